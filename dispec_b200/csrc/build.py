@@ -36,6 +36,9 @@ CORE_SOURCES = [
     "attn_combine.cu",
     "dense_chain.cu",
     "sampling.cu",
+    "tree_attn.cu",
+    "tree_keep.cu",
+    "tree_verify.cu",
     "random_fill.cu",
     "selftest.cu",
 ]

@@ -6,6 +6,7 @@ from dispec_b200.ops.elementwise import GLU_ACTS, embed, feed_tokens, fill_norma
 from dispec_b200.ops.gemm import linear
 from dispec_b200.ops.library import KernelError, device_error, raise_on_device_error
 from dispec_b200.ops.sampling import argmax, sample
+from dispec_b200.ops.tree import keep_path, tree_attention, verify_tree
 
 __all__ = ["GLU_ACTS", "paged_attention", "embed", "feed_tokens", "fill_normal", "rms_norm", "rope_kv_store", "swiglu", "linear",
-           "KernelError", "device_error", "raise_on_device_error", "argmax", "sample"]
+           "KernelError", "device_error", "raise_on_device_error", "argmax", "sample", "keep_path", "tree_attention", "verify_tree"]
