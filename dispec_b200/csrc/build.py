@@ -167,6 +167,7 @@ def build_all(head_dims=(16, 32, 64, 128)) -> list[str]:
         libs.append(attention_library(d))
         if d in (64, 128):
             libs.append(prefill_attention_library(d))
+            libs.append(tree_attention_library(d))
     libs += [mixer_library(name) for name in MIXER_LIBRARIES]
     # the attention with widths of their own for keys and values is compiled per pair of widths
     libs += [sink_attention_library(dk, dv) for dk, dv in ((64, 64), (128, 64), (128, 128))]
@@ -180,6 +181,11 @@ def attention_library(head_dim: int) -> str:
 
 def prefill_attention_library(head_dim: int) -> str:
     return specialised_library(f"attn_tcgen05_d{head_dim}", "attn_tcgen05.cu", {"DSP_HEAD_DIM": head_dim})
+
+
+def tree_attention_library(head_dim: int) -> str:
+    """The attention of drafted trees on the tensor cores."""
+    return specialised_library(f"tree_attn_tcgen05_d{head_dim}", "tree_attn_tcgen05.cu", {"DSP_HEAD_DIM": head_dim})
 
 
 def sink_attention_library(key_dim: int, value_dim: int) -> str:

@@ -222,6 +222,8 @@ __global__ void __launch_bounds__(128)
 tree_combine_kernel(const Shape sh, const float* __restrict__ part_o, const float* __restrict__ part_ml,
                     T* __restrict__ out, long out_stride, int D, int ctas) {
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
   long total;
   const long chunk = units_per_cta(sh, ctas, &total);
   const long last = min(total, chunk * (c + 1)) - 1;  // last unit of CTA c
@@ -282,8 +284,14 @@ cudaError_t tree_combine(const tree::Shape& sh, const float* part_o, const float
                          int D, int ctas, int dtype, cudaStream_t stream) {
   const dim3 grid(ctas, (sh.rows_per_tile + 15) / 16);
   return dtype == DSP_F32
-             ? launch_plain(tree_combine_kernel<float>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (float*)out, out_stride, D, ctas)
-             : launch_plain(tree_combine_kernel<bf16>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (bf16*)out, out_stride, D, ctas);
+             ? launch_pdl(tree_combine_kernel<float>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (float*)out, out_stride, D, ctas)
+             : launch_pdl(tree_combine_kernel<bf16>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (bf16*)out, out_stride, D, ctas);
+}
+
+// The same for kernels that live in other libraries.
+extern "C" int dsp_tree_combine(const tree::Shape* sh, const float* part_o, const float* part_ml, void* out, long out_stride,
+                                int D, int ctas, int dtype, cudaStream_t stream) {
+  return tree_combine(*sh, part_o, part_ml, out, out_stride, D, ctas, dtype, stream) == cudaSuccess ? 0 : 1;
 }
 
 // What the Python side packs, in this order (ops/tree.py).
@@ -296,9 +304,6 @@ struct DspTreeAttention {
   long q_stride, out_stride, pt_stride, words, S, H, KVH, D, page_size, num_pages, window, dtype, ctas;
   double scale;
 };
-
-// Floats of scratch that dsp_tree_attention wants.
-extern "C" long dsp_tree_attention_scratch(int ctas, int D) { return 2L * ctas * ROWS * (D + 2); }
 
 extern "C" int dsp_tree_attention(const DspTreeAttention* p, cudaStream_t stream) {
   if (p->S == 0) return 0;

@@ -1,0 +1,651 @@
+// Attention of drafted trees over the paged cache on the fifth-generation tensor cores, bfloat16 in, 32-bit softmax and
+// accumulation (the formula: tree_attn.cu; how the work is cut: tree_schedule.cuh).  Compiled once per head size
+// (-DDSP_HEAD_DIM=64 or 128).
+//
+// One CTA an SM walks its run of units: for each item's share, 128 query rows of one key/value head and key tiles of 64.
+// S = Q K^T and O += P V are tcgen05.mma with S, O and the A operands Q and P in tensor memory; keys and values arrive by
+// TMA in rings of their own that run on from share to share.  Roles:
+//   warp 0      requests the key and value tiles;
+//   warps 1, 11 issue the score products of softmax group 0 and of group 1;
+//   warp 10     issues the output products;
+//   warps 2..9  two softmax groups of four warps: group g owns the key tiles g, g + 2, ... of a share with a score buffer,
+//               output accumulator, P, running maximum and sum of its own; thread r of a group owns row r.
+// At the end of a share group 0 merges the two halves and stores the rows (or leaves a partial result) while group 1
+// brings the next share's queries.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
+// its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output
+// product.  Every wait is bounded; one that runs out sets the device error word.
+#include "tcgen05_common.cuh"
+#include "tree_schedule.cuh"
+
+#ifndef DSP_HEAD_DIM
+#error "compile with -DDSP_HEAD_DIM=<head size>"
+#endif
+#define DSP_CAT2(a, b) a##b
+#define DSP_CAT(a, b) DSP_CAT2(a, b)
+
+namespace {
+using namespace tc;
+using namespace tree;
+
+constexpr int D = DSP_HEAD_DIM;
+static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
+constexpr int BM = 128, BN = 64, THREADS = 384;
+constexpr int K_STAGES = 5, V_STAGES = 7;
+constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
+static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
+constexpr int PV_WARP = 10, S1_WARP = 11;
+constexpr int KD = D / 64;
+constexpr int KV_SLICE = BN * 128;
+constexpr int KV_BYTES = KD * KV_SLICE;
+constexpr int SMEM_BYTES = (K_STAGES + V_STAGES) * KV_BYTES + 1024;
+// tensor memory, 32-bit columns
+constexpr int S_COLS = BN;
+constexpr int O_COL = 2 * S_COLS;
+constexpr int P_COLS = BN / 2;
+constexpr int P_COL = O_COL + 2 * D;
+constexpr int Q_COL = P_COL + 2 * P_COLS;
+constexpr int TMEM_COLS = 512;
+static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
+constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
+
+struct Params {
+  Shape sh;
+  const bf16* q;
+  const int *page_table, *depth;
+  const unsigned long long* visible;
+  bf16* out;
+  float *part_o, *part_ml;
+  long q_stride, out_stride;
+  int pt_stride, words, page_size, num_pages;
+  int page_runs;  // the run maps are valid
+  float scale_log2;
+  int* err;
+};
+
+// Which keys key0 .. key0 + 63 the row of a node sees: stored ones, and nodes of the tree by the row's words.
+__device__ __forceinline__ unsigned long long seen_keys(const Params& p, const Tree& t, int row, int depth, int key0) {
+  unsigned long long stored = 0ull, drafted = 0ull;
+  const int off = key0 - t.ctx;  // number of the first key as a node
+  if (off < 0) {
+    stored = off <= -64 ? ~0ull : (1ull << -off) - 1ull;
+    if (p.sh.window > 0) {
+      const int hidden = t.ctx + depth - p.sh.window + 1 - key0;  // so many first keys are out of the window
+      if (hidden > 0) stored = hidden >= 64 ? 0ull : stored & ~((1ull << hidden) - 1ull);
+    }
+  }
+  if (off > -64 && off < t.n) {
+    const unsigned long long* w = p.visible + (size_t)row * p.words;
+    if (off <= 0) {
+      drafted = w[0] << -off;
+    } else {
+      const int k = off >> 6, sft = off & 63;
+      drafted = k < p.words ? w[k] >> sft : 0ull;
+      if (sft && k + 1 < p.words) drafted |= w[k + 1] << (64 - sft);
+    }
+    const int there = t.n - off;  // keys up to the tree's last node
+    if (there < 64) drafted &= (1ull << there) - 1ull;
+    if (p.sh.window > 0 && depth >= p.sh.window) {  // a tree deeper than the window
+      for (unsigned long long left = drafted; left != 0ull; left &= left - 1ull) {
+        const int c = __ffsll((long long)left) - 1;
+        if (p.depth[t.first + off + c] <= depth - p.sh.window) drafted &= ~(1ull << c);
+      }
+    }
+  }
+  return stored | drafted;
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap runs_k,
+                         const __grid_constant__ CUtensorMap runs_v) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);  // swizzle atoms are 1024 bytes
+  __shared__ __align__(8) uint64_t k_full[K_STAGES], k_empty[K_STAGES];  // landed; its scores are complete
+  __shared__ __align__(8) uint64_t v_full[V_STAGES], v_empty[V_STAGES];  // landed; its output product is complete
+  __shared__ __align__(8) uint64_t s_full[2], s_free[2];  // a score buffer is complete; the group has read it
+  __shared__ __align__(8) uint64_t p_full[2], o_done[2];  // P written, O rescaled, V rows zeroed; the output product is complete
+  __shared__ __align__(8) uint64_t q_ready[2];            // the queries of a share with tiles for the group are in tensor memory
+  __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
+  __shared__ float merge_m[2][BM], merge_l[2][BM];        // group 1's maximum and sum per row, by share in turn
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed, failed_share;  // a wait ran out; the first share in which one of a softmax warp did
+  __shared__ uint32_t bad_pages[BAD_SLOTS];  // of key tile n, in slot n % BAD_SLOTS; bit j: page j had no valid id (not loaded)
+
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
+  const Shape& sh = p.sh;
+  Walk w;
+  if (!w.begin(sh, cta, gridDim.x)) return;
+  const int G = sh.G;
+  unsigned char* k_s = smem;  // [stage][slice][64 keys][128 bytes]
+  unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
+
+  if (tid == 0) {
+    for (int s = 0; s < K_STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < V_STAGES; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&s_free[b], 4);
+      mbar_init(&p_full[b], 4);
+      mbar_init(&o_done[b], 1);
+    }
+    mbar_init(&q_ready[0], 4);
+    mbar_init(&q_ready[1], 4);
+    mbar_init(&o_free, 4);
+    failed = 0;
+    failed_share = 0x7fffffff;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    // ---- requests of the K and V tiles.  Page ids are looked up for a chunk of 32 / pages_per_tile tiles at a time, a
+    // chunk ahead; two tiles per turn, each with a lane of its own that waits for the ring slots and makes the requests.
+    const int pages_per_tile = BN / p.page_size;
+    const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.page_size * 128u;
+    const int ppt_shift = __ffs(pages_per_tile) - 1, page_shift = __ffs(p.page_size) - 1;  // powers of two here
+    const int chunk_shift = 5 - ppt_shift, chunk_mask = (1 << chunk_shift) - 1;
+    const int page_in_tile = lane & (pages_per_tile - 1);
+    const uint32_t tile_lanes = pages_per_tile == 32 ? 0xffffffffu : ((1u << pages_per_tile) - 1u);
+    int sk = 0, rk = 0, sv = 0, rv = 0;  // ring slots of the turn's first tile, and their use counts
+    int done = 0;                        // tiles of the shares before
+    do {
+      const int n_kt = w.kt_end - w.kt_begin, kt_begin = w.kt_begin;
+      const int lo = sh.window > 0 ? max(0, w.t.ctx - sh.window + 1) : 0, last = w.t.ctx + w.t.n - 1;
+      const int* table = p.page_table + (size_t)w.at.seq * p.pt_stride;
+      auto load_chunk = [&](int c) -> int {
+        const int i = (c << chunk_shift) + (lane >> ppt_shift);
+        const int first = (kt_begin + i) * BN + page_in_tile * p.page_size;
+        if (i < n_kt && first <= last && first + p.page_size > lo) {
+          const int j = first >> page_shift;
+          return j < p.pt_stride ? table[j] : -1;
+        }
+        return -2;  // not wanted
+      };
+      int pg = -2, pg_next = load_chunk(0);
+      uint32_t bad_mask = 0, live_mask = 0, run_mask = 0;
+      for (int i = 0; i < n_kt; i += 2) {
+        const int in_chunk = i & chunk_mask;
+        if (in_chunk == 0) {
+          pg = pg_next;
+          pg_next = load_chunk((i >> chunk_shift) + 1);
+          const bool bad = pg != -2 && (pg < 0 || pg >= p.num_pages);  // recorded, not loaded, its keys are hidden
+          if (bad) {
+            atomicOr(p.err, DSP_ERR_BAD_PAGE);
+            pg = -1;
+          }
+          bad_mask = __ballot_sync(0xffffffffu, bad);
+          live_mask = __ballot_sync(0xffffffffu, pg >= 0);
+          const int first_pg = __shfl_sync(0xffffffffu, pg, lane & ~(pages_per_tile - 1));
+          run_mask = __ballot_sync(0xffffffffu, pg >= 0 && pg == first_pg + page_in_tile &&
+                                                    first_pg + pages_per_tile <= p.num_pages);
+        }
+        const int second = (lane >> ppt_shift) - in_chunk;  // 0, 1: this lane holds a page of the turn's first, second tile
+        const bool mine = (second == 0 || second == 1) && i + second < n_kt;
+        const int shift = (in_chunk + (second == 1 ? 1 : 0)) << ppt_shift;
+        const uint32_t live = (live_mask >> shift) & tile_lanes;
+        const bool in_run = p.page_runs && ((run_mask >> shift) & tile_lanes) == tile_lanes;
+        const bool leader = mine && lane == shift;
+        int my_sk = sk, my_rk = rk, my_sv = sv, my_rv = rv;
+        if (second == 1) {
+          if (++my_sk == K_STAGES) {
+            my_sk = 0;
+            ++my_rk;
+          }
+          if (++my_sv == V_STAGES) {
+            my_sv = 0;
+            ++my_rv;
+          }
+        }
+        if (leader) {
+          if (*(volatile int*)&failed == 0 &&
+              mbar_wait_both(&k_empty[my_sk], (my_rk & 1) ^ 1, &v_empty[my_sv], (my_rv & 1) ^ 1)) {
+            bad_pages[(done + i + second) % BAD_SLOTS] = (bad_mask >> shift) & tile_lanes;  // published by the arrival on k_full
+            if (live == 0) {
+              mbar_arrive(&k_full[my_sk]);
+              mbar_arrive(&v_full[my_sv]);
+            } else {
+              mbar_expect_tx(&k_full[my_sk], (uint32_t)__popc(live) * page_bytes);
+              mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
+            }
+            if (in_run) {  // the tile's pages lie one after the other in the pool: one request per operand
+              tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, w.head * p.page_size, pg, 0);
+              tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, w.head * p.page_size, pg, 0);
+            }
+          } else {
+            failed = 1;
+          }
+        }
+        if (!__all_sync(0xffffffffu, !mine || in_run)) {
+          if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
+            const int row = (pg * sh.KVH + w.head) * p.page_size;
+            const int dst = page_in_tile * p.page_size * 128;
+#pragma unroll
+            for (int h = 0; h < KD; ++h) {
+              tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
+              tma_load_2d(v_s + my_sv * KV_BYTES + dst + h * KV_SLICE, &map_v, &v_full[my_sv], h * 64, row);
+            }
+          }
+        }
+        for (int u = 0; u < min(2, n_kt - i); ++u) {
+          if (++sk == K_STAGES) {
+            sk = 0;
+            ++rk;
+          }
+          if (++sv == V_STAGES) {
+            sv = 0;
+            ++rv;
+          }
+        }
+      }
+      done += n_kt;
+    } while (w.next(sh, cta));
+  } else if (warp == 1 || warp == S1_WARP) {
+    // ---- score products of one softmax group
+    const int g = warp == 1 ? 0 : 1;
+    const bool leader = elect_one();
+    const uint32_t idesc_s = umma_idesc(BM, BN);
+    const uint64_t k_desc0 = umma_desc(smem_u32(k_s));
+    const uint32_t tmem_s = tmem_base + (uint32_t)(g * S_COLS);
+    int done = 0, count = 0, share = 0;  // tiles of the shares before; this group's tiles, and shares with any, so far
+    bool ok = true;
+    do {
+      const int n_kt = w.kt_end - w.kt_begin;
+      if (g < n_kt) {
+        ok = mbar_wait(&q_ready[g], share & 1);
+        ++share;
+        tc_fence_after();
+        for (int a = g; a < n_kt && ok; a += 2, ++count) {
+          const int s = (done + a) % K_STAGES, use = (done + a) / K_STAGES;
+          ok = count == 0 ? mbar_wait(&k_full[s], use & 1)
+                          : mbar_wait_both(&k_full[s], use & 1, &s_free[g], (count - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t k_desc = k_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (uint32_t)(k >> 2), in = (uint32_t)(k & 3) * 32u;
+              umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * KV_SLICE + in) >> 4), idesc_s, k != 0);
+            }
+            umma_commit(&s_full[g]);
+            umma_commit(&k_empty[s]);
+          }
+        }
+      }
+      done += n_kt;
+    } while (ok && w.next(sh, cta));
+    if (!ok) failed = 1;
+  } else if (warp == PV_WARP) {
+    // ---- output products: O[g] += P[g] V of the share's tiles in turn
+    const bool leader = elect_one();
+    const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
+    const uint64_t v_desc0 = umma_desc_mn(smem_u32(v_s), KV_SLICE);
+    int done = 0, share = 0, count[2] = {0, 0};
+    bool ok = true;
+    do {
+      const int n_kt = w.kt_end - w.kt_begin;
+      if (share > 0) ok = mbar_wait(&o_free, (share - 1) & 1);
+      for (int b = 0; b < n_kt && ok; ++b) {
+        const int g = b & 1, st = (done + b) % V_STAGES;
+        ok = mbar_wait_both(&v_full[st], ((done + b) / V_STAGES) & 1, &p_full[g], (g ? count[1] : count[0]) & 1);
+        if (!ok) break;
+        if (g)
+          ++count[1];
+        else
+          ++count[0];
+        tc_fence_after();
+        const uint64_t v_desc = v_desc0 + (uint64_t)(st * (KV_BYTES >> 4));
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k)
+            umma_a_tmem(tmem_base + (uint32_t)(O_COL + g * D), tmem_base + (uint32_t)(P_COL + g * P_COLS + k * 8),
+                        v_desc + (uint64_t)(k * 128), idesc_o, (b >= 2) || k != 0);
+          umma_commit(&v_empty[st]);
+          umma_commit(&o_done[g]);
+        }
+      }
+      done += n_kt;
+      ++share;
+    } while (ok && w.next(sh, cta));
+    if (!ok) failed = 1;
+  } else {
+    // ---- softmax groups
+    const int g = (warp - 2) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
+    const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
+    const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
+    const float scale = p.scale_log2;
+    const int page_shift = __ffs(p.page_size) - 1;
+    // the queries of a share: row r of the tile, lane r, two bfloat16 per column (rows past the item are zero)
+    auto bring_queries = [&]() {
+      const int row0 = w.row_tile * BM, rr = row0 + r;
+      const bool valid = rr < w.t.n * G;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q);
+      if (valid)
+        src = reinterpret_cast<const uint4*>(p.q + (size_t)(w.t.first + rr / G) * p.q_stride +
+                                             (size_t)(w.head * G + rr % G) * D);
+#pragma unroll
+      for (int c0 = 0; c0 < D / 2; c0 += 32) {
+        uint32_t x[32];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 v = valid ? __ldg(src + c0 / 4 + c) : make_uint4(0, 0, 0, 0);
+          x[4 * c] = v.x;
+          x[4 * c + 1] = v.y;
+          x[4 * c + 2] = v.z;
+          x[4 * c + 3] = v.w;
+        }
+        tmem_st32(lane_addr + (uint32_t)(Q_COL + c0), x);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&q_ready[0]);
+        if (w.kt_end - w.kt_begin > 1) mbar_arrive(&q_ready[1]);
+      }
+    };
+    if (g == 1) bring_queries();
+    int done = 0, count = 0, share = 0;
+    bool more = true;
+    do {
+      const Tree t = w.t;
+      const int n_kt = w.kt_end - w.kt_begin, kt_begin = w.kt_begin, row0 = w.row_tile * BM, slot = w.slot, head = w.head;
+      const int nrows = min(BM, t.n * G - row0);
+      const bool row_ok = r < nrows;
+      const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
+      const int node = row_ok ? t.first + (row0 + r) / G : t.first;
+      const int depth = sh.window > 0 ? p.depth[node] : 0;
+      const int total = t.ctx + t.n;
+      const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;  // first key any row sees
+      const int lo_r = sh.window > 0 ? t.ctx + depth - sh.window + 1 : 0;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool ok = true;
+      int j = 0;  // tiles of this group in this share
+      for (int i = g; i < n_kt; i += 2, ++j, ++count) {
+        const int key0 = (kt_begin + i) * BN;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], count & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sv[64];
+        const uint32_t bad = bad_pages[(done + i) % BAD_SLOTS];
+        float alpha = 1.f;
+        uint32_t pk[32];
+        if (warp_ok) {
+          uint32_t a[32], b[32];
+          tmem_ld32_nowait(s_addr, a);
+          tmem_ld32_nowait(s_addr + 32, b);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            sv[c] = a[c];
+            sv[32 + c] = b[c];
+          }
+        }
+        // the scores are in registers: the next scores of this group may overwrite S[g]
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[g]);
+        if (warp_ok) {
+          if (key0 + BN > t.ctx || bad != 0u || __any_sync(0xffffffffu, key0 < lo_r)) {
+            unsigned long long seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
+            if (bad != 0u)
+              for (int b = 0; b < BN >> page_shift; ++b)
+                if ((bad >> b) & 1u)
+                  seen &= ~((p.page_size == 64 ? ~0ull : (1ull << p.page_size) - 1ull) << (b << page_shift));
+            const uint32_t s_lo = (uint32_t)seen, s_hi = (uint32_t)(seen >> 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              sv[c] = (s_lo >> c) & 1u ? sv[c] : 0xff800000u;  // -inf
+              sv[32 + c] = (s_hi >> c) & 1u ? sv[32 + c] : 0xff800000u;
+            }
+          }
+          float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            t0 = fmaxf(t0, __uint_as_float(sv[c]));
+            t1 = fmaxf(t1, __uint_as_float(sv[c + 1]));
+            t2 = fmaxf(t2, __uint_as_float(sv[c + 2]));
+            t3 = fmaxf(t3, __uint_as_float(sv[c + 3]));
+          }
+          const float tmax = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;  // the scale is positive
+          const float m_new = (tmax > m_run + RESCALE_STEP || m_run == -INFINITY) ? fmaxf(tmax, m_run) : m_run;
+          alpha = m_new == m_run ? 1.f : ex2(m_run - m_new);  // 0 on a row's first visible tile
+          m_run = m_new;
+          const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+          float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const float e0 = ex2(fmaf(__uint_as_float(sv[c]), scale, neg_m));
+            const float e1 = ex2(fmaf(__uint_as_float(sv[c + 1]), scale, neg_m));
+            const float e2 = ex2(fmaf(__uint_as_float(sv[c + 2]), scale, neg_m));
+            const float e3 = ex2(fmaf(__uint_as_float(sv[c + 3]), scale, neg_m));
+            a0 += e0;
+            a1 += e1;
+            a2 += e2;
+            a3 += e3;
+            pk[c / 2] = pack2(e0, e1);
+            pk[c / 2 + 1] = pack2(e2, e3);
+          }
+          l_run = l_run * alpha + ((a0 + a1) + (a2 + a3));
+        }
+        // the group's previous O[g] += P V must be complete before O[g] is rescaled and P[g] rewritten
+        if (j > 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (warp_ok && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              uint32_t ov[32];
+              tmem_ld32(o_addr + (uint32_t)c0, ov);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+              tmem_st32(o_addr + (uint32_t)c0, ov);
+            }
+          }
+        }
+        if (warp_ok) tmem_st32(p_addr, pk);  // 64 bfloat16 in the 32 columns of the group's A operand
+        // value rows no row of this item may see: zero them (whole 128-byte rows, every slice)
+        if (key0 < lo || key0 + BN > total || bad != 0u) {
+          const int st = (done + i) % V_STAGES;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], ((done + i) / V_STAGES) & 1))) {
+            ok = false;
+            break;
+          }
+          const int key_row = r >> 1;  // two threads per key row
+          const int key = key0 + key_row;
+          const bool dead = key >= total || key < lo || ((bad >> (key_row >> page_shift)) & 1u);
+          if (dead) {
+            const uint32_t row_addr = smem_u32(v_s + st * KV_BYTES) + (uint32_t)key_row * 128u + (uint32_t)(r & 1) * 64u;
+#pragma unroll
+            for (int h = 0; h < KD; ++h)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * KV_SLICE + c * 16, make_uint4(0, 0, 0, 0));
+          }
+          fence_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+      }
+      // the group's last product of the share
+      if (ok && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) ok = false;
+      if (!ok) {
+        failed = 1;
+        atomicMin(&failed_share, share);
+      }
+      if (g == 1) {
+        merge_m[share & 1][r] = m_run;
+        merge_l[share & 1][r] = l_run;
+      }
+      tc_fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
+      if (*(volatile int*)&failed_share <= share) break;  // all of them see the same
+      tc_fence_after();
+      if (g == 1) {
+        more = w.next(sh, cta);
+        if (more) bring_queries();
+      } else {
+        // ---- merge the two groups' halves of the share; store the rows, or the partial result of the share
+        const bool two = n_kt > 1;
+        const float m1 = two ? merge_m[share & 1][r] : -INFINITY, l1 = two ? merge_l[share & 1][r] : 0.f;
+        const float M = fmaxf(m_run, m1);
+        const float w0 = m_run == -INFINITY ? 0.f : ex2(m_run - M);
+        const float w1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+        const float denom = l_run * w0 + l1 * w1;
+        const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
+        const float f0 = w0 * inv, f1 = w1 * inv;
+        if (warp_ok) {
+          bf16* dst = p.out;
+          float* part = p.part_o;
+          if (slot >= 0)
+            part += ((size_t)slot * BM + r) * D;
+          else if (row_ok)
+            dst += (size_t)node * p.out_stride + (size_t)(head * G + (row0 + r) % G) * D;
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t ov[32], ow[32];
+            tmem_ld32_nowait(lane_addr + (uint32_t)(O_COL + c0), ov);
+            if (two) tmem_ld32_nowait(lane_addr + (uint32_t)(O_COL + D + c0), ow);
+            tmem_ld_wait();
+            // (a half that saw no key has weight 0, and an accumulator of zeros)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              ov[c] = __float_as_uint(two ? __uint_as_float(ov[c]) * f0 + __uint_as_float(ow[c]) * f1
+                                          : __uint_as_float(ov[c]) * f0);
+            if (row_ok && slot >= 0) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
+            } else if (row_ok) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+                uint4 x;
+                x.x = pack2(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]));
+                x.y = pack2(__uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3]));
+                x.z = pack2(__uint_as_float(ov[c + 4]), __uint_as_float(ov[c + 5]));
+                x.w = pack2(__uint_as_float(ov[c + 6]), __uint_as_float(ov[c + 7]));
+                *reinterpret_cast<uint4*>(dst + c0 + c) = x;
+              }
+            }
+            __syncwarp();
+          }
+          if (slot >= 0 && row_ok) reinterpret_cast<float2*>(p.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free);
+        more = w.next(sh, cta);
+      }
+      done += n_kt;
+      ++share;
+    } while (more);
+  }
+
+  pdl_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (failed) {
+    if (threadIdx.x == 0) atomicOr(p.err, DSP_ERR_WAIT_LIMIT);
+    // let copies that are still on their way land before the shared memory goes away
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);
+  }
+  tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+}  // namespace
+
+// As dsp_tree_attention (tree_attn.cu), whose merge of partial results it calls at `combine`.  Returns 0, or: 1 launch
+// failed, 2 unsupported sizes (page sizes are 8, 16, 32 or 64), 3 misaligned rows, 4 the shared-memory opt-in or the tensor
+// maps failed.
+struct DspTreeAttention {
+  const void *q, *k_pool, *v_pool;
+  const int *page_table, *ctx_len, *node_start, *depth;
+  const unsigned long long* visible;
+  void* out;
+  float* scratch;
+  long q_stride, out_stride, pt_stride, words, S, H, KVH, D, page_size, num_pages, window, dtype, ctas;
+  double scale;
+};
+typedef int (*TreeCombine)(const Shape*, const float*, const float*, void*, long, int, int, int, cudaStream_t);
+
+extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTreeAttention* a, void* combine, int* err,
+                                                                   cudaStream_t stream) {
+  if (a->S <= 0) return a->S == 0 ? 0 : 2;
+  const int page = (int)a->page_size;
+  if (a->D != D || a->KVH <= 0 || a->H <= 0 || a->H % a->KVH != 0 || a->dtype != DSP_BF16) return 2;
+  if (page != 8 && page != 16 && page != 32 && page != 64) return 2;
+  if (!(a->scale > 0.) || a->ctas < 1 || a->words < 1 || a->num_pages < 1) return 2;
+  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->k_pool | (uintptr_t)a->v_pool | (uintptr_t)a->out;
+  if (bits % 16 != 0 || a->q_stride % 8 != 0 || a->out_stride % 8 != 0) return 3;
+  Params p = {};
+  p.sh.node_start = a->node_start;
+  p.sh.ctx_len = a->ctx_len;
+  p.sh.S = (int)a->S;
+  p.sh.KVH = (int)a->KVH;
+  p.sh.G = (int)(a->H / a->KVH);
+  p.sh.rows_per_tile = BM;
+  p.sh.keys_per_tile = BN;
+  p.sh.window = (int)a->window;
+  p.sh.min_units = 2;  // one tile for each softmax group
+  p.q = (const bf16*)a->q;
+  p.page_table = a->page_table;
+  p.depth = a->depth;
+  p.visible = a->visible;
+  p.out = (bf16*)a->out;
+  p.part_o = a->scratch;
+  p.part_ml = a->scratch + 2 * a->ctas * BM * D;
+  p.q_stride = a->q_stride;
+  p.out_stride = a->out_stride;
+  p.pt_stride = (int)a->pt_stride;
+  p.words = (int)a->words;
+  p.page_size = page;
+  p.num_pages = (int)a->num_pages;
+  p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+  p.err = err;
+  CUtensorMap map_k, map_v, runs_k, runs_v;
+  const long rows = a->num_pages * a->KVH * page;
+  if (!make_map(&map_k, a->k_pool, rows, D, D, page) || !make_map(&map_v, a->v_pool, rows, D, D, page)) return 4;
+  // a pool of fewer pages than a key tile has gives no map of runs
+  p.page_runs = make_map_page_runs(&runs_k, a->k_pool, a->num_pages, p.sh.KVH, page, D, BN / page) &&
+                make_map_page_runs(&runs_v, a->v_pool, a->num_pages, p.sh.KVH, page, D, BN / page);
+  if (!p.page_runs) {
+    runs_k = map_k;
+    runs_v = map_v;
+  }
+  if (cudaFuncSetAttribute(tree_attn_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+    return 4;
+  if (launch_pdl(tree_attn_tcgen05_kernel, dim3((unsigned)a->ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, p, map_k, map_v,
+                 runs_k, runs_v) != cudaSuccess)
+    return 1;
+  return reinterpret_cast<TreeCombine>(combine)(&p.sh, p.part_o, p.part_ml, p.out, p.out_stride, D, (int)a->ctas, DSP_BF16, stream);
+}

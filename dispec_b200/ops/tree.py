@@ -8,6 +8,7 @@ keeps its key and value at place ``ctx_len[s] + i`` of its request's cache until
 of the accepted branch."""
 from __future__ import annotations
 
+import ctypes
 import struct
 from dataclasses import dataclass
 
@@ -15,8 +16,10 @@ import torch
 
 from dispec_b200.ops import library as L
 from dispec_b200.ops import tuning
+from dispec_b200.ops.attention import _TCGEN05_ERRORS, _device_error_address
 
 MAX_HEAD_DIM = 256
+TENSOR_CORE_ROWS, FMA_ROWS = 128, 32  # rows of a tile of the two attention kernels
 MAX_POOLS = 8
 _ATTENTION = struct.Struct("10q13qd")
 _VERIFY = struct.Struct("11q6q")
@@ -91,14 +94,25 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         return out
     lib = L.core()
     ctas = tuning.sm_count(dev)
-    # scratch of this call alone: calls on several streams do not meet in it
-    scratch = torch.empty((lib.dsp_tree_attention_scratch(ctas, dim),), dtype=torch.float32, device=dev)
+    # the tensor-core kernel is built for these head and page sizes; bfloat16 in others and float32 take the 32-bit kernel
+    tensor_cores = q.dtype == torch.bfloat16 and dim in (64, 128) and page_size in (8, 16, 32, 64) and num_pages > 0
+    rows = TENSOR_CORE_ROWS if tensor_cores else FMA_ROWS
+    # scratch of this call alone (calls on several streams do not meet in it): two partial results for each CTA
+    scratch = torch.empty((2 * ctas * rows * (dim + 2),), dtype=torch.float32, device=dev)
     args = _ATTENTION.pack(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ctx_len.data_ptr(), node_start.data_ptr(),
         0 if depth is None else depth.data_ptr(), visible.data_ptr(), out.data_ptr(), scratch.data_ptr(), q.stride(0),
         out.stride(0), page_table.stride(0), visible.shape[1], S, heads, kv_heads, dim, page_size, num_pages, window, dtype,
         ctas, scale)
-    L.check(lib.dsp_tree_attention(args, L.stream_handle()), launches=2)
+    if tensor_cores:
+        kernel = getattr(L.tree_attention_library(dim), f"dsp_tree_attention_tcgen05_d{dim}")
+        rc = kernel(args, ctypes.c_void_p(L.address_of(lib, "dsp_tree_combine")),
+                    ctypes.c_void_p(_device_error_address(dev)), L.stream_handle())
+        L.LaunchCounter.n += 2
+        if rc != 0:
+            _refuse(what, _TCGEN05_ERRORS.get(rc, str(rc)))
+    else:
+        L.check(lib.dsp_tree_attention(args, L.stream_handle()), launches=2)
     return out
 
 

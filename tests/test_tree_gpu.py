@@ -31,9 +31,19 @@ def test_attention_head_layouts(dtype, heads, kv_heads, dim):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("spec", [[(0, 1)], [(1, 1)], [(0, 64)], [(0, 65), (130, 130)], [(5000, 3)], [(62, 2), (63, 2), (64, 2)],
-                                  [(10, 0), (20, 4), (30, 0)], [(700, 256)], [(40, 4)] * 70, [(3, 1)] * 200])
+                                  [(10, 0), (20, 4), (30, 0)], [(700, 256)], [(40, 4)] * 70, [(3, 1)] * 200,
+                                  [(130, 5), (64, 3), (190, 20)] * 40])
 def test_attention_lengths(dtype, spec):
     AttentionCase(trees(spec), 12, 2, 128, dtype, seed=3).check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kv_heads,window", [(8, 0), (3, 50), (5, 0), (7, 100)])
+def test_attention_many_shares_a_cta(dim, kv_heads, window):
+    """Work that is cut at every place: shares of one key tile and of many follow one another in a CTA."""
+    spec = [(100 + 61 * i % 400, 1 + 7 * i % 40) for i in range(60)]
+    AttentionCase(trees(spec), 4 * kv_heads, kv_heads, dim, BF16, window=window).check()
     no_device_error()
 
 
