@@ -12,11 +12,23 @@
 // accepted tokens and the drawn one together are distributed as the target's own samples.  Where no child is taken, the
 // token is the first v whose masses up to v exceed min(R - 1, floor(draw R)).  NaN counts as -inf; a row without a finite
 // or infinite largest logit gives token 0.
+//
+// A cluster of up to 16 CTAs works on one tree and reads only the rows of the nodes that the walk comes to, each of them
+// once: every CTA keeps its share of the row in shared memory, first as scaled logits, then as exponentials, and the CTAs
+// exchange the largest logit and the sums of masses through each other's shared memory (one cluster barrier each).  The
+// tests of a node's children need R and a few numbers that are read while the row arrives; every CTA makes them for itself, with the same result.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace {
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_CTAS = 16, MAX_NODES = 1024;
+constexpr int SHARE = 24 * 1024;      // logits of a row in a CTA's shared memory, two CTAs an SM
+constexpr int MAX_VOCAB = 1 << 19;    // 32,768 logits in each of 16 CTAs
 typedef long long mass_t;
+constexpr mass_t ONE = (mass_t)1 << 40;
 
 struct Args {
   const void* logits;
@@ -25,7 +37,7 @@ struct Args {
   const float *temperature, *uniforms, *draws;
   int *path, *count, *token;
   long ld, ldq;
-  int V, max_nodes;
+  int V, share, max_nodes;
   int* err;
 };
 
@@ -34,161 +46,314 @@ __device__ __forceinline__ mass_t warp_sum_mass(mass_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float scale_logit(float l, float temp) {
+  return isnan(l) ? -INFINITY : temp > 0.f ? __fdiv_rn(l, temp) : l;
+}
+__device__ __forceinline__ float exponential(float x, float top) { return x == top ? 1.f : expf(x - top); }
+__device__ __forceinline__ mass_t mass_of(float e) { return (mass_t)(e * 1099511627776.f); }
 
-// What a pass over a row needs to know.
-template <typename T>
-struct Row {
-  const T* x;
-  const float* q;   // draft probabilities, or null
-  float temp, top;  // largest scaled logit
-  int first;        // lowest index of it
-  bool alone;       // all the mass is on `first`
-  int refused;      // refusals so far
-  const float* left;  // with draft probabilities: R at each refusal
-  const int* gone;    // without: the refused tokens
-
-  __device__ __forceinline__ float scaled(int v) const {
-    const float l = to_f32(x[v]);
-    return isnan(l) ? -INFINITY : temp > 0.f ? __fdiv_rn(l, temp) : l;
-  }
-  __device__ __forceinline__ mass_t mass(int v) const {
-    mass_t m;
-    if (alone) {
-      m = v == first ? (mass_t)1 << 40 : 0;
-    } else {
-      const float s = scaled(v);
-      m = s == top ? (mass_t)1 << 40 : (mass_t)(expf(s - top) * 1099511627776.f);
-    }
-    if (q != nullptr) {
-      const float qv = refused > 0 ? q[v] : 0.f;
-      for (int k = 0; k < refused; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qv, left[k]));
-    } else {
-      for (int k = 0; k < refused; ++k)
-        if (gone[k] == v) m = 0;
-    }
-    return m;
-  }
+// One exchange: every CTA of the cluster tells every other one a number.
+struct Mailbox {
+  float value[2][MAX_CTAS];
+  mass_t mass[2][MAX_CTAS];
 };
 
-template <typename T>
+template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(THREADS)
 tree_verify_kernel(const Args a) {
-  extern __shared__ int list[];  // [max_nodes] refused tokens, or the R at each refusal
-  __shared__ float f_scratch[32];
-  __shared__ mass_t m_scratch[32];
-  __shared__ int found;
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
+  extern __shared__ float xs[];  // [share] this CTA's part of the row
+  __shared__ Mailbox box;
+  __shared__ int parents[MAX_NODES];
+  __shared__ float cand_x[MAX_NODES], cand_q[MAX_NODES], cand_u[MAX_NODES];  // of the children of the present node
+  __shared__ int cand_t[MAX_NODES];
+  __shared__ int gone[MAX_NODES];    // refused tokens, without draft probabilities
+  __shared__ float left[MAX_NODES];  // R at each refusal, with them
+  __shared__ float warp_value[WARPS];
+  __shared__ mass_t warp_mass[WARPS];
+  __shared__ mass_t cta_mass[MAX_CTAS];  // the masses of every CTA's part
+  __shared__ mass_t total;               // R
+  __shared__ int decided, refused, first_top;
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int s = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (ctas > 1) cluster.sync();  // every CTA of the cluster is there before another one writes to it
+  pdl_wait();
+  pdl_launch_dependents();
   const int first = a.node_start[s], n = min(a.node_start[s + 1] - first, a.max_nodes);
   int* path = a.path + (size_t)s * a.max_nodes;
-  for (int i = tid; i < a.max_nodes; i += THREADS) path[i] = -1;
-  if (n <= 0) {
-    if (tid == 0) {
+  if (rank == 0)
+    for (int i = tid; i < a.max_nodes; i += THREADS) path[i] = i == 0 && n > 0 ? 0 : -1;
+  if (n <= 0) {  // (the whole cluster leaves)
+    if (rank == 0 && tid == 0) {
       a.count[s] = 0;
       a.token[s] = -1;
     }
     return;
   }
-  auto sum = [&](mass_t v) -> mass_t {
+  for (int i = tid; i < n; i += THREADS) parents[i] = a.parents[first + i];
+  const float temp = a.temperature[s];
+  const int begin = min(a.V, rank * a.share), end = min(a.V, begin + a.share), mine = end - begin;
+  int turn = 0;
+
+  // the largest of all threads' values in the cluster
+  auto cluster_max = [&](float v) -> float {
+    v = warp_max(v);
+    __syncthreads();
+    if (lane == 0) warp_value[warp] = v;
+    __syncthreads();
+    v = lane < WARPS ? warp_value[lane] : -INFINITY;
+    v = warp_max(v);
+    if (ctas == 1) return v;
+    if (tid < ctas) cluster.map_shared_rank(&box, tid)->value[turn][rank] = v;
+    cluster.sync();
+    v = lane < ctas ? box.value[turn][lane] : -INFINITY;
+    turn ^= 1;
+    return warp_max(v);
+  };
+  // the sum of all threads' masses in the cluster; cta_mass has every CTA's afterwards (behind the next block barrier)
+  auto cluster_sum = [&](mass_t v) -> mass_t {
     v = warp_sum_mass(v);
     __syncthreads();
-    if (lane == 0) m_scratch[warp] = v;
+    if (lane == 0) warp_mass[warp] = v;
     __syncthreads();
-    mass_t total = 0;
-    for (int w = 0; w < THREADS / 32; ++w) total += m_scratch[w];
-    return total;
+    v = warp_sum_mass(lane < WARPS ? warp_mass[lane] : 0);
+    if (ctas > 1) {
+      if (tid < ctas) cluster.map_shared_rank(&box, tid)->mass[turn][rank] = v;
+      cluster.sync();
+      const mass_t each = lane < ctas ? box.mass[turn][lane] : 0;
+      if (tid < ctas) cta_mass[tid] = each;
+      turn ^= 1;
+      return warp_sum_mass(each);
+    }
+    if (tid == 0) cta_mass[0] = v;
+    return v;
   };
-  Row<T> row;
-  row.temp = a.temperature[s];
-  row.left = reinterpret_cast<const float*>(list);
-  row.gone = list;
+
   int cur = 0, count = 1;
-  mass_t R = 0;
-  auto total_of_row = [&]() -> mass_t {
-    mass_t v = 0;
-    for (int i = tid; i < V; i += THREADS) v += row.mass(i);
-    return sum(v);
-  };
-  auto enter = [&](int node) {
-    row.x = (const T*)a.logits + (size_t)(first + node) * a.ld;
-    row.q = a.draft ? a.draft + (size_t)(first + node) * a.ldq : nullptr;
-    row.refused = 0;
+  for (;;) {
+    // ---- the row of node cur
+    const T* row = (const T*)a.logits + (size_t)(first + cur) * a.ld;
+    const float* q = DRAFT ? a.draft + (size_t)(first + cur) * a.ldq : nullptr;
+    __syncthreads();  // parents are there; nobody reads the last row any more
+    for (int i = cur + 1 + tid; i < n; i += THREADS) {
+      if (parents[i] != cur) continue;
+      const int t = a.tokens[first + i];
+      const bool known = t >= 0 && t < a.V;
+      if (!known) atomicOr(a.err, DSP_ERR_BAD_TOKEN);
+      cand_t[i] = known ? t : -1;
+      cand_u[i] = a.uniforms[first + i];
+      cand_x[i] = known ? scale_logit(to_f32(row[t]), temp) : 0.f;
+      cand_q[i] = DRAFT && known ? q[t] : 1.f;
+    }
     float top = -INFINITY;
-    for (int i = tid; i < V; i += THREADS) top = fmaxf(top, row.scaled(i));
-    row.top = block_max(top, f_scratch);
-    row.alone = !(row.temp > 0.f) || row.top == -INFINITY;
-    int low = V;
-    if (row.alone) {
-      for (int i = tid; i < V; i += THREADS)
-        if (row.scaled(i) == row.top) low = min(low, i);
-      if (tid == 0) found = V;
-      __syncthreads();
-      if (low < V) atomicMin(&found, low);
-      __syncthreads();
-      low = found;
-      __syncthreads();
-    }
-    row.first = low;
-    R = total_of_row();
-  };
-  __syncthreads();
-  if (tid == 0) path[0] = 0;
-  enter(0);
-  for (int i = 1; i < n; ++i) {
-    if (a.parents[first + i] != cur) continue;
-    const int t = a.tokens[first + i];
-    if (t < 0 || t >= V) {
-      if (tid == 0) atomicOr(a.err, DSP_ERR_BAD_TOKEN);
-      continue;  // no draft: never taken, nothing to refuse
-    }
-    const float u = a.uniforms[first + i];
-    const float limit = __fmul_rn(row.q ? __fmul_rn(u, row.q[t]) : u, (float)R);
-    if (limit < (float)row.mass(t)) {
-      cur = i;
-      if (tid == 0) path[count] = i;
-      ++count;
-      enter(i);
-      continue;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      if (row.q)
-        reinterpret_cast<float*>(list)[row.refused] = (float)R;
-      else
-        list[row.refused] = t;
-    }
-    __syncthreads();
-    ++row.refused;
-    const mass_t rest = total_of_row();
-    if (rest > 0)
-      R = rest;
-    else
-      --row.refused;
-  }
-  // the draw: thread t owns a run of neighbouring tokens
-  const mass_t aim = max((mass_t)0, min((mass_t)__fmul_rn(a.draws[s], (float)R), R - 1));
-  const int per = (V + THREADS - 1) / THREADS, begin = min(V, tid * per), end = min(V, begin + per);
-  mass_t mine = 0;
-  for (int i = begin; i < end; ++i) mine += row.mass(i);
-  mass_t upto = mine;
+    {
+      constexpr int N = 16 / sizeof(T);
+      const T* src = row + begin;
+      int done = 0;
+      if (((uintptr_t)src & 15) == 0) {  // (a share is a multiple of 16 bytes)
+        const int pieces = mine / N;
+        constexpr int AHEAD = 5;  // requests of a thread under way: a share of 151,936 / 16 logits at once
+        for (int i0 = tid; i0 < pieces; i0 += AHEAD * THREADS) {
+          uint4 v[AHEAD];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const mass_t up = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += up;
-  }
-  __syncthreads();
-  if (lane == 31) m_scratch[warp] = upto;
-  __syncthreads();
-  mass_t before = upto - mine;
-  for (int w = 0; w < warp; ++w) before += m_scratch[w];
-  if (before <= aim && aim < before + mine) {
-    int v = begin;
-    for (; v < end; ++v) {
-      before += row.mass(v);
-      if (before > aim) break;
+          for (int k = 0; k < AHEAD; ++k)
+            if (i0 + k * THREADS < pieces) v[k] = __ldg(reinterpret_cast<const uint4*>(src) + i0 + k * THREADS);
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const int i = i0 + k * THREADS;
+            if (i >= pieces) continue;
+            const T* l = reinterpret_cast<const T*>(&v[k]);
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+              const float x = scale_logit(to_f32(l[c]), temp);
+              xs[i * N + c] = x;
+              top = fmaxf(top, x);
+            }
+          }
+        }
+        done = pieces * N;
+      }
+#pragma unroll 4
+      for (int i = done + tid; i < mine; i += THREADS) {
+        const float x = scale_logit(to_f32(src[i]), temp);
+        xs[i] = x;
+        top = fmaxf(top, x);
+      }
     }
-    a.token[s] = v;
+    top = cluster_max(top);
+    const bool alone = !(temp > 0.f) || top == -INFINITY;  // all the mass on the lowest index of `top`
+    if (alone) {
+      int low = a.V;
+      for (int i = tid; i < mine; i += THREADS)
+        if (xs[i] == top) low = min(low, begin + i);
+      first_top = (int)-cluster_max((float)-low);  // (whole numbers up to 2^24 are exact)
+      __syncthreads();
+      const int at = first_top;
+      for (int i = tid; i < mine; i += THREADS) xs[i] = begin + i == at ? 1.f : 0.f;
+      if (tid < ctas) cta_mass[tid] = at >= tid * a.share && at < (tid + 1) * a.share ? ONE : 0;
+      if (tid == 0) total = ONE;
+    } else {
+      mass_t sum = 0;
+#pragma unroll 4
+      for (int i = tid; i < mine; i += THREADS) {
+        const float e = exponential(xs[i], top);
+        xs[i] = e;
+        sum += mass_of(e);
+      }
+      sum = cluster_sum(sum);
+      if (tid == 0) total = sum;
+    }
+    if (tid == 0) refused = 0;
+    __syncthreads();
+
+    // ---- its children, in the order of their numbers
+    int next = cur + 1;
+    for (;;) {
+      if (warp == 0) {
+        mass_t R = total;
+        int found = 0, nr = refused;
+        for (int i0 = next & ~31; i0 < n && found == 0; i0 += 32) {
+          const int me = i0 + lane;
+          uint32_t todo = __ballot_sync(0xffffffffu, me >= next && me < n && parents[me] == cur);
+          while (todo != 0u && found == 0) {
+            const int i = i0 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int t = cand_t[i];
+            if (t < 0) continue;
+            const float e = alone ? (t == first_top ? 1.f : 0.f) : exponential(cand_x[i], top);
+            mass_t m = mass_of(e);
+            if (DRAFT) {
+              for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(cand_q[i], left[k]));
+              if (__fmul_rn(__fmul_rn(cand_u[i], cand_q[i]), (float)R) < (float)m)
+                found = i;
+              else
+                found = -i;  // refused: the masses have to be summed again
+            } else {
+              bool was = false;  // refused before: no mass
+              for (int k = lane; k < nr; k += 32) was |= gone[k] == t;
+              if (__any_sync(0xffffffffu, was)) m = 0;
+              if (__fmul_rn(cand_u[i], (float)R) < (float)m) {
+                found = i;
+              } else if (m > 0 && R > m) {
+                R -= m;
+                if (lane == 0) {
+                  gone[nr] = t;
+                  cta_mass[t / a.share] -= m;
+                }
+                ++nr;
+                __syncwarp();
+              }
+            }
+          }
+        }
+        if (lane == 0) {
+          decided = found;
+          if (!DRAFT) {
+            total = R;
+            refused = nr;
+          } else if (found < 0) {
+            left[nr] = (float)R;
+          }
+        }
+      }
+      __syncthreads();
+      if (!DRAFT || decided >= 0) break;
+      const int nr = refused + 1;
+      mass_t sum = 0;
+#pragma unroll 4
+      for (int i = tid; i < mine; i += THREADS) {
+        mass_t m = mass_of(xs[i]);
+        const float qv = q[begin + i];
+        for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qv, left[k]));
+        sum += m;
+      }
+      next = -decided + 1;
+      // (where nothing would be left, the masses and every CTA's sum stay)
+      const mass_t kept = tid < ctas ? cta_mass[tid] : 0;
+      const mass_t rest = cluster_sum(sum);
+      if (rest == 0 && tid < ctas) cta_mass[tid] = kept;
+      if (rest > 0 && tid == 0) {
+        total = rest;
+        refused = nr;
+      }
+      __syncthreads();
+    }
+    if (decided <= 0) {
+      // ---- no child was taken: the draw, by the CTA whose part holds the mass it aims at
+      const mass_t R = total, aim = max((mass_t)0, min((mass_t)__fmul_rn(a.draws[s], (float)R), R - 1));
+      mass_t before = 0;
+      for (int r = 0; r < rank; ++r) before += cta_mass[r];
+      if (before <= aim && aim < before + cta_mass[rank]) {
+        const int nr = refused;
+        auto mass_at = [&](int i) -> mass_t {
+          mass_t m = mass_of(xs[i]);
+          if (DRAFT) {
+            const float qv = nr > 0 ? q[begin + i] : 0.f;
+            for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qv, left[k]));
+          } else {
+            for (int k = 0; k < nr; ++k)
+              if (gone[k] == begin + i) m = 0;
+          }
+          return m;
+        };
+        // every warp has a run of neighbouring tokens, 32 at a time
+        const int per = (mine + WARPS * 32 - 1) / (WARPS * 32) * 32, w0 = min(mine, warp * per), w1 = min(mine, w0 + per);
+        mass_t sum = 0;
+#pragma unroll 4
+        for (int i = w0 + lane; i < w1; i += 32) sum += mass_at(i);
+        sum = warp_sum_mass(sum);
+        if (lane == 0) warp_mass[warp] = sum;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) before += warp_mass[w];
+        if (before <= aim && aim < before + sum) {
+          for (int i0 = w0;; i0 += 32) {
+            mass_t upto = i0 + lane < w1 ? mass_at(i0 + lane) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const mass_t up = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += up;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > aim);
+            if (past != 0u) {
+              if (lane == 0) a.token[s] = begin + i0 + __ffs(past) - 1;
+              break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+          }
+        }
+      }
+      if (rank == 0 && tid == 0) a.count[s] = count;
+      break;
+    }
+    cur = decided;
+    if (rank == 0 && tid == 0) path[count] = cur;
+    ++count;
   }
-  if (tid == 0) a.count[s] = count;
+  // (nobody writes to another CTA after the last exchange, whose barrier all of them passed)
+}
+
+template <typename T, bool DRAFT>
+int launch(const Args& a, int S, int ctas, cudaStream_t stream) {
+  auto kernel = tree_verify_kernel<T, DRAFT>;
+  const size_t smem = (size_t)a.share * sizeof(float);
+  prefer_max_shared(reinterpret_cast<const void*>(kernel));
+  DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (ctas > 8) DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(S * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  DSP_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  return 0;
 }
 }  // namespace
 
@@ -204,8 +369,8 @@ struct DspTreeVerify {
 
 extern "C" int dsp_tree_verify(const DspTreeVerify* p, cudaStream_t stream) {
   if (p->S == 0) return 0;
-  DSP_REQUIRE(p->S > 0 && p->V > 0 && p->V <= (1 << 22), "dsp_tree_verify: a vocabulary of %ld (at most 2^22)", p->V);
-  DSP_REQUIRE(p->max_nodes > 0 && p->max_nodes <= 4096, "dsp_tree_verify: max_nodes=%ld", p->max_nodes);
+  DSP_REQUIRE(p->S > 0 && p->V > 0 && p->V <= MAX_VOCAB, "dsp_tree_verify: a vocabulary of %ld (at most 2^19)", p->V);
+  DSP_REQUIRE(p->max_nodes > 0 && p->max_nodes <= MAX_NODES, "dsp_tree_verify: max_nodes=%ld", p->max_nodes);
   DSP_REQUIRE(p->dtype == DSP_F32 || p->dtype == DSP_BF16, "dsp_tree_verify: unknown dtype %ld", p->dtype);
   Args a = {};
   a.logits = p->logits;
@@ -225,11 +390,16 @@ extern "C" int dsp_tree_verify(const DspTreeVerify* p, cudaStream_t stream) {
   a.max_nodes = (int)p->max_nodes;
   a.err = dsp_device_error_ptr();
   DSP_REQUIRE(a.err != nullptr, "dsp_tree_verify: no device error word");
-  const size_t smem = (size_t)p->max_nodes * sizeof(int);
-  if (p->dtype == DSP_F32)
-    DSP_CUDA(launch_plain(tree_verify_kernel<float>, dim3((unsigned)p->S), dim3(THREADS), smem, stream, a));
-  else
-    DSP_CUDA(launch_plain(tree_verify_kernel<bf16>, dim3((unsigned)p->S), dim3(THREADS), smem, stream, a));
+  // CTAs a tree: as many as keep the device's SMs busy with the trees there are, at least 2,048 logits each, and so many
+  // that a share fits
+  const int sms = dsp_num_sms();
+  int ctas = 1;
+  while (ctas < MAX_CTAS && ((p->V + ctas - 1) / ctas > SHARE || (ctas * 2 * 2048 <= p->V && ctas * 2 * p->S <= 2 * sms))) ctas *= 2;
+  a.share = (int)(((p->V + ctas - 1) / ctas + 7) / 8 * 8);
+  const int S = (int)p->S;
+  const int rc = p->dtype == DSP_F32 ? (a.draft ? launch<float, true>(a, S, ctas, stream) : launch<float, false>(a, S, ctas, stream))
+                                     : (a.draft ? launch<bf16, true>(a, S, ctas, stream) : launch<bf16, false>(a, S, ctas, stream));
+  if (rc != 0) return rc;
   DSP_CHECK_LAUNCH("dsp_tree_verify");
   return 0;
 }

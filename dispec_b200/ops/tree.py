@@ -21,6 +21,7 @@ from dispec_b200.ops.attention import _TCGEN05_ERRORS, _device_error_address
 MAX_HEAD_DIM = 256
 TENSOR_CORE_ROWS, FMA_ROWS = 128, 32  # rows of a tile of the two attention kernels
 MAX_POOLS = 8
+MAX_TREE = 1024  # nodes of a tree that is verified
 _ATTENTION = struct.Struct("10q13qd")
 _VERIFY = struct.Struct("11q6q")
 _KEEP = struct.Struct("4q6q40q")
@@ -157,8 +158,8 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     what = "verify_tree"
     if not logits.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")
-    if logits.dim() != 2 or logits.stride(1) != 1 or not 1 <= logits.shape[1] <= 1 << 22:
-        _refuse(what, f"logits must be [T, V] with neighbouring columns and V up to 2^22, not {list(logits.shape)}")
+    if logits.dim() != 2 or logits.stride(1) != 1 or not 1 <= logits.shape[1] <= 1 << 19:
+        _refuse(what, f"logits must be [T, V] with neighbouring columns and V up to 2^19, not {list(logits.shape)}")
     (T, V), S, dev = logits.shape, temperature.shape[0], logits.device
     dtype = L.dtype_code(logits.dtype)
     _ints(what, "tokens", tokens, (T,), dev)
@@ -170,8 +171,8 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.device != dev
                                     or draft_probs.shape != (T, V) or draft_probs.stride(1) != 1):
         _refuse(what, f"draft_probs must be float32 [{T}, {V}] with neighbouring columns on {dev}")
-    if not 1 <= max_nodes <= 4096:
-        _refuse(what, f"max_nodes {max_nodes} outside 1 .. 4096")
+    if not 1 <= max_nodes <= MAX_TREE:
+        _refuse(what, f"max_nodes {max_nodes} outside 1 .. {MAX_TREE}")
     got = torch.empty((S, max_nodes + 2), dtype=torch.int32, device=dev) if S else torch.empty((0, 2), dtype=torch.int32, device=dev)
     flat = got.view(-1)
     count, token, path = flat[:S], flat[S:2 * S], flat[2 * S:].view(S, max_nodes)
