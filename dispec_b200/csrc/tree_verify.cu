@@ -14,19 +14,18 @@
 // or infinite largest logit gives token 0.
 //
 // A cluster of up to 16 CTAs works on one tree and reads only the rows of the nodes that the walk comes to, each of them
-// once: every CTA keeps its share of the row in shared memory, first as scaled logits, then as exponentials, and the CTAs
-// exchange the largest logit and the sums of masses through each other's shared memory (one cluster barrier each).  The
-// tests of a node's children need R and a few numbers that are read while the row arrives; every CTA makes them for itself, with the same result.
-#include <cooperative_groups.h>
-
-#include "common.cuh"
-
-namespace cg = cooperative_groups;
+// once: every CTA keeps its share of the row in shared memory, and the CTAs exchange the largest logit and the sums of
+// masses through each other's shared memory (one cluster barrier each).  The tests of a node's children need R and a few
+// numbers that are read while the row arrives; every CTA makes them for itself, with the same result.
+//
+// What bounds it: for a few trees the latencies of a node in a row (the row's arrival, two exchanges, the pass of
+// exponentials, the tests), for many the instructions of the exponentials' pass.
+#include "tcgen05_common.cuh"  // bounded mbarrier waits, cluster addresses, counted remote stores
 
 namespace {
 constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_CTAS = 16, MAX_NODES = 1024;
 constexpr int SHARE = 24 * 1024;      // logits of a row in a CTA's shared memory, two CTAs an SM
-constexpr int MAX_VOCAB = 1 << 19;    // 32,768 logits in each of 16 CTAs
+constexpr int MAX_VOCAB = 3 << 17;    // 24,576 logits in each of 16 CTAs
 typedef long long mass_t;
 constexpr mass_t ONE = (mass_t)1 << 40;
 
@@ -46,44 +45,91 @@ __device__ __forceinline__ mass_t warp_sum_mass(mass_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float scale_logit(float l, float temp) {
-  return isnan(l) ? -INFINITY : temp > 0.f ? __fdiv_rn(l, temp) : l;
-}
-__device__ __forceinline__ float exponential(float x, float top) { return x == top ? 1.f : expf(x - top); }
 __device__ __forceinline__ mass_t mass_of(float e) { return (mass_t)(e * 1099511627776.f); }
 
-// One exchange: every CTA of the cluster tells every other one a number.
-struct Mailbox {
-  float value[2][MAX_CTAS];
-  mass_t mass[2][MAX_CTAS];
+// exp(l / temp - top) with the correctly rounded quotient; 0 for a logit that is no number.
+//   UNIT     temp is 1
+//   PLAIN    inv = 1 / temp rounded once and two of Markstein's corrections q <- q + inv (l - q temp), which round the quotient
+//            correctly where nothing over- or underflows (temp and the largest logit are far from that).  A quotient of
+//            -inf comes out as no number, whose exponential is 0 as it should be; one so small that a remainder
+//            is not exact changes no exponential.  Five instructions for a division's ten, and no reciprocal.
+//   GENERAL  a division; the largest logit may be infinite
+enum Mode { UNIT, PLAIN, GENERAL };
+struct Scale {
+  float temp, inv, top;
+  Mode mode;
+  template <Mode M>
+  __device__ __forceinline__ float exponential(float l) const {
+    float x = l;
+    if (M == PLAIN) {
+      float q = l * inv;
+      q = fmaf(fmaf(-q, temp, l), inv, q);
+      x = fmaf(fmaf(-q, temp, l), inv, q);
+    }
+    if (M == GENERAL) x = __fdiv_rn(l, temp);
+    const float e = fmaxf(expf(x - top), 0.f);
+    return M == GENERAL && x == top ? 1.f : e;
+  }
+  __device__ __forceinline__ float exponential(float l) const {
+    return mode == UNIT ? exponential<UNIT>(l) : mode == PLAIN ? exponential<PLAIN>(l) : exponential<GENERAL>(l);
+  }
 };
 
+__device__ __forceinline__ void near(const void* p, int bytes) {  // into the L2
+  for (int i = threadIdx.x * 128; i < bytes; i += THREADS * 128)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p) + i));
+}
+
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 tree_verify_kernel(const Args a) {
-  extern __shared__ float xs[];  // [share] this CTA's part of the row
-  __shared__ Mailbox box;
-  __shared__ int parents[MAX_NODES];
-  __shared__ float cand_x[MAX_NODES], cand_q[MAX_NODES], cand_u[MAX_NODES];  // of the children of the present node
-  __shared__ int cand_t[MAX_NODES];
-  __shared__ int gone[MAX_NODES];    // refused tokens, without draft probabilities
-  __shared__ float left[MAX_NODES];  // R at each refusal, with them
+  extern __shared__ __align__(16) float xs[];  // [share] this CTA's part of the row; with draft probabilities [share] of them
+  __shared__ __align__(8) uint64_t bar[2];     // exchange k uses box and barrier k % 2
+  __shared__ __align__(8) float2 box[2][MAX_CTAS];
+  __shared__ int parents[MAX_NODES], tokens[MAX_NODES];
+  __shared__ float uniforms[MAX_NODES];
+  __shared__ float cand_x[MAX_NODES], cand_q[DRAFT ? MAX_NODES : 1];  // logit and draft probability of the present node's children
+  __shared__ int gone[DRAFT ? 1 : MAX_NODES];    // refused tokens, without draft probabilities
+  __shared__ float left[DRAFT ? MAX_NODES : 1];  // R at each refusal, with them
   __shared__ float warp_value[WARPS];
   __shared__ mass_t warp_mass[WARPS];
   __shared__ mass_t cta_mass[MAX_CTAS];  // the masses of every CTA's part
-  __shared__ mass_t total;               // R
-  __shared__ int decided, refused, first_top;
+  __shared__ float sh_top;
+  __shared__ mass_t total;  // R
+  __shared__ int decided, refused, broken;
 
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int s = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (ctas > 1) cluster.sync();  // every CTA of the cluster is there before another one writes to it
+  const int ctas = gridDim.y, rank = blockIdx.y;  // (a cluster is the CTAs of one blockIdx.x)
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* qs = xs + a.share;
+  if (tid == 0) {
+    for (int k = 0; k < 2; ++k) {
+      tc::mbar_init(&bar[k], 1);
+      tc::mbar_expect_tx(&bar[k], (uint32_t)ctas * 8u);
+    }
+    broken = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  // every CTA of the cluster is there, its barriers with it, before another one writes to it (waited for below)
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   pdl_wait();
   pdl_launch_dependents();
   const int first = a.node_start[s], n = min(a.node_start[s + 1] - first, a.max_nodes);
+  const float temp = a.temperature[s];
+  const int begin = min(a.V, rank * a.share), end = min(a.V, begin + a.share), mine = end - begin;
+  const int per = ((mine + THREADS - 1) / THREADS) | 1;  // logits of a thread: neighbours, and odd, so that banks do not meet
+  if (n > 0) near((const T*)a.logits + (size_t)first * a.ld + begin, mine * (int)sizeof(T));
   int* path = a.path + (size_t)s * a.max_nodes;
   if (rank == 0)
     for (int i = tid; i < a.max_nodes; i += THREADS) path[i] = i == 0 && n > 0 ? 0 : -1;
+  for (int i = tid; i < n; i += THREADS) {
+    const int t = a.tokens[first + i];
+    parents[i] = a.parents[first + i];
+    uniforms[i] = a.uniforms[first + i];
+    tokens[i] = t >= 0 && t < a.V ? t : -1;
+    if (i > 0 && (t < 0 || t >= a.V)) atomicOr(a.err, DSP_ERR_BAD_TOKEN);  // (the root is not tried)
+  }
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (n <= 0) {  // (the whole cluster leaves)
     if (rank == 0 && tid == 0) {
       a.count[s] = 0;
@@ -91,65 +137,69 @@ tree_verify_kernel(const Args a) {
     }
     return;
   }
-  for (int i = tid; i < n; i += THREADS) parents[i] = a.parents[first + i];
-  const float temp = a.temperature[s];
-  const int begin = min(a.V, rank * a.share), end = min(a.V, begin + a.share), mine = end - begin;
-  int turn = 0;
 
+  int turn = 0, phases = 0;  // bit k of `phases`: the parity that barrier k is waited for with
+  // By warp 0: sends eight bytes to every CTA of the cluster and returns, in lane r, what CTA r sent.  Nobody writes to a box
+  // that is still being read: a box is used again two exchanges later, which takes a message from here in between.
+  auto exchange = [&](float2 v) -> float2 {
+    if (ctas == 1) return v;
+    if (lane < ctas)
+      tc::st_async_v2(tc::mapa_u32(tc::smem_u32(&box[turn][rank]), (uint32_t)lane), v,
+                      tc::mapa_u32(tc::smem_u32(&bar[turn]), (uint32_t)lane));
+    if (!broken && !__all_sync(0xffffffffu, tc::mbar_wait(&bar[turn], (phases >> turn) & 1))) {
+      if (lane == 0) {
+        broken = 1;  // the numbers are worthless from here on; nothing waits any more
+        atomicOr(a.err, DSP_ERR_WAIT_LIMIT);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) tc::mbar_expect_tx(&bar[turn], (uint32_t)ctas * 8u);
+    const float2 got = box[turn][lane & (MAX_CTAS - 1)];
+    phases ^= 1 << turn;
+    turn ^= 1;
+    __syncwarp();
+    return got;
+  };
   // the largest of all threads' values in the cluster
   auto cluster_max = [&](float v) -> float {
     v = warp_max(v);
-    __syncthreads();
     if (lane == 0) warp_value[warp] = v;
     __syncthreads();
-    v = lane < WARPS ? warp_value[lane] : -INFINITY;
-    v = warp_max(v);
-    if (ctas == 1) return v;
-    if (tid < ctas) cluster.map_shared_rank(&box, tid)->value[turn][rank] = v;
-    cluster.sync();
-    v = lane < ctas ? box.value[turn][lane] : -INFINITY;
-    turn ^= 1;
-    return warp_max(v);
-  };
-  // the sum of all threads' masses in the cluster; cta_mass has every CTA's afterwards (behind the next block barrier)
-  auto cluster_sum = [&](mass_t v) -> mass_t {
-    v = warp_sum_mass(v);
-    __syncthreads();
-    if (lane == 0) warp_mass[warp] = v;
-    __syncthreads();
-    v = warp_sum_mass(lane < WARPS ? warp_mass[lane] : 0);
-    if (ctas > 1) {
-      if (tid < ctas) cluster.map_shared_rank(&box, tid)->mass[turn][rank] = v;
-      cluster.sync();
-      const mass_t each = lane < ctas ? box.mass[turn][lane] : 0;
-      if (tid < ctas) cta_mass[tid] = each;
-      turn ^= 1;
-      return warp_sum_mass(each);
+    if (warp == 0) {
+      v = warp_max(lane < WARPS ? warp_value[lane] : -INFINITY);
+      const float2 got = exchange(make_float2(v, 0.f));
+      v = warp_max(lane < ctas ? got.x : -INFINITY);
+      if (lane == 0) sh_top = v;
     }
-    if (tid == 0) cta_mass[0] = v;
-    return v;
+    __syncthreads();
+    return sh_top;
+  };
+  // By warp 0, behind a block barrier: the sum of the warps' masses in the cluster, and in lane r that of CTA r.
+  auto cluster_sum = [&](mass_t& each) -> mass_t {
+    const mass_t v = warp_sum_mass(lane < WARPS ? warp_mass[lane] : 0);
+    const float2 got = exchange(make_float2(__int_as_float((int)(v & 0xffffffffll)), __int_as_float((int)(v >> 32))));
+    each = lane < ctas ? ((mass_t)__float_as_int(got.y) << 32) | (mass_t)(uint32_t)__float_as_int(got.x) : 0;
+    return warp_sum_mass(each);
   };
 
   int cur = 0, count = 1;
   for (;;) {
     // ---- the row of node cur
     const T* row = (const T*)a.logits + (size_t)(first + cur) * a.ld;
+    const T* src = row + begin;
     const float* q = DRAFT ? a.draft + (size_t)(first + cur) * a.ldq : nullptr;
     __syncthreads();  // parents are there; nobody reads the last row any more
-    for (int i = cur + 1 + tid; i < n; i += THREADS) {
-      if (parents[i] != cur) continue;
-      const int t = a.tokens[first + i];
-      const bool known = t >= 0 && t < a.V;
-      if (!known) atomicOr(a.err, DSP_ERR_BAD_TOKEN);
-      cand_t[i] = known ? t : -1;
-      cand_u[i] = a.uniforms[first + i];
-      cand_x[i] = known ? scale_logit(to_f32(row[t]), temp) : 0.f;
-      cand_q[i] = DRAFT && known ? q[t] : 1.f;
+    // a thread's first child is asked for here and put down behind the requests for the row
+    float my_x = 0.f, my_q = 1.f;
+    const int my_child = cur + 1 + tid;
+    const bool has_child = my_child < n && parents[my_child] == cur && tokens[my_child] >= 0;
+    if (has_child) {
+      my_x = to_f32(row[tokens[my_child]]);
+      if (DRAFT) my_q = q[tokens[my_child]];
     }
     float top = -INFINITY;
     {
       constexpr int N = 16 / sizeof(T);
-      const T* src = row + begin;
       int done = 0;
       if (((uintptr_t)src & 15) == 0) {  // (a share is a multiple of 16 bytes)
         const int pieces = mine / N;
@@ -165,10 +215,10 @@ tree_verify_kernel(const Args a) {
             if (i >= pieces) continue;
             const T* l = reinterpret_cast<const T*>(&v[k]);
 #pragma unroll
-            for (int c = 0; c < N; ++c) {
-              const float x = scale_logit(to_f32(l[c]), temp);
-              xs[i * N + c] = x;
-              top = fmaxf(top, x);
+            for (int c = 0; c < N; c += 4) {
+              const float4 x = make_float4(to_f32(l[c]), to_f32(l[c + 1]), to_f32(l[c + 2]), to_f32(l[c + 3]));
+              *reinterpret_cast<float4*>(xs + i * N + c) = x;
+              top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));  // (no number is smaller than any)
             }
           }
         }
@@ -176,56 +226,105 @@ tree_verify_kernel(const Args a) {
       }
 #pragma unroll 4
       for (int i = done + tid; i < mine; i += THREADS) {
-        const float x = scale_logit(to_f32(src[i]), temp);
+        const float x = to_f32(src[i]);
         xs[i] = x;
         top = fmaxf(top, x);
       }
     }
+    if (has_child) {
+      cand_x[my_child] = my_x;
+      if (DRAFT) cand_q[my_child] = my_q;
+    }
+    for (int i = my_child + THREADS; i < n; i += THREADS)
+      if (parents[i] == cur && tokens[i] >= 0) {
+        cand_x[i] = to_f32(row[tokens[i]]);
+        if (DRAFT) cand_q[i] = q[tokens[i]];
+      }
+    // the node's first child: its row is likely to be read next and comes nearer meanwhile.  A node with children
+    // will mostly see one refused, and needs its draft probabilities then.
+    int child = 0;
+    for (int i0 = cur + 1; i0 < n && child == 0; i0 += 32) {
+      const uint32_t is = __ballot_sync(0xffffffffu, i0 + lane < n && parents[min(i0 + lane, n - 1)] == cur);
+      if (is != 0u) child = i0 + __ffs(is) - 1;
+    }
+    if (child != 0) {
+      near((const T*)a.logits + (size_t)(first + child) * a.ld + begin, mine * (int)sizeof(T));
+      if (DRAFT)
+        for (int i = tid; i < mine; i += THREADS)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(qs + i)), "l"(q + begin + i) : "memory");
+    }
     top = cluster_max(top);
     const bool alone = !(temp > 0.f) || top == -INFINITY;  // all the mass on the lowest index of `top`
+    int first_top = -1;
+    Scale scale = {};
+    mass_t my_mass = 0;  // of the thread's own logits, per * tid .. per * (tid + 1) - 1
+    const int t0 = min(mine, per * tid), t1 = min(mine, t0 + per);
     if (alone) {
       int low = a.V;
-      for (int i = tid; i < mine; i += THREADS)
-        if (xs[i] == top) low = min(low, begin + i);
+      for (int i = tid; i < mine; i += THREADS) {
+        const float x = xs[i];
+        if (x == top || (top == -INFINITY && isnan(x))) low = min(low, begin + i);  // (no number counts as -inf)
+      }
       first_top = (int)-cluster_max((float)-low);  // (whole numbers up to 2^24 are exact)
-      __syncthreads();
-      const int at = first_top;
-      for (int i = tid; i < mine; i += THREADS) xs[i] = begin + i == at ? 1.f : 0.f;
-      if (tid < ctas) cta_mass[tid] = at >= tid * a.share && at < (tid + 1) * a.share ? ONE : 0;
+      const int at = first_top - begin;
+      if (at >= t0 && at < t1) my_mass = ONE;
+      if (DRAFT)
+        for (int i = tid; i < mine; i += THREADS) xs[i] = i == at ? 1.f : 0.f;
+      if (tid < ctas) cta_mass[tid] = first_top >= tid * a.share && first_top < (tid + 1) * a.share ? ONE : 0;
       if (tid == 0) total = ONE;
     } else {
-      mass_t sum = 0;
+      scale.temp = temp;
+      scale.inv = __frcp_rn(temp);
+      scale.top = __fdiv_rn(top, temp);  // (a quotient grows with its numerator, so this is the largest of them)
+      scale.mode = !(fabsf(top) < 1.1e18f && temp > 9.3e-10f && temp < 1.1e9f) ? GENERAL : temp == 1.f ? UNIT : PLAIN;
+      auto pass = [&](auto exponential) {
 #pragma unroll 4
-      for (int i = tid; i < mine; i += THREADS) {
-        const float e = exponential(xs[i], top);
-        xs[i] = e;
-        sum += mass_of(e);
+        for (int i = t0; i < t1; ++i) {
+          const float e = exponential(xs[i]);
+          if (DRAFT) xs[i] = e;  // refusals come back to them
+          my_mass += mass_of(e);
+        }
+      };
+      if (scale.mode == UNIT)
+        pass([&](float l) { return scale.exponential<UNIT>(l); });
+      else if (scale.mode == PLAIN)
+        pass([&](float l) { return scale.exponential<PLAIN>(l); });
+      else
+        pass([&](float l) { return scale.exponential<GENERAL>(l); });
+      const mass_t sum = warp_sum_mass(my_mass);
+      if (lane == 0) warp_mass[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
+        mass_t each;
+        const mass_t all = cluster_sum(each);
+        if (lane < ctas) cta_mass[lane] = each;
+        if (lane == 0) total = all;
+        __syncwarp();
       }
-      sum = cluster_sum(sum);
-      if (tid == 0) total = sum;
     }
     if (tid == 0) refused = 0;
-    __syncthreads();
+    if (DRAFT) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (alone) __syncthreads();  // (else all that follows is warp 0's until the next barrier)
 
     // ---- its children, in the order of their numbers
     int next = cur + 1;
     for (;;) {
       if (warp == 0) {
         mass_t R = total;
-        int found = 0, nr = refused;
+        int found = 0, nr = next == cur + 1 ? 0 : refused;
         for (int i0 = next & ~31; i0 < n && found == 0; i0 += 32) {
           const int me = i0 + lane;
           uint32_t todo = __ballot_sync(0xffffffffu, me >= next && me < n && parents[me] == cur);
           while (todo != 0u && found == 0) {
             const int i = i0 + __ffs(todo) - 1;
             todo &= todo - 1;
-            const int t = cand_t[i];
+            const int t = tokens[i];
             if (t < 0) continue;
-            const float e = alone ? (t == first_top ? 1.f : 0.f) : exponential(cand_x[i], top);
+            const float u = uniforms[i], e = alone ? (t == first_top ? 1.f : 0.f) : scale.exponential(cand_x[i]);
             mass_t m = mass_of(e);
             if (DRAFT) {
               for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(cand_q[i], left[k]));
-              if (__fmul_rn(__fmul_rn(cand_u[i], cand_q[i]), (float)R) < (float)m)
+              if (__fmul_rn(__fmul_rn(u, cand_q[i]), (float)R) < (float)m)
                 found = i;
               else
                 found = -i;  // refused: the masses have to be summed again
@@ -233,7 +332,7 @@ tree_verify_kernel(const Args a) {
               bool was = false;  // refused before: no mass
               for (int k = lane; k < nr; k += 32) was |= gone[k] == t;
               if (__any_sync(0xffffffffu, was)) m = 0;
-              if (__fmul_rn(cand_u[i], (float)R) < (float)m) {
+              if (__fmul_rn(u, (float)R) < (float)m) {
                 found = i;
               } else if (m > 0 && R > m) {
                 R -= m;
@@ -249,105 +348,122 @@ tree_verify_kernel(const Args a) {
         }
         if (lane == 0) {
           decided = found;
-          if (!DRAFT) {
+          refused = nr;
+          if (!DRAFT)
             total = R;
-            refused = nr;
-          } else if (found < 0) {
+          else if (found < 0)
             left[nr] = (float)R;
-          }
         }
       }
       __syncthreads();
-      if (!DRAFT || decided >= 0) break;
+      const int decision = decided;
+      if (!DRAFT || decision >= 0 || broken) break;
       const int nr = refused + 1;
       mass_t sum = 0;
 #pragma unroll 4
-      for (int i = tid; i < mine; i += THREADS) {
+      for (int i = t0; i < t1; ++i) {
         mass_t m = mass_of(xs[i]);
-        const float qv = q[begin + i];
+        const float qv = qs[i];
         for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qv, left[k]));
         sum += m;
       }
-      next = -decided + 1;
-      // (where nothing would be left, the masses and every CTA's sum stay)
-      const mass_t kept = tid < ctas ? cta_mass[tid] : 0;
-      const mass_t rest = cluster_sum(sum);
-      if (rest == 0 && tid < ctas) cta_mass[tid] = kept;
-      if (rest > 0 && tid == 0) {
-        total = rest;
-        refused = nr;
-      }
-      __syncthreads();
-    }
-    if (decided <= 0) {
-      // ---- no child was taken: the draw, by the CTA whose part holds the mass it aims at
-      const mass_t R = total, aim = max((mass_t)0, min((mass_t)__fmul_rn(a.draws[s], (float)R), R - 1));
-      mass_t before = 0;
-      for (int r = 0; r < rank; ++r) before += cta_mass[r];
-      if (before <= aim && aim < before + cta_mass[rank]) {
-        const int nr = refused;
-        auto mass_at = [&](int i) -> mass_t {
-          mass_t m = mass_of(xs[i]);
-          if (DRAFT) {
-            const float qv = nr > 0 ? q[begin + i] : 0.f;
-            for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qv, left[k]));
-          } else {
-            for (int k = 0; k < nr; ++k)
-              if (gone[k] == begin + i) m = 0;
-          }
-          return m;
-        };
-        // every warp has a run of neighbouring tokens, 32 at a time
-        const int per = (mine + WARPS * 32 - 1) / (WARPS * 32) * 32, w0 = min(mine, warp * per), w1 = min(mine, w0 + per);
-        mass_t sum = 0;
-#pragma unroll 4
-        for (int i = w0 + lane; i < w1; i += 32) sum += mass_at(i);
-        sum = warp_sum_mass(sum);
-        if (lane == 0) warp_mass[warp] = sum;
+      next = -decision + 1;
+      {
+        const mass_t of_warp = warp_sum_mass(sum);
+        if (lane == 0) warp_mass[warp] = of_warp;
         __syncthreads();
-        for (int w = 0; w < warp; ++w) before += warp_mass[w];
-        if (before <= aim && aim < before + sum) {
-          for (int i0 = w0;; i0 += 32) {
-            mass_t upto = i0 + lane < w1 ? mass_at(i0 + lane) : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const mass_t up = __shfl_up_sync(0xffffffffu, upto, o);
-              if (lane >= o) upto += up;
+        if (warp == 0) {
+          mass_t each;
+          const mass_t rest = cluster_sum(each);
+          if (rest > 0) {  // (where nothing would be left, the masses stay)
+            if (lane < ctas) cta_mass[lane] = each;
+            if (lane == 0) {
+              total = rest;
+              refused = nr;
             }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > aim);
-            if (past != 0u) {
-              if (lane == 0) a.token[s] = begin + i0 + __ffs(past) - 1;
-              break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
           }
+          __syncwarp();
         }
+        __syncthreads();
+        if (refused == nr) my_mass = sum;
       }
-      if (rank == 0 && tid == 0) a.count[s] = count;
-      break;
     }
-    cur = decided;
-    if (rank == 0 && tid == 0) path[count] = cur;
-    ++count;
+    const int decision = decided;
+    if (decision > 0 && !broken) {
+      cur = decision;
+      if (rank == 0 && tid == 0) path[count] = cur;
+      ++count;
+      continue;
+    }
+    // ---- no child was taken: the draw, by the CTA whose part holds the mass it aims at
+    if (rank == 0 && tid == 0) a.count[s] = count;
+    const mass_t R = total, aim = max((mass_t)0, min((mass_t)__fmul_rn(a.draws[s], (float)R), R - 1));
+    mass_t before = 0;
+    for (int r = 0; r < rank; ++r) before += cta_mass[r];
+    if (aim < before || aim >= before + cta_mass[rank]) break;
+    const int nr = refused;
+    auto mass_at = [&](int i) -> mass_t {
+      mass_t m = mass_of(DRAFT ? xs[i] : alone ? (begin + i == first_top ? 1.f : 0.f) : scale.exponential(xs[i]));
+      if (DRAFT) {
+        for (int k = 0; k < nr; ++k) m = max((mass_t)0, m - (mass_t)__fmul_rn(qs[i], left[k]));
+      } else {
+        for (int k = 0; k < nr; ++k)
+          if (gone[k] == begin + i) m = 0;
+      }
+      return m;
+    };
+    if (!DRAFT)
+      for (int k = 0; k < nr; ++k) {
+        const int i = gone[k] - begin;
+        if (i >= t0 && i < t1) my_mass -= mass_of(alone ? (gone[k] == first_top ? 1.f : 0.f) : scale.exponential(xs[i]));
+      }
+    auto scan = [&](mass_t v) -> mass_t {  // inclusive, over a warp
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const mass_t up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+      }
+      return v;
+    };
+    const mass_t upto = scan(my_mass);
+    __syncthreads();
+    if (lane == 31) warp_mass[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before += warp_mass[w];
+    const mass_t mine_from = before + upto - my_mass;
+    const uint32_t holds = __ballot_sync(0xffffffffu, mine_from <= aim && aim < mine_from + my_mass);
+    if (holds != 0u) {  // one thread of the CTA: its warp looks at its logits, 32 at a time
+      const int who = __ffs(holds) - 1, i_end = __shfl_sync(0xffffffffu, t1, who);
+      mass_t from = __shfl_sync(0xffffffffu, mine_from, who);
+      for (int i0 = __shfl_sync(0xffffffffu, t0, who); i0 < i_end; i0 += 32) {
+        const mass_t sums = scan(i0 + lane < i_end ? mass_at(i0 + lane) : 0);
+        const uint32_t past = __ballot_sync(0xffffffffu, from + sums > aim);
+        if (past != 0u) {
+          if (lane == 0) a.token[s] = begin + i0 + __ffs(past) - 1;
+          break;
+        }
+        from += __shfl_sync(0xffffffffu, sums, 31);
+      }
+    }
+    break;
   }
-  // (nobody writes to another CTA after the last exchange, whose barrier all of them passed)
 }
 
 template <typename T, bool DRAFT>
 int launch(const Args& a, int S, int ctas, cudaStream_t stream) {
   auto kernel = tree_verify_kernel<T, DRAFT>;
-  const size_t smem = (size_t)a.share * sizeof(float);
+  const size_t smem = (size_t)a.share * sizeof(float) * (DRAFT ? 2 : 1);
   prefer_max_shared(reinterpret_cast<const void*>(kernel));
   DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (ctas > 8) DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(S * ctas));
+  cfg.gridDim = dim3((unsigned)S, (unsigned)ctas);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  attr[0].val.clusterDim = {1, (unsigned)ctas, 1};
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
@@ -369,7 +485,7 @@ struct DspTreeVerify {
 
 extern "C" int dsp_tree_verify(const DspTreeVerify* p, cudaStream_t stream) {
   if (p->S == 0) return 0;
-  DSP_REQUIRE(p->S > 0 && p->V > 0 && p->V <= MAX_VOCAB, "dsp_tree_verify: a vocabulary of %ld (at most 2^19)", p->V);
+  DSP_REQUIRE(p->S > 0 && p->V > 0 && p->V <= MAX_VOCAB, "dsp_tree_verify: a vocabulary of %ld (at most 393,216)", p->V);
   DSP_REQUIRE(p->max_nodes > 0 && p->max_nodes <= MAX_NODES, "dsp_tree_verify: max_nodes=%ld", p->max_nodes);
   DSP_REQUIRE(p->dtype == DSP_F32 || p->dtype == DSP_BF16, "dsp_tree_verify: unknown dtype %ld", p->dtype);
   Args a = {};
@@ -391,10 +507,10 @@ extern "C" int dsp_tree_verify(const DspTreeVerify* p, cudaStream_t stream) {
   a.err = dsp_device_error_ptr();
   DSP_REQUIRE(a.err != nullptr, "dsp_tree_verify: no device error word");
   // CTAs a tree: as many as keep the device's SMs busy with the trees there are, at least 2,048 logits each, and so many
-  // that a share fits
-  const int sms = dsp_num_sms();
+  // that two CTAs' shares fit an SM
+  const int sms = dsp_num_sms(), fits = a.draft ? SHARE / 2 : SHARE;
   int ctas = 1;
-  while (ctas < MAX_CTAS && ((p->V + ctas - 1) / ctas > SHARE || (ctas * 2 * 2048 <= p->V && ctas * 2 * p->S <= 2 * sms))) ctas *= 2;
+  while (ctas < MAX_CTAS && ((p->V + ctas - 1) / ctas > fits || (ctas * 2 * 2048 <= p->V && ctas * 2 * p->S <= 2 * sms))) ctas *= 2;
   a.share = (int)(((p->V + ctas - 1) / ctas + 7) / 8 * 8);
   const int S = (int)p->S;
   const int rc = p->dtype == DSP_F32 ? (a.draft ? launch<float, true>(a, S, ctas, stream) : launch<float, false>(a, S, ctas, stream))

@@ -21,6 +21,7 @@ from dispec_b200.ops.attention import _TCGEN05_ERRORS, _device_error_address
 MAX_HEAD_DIM = 256
 TENSOR_CORE_ROWS, FMA_ROWS = 128, 32  # rows of a tile of the two attention kernels
 MAX_POOLS = 8
+MAX_VOCAB = 3 << 17  # of a verified tree: a row is shared by at most 16 CTAs
 MAX_TREE = 1024  # nodes of a tree that is verified
 _ATTENTION = struct.Struct("10q13qd")
 _VERIFY = struct.Struct("11q6q")
@@ -158,8 +159,8 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     what = "verify_tree"
     if not logits.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")
-    if logits.dim() != 2 or logits.stride(1) != 1 or not 1 <= logits.shape[1] <= 1 << 19:
-        _refuse(what, f"logits must be [T, V] with neighbouring columns and V up to 2^19, not {list(logits.shape)}")
+    if logits.dim() != 2 or logits.stride(1) != 1 or not 1 <= logits.shape[1] <= MAX_VOCAB:
+        _refuse(what, f"logits must be [T, V] with neighbouring columns and V up to {MAX_VOCAB}, not {list(logits.shape)}")
     (T, V), S, dev = logits.shape, temperature.shape[0], logits.device
     dtype = L.dtype_code(logits.dtype)
     _ints(what, "tokens", tokens, (T,), dev)
