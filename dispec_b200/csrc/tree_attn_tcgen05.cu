@@ -642,8 +642,13 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
     runs_k = map_k;
     runs_v = map_v;
   }
-  if (cudaFuncSetAttribute(tree_attn_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
-    return 4;
+  static bool allowed[MAX_DEVICES] = {};  // asked for once a device
+  const int device = current_device();
+  if (device < 0 || !allowed[device]) {
+    if (cudaFuncSetAttribute(tree_attn_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+      return 4;
+    if (device >= 0) allowed[device] = true;
+  }
   if (launch_pdl(tree_attn_tcgen05_kernel, dim3((unsigned)a->ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, p, map_k, map_v,
                  runs_k, runs_v) != cudaSuccess)
     return 1;

@@ -453,9 +453,15 @@ template <typename T, bool DRAFT>
 int launch(const Args& a, int S, int ctas, cudaStream_t stream) {
   auto kernel = tree_verify_kernel<T, DRAFT>;
   const size_t smem = (size_t)a.share * sizeof(float) * (DRAFT ? 2 : 1);
-  prefer_max_shared(reinterpret_cast<const void*>(kernel));
-  DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  if (ctas > 8) DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  static bool allowed[MAX_DEVICES] = {};  // asked for once a device: the largest share, clusters of 16
+  const int device = current_device();
+  if (device < 0 || !allowed[device]) {
+    prefer_max_shared(reinterpret_cast<const void*>(kernel));
+    DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  MAX_VOCAB / MAX_CTAS * (int)sizeof(float) * (DRAFT ? 2 : 1)));
+    DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (device >= 0) allowed[device] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)S, (unsigned)ctas);
   cfg.blockDim = dim3(THREADS);
