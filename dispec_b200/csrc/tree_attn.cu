@@ -60,19 +60,19 @@ tree_attn_kernel(const Args a) {
   const Shape& sh = a.sh;
   Walk w;
   if (!w.begin(sh, cta, gridDim.x)) return;
-  const int G = sh.G, H = G * sh.KVH;
+  const int G = sh.G;
   do {
-    const Tree& t = w.t;
-    const int row0 = w.row_tile * ROWS, rows = min(ROWS, t.n * G - row0);
+    const Share& t = w.at;
+    const int row0 = t.row_tile * ROWS, rows = min(ROWS, t.n * G - row0);
     const int total = t.ctx + t.n;
-    const int* table = a.page_table + (size_t)w.at.seq * a.pt_stride;
+    const int* table = a.page_table + (size_t)t.seq * a.pt_stride;
     __syncthreads();
     for (int i = tid; i < ROWS * (D / 4); i += THREADS) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows) {
         const int rr = row0 + r;
-        v = load4((const T*)a.q + (size_t)(t.first + rr / G) * a.q_stride + (size_t)(w.head * G + rr % G) * D + d);
+        v = load4((const T*)a.q + (size_t)(t.first + rr / G) * a.q_stride + (size_t)(t.head * G + rr % G) * D + d);
       }
       *reinterpret_cast<float4*>(qs + r * LD + d) = v;
     }
@@ -88,7 +88,7 @@ tree_attn_kernel(const Args a) {
 #pragma unroll
       for (int d = 0; d < 4 * DJ; ++d) acc[i][d] = 0.f;
     }
-    for (int kt = w.kt_begin; kt < w.kt_end; ++kt) {
+    for (int kt = t.kt_begin; kt < t.kt_end; ++kt) {
       const int key0 = kt * KEYS;
       __syncthreads();
       if (tid < KEYS) {
@@ -98,7 +98,7 @@ tree_attn_kernel(const Args a) {
         if (wanted) {
           const int page = key / a.page_size < a.pt_stride ? table[key / a.page_size] : -1;
           if (page >= 0 && page < a.num_pages)
-            at = ((long)page * sh.KVH + w.head) * a.page_size + key % a.page_size;
+            at = ((long)page * sh.KVH + t.head) * a.page_size + key % a.page_size;
           else
             atomicOr(a.err, DSP_ERR_BAD_PAGE);
         }
@@ -196,75 +196,99 @@ tree_attn_kernel(const Args a) {
       const int r = ty + i * 16;
       if (r >= rows) continue;
       const int rr = row0 + r;
-      const float inv = w.slot >= 0 ? 1.f : l[i] > 0.f ? 1.f / l[i] : 0.f;
+      const float inv = t.slot >= 0 ? 1.f : l[i] > 0.f ? 1.f / l[i] : 0.f;
 #pragma unroll
       for (int c = 0; c < DJ; ++c) {
         const int d = c * 64 + tx * 4;
         if (d >= D) continue;
         const float4 v = make_float4(acc[i][4 * c] * inv, acc[i][4 * c + 1] * inv, acc[i][4 * c + 2] * inv,
                                      acc[i][4 * c + 3] * inv);
-        if (w.slot >= 0)
-          store4(a.part_o + ((size_t)w.slot * ROWS + r) * D + d, v);
+        if (t.slot >= 0)
+          store4(a.part_o + ((size_t)t.slot * ROWS + r) * D + d, v);
         else
-          store4((T*)a.out + (size_t)(t.first + rr / G) * a.out_stride + (size_t)(w.head * G + rr % G) * D + d, v);
+          store4((T*)a.out + (size_t)(t.first + rr / G) * a.out_stride + (size_t)(t.head * G + rr % G) * D + d, v);
       }
-      if (w.slot >= 0 && tx == 0)
-        reinterpret_cast<float2*>(a.part_ml)[(size_t)w.slot * ROWS + r] = make_float2(m[i] * 1.4426950408889634f, l[i]);
+      if (t.slot >= 0 && tx == 0)
+        reinterpret_cast<float2*>(a.part_ml)[(size_t)t.slot * ROWS + r] = make_float2(m[i] * 1.4426950408889634f, l[i]);
     }
-    (void)H;
   } while (w.next(sh, cta));
 }
 
-// Block (c, y): the item that begins in CTA c and ends in a later one, if there is one; its rows y, y + gridDim.y, ..., one
-// a warp.
+// Block (c, y): the item that begins in CTA c and ends in a later one, if there is one; four of its rows, one a warp.  Which
+// item that is does not depend on the kernel in front, so it is found out before the wait.  A lane holds the weights
+// of up to 32 partial results, and the outputs of eight are asked for together.
 template <typename T>
 __global__ void __launch_bounds__(128)
 tree_combine_kernel(const Shape sh, const float* __restrict__ part_o, const float* __restrict__ part_ml,
                     T* __restrict__ out, long out_stride, int D, int ctas) {
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
+  // last unit of CTA c
+  const Found f = find_unit(sh, ctas, [&](const Found& g) {
+    const long last = min((long)g.total, (long)g.chunk * (c + 1)) - 1;
+    return last + 1 >= g.total ? g.total : (int)last;  // (nothing follows the last CTA with work)
+  });
+  bool mine = f.seq >= 0;
+  int c_end = 0, head = 0, row0 = 0, rows = 0;
+  Tree t = {};
+  if (mine) {
+    t = load_tree(sh, f.seq);
+    const int last = f.chunk * (c + 1) - 1;
+    head = (last - f.start) / t.key_tiles;
+    const int begin = f.start + head * t.key_tiles, end = begin + t.key_tiles;
+    mine = end != last + 1 && begin >= f.chunk * c;  // it goes on, and began here
+    c_end = (end - 1) / f.chunk;
+    row0 = f.row_tile * sh.rows_per_tile;
+    rows = min(sh.rows_per_tile, t.n * sh.G - row0);
+  }
+  const int r = blockIdx.y * 4 + warp;
   pdl_wait();
-  long total;
-  const long chunk = units_per_cta(sh, ctas, &total);
-  const long last = min(total, chunk * (c + 1)) - 1;  // last unit of CTA c
-  if (last + 1 >= total || last < chunk * c) return;
-  const Place p = find_unit(sh, last);
-  const Tree t = load_tree(sh, p.seq);
-  const long item_end = p.item_start + t.key_tiles;
-  if (item_end == last + 1 || p.item_start < chunk * c) return;  // it ends here, or began before
-  const int c_end = (int)((item_end - 1) / chunk);
-  const int head = p.item / t.row_tiles, row0 = (p.item - head * t.row_tiles) * sh.rows_per_tile;
-  const int rows = min(sh.rows_per_tile, t.n * sh.G - row0);
+  if (!mine || r >= rows) return;
   const float2* ml = reinterpret_cast<const float2*>(part_ml);
-  auto slot = [&](int k) -> size_t { return k == c ? 2 * (size_t)c + 1 : 2 * (size_t)k; };
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += 4 * gridDim.y) {
-    float M = -INFINITY;
-    for (int k = c + lane; k <= c_end; k += 32) M = fmaxf(M, ml[slot(k) * sh.rows_per_tile + r].x);
-    M = warp_max(M);
-    float L = 0.f;
-    for (int k = c + lane; k <= c_end; k += 32) {
-      const float2 v = ml[slot(k) * sh.rows_per_tile + r];
-      if (v.x != -INFINITY) L += v.y * exp2f(v.x - M);
-    }
-    L = warp_sum(L);
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    const int rr = row0 + r;
-    T* dst = out + (size_t)(t.first + rr / sh.G) * out_stride + (size_t)(head * sh.G + rr % sh.G) * D;
-    for (int d = lane * 4; d < D; d += 128) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = c; k <= c_end; ++k) {
-        const size_t row = slot(k) * sh.rows_per_tile + r;
-        const float mk = ml[row].x;
-        if (mk == -INFINITY) continue;
-        const float wk = exp2f(mk - M);
-        const float4 v = load4(part_o + row * D + d);
-        acc.x = fmaf(wk, v.x, acc.x);
-        acc.y = fmaf(wk, v.y, acc.y);
-        acc.z = fmaf(wk, v.z, acc.z);
-        acc.w = fmaf(wk, v.w, acc.w);
+  const int R = sh.rows_per_tile, parts = c_end - c + 1;
+  auto slot = [&](int k) -> size_t { return k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k); };  // of the k-th part
+  float M = -INFINITY, L = 0.f;
+  float2 mine_ml = make_float2(-INFINITY, 0.f);
+  for (int k = lane; k < parts; k += 32) {
+    const float2 v = ml[slot(k) * R + r];
+    if (k < 32) mine_ml = v;
+    M = fmaxf(M, v.x);
+  }
+  M = warp_max(M);
+  for (int k = lane; k < parts; k += 32) {
+    const float2 v = k < 32 ? mine_ml : ml[slot(k) * R + r];
+    if (v.x != -INFINITY) L += v.y * exp2f(v.x - M);
+  }
+  L = warp_sum(L);
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int rr = row0 + r;
+  T* dst = out + (size_t)(t.first + rr / sh.G) * out_stride + (size_t)(head * sh.G + rr % sh.G) * D;
+  for (int d0 = 0; d0 < D; d0 += 128) {  // the same trips for a whole warp (shuffles)
+    const int d = d0 + lane * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < parts; k0 += 8) {
+      float4 v[8];
+      float wk[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int part = k0 + k;
+        float m = -INFINITY;
+        if (part < 32)
+          m = __shfl_sync(0xffffffffu, mine_ml.x, part);
+        else if (part < parts)
+          m = ml[slot(part) * R + r].x;
+        wk[k] = part < parts && m != -INFINITY ? exp2f(m - M) : 0.f;
+        v[k] = wk[k] != 0.f && d < D ? load4(part_o + (slot(part) * R + r) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        acc.x = fmaf(wk[k], v[k].x, acc.x);
+        acc.y = fmaf(wk[k], v[k].y, acc.y);
+        acc.z = fmaf(wk[k], v[k].z, acc.z);
+        acc.w = fmaf(wk[k], v[k].w, acc.w);
+      }
     }
+    if (d < D) store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
 
@@ -282,7 +306,7 @@ int launch(const Args& a, int ctas, cudaStream_t stream) {
 
 cudaError_t tree_combine(const tree::Shape& sh, const float* part_o, const float* part_ml, void* out, long out_stride,
                          int D, int ctas, int dtype, cudaStream_t stream) {
-  const dim3 grid(ctas, (sh.rows_per_tile + 15) / 16);
+  const dim3 grid(ctas, (sh.rows_per_tile + 3) / 4);
   return dtype == DSP_F32
              ? launch_pdl(tree_combine_kernel<float>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (float*)out, out_stride, D, ctas)
              : launch_pdl(tree_combine_kernel<bf16>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (bf16*)out, out_stride, D, ctas);

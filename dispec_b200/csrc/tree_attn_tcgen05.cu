@@ -10,8 +10,9 @@
 //   warp 10     issues the output products;
 //   warps 2..9  two softmax groups of four warps: group g owns the key tiles g, g + 2, ... of a share with a score buffer,
 //               output accumulator, P, running maximum and sum of its own; thread r of a group owns row r.
-// At the end of a share group 0 merges the two halves and stores the rows (or leaves a partial result) while group 1
-// brings the next share's queries.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
+// The whole block meets once a share.  Behind that barrier group 0 merges the two halves and stores the rows (or leaves a
+// partial result) while group 1 brings the next share's queries; warp 0 has worked the next share out and asked for its
+// first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
 // its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output
 // product.  Every wait is bounded; one that runs out sets the device error word.
 #include "tcgen05_common.cuh"
@@ -30,7 +31,12 @@ using namespace tree;
 constexpr int D = DSP_HEAD_DIM;
 static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
 constexpr int BM = 128, BN = 64, THREADS = 384;
-constexpr int K_STAGES = 5, V_STAGES = 7;
+// Key tiles of a share go to two issuing warps in turn, and each waits for its own tiles only.  With an even ring a slot's
+// tiles all belong to one of them; with an odd one a warp that is ahead (its tile landed, an older one of the
+// other's has not) could take the slot's last phase but one for the phase it waits for.
+constexpr int K_STAGES = 6, V_STAGES = 6;
+static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing warp");
+constexpr int SHARES = 4;      // the shares remembered: the next one, the present one and the one whose rows are being stored
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 constexpr int PV_WARP = 10, S1_WARP = 11;
@@ -63,7 +69,7 @@ struct Params {
 };
 
 // Which keys key0 .. key0 + 63 the row of a node sees: stored ones, and nodes of the tree by the row's words.
-__device__ __forceinline__ unsigned long long seen_keys(const Params& p, const Tree& t, int row, int depth, int key0) {
+__device__ __forceinline__ unsigned long long seen_keys(const Params& p, const Share& t, int row, int depth, int key0) {
   unsigned long long stored = 0ull, drafted = 0ull;
   const int off = key0 - t.ctx;  // number of the first key as a node
   if (off < 0) {
@@ -94,6 +100,18 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const T
   return stored | drafted;
 }
 
+// Multiplies a row's accumulators by alpha.
+__device__ __forceinline__ void rescale(uint32_t o_addr, float alpha) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    uint32_t ov[32];
+    tmem_ld32(o_addr + (uint32_t)c0, ov);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+    tmem_st32(o_addr + (uint32_t)c0, ov);
+  }
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap runs_k,
@@ -108,20 +126,33 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ __align__(8) uint64_t q_ready[2];            // the queries of a share with tiles for the group are in tensor memory
   __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
   __shared__ float merge_m[2][BM], merge_l[2][BM];        // group 1's maximum and sum per row, by share in turn
+  __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 before the barrier in front of it
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed, failed_share;  // a wait ran out; the first share in which one of a softmax warp did
+  __shared__ int failed;        // a wait ran out
+  __shared__ int failed_share;  // the first share in which one did: the block leaves together behind that share's barrier
   __shared__ uint32_t bad_pages[BAD_SLOTS];  // of key tile n, in slot n % BAD_SLOTS; bit j: page j had no valid id (not loaded)
 
-  pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const Shape& sh = p.sh;
-  Walk w;
-  if (!w.begin(sh, cta, gridDim.x)) return;
   const int G = sh.G;
   unsigned char* k_s = smem;  // [stage][slice][64 keys][128 bytes]
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
-  if (tid == 0) {
+  pdl_wait();
+  Walk w;  // warp 0's
+  bool more = false;
+  if (warp == 0) {
+    more = w.begin(sh, cta, gridDim.x);
+    if (lane == 0) {
+      if (!more) w.at.seq = -1;
+      shares[0] = w.at;
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid == 64) {
     for (int s = 0; s < K_STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -143,234 +174,307 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     failed_share = 0x7fffffff;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                 "r"(TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  auto give_up = [&](int share) {
+    failed = 1;
+    atomicMin(&failed_share, share);
+  };
 
-  if (warp == 0) {
-    // ---- requests of the K and V tiles.  Page ids are looked up for a chunk of 32 / pages_per_tile tiles at a time, a
-    // chunk ahead; two tiles per turn, each with a lane of its own that waits for the ring slots and makes the requests.
+  int done = 0;   // key tiles of the shares before
+  int share = 0;
+  // warp 0: ring slots of the next tile, and their use counts; tiles of the coming share that have been asked for
+  int sk = 0, rk = 0, sv = 0, rv = 0, asked = 0;
+  int pg = -2, pg_next = -2;                                // the page ids of a chunk of tiles, and of the next one
+  uint32_t bad_mask = 0, live_mask = 0, run_mask = 0;
+  // warps 1, 10, 11: shares of the group with tiles, tiles of each group
+  int active = 0, count0 = 0, count1 = 0;
+  // softmax warps: the group's tiles so far, running maximum and sum of the present share
+  int count = 0;
+  float m_run = -INFINITY, l_run = 0.f;
+  const bool leader = elect_one();
+
+  // Rows of tile `quarter` of the softmax warps.
+  const int g = warp >= 2 && warp < PV_WARP ? (warp - 2) >> 2 : warp == S1_WARP ? 1 : 0;  // the group of warps 1 to 9 and 11
+  const int quarter = warp & 3, r = quarter * 32 + lane;
+  const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+
+  // Requests the tiles asked .. upto - 1 of a share, two a turn (`upto` is even or the share's last).
+  auto request = [&](const Share& t, int upto, int first_tile) {
     const int pages_per_tile = BN / p.page_size;
     const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.page_size * 128u;
     const int ppt_shift = __ffs(pages_per_tile) - 1, page_shift = __ffs(p.page_size) - 1;  // powers of two here
     const int chunk_shift = 5 - ppt_shift, chunk_mask = (1 << chunk_shift) - 1;
     const int page_in_tile = lane & (pages_per_tile - 1);
     const uint32_t tile_lanes = pages_per_tile == 32 ? 0xffffffffu : ((1u << pages_per_tile) - 1u);
-    int sk = 0, rk = 0, sv = 0, rv = 0;  // ring slots of the turn's first tile, and their use counts
-    int done = 0;                        // tiles of the shares before
-    do {
-      const int n_kt = w.kt_end - w.kt_begin, kt_begin = w.kt_begin;
-      const int lo = sh.window > 0 ? max(0, w.t.ctx - sh.window + 1) : 0, last = w.t.ctx + w.t.n - 1;
-      const int* table = p.page_table + (size_t)w.at.seq * p.pt_stride;
-      auto load_chunk = [&](int c) -> int {
-        const int i = (c << chunk_shift) + (lane >> ppt_shift);
-        const int first = (kt_begin + i) * BN + page_in_tile * p.page_size;
-        if (i < n_kt && first <= last && first + p.page_size > lo) {
-          const int j = first >> page_shift;
-          return j < p.pt_stride ? table[j] : -1;
+    const int n_kt = t.kt_end - t.kt_begin, kt_begin = t.kt_begin, head = t.head;
+    const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0, last = t.ctx + t.n - 1;
+    const int* table = p.page_table + (size_t)t.seq * p.pt_stride;
+    // Page ids are looked up for a chunk of 32 / pages_per_tile tiles at a time, a chunk ahead.
+    auto load_chunk = [&](int c) -> int {
+      const int i = (c << chunk_shift) + (lane >> ppt_shift);
+      const int first = (kt_begin + i) * BN + page_in_tile * p.page_size;
+      if (i < n_kt && first <= last && first + p.page_size > lo) {
+        const int j = first >> page_shift;
+        return j < p.pt_stride ? table[j] : -1;
+      }
+      return -2;  // not wanted
+    };
+    if (asked == 0) pg_next = load_chunk(0);
+    for (; asked < upto; asked += 2) {
+      const int in_chunk = asked & chunk_mask;
+      if (in_chunk == 0) {
+        pg = pg_next;
+        pg_next = load_chunk((asked >> chunk_shift) + 1);
+        const bool bad = pg != -2 && (pg < 0 || pg >= p.num_pages);  // recorded, not loaded, its keys are hidden
+        if (bad) {
+          atomicOr(p.err, DSP_ERR_BAD_PAGE);
+          pg = -1;
         }
-        return -2;  // not wanted
-      };
-      int pg = -2, pg_next = load_chunk(0);
-      uint32_t bad_mask = 0, live_mask = 0, run_mask = 0;
-      for (int i = 0; i < n_kt; i += 2) {
-        const int in_chunk = i & chunk_mask;
-        if (in_chunk == 0) {
-          pg = pg_next;
-          pg_next = load_chunk((i >> chunk_shift) + 1);
-          const bool bad = pg != -2 && (pg < 0 || pg >= p.num_pages);  // recorded, not loaded, its keys are hidden
-          if (bad) {
-            atomicOr(p.err, DSP_ERR_BAD_PAGE);
-            pg = -1;
-          }
-          bad_mask = __ballot_sync(0xffffffffu, bad);
-          live_mask = __ballot_sync(0xffffffffu, pg >= 0);
-          const int first_pg = __shfl_sync(0xffffffffu, pg, lane & ~(pages_per_tile - 1));
-          run_mask = __ballot_sync(0xffffffffu, pg >= 0 && pg == first_pg + page_in_tile &&
-                                                    first_pg + pages_per_tile <= p.num_pages);
+        bad_mask = __ballot_sync(0xffffffffu, bad);
+        live_mask = __ballot_sync(0xffffffffu, pg >= 0);
+        const int first_pg = __shfl_sync(0xffffffffu, pg, lane & ~(pages_per_tile - 1));
+        run_mask = __ballot_sync(0xffffffffu, pg >= 0 && pg == first_pg + page_in_tile &&
+                                                  first_pg + pages_per_tile <= p.num_pages);
+      }
+      // Two tiles per turn, each with a lane of its own that waits for the tile's ring slots and makes the requests.
+      const int second = (lane >> ppt_shift) - in_chunk;  // 0, 1: this lane holds a page of the turn's first, second tile
+      const bool mine = (second == 0 || second == 1) && asked + second < n_kt;
+      const int shift = (in_chunk + (second == 1 ? 1 : 0)) << ppt_shift;
+      const uint32_t live = (live_mask >> shift) & tile_lanes;
+      const bool in_run = p.page_runs && ((run_mask >> shift) & tile_lanes) == tile_lanes;
+      int my_sk = sk, my_rk = rk, my_sv = sv, my_rv = rv;
+      if (second == 1) {
+        if (++my_sk == K_STAGES) {
+          my_sk = 0;
+          ++my_rk;
         }
-        const int second = (lane >> ppt_shift) - in_chunk;  // 0, 1: this lane holds a page of the turn's first, second tile
-        const bool mine = (second == 0 || second == 1) && i + second < n_kt;
-        const int shift = (in_chunk + (second == 1 ? 1 : 0)) << ppt_shift;
-        const uint32_t live = (live_mask >> shift) & tile_lanes;
-        const bool in_run = p.page_runs && ((run_mask >> shift) & tile_lanes) == tile_lanes;
-        const bool leader = mine && lane == shift;
-        int my_sk = sk, my_rk = rk, my_sv = sv, my_rv = rv;
-        if (second == 1) {
-          if (++my_sk == K_STAGES) {
-            my_sk = 0;
-            ++my_rk;
-          }
-          if (++my_sv == V_STAGES) {
-            my_sv = 0;
-            ++my_rv;
-          }
+        if (++my_sv == V_STAGES) {
+          my_sv = 0;
+          ++my_rv;
         }
-        if (leader) {
-          if (*(volatile int*)&failed == 0 &&
-              mbar_wait_both(&k_empty[my_sk], (my_rk & 1) ^ 1, &v_empty[my_sv], (my_rv & 1) ^ 1)) {
-            bad_pages[(done + i + second) % BAD_SLOTS] = (bad_mask >> shift) & tile_lanes;  // published by the arrival on k_full
-            if (live == 0) {
-              mbar_arrive(&k_full[my_sk]);
-              mbar_arrive(&v_full[my_sv]);
-            } else {
-              mbar_expect_tx(&k_full[my_sk], (uint32_t)__popc(live) * page_bytes);
-              mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
-            }
-            if (in_run) {  // the tile's pages lie one after the other in the pool: one request per operand
-              tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, w.head * p.page_size, pg, 0);
-              tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, w.head * p.page_size, pg, 0);
-            }
+      }
+      if (mine && lane == shift) {
+        if (*(volatile int*)&failed == 0 &&
+            mbar_wait_both(&k_empty[my_sk], (my_rk & 1) ^ 1, &v_empty[my_sv], (my_rv & 1) ^ 1)) {
+          bad_pages[(first_tile + asked + second) % BAD_SLOTS] = (bad_mask >> shift) & tile_lanes;  // published by the arrival on k_full
+          if (live == 0) {
+            mbar_arrive(&k_full[my_sk]);
+            mbar_arrive(&v_full[my_sv]);
           } else {
-            failed = 1;
+            mbar_expect_tx(&k_full[my_sk], (uint32_t)__popc(live) * page_bytes);
+            mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
           }
+          if (in_run) {  // the tile's pages lie one after the other in the pool: one request per operand
+            tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, head * p.page_size, pg, 0);
+            tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, head * p.page_size, pg, 0);
+          }
+        } else {
+          give_up(share);
         }
-        if (!__all_sync(0xffffffffu, !mine || in_run)) {
-          if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
-            const int row = (pg * sh.KVH + w.head) * p.page_size;
-            const int dst = page_in_tile * p.page_size * 128;
+      }
+      if (!__all_sync(0xffffffffu, !mine || in_run)) {
+        if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
+          const int row = (pg * sh.KVH + head) * p.page_size;
+          const int dst = page_in_tile * p.page_size * 128;
 #pragma unroll
-            for (int h = 0; h < KD; ++h) {
-              tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
-              tma_load_2d(v_s + my_sv * KV_BYTES + dst + h * KV_SLICE, &map_v, &v_full[my_sv], h * 64, row);
-            }
-          }
-        }
-        for (int u = 0; u < min(2, n_kt - i); ++u) {
-          if (++sk == K_STAGES) {
-            sk = 0;
-            ++rk;
-          }
-          if (++sv == V_STAGES) {
-            sv = 0;
-            ++rv;
+          for (int h = 0; h < KD; ++h) {
+            tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
+            tma_load_2d(v_s + my_sv * KV_BYTES + dst + h * KV_SLICE, &map_v, &v_full[my_sv], h * 64, row);
           }
         }
       }
-      done += n_kt;
-    } while (w.next(sh, cta));
-  } else if (warp == 1 || warp == S1_WARP) {
-    // ---- score products of one softmax group
-    const int g = warp == 1 ? 0 : 1;
-    const bool leader = elect_one();
-    const uint32_t idesc_s = umma_idesc(BM, BN);
-    const uint64_t k_desc0 = umma_desc(smem_u32(k_s));
-    const uint32_t tmem_s = tmem_base + (uint32_t)(g * S_COLS);
-    int done = 0, count = 0, share = 0;  // tiles of the shares before; this group's tiles, and shares with any, so far
-    bool ok = true;
-    do {
-      const int n_kt = w.kt_end - w.kt_begin;
+      for (int u = 0; u < min(2, n_kt - asked); ++u) {
+        if (++sk == K_STAGES) {
+          sk = 0;
+          ++rk;
+        }
+        if (++sv == V_STAGES) {
+          sv = 0;
+          ++rv;
+        }
+      }
+    }
+  };
+
+  // The queries of a share, by the warps of group 1: row r of the tile, lane r, two bfloat16 per column (rows past the item
+  // are zero).
+  auto bring_queries = [&](const Share& t) {
+    const int rr = t.row_tile * BM + r;
+    const bool valid = rr < t.n * G;
+    const uint4* src = reinterpret_cast<const uint4*>(p.q);
+    if (valid)
+      src = reinterpret_cast<const uint4*>(p.q + (size_t)(t.first + rr / G) * p.q_stride + (size_t)(t.head * G + rr % G) * D);
+#pragma unroll
+    for (int c0 = 0; c0 < D / 2; c0 += 32) {
+      uint32_t x[32];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 v = valid ? __ldg(src + c0 / 4 + c) : make_uint4(0, 0, 0, 0);
+        x[4 * c] = v.x;
+        x[4 * c + 1] = v.y;
+        x[4 * c + 2] = v.z;
+        x[4 * c + 3] = v.w;
+      }
+      __syncwarp();
+      tmem_st32(lane_addr + (uint32_t)(Q_COL + c0), x);
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&q_ready[0]);
+      if (t.kt_end - t.kt_begin > 1) mbar_arrive(&q_ready[1]);
+    }
+  };
+
+  // By the warps of group 0, behind the barrier of share k: merges the two groups' halves and stores the rows, or the partial
+  // result of the share.
+  auto finish = [&](int k) {
+    const Share& t = shares[k % SHARES];
+    const int row0 = t.row_tile * BM, nrows = min(BM, t.n * G - row0), slot = t.slot;
+    const bool row_ok = r < nrows;
+    const bool two = t.kt_end - t.kt_begin > 1;
+    const float m1 = two ? merge_m[k & 1][r] : -INFINITY, l1 = two ? merge_l[k & 1][r] : 0.f;
+    const float M = fmaxf(m_run, m1);
+    const float w0 = m_run == -INFINITY ? 0.f : ex2(m_run - M);
+    const float w1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+    const float denom = l_run * w0 + l1 * w1;
+    const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
+    const float f0 = w0 * inv, f1 = w1 * inv;
+    if (quarter * 32 < nrows) {
+      bf16* dst = p.out;
+      float* part = p.part_o;
+      if (slot >= 0)
+        part += ((size_t)slot * BM + r) * D;
+      else if (row_ok)
+        dst += (size_t)(t.first + (row0 + r) / G) * p.out_stride + (size_t)(t.head * G + (row0 + r) % G) * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t ov[32], ow[32];
+        __syncwarp();
+        tmem_ld32(lane_addr + (uint32_t)(O_COL + c0), ov);
+        // (a half that saw no key has weight 0, and an accumulator of zeros)
+        if (two) {
+          tmem_ld32(lane_addr + (uint32_t)(O_COL + D + c0), ow);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            ov[c] = __float_as_uint(__uint_as_float(ov[c]) * f0 + __uint_as_float(ow[c]) * f1);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * f0);
+        }
+        if (row_ok && slot >= 0) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
+        } else if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint4 x;
+            x.x = pack2(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]));
+            x.y = pack2(__uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3]));
+            x.z = pack2(__uint_as_float(ov[c + 4]), __uint_as_float(ov[c + 5]));
+            x.w = pack2(__uint_as_float(ov[c + 6]), __uint_as_float(ov[c + 7]));
+            *reinterpret_cast<uint4*>(dst + c0 + c) = x;
+          }
+        }
+        __syncwarp();
+      }
+      if (slot >= 0 && row_ok) reinterpret_cast<float2*>(p.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&o_free);
+  };
+
+  // Every wait of a share is for something that happens in that share, or, in warp 0's requests for the coming one, for
+  // slots that this share's tiles leave; the whole block passes the barrier at its end.
+  for (;; ++share) {
+    const Share& t = shares[share % SHARES];
+    if (failed_share < share || t.seq < 0) break;  // (written before the last barrier; all see the same)
+    const int n_kt = t.kt_end - t.kt_begin;
+    if (warp == 0) {
+      request(t, n_kt, done);
+      more = w.next(sh, cta);
+      if (lane == 0) {
+        if (!more) w.at.seq = -1;
+        shares[(share + 1) % SHARES] = w.at;
+      }
+      asked = 0;
+      // the coming share's first tiles: as many as slots that this share's tiles are sure to leave
+      if (more) request(w.at, min(K_STAGES - 2, w.at.kt_end - w.at.kt_begin), done + n_kt);
+    } else if (warp == 1 || warp == S1_WARP) {
+      // ---- score products of one softmax group
+      const uint32_t idesc_s = umma_idesc(BM, BN);
+      const uint64_t k_desc0 = umma_desc(smem_u32(k_s));
+      const uint32_t tmem_s = tmem_base + (uint32_t)(g * S_COLS);
+      bool ok = true;
       if (g < n_kt) {
-        ok = mbar_wait(&q_ready[g], share & 1);
-        ++share;
+        ok = __all_sync(0xffffffffu, mbar_wait(&q_ready[g], active & 1));
+        ++active;
         tc_fence_after();
-        for (int a = g; a < n_kt && ok; a += 2, ++count) {
-          const int s = (done + a) % K_STAGES, use = (done + a) / K_STAGES;
-          ok = count == 0 ? mbar_wait(&k_full[s], use & 1)
-                          : mbar_wait_both(&k_full[s], use & 1, &s_free[g], (count - 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t k_desc = k_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
-          if (leader) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (uint32_t)(k >> 2), in = (uint32_t)(k & 3) * 32u;
-              umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * KV_SLICE + in) >> 4), idesc_s, k != 0);
-            }
-            umma_commit(&s_full[g]);
-            umma_commit(&k_empty[s]);
-          }
-        }
       }
-      done += n_kt;
-    } while (ok && w.next(sh, cta));
-    if (!ok) failed = 1;
-  } else if (warp == PV_WARP) {
-    // ---- output products: O[g] += P[g] V of the share's tiles in turn
-    const bool leader = elect_one();
-    const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
-    const uint64_t v_desc0 = umma_desc_mn(smem_u32(v_s), KV_SLICE);
-    int done = 0, share = 0, count[2] = {0, 0};
-    bool ok = true;
-    do {
-      const int n_kt = w.kt_end - w.kt_begin;
-      if (share > 0) ok = mbar_wait(&o_free, (share - 1) & 1);
-      for (int b = 0; b < n_kt && ok; ++b) {
-        const int g = b & 1, st = (done + b) % V_STAGES;
-        ok = mbar_wait_both(&v_full[st], ((done + b) / V_STAGES) & 1, &p_full[g], (g ? count[1] : count[0]) & 1);
+      for (int a = g; a < n_kt && ok; a += 2, ++count0) {
+        const int s = (done + a) % K_STAGES, use = (done + a) / K_STAGES;
+        ok = __all_sync(0xffffffffu, count0 == 0 ? mbar_wait(&k_full[s], use & 1)
+                                                 : mbar_wait_both(&k_full[s], use & 1, &s_free[g], (count0 - 1) & 1));
         if (!ok) break;
-        if (g)
-          ++count[1];
+        tc_fence_after();
+        const uint64_t k_desc = k_desc0 + (uint64_t)(s * (KV_BYTES >> 4));
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (uint32_t)(k >> 2), in = (uint32_t)(k & 3) * 32u;
+            umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * KV_SLICE + in) >> 4), idesc_s, k != 0);
+          }
+          umma_commit(&s_full[g]);
+          umma_commit(&k_empty[s]);
+        }
+        __syncwarp();
+      }
+      if (!ok) give_up(share);
+    } else if (warp == PV_WARP) {
+      // ---- output products: O[g] += P[g] V of the share's tiles in turn
+      const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
+      const uint64_t v_desc0 = umma_desc_mn(smem_u32(v_s), KV_SLICE);
+      bool ok = share == 0 || __all_sync(0xffffffffu, mbar_wait(&o_free, (share - 1) & 1));
+      for (int b = 0; b < n_kt && ok; ++b) {
+        const int og = b & 1, st = (done + b) % V_STAGES;
+        ok = __all_sync(0xffffffffu, mbar_wait_both(&v_full[st], ((done + b) / V_STAGES) & 1, &p_full[og],
+                                                    (og ? count1 : count0) & 1));
+        if (!ok) break;
+        if (og)
+          ++count1;
         else
-          ++count[0];
+          ++count0;
         tc_fence_after();
         const uint64_t v_desc = v_desc0 + (uint64_t)(st * (KV_BYTES >> 4));
         if (leader) {
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
-            umma_a_tmem(tmem_base + (uint32_t)(O_COL + g * D), tmem_base + (uint32_t)(P_COL + g * P_COLS + k * 8),
+            umma_a_tmem(tmem_base + (uint32_t)(O_COL + og * D), tmem_base + (uint32_t)(P_COL + og * P_COLS + k * 8),
                         v_desc + (uint64_t)(k * 128), idesc_o, (b >= 2) || k != 0);
           umma_commit(&v_empty[st]);
-          umma_commit(&o_done[g]);
+          umma_commit(&o_done[og]);
         }
+        __syncwarp();
       }
-      done += n_kt;
-      ++share;
-    } while (ok && w.next(sh, cta));
-    if (!ok) failed = 1;
-  } else {
-    // ---- softmax groups
-    const int g = (warp - 2) >> 2;
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
-    const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
-    const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
-    const float scale = p.scale_log2;
-    const int page_shift = __ffs(p.page_size) - 1;
-    // the queries of a share: row r of the tile, lane r, two bfloat16 per column (rows past the item are zero)
-    auto bring_queries = [&]() {
-      const int row0 = w.row_tile * BM, rr = row0 + r;
-      const bool valid = rr < w.t.n * G;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q);
-      if (valid)
-        src = reinterpret_cast<const uint4*>(p.q + (size_t)(w.t.first + rr / G) * p.q_stride +
-                                             (size_t)(w.head * G + rr % G) * D);
-#pragma unroll
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
-        uint32_t x[32];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 v = valid ? __ldg(src + c0 / 4 + c) : make_uint4(0, 0, 0, 0);
-          x[4 * c] = v.x;
-          x[4 * c + 1] = v.y;
-          x[4 * c + 2] = v.z;
-          x[4 * c + 3] = v.w;
-        }
-        tmem_st32(lane_addr + (uint32_t)(Q_COL + c0), x);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&q_ready[0]);
-        if (w.kt_end - w.kt_begin > 1) mbar_arrive(&q_ready[1]);
-      }
-    };
-    if (g == 1) bring_queries();
-    int done = 0, count = 0, share = 0;
-    bool more = true;
-    do {
-      const Tree t = w.t;
-      const int n_kt = w.kt_end - w.kt_begin, kt_begin = w.kt_begin, row0 = w.row_tile * BM, slot = w.slot, head = w.head;
+      if (!ok) give_up(share);
+    } else {
+      // ---- softmax groups: first the end of the last share, or the queries of this one
+      if (g == 1)
+        bring_queries(t);
+      else if (share > 0)
+        finish(share - 1);
+      const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
+      const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
+      const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
+      const float scale = p.scale_log2;
+      const int page_shift = __ffs(p.page_size) - 1;
+      const int kt_begin = t.kt_begin, row0 = t.row_tile * BM;
       const int nrows = min(BM, t.n * G - row0);
       const bool row_ok = r < nrows;
       const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
@@ -379,97 +483,92 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       const int total = t.ctx + t.n;
       const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;  // first key any row sees
       const int lo_r = sh.window > 0 ? t.ctx + depth - sh.window + 1 : 0;
-      float m_run = -INFINITY, l_run = 0.f;
+      m_run = -INFINITY;
+      l_run = 0.f;
       bool ok = true;
       int j = 0;  // tiles of this group in this share
       for (int i = g; i < n_kt; i += 2, ++j, ++count) {
         const int key0 = (kt_begin + i) * BN;
+        // what the row sees of a tile that not every row sees whole, while its scores are being formed
+        const bool some = key0 + BN > t.ctx || __any_sync(0xffffffffu, key0 < lo_r);
+        unsigned long long seen = ~0ull;
+        if (some && warp_ok) seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], count & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t sv[64];
         const uint32_t bad = bad_pages[(done + i) % BAD_SLOTS];
-        float alpha = 1.f;
-        uint32_t pk[32];
+        if (bad != 0u)
+          for (int b = 0; b < BN >> page_shift; ++b)
+            if ((bad >> b) & 1u)
+              seen &= ~((p.page_size == 64 ? ~0ull : (1ull << p.page_size) - 1ull) << (b << page_shift));
+        __syncwarp();
         if (warp_ok) {
           uint32_t a[32], b[32];
           tmem_ld32_nowait(s_addr, a);
           tmem_ld32_nowait(s_addr + 32, b);
           tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            sv[c] = a[c];
-            sv[32 + c] = b[c];
-          }
-        }
-        // the scores are in registers: the next scores of this group may overwrite S[g]
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[g]);
-        if (warp_ok) {
-          if (key0 + BN > t.ctx || bad != 0u || __any_sync(0xffffffffu, key0 < lo_r)) {
-            unsigned long long seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
-            if (bad != 0u)
-              for (int b = 0; b < BN >> page_shift; ++b)
-                if ((bad >> b) & 1u)
-                  seen &= ~((p.page_size == 64 ? ~0ull : (1ull << p.page_size) - 1ull) << (b << page_shift));
+          // the scores are in registers: the next scores of this group may overwrite S[g]
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[g]);
+          if (some || bad != 0u) {
             const uint32_t s_lo = (uint32_t)seen, s_hi = (uint32_t)(seen >> 32);
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
-              sv[c] = (s_lo >> c) & 1u ? sv[c] : 0xff800000u;  // -inf
-              sv[32 + c] = (s_hi >> c) & 1u ? sv[32 + c] : 0xff800000u;
+              a[c] = (s_lo >> c) & 1u ? a[c] : 0xff800000u;  // -inf
+              b[c] = (s_hi >> c) & 1u ? b[c] : 0xff800000u;
             }
           }
           float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            t0 = fmaxf(t0, __uint_as_float(sv[c]));
-            t1 = fmaxf(t1, __uint_as_float(sv[c + 1]));
-            t2 = fmaxf(t2, __uint_as_float(sv[c + 2]));
-            t3 = fmaxf(t3, __uint_as_float(sv[c + 3]));
+          for (int c = 0; c < 32; c += 2) {
+            t0 = fmaxf(t0, __uint_as_float(a[c]));
+            t1 = fmaxf(t1, __uint_as_float(a[c + 1]));
+            t2 = fmaxf(t2, __uint_as_float(b[c]));
+            t3 = fmaxf(t3, __uint_as_float(b[c + 1]));
           }
           const float tmax = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;  // the scale is positive
           const float m_new = (tmax > m_run + RESCALE_STEP || m_run == -INFINITY) ? fmaxf(tmax, m_run) : m_run;
-          alpha = m_new == m_run ? 1.f : ex2(m_run - m_new);  // 0 on a row's first visible tile
+          const float alpha = m_new == m_run ? 1.f : ex2(m_run - m_new);  // 0 on a row's first visible tile
           m_run = m_new;
           const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
           float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+          uint32_t pk[32];
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            const float e0 = ex2(fmaf(__uint_as_float(sv[c]), scale, neg_m));
-            const float e1 = ex2(fmaf(__uint_as_float(sv[c + 1]), scale, neg_m));
-            const float e2 = ex2(fmaf(__uint_as_float(sv[c + 2]), scale, neg_m));
-            const float e3 = ex2(fmaf(__uint_as_float(sv[c + 3]), scale, neg_m));
+          for (int c = 0; c < 32; c += 2) {
+            const float e0 = ex2(fmaf(__uint_as_float(a[c]), scale, neg_m));
+            const float e1 = ex2(fmaf(__uint_as_float(a[c + 1]), scale, neg_m));
+            const float e2 = ex2(fmaf(__uint_as_float(b[c]), scale, neg_m));
+            const float e3 = ex2(fmaf(__uint_as_float(b[c + 1]), scale, neg_m));
             a0 += e0;
             a1 += e1;
             a2 += e2;
             a3 += e3;
             pk[c / 2] = pack2(e0, e1);
-            pk[c / 2 + 1] = pack2(e2, e3);
+            pk[16 + c / 2] = pack2(e2, e3);
           }
           l_run = l_run * alpha + ((a0 + a1) + (a2 + a3));
-        }
-        // the group's previous O[g] += P V must be complete before O[g] is rescaled and P[g] rewritten
-        if (j > 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
+          // the group's previous O[g] += P V must be complete before O[g] is rescaled and P[g] rewritten
+          if (j > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (__any_sync(0xffffffffu, alpha != 1.f)) rescale(o_addr, alpha);
+          }
+          __syncwarp();
+          tmem_st32(p_addr, pk);  // 64 bfloat16 in the 32 columns of the group's A operand
+        } else {
+          if (lane == 0) mbar_arrive(&s_free[g]);
+          // (no arrival for a tile before every warp's for the one before has been counted)
+          if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          if (warp_ok && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t ov[32];
-              tmem_ld32(o_addr + (uint32_t)c0, ov);
-#pragma unroll
-              for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-              tmem_st32(o_addr + (uint32_t)c0, ov);
-            }
-          }
         }
-        if (warp_ok) tmem_st32(p_addr, pk);  // 64 bfloat16 in the 32 columns of the group's A operand
         // value rows no row of this item may see: zero them (whole 128-byte rows, every slice)
         if (key0 < lo || key0 + BN > total || bad != 0u) {
           const int st = (done + i) % V_STAGES;
@@ -489,6 +588,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           }
           fence_async_smem();
         }
+        __syncwarp();
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -496,79 +596,22 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       // the group's last product of the share
       if (ok && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) ok = false;
-      if (!ok) {
-        failed = 1;
-        atomicMin(&failed_share, share);
-      }
+      if (!ok) give_up(share);
       if (g == 1) {
         merge_m[share & 1][r] = m_run;
         merge_l[share & 1][r] = l_run;
       }
-      tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
-      if (*(volatile int*)&failed_share <= share) break;  // all of them see the same
-      tc_fence_after();
-      if (g == 1) {
-        more = w.next(sh, cta);
-        if (more) bring_queries();
-      } else {
-        // ---- merge the two groups' halves of the share; store the rows, or the partial result of the share
-        const bool two = n_kt > 1;
-        const float m1 = two ? merge_m[share & 1][r] : -INFINITY, l1 = two ? merge_l[share & 1][r] : 0.f;
-        const float M = fmaxf(m_run, m1);
-        const float w0 = m_run == -INFINITY ? 0.f : ex2(m_run - M);
-        const float w1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-        const float denom = l_run * w0 + l1 * w1;
-        const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
-        const float f0 = w0 * inv, f1 = w1 * inv;
-        if (warp_ok) {
-          bf16* dst = p.out;
-          float* part = p.part_o;
-          if (slot >= 0)
-            part += ((size_t)slot * BM + r) * D;
-          else if (row_ok)
-            dst += (size_t)node * p.out_stride + (size_t)(head * G + (row0 + r) % G) * D;
-#pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t ov[32], ow[32];
-            tmem_ld32_nowait(lane_addr + (uint32_t)(O_COL + c0), ov);
-            if (two) tmem_ld32_nowait(lane_addr + (uint32_t)(O_COL + D + c0), ow);
-            tmem_ld_wait();
-            // (a half that saw no key has weight 0, and an accumulator of zeros)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              ov[c] = __float_as_uint(two ? __uint_as_float(ov[c]) * f0 + __uint_as_float(ow[c]) * f1
-                                          : __uint_as_float(ov[c]) * f0);
-            if (row_ok && slot >= 0) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 4)
-                *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
-            } else if (row_ok) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 8) {
-                uint4 x;
-                x.x = pack2(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]));
-                x.y = pack2(__uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3]));
-                x.z = pack2(__uint_as_float(ov[c + 4]), __uint_as_float(ov[c + 5]));
-                x.w = pack2(__uint_as_float(ov[c + 6]), __uint_as_float(ov[c + 7]));
-                *reinterpret_cast<uint4*>(dst + c0 + c) = x;
-              }
-            }
-            __syncwarp();
-          }
-          if (slot >= 0 && row_ok) reinterpret_cast<float2*>(p.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free);
-        more = w.next(sh, cta);
-      }
-      done += n_kt;
-      ++share;
-    } while (more);
+    }
+    done += n_kt;
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    __syncwarp();
   }
-
   pdl_launch_dependents();
+  if (share > 0 && failed_share >= share && warp >= 2 && warp < 6) finish(share - 1);
+
   tc_fence_before();
   __syncthreads();
   if (failed) {
@@ -577,6 +620,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     for (int i = 0; i < 2000; ++i) __nanosleep(100);
   }
   tc_fence_after();
+  __syncwarp();
   if (warp == 1) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }

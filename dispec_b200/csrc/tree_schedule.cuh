@@ -2,10 +2,12 @@
 //
 // Tree s has n_s nodes behind ctx_s stored tokens.  An item is one tile of query rows (rows are (node, head-in-group)
 // pairs, G heads a node) of one key/value head of one tree; it walks the key tiles from the first key that any of its
-// tree's nodes sees to the tree's last node.  A unit is one key tile of one item.  All units, in the order (tree, head,
-// row tile, key tile), are cut into equal runs, one per CTA, wherever that falls: trees of any lengths load every SM
-// alike, and nothing about lengths is needed on the host.  Row tiles of one head follow one another, so CTAs that run
-// at the same time share its keys through the L2.
+// tree's nodes sees to the tree's last node.  A unit is one key tile of one item.  All units, in the order (row tile, tree,
+// head, key tile), are cut into equal runs, one per CTA, wherever that falls: trees of any lengths load every SM alike, and
+// nothing about lengths is needed on the host.  Where all trees have R row tiles and the number of CTAs is a multiple of R, the
+// CTAs c, c + ctas / R, ... walk the same keys at the same time, which then come from memory once and from the L2
+// for the others (64 trees of 320 rows, whose row tiles followed one another in one CTA: 1.28 GB read where
+// the keys and values are 0.42).
 //
 // An item that ends in the CTA it began in is finished there.  The others leave one partial result (32-bit sums that are
 // not divided yet, running maximum, sum of weights) per CTA in scratch: slot 2 c + 1 for the item that begins in CTA c,
@@ -37,111 +39,136 @@ __device__ __forceinline__ Tree load_tree(const Shape& sh, int s) {
   const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;
   t.lo_tile = lo / sh.keys_per_tile;
   t.key_tiles = t.n > 0 ? (t.ctx + t.n + sh.keys_per_tile - 1) / sh.keys_per_tile - t.lo_tile : 0;
-  t.row_tiles = (int)(((long)t.n * sh.G + sh.rows_per_tile - 1) / sh.rows_per_tile);
+  t.row_tiles = (t.n * sh.G + sh.rows_per_tile - 1) / sh.rows_per_tile;
   return t;
 }
-__device__ __forceinline__ long units_of(const Shape& sh, const Tree& t) {
-  return (long)t.row_tiles * t.key_tiles * sh.KVH;
-}
+// Units of a tree in one of its row tiles.
+__device__ __forceinline__ int units_of(const Shape& sh, const Tree& t) { return t.key_tiles * sh.KVH; }
 
-__device__ __forceinline__ long warp_scan(long v) {
+__device__ __forceinline__ int warp_sum_int(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long up = __shfl_up_sync(0xffffffffu, v, o);
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   return v;
 }
 
-// Units a CTA takes: the same number for all, at least min_units.  Called by whole warps.
-__device__ __forceinline__ long units_per_cta(const Shape& sh, int ctas, long* total) {
-  const int lane = threadIdx.x & 31;
-  long mine = 0;
-  for (int s = lane; s < sh.S; s += 32) mine += units_of(sh, load_tree(sh, s));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  *total = mine;
-  return max((mine + ctas - 1) / ctas, (long)sh.min_units);
-}
-
-// Where unit u lies.
-struct Place {
-  int seq, item, key_tile;  // item inside the tree: head * row_tiles + row tile; key tile counted from lo_tile
-  long item_start;          // first unit of the item
+// Where a unit lies.
+struct Found {
+  int total, chunk;         // all units; units a CTA takes (the same number for all, at least min_units)
+  int seq, row_tile, start; // the tree (-1: there is no such unit), the row tile, first unit of that tree in that row tile
 };
-
-// Called by whole warps; u is inside the total.
-__device__ __forceinline__ Place find_unit(const Shape& sh, long u) {
+// Called by whole warps.  `pick` names the unit once total and chunk are known.  The trees of up to 32 requests are read once.
+template <typename Pick>
+__device__ __forceinline__ Found find_unit(const Shape& sh, int ctas, Pick pick) {
   const int lane = threadIdx.x & 31;
-  Place p = {0, 0, 0, 0};
-  long before = 0;
-  for (int s0 = 0; s0 < sh.S; s0 += 32) {
-    const int s = s0 + lane;
-    Tree t = {};
-    long n = 0;
-    if (s < sh.S) {
-      t = load_tree(sh, s);
-      n = units_of(sh, t);
-    }
-    const long upto = before + warp_scan(n);
-    const uint32_t past = __ballot_sync(0xffffffffu, upto > u);
-    if (past != 0u) {
-      const int who = __ffs(past) - 1;
-      const long start = __shfl_sync(0xffffffffu, upto - n, who);
-      const int per_item = __shfl_sync(0xffffffffu, t.key_tiles, who);
-      p.seq = s0 + who;
-      p.item = (int)((u - start) / per_item);
-      p.key_tile = (int)((u - start) - (long)p.item * per_item);
-      p.item_start = start + (long)p.item * per_item;
-      return p;
-    }
-    before = __shfl_sync(0xffffffffu, upto, 31);
+  Found f = {0, 0, -1, 0, 0};
+  int mine = 0, held = 0, held_tiles = 0;
+  for (int s = lane; s < sh.S; s += 32) {
+    const Tree t = load_tree(sh, s);
+    held = units_of(sh, t);
+    held_tiles = t.row_tiles;
+    mine += held * held_tiles;
   }
-  return p;
+  auto units = [&](int s, int tile) -> int {  // of lane's tree s in a row tile
+    if (s >= sh.S) return 0;
+    if (sh.S <= 32) return held_tiles > tile ? held : 0;
+    const Tree t = load_tree(sh, s);
+    return t.row_tiles > tile ? units_of(sh, t) : 0;
+  };
+  f.total = warp_sum_int(mine);
+  f.chunk = max((f.total + ctas - 1) / ctas, sh.min_units);
+  const int u = pick(f);
+  if (u >= f.total) return f;
+  int before = 0;
+  for (int tile = 0;; ++tile) {
+    int of_tile = 0;
+    for (int s = lane; s < sh.S; s += 32) of_tile += units(s, tile);
+    of_tile = warp_sum_int(of_tile);
+    if (u >= before + of_tile) {
+      before += of_tile;
+      continue;  // (ends: u is below the total)
+    }
+    for (int s0 = 0; s0 < sh.S; s0 += 32) {
+      const int n = units(s0 + lane, tile);
+      const int upto = before + warp_scan(n);
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > u);
+      if (past != 0u) {
+        const int who = __ffs(past) - 1;
+        f.seq = s0 + who;
+        f.row_tile = tile;
+        f.start = __shfl_sync(0xffffffffu, upto - n, who);
+        return f;
+      }
+      before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return f;
+  }
 }
+
+// One item's part of a CTA's run.
+struct Share {
+  int seq, first, n, ctx;  // the tree (seq -1: the run has ended)
+  int head, row_tile;
+  int kt_begin, kt_end;    // key tiles, counted from key 0
+  int slot;                // scratch slot of the partial result, -1: the item is finished here
+};
 
 // A CTA's walk over its run of units, one item's share at a time.
 struct Walk {
-  long u, end, chunk;
-  Place at;
-  Tree t;
-  // the current share
-  int head, row_tile, kt_begin, kt_end;  // key tiles counted from key 0
-  int slot;                              // scratch slot of the partial result, -1: the item is finished here
+  int u, end;
+  int item_start, key_tiles, lo_tile;
+  Share at;
 
-  // false: this CTA has no work
+  // Called by whole warps.  False: this CTA has no work.
   __device__ __forceinline__ bool begin(const Shape& sh, int cta, int ctas) {
-    long total;
-    chunk = units_per_cta(sh, ctas, &total);
-    u = chunk * cta;
-    end = min(total, u + chunk);
-    if (u >= end) return false;
-    at = find_unit(sh, u);
-    t = load_tree(sh, at.seq);
+    const Found f = find_unit(sh, ctas, [&](const Found& g) { return (int)min((long)g.chunk * cta, (long)g.total); });
+    if (f.seq < 0) return false;
+    u = f.chunk * cta;
+    end = min(f.total, u + f.chunk);
+    at.seq = f.seq;
+    at.row_tile = f.row_tile;
+    enter(load_tree(sh, at.seq));
+    at.head = (u - f.start) / key_tiles;
+    item_start = f.start + at.head * key_tiles;
     share(cta);
     return true;
   }
+  __device__ __forceinline__ void enter(const Tree& t) {
+    at.first = t.first;
+    at.n = t.n;
+    at.ctx = t.ctx;
+    key_tiles = t.key_tiles;
+    lo_tile = t.lo_tile;
+  }
   __device__ __forceinline__ void share(int cta) {
-    head = at.item / t.row_tiles;
-    row_tile = at.item - head * t.row_tiles;
-    const long item_end = at.item_start + t.key_tiles;
-    const long stop = min(end, item_end);
-    kt_begin = t.lo_tile + at.key_tile;
-    kt_end = kt_begin + (int)(stop - u);
-    slot = at.key_tile == 0 ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
+    const int item_end = item_start + key_tiles, stop = min(end, item_end);
+    at.kt_begin = lo_tile + (u - item_start);
+    at.kt_end = at.kt_begin + (stop - u);
+    at.slot = u == item_start ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
   }
   __device__ __forceinline__ bool next(const Shape& sh, int cta) {
-    u += kt_end - kt_begin;
+    u += at.kt_end - at.kt_begin;
     if (u >= end) return false;
-    at.key_tile = 0;
-    at.item_start = u;
-    if (++at.item == t.row_tiles * sh.KVH) {
-      at.item = 0;
-      do {
-        ++at.seq;
+    item_start = u;
+    if (++at.head == sh.KVH) {
+      at.head = 0;
+      Tree t;
+      do {  // (there is such a tree: units are left)
+        if (++at.seq == sh.S) {
+          at.seq = 0;
+          ++at.row_tile;
+        }
         t = load_tree(sh, at.seq);
-      } while (t.n == 0);
+      } while (t.row_tiles <= at.row_tile);
+      enter(t);
     }
     share(cta);
     return true;

@@ -118,6 +118,10 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     # the tensor-core kernel is built for these head and page sizes; bfloat16 in others and float32 take the 32-bit kernel
     tensor_cores = code == L.BF16 and dim in (64, 128) and page_size in (8, 16, 32, 64) and num_pages > 0
     rows = TENSOR_CORE_ROWS if tensor_cores else FMA_ROWS
+    # a multiple of the row tiles that trees have: then those of one head read its keys at the same time
+    row_tiles = -(-max_nodes * (heads // kv_heads) // rows)
+    if row_tiles < ctas:
+        ctas -= ctas % row_tiles
     # scratch of this call alone (calls on several streams do not meet in it): two partial results for each CTA
     scratch = node_start.new_empty(2 * ctas * rows * (dim + 2))
     args = _ATTENTION.pack(
