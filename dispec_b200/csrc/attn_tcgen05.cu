@@ -40,7 +40,11 @@ using namespace tc;
 constexpr int D = DSP_HEAD_DIM;
 static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
 constexpr int BM = 128, BN = 64, THREADS = 384;
-constexpr int K_STAGES = 5, V_STAGES = 7;  // tiles in the ring of keys and in the ring of values
+// Tiles in the ring of keys and in the ring of values.  Even and odd key tiles have issuing warps of their own, each of which
+// waits for its own tiles only: with an even ring a slot's tiles all belong to one of them.  (With five slots a warp
+// whose tile landed before an older one of the other's could take a slot's last phase but one for the one it waits for.)
+constexpr int K_STAGES = 6, V_STAGES = 6;
+static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing warp");
 constexpr int BAD_SLOTS = 16;              // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 // warp 0: TMA, warps 1 and 11: issue S = Q K^T for softmax group 0 and 1, warps 2-9: softmax, warp 10: issues O += P V

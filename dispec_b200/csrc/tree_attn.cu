@@ -23,7 +23,7 @@ struct Args {
   const int *page_table, *depth;
   const unsigned long long* visible;
   void* out;
-  float *part_o, *part_ml;
+  TreeScratch scratch;
   long q_stride, out_stride;
   int pt_stride, words, D, page_size, num_pages;
   float scale;
@@ -59,8 +59,12 @@ tree_attn_kernel(const Args a) {
   __shared__ long slot_of_key[KEYS];
   const Shape& sh = a.sh;
   Walk w;
-  if (!w.begin(sh, cta, gridDim.x)) return;
+  if (!w.begin(sh, cta, gridDim.x)) {
+    if (tid == 0) a.scratch.splits[cta].parts = 0;
+    return;
+  }
   const int G = sh.G;
+  bool more;
   do {
     const Share& t = w.at;
     const int row0 = t.row_tile * ROWS, rows = min(ROWS, t.n * G - row0);
@@ -204,91 +208,90 @@ tree_attn_kernel(const Args a) {
         const float4 v = make_float4(acc[i][4 * c] * inv, acc[i][4 * c + 1] * inv, acc[i][4 * c + 2] * inv,
                                      acc[i][4 * c + 3] * inv);
         if (t.slot >= 0)
-          store4(a.part_o + ((size_t)t.slot * ROWS + r) * D + d, v);
+          store4(a.scratch.part_o + ((size_t)t.slot * ROWS + r) * D + d, v);
         else
           store4((T*)a.out + (size_t)(t.first + rr / G) * a.out_stride + (size_t)(t.head * G + rr % G) * D + d, v);
       }
       if (t.slot >= 0 && tx == 0)
-        reinterpret_cast<float2*>(a.part_ml)[(size_t)t.slot * ROWS + r] = make_float2(m[i] * 1.4426950408889634f, l[i]);
+        reinterpret_cast<float2*>(a.scratch.part_ml)[(size_t)t.slot * ROWS + r] = make_float2(m[i] * 1.4426950408889634f, l[i]);
     }
-  } while (w.next(sh, cta));
+    const Split split = w.split(sh, cta);
+    more = w.next(sh, cta);
+    if (!more && tid == 0) a.scratch.splits[cta] = split;
+  } while (more);
 }
 
-// Block (c, y): the item that begins in CTA c and ends in a later one, if there is one; four of its rows, one a warp.  Which
-// item that is does not depend on the kernel in front, so it is found out before the wait.  A lane holds the weights
-// of up to 32 partial results, and the outputs of eight are asked for together.
+// Every block makes out which CTAs began an item that others share (one read of the list, a thread each), and the warps of the
+// whole grid take those items' rows in turn.  A row's partial results are asked for eight at a time, maxima, sums and outputs
+// together: two latencies stand between the wait and the store.
+constexpr int COMBINE_THREADS = 256, COMBINE_WARPS = COMBINE_THREADS / 32, COMBINE_BLOCKS_PER_SM = 4;
 template <typename T>
-__global__ void __launch_bounds__(128)
-tree_combine_kernel(const Shape sh, const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                    T* __restrict__ out, long out_stride, int D, int ctas) {
-  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_BLOCKS_PER_SM)
+tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_stride, int G, int D, int R, int ctas) {
+  __shared__ int items[COMBINE_THREADS];  // CTAs that began one
+  __shared__ int of_warp[COMBINE_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
-  // last unit of CTA c
-  const Found f = find_unit(sh, ctas, [&](const Found& g) {
-    const long last = min((long)g.total, (long)g.chunk * (c + 1)) - 1;
-    return last + 1 >= g.total ? g.total : (int)last;  // (nothing follows the last CTA with work)
-  });
-  bool mine = f.seq >= 0;
-  int c_end = 0, head = 0, row0 = 0, rows = 0;
-  Tree t = {};
-  if (mine) {
-    t = load_tree(sh, f.seq);
-    const int last = f.chunk * (c + 1) - 1;
-    head = (last - f.start) / t.key_tiles;
-    const int begin = f.start + head * t.key_tiles, end = begin + t.key_tiles;
-    mine = end != last + 1 && begin >= f.chunk * c;  // it goes on, and began here
-    c_end = (end - 1) / f.chunk;
-    row0 = f.row_tile * sh.rows_per_tile;
-    rows = min(sh.rows_per_tile, t.n * sh.G - row0);
-  }
-  const int r = blockIdx.y * 4 + warp;
   pdl_wait();
-  if (!mine || r >= rows) return;
-  const float2* ml = reinterpret_cast<const float2*>(part_ml);
-  const int R = sh.rows_per_tile, parts = c_end - c + 1;
-  auto slot = [&](int k) -> size_t { return k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k); };  // of the k-th part
-  float M = -INFINITY, L = 0.f;
-  float2 mine_ml = make_float2(-INFINITY, 0.f);
-  for (int k = lane; k < parts; k += 32) {
-    const float2 v = ml[slot(k) * R + r];
-    if (k < 32) mine_ml = v;
-    M = fmaxf(M, v.x);
-  }
-  M = warp_max(M);
-  for (int k = lane; k < parts; k += 32) {
-    const float2 v = k < 32 ? mine_ml : ml[slot(k) * R + r];
-    if (v.x != -INFINITY) L += v.y * exp2f(v.x - M);
-  }
-  L = warp_sum(L);
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  const int rr = row0 + r;
-  T* dst = out + (size_t)(t.first + rr / sh.G) * out_stride + (size_t)(head * sh.G + rr % sh.G) * D;
-  for (int d0 = 0; d0 < D; d0 += 128) {  // the same trips for a whole warp (shuffles)
-    const int d = d0 + lane * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < parts; k0 += 8) {
-      float4 v[8];
-      float wk[8];
+  for (int c0 = 0; c0 < ctas; c0 += COMBINE_THREADS) {
+    const bool has = c0 + tid < ctas && scratch.splits[c0 + tid].parts > 0;
+    // the same list in every block: in the order of the CTAs
+    const uint32_t those = __ballot_sync(0xffffffffu, has);
+    __syncthreads();
+    if (lane == 0) of_warp[warp] = __popc(those);
+    __syncthreads();
+    int before = 0, n_items = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int part = k0 + k;
-        float m = -INFINITY;
-        if (part < 32)
-          m = __shfl_sync(0xffffffffu, mine_ml.x, part);
-        else if (part < parts)
-          m = ml[slot(part) * R + r].x;
-        wk[k] = part < parts && m != -INFINITY ? exp2f(m - M) : 0.f;
-        v[k] = wk[k] != 0.f && d < D ? load4(part_o + (slot(part) * R + r) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+    for (int w = 0; w < COMBINE_WARPS; ++w) {
+      before += w < warp ? of_warp[w] : 0;
+      n_items += of_warp[w];
+    }
+    if (has) items[before + __popc(those & ((1u << lane) - 1u))] = c0 + tid;
+    __syncthreads();
+    for (int i = blockIdx.x * COMBINE_WARPS + warp; i < n_items * R; i += gridDim.x * COMBINE_WARPS) {
+      // neighbouring warps take neighbouring rows
+      const int c = items[i / R], r = i % R;
+      const Split x = scratch.splits[c];
+      if (r >= x.rows) continue;
+      const float2* ml = reinterpret_cast<const float2*>(scratch.part_ml);
+      auto row_of = [&](int k) -> size_t { return (k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * R + r; };  // of the k-th part
+      const int rr = x.row0 + r;
+      T* dst = out + (size_t)(x.first + rr / G) * out_stride + (size_t)(x.head * G + rr % G) * D;
+      for (int d = lane * 4; d < D; d += 128) {
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < x.parts; k0 += 8) {
+          float4 v[8];
+          float2 p[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        acc.x = fmaf(wk[k], v[k].x, acc.x);
-        acc.y = fmaf(wk[k], v[k].y, acc.y);
-        acc.z = fmaf(wk[k], v[k].z, acc.z);
-        acc.w = fmaf(wk[k], v[k].w, acc.w);
+          for (int k = 0; k < 8; ++k) {
+            const size_t row = row_of(min(k0 + k, x.parts - 1));
+            p[k] = ml[row];
+            v[k] = load4(scratch.part_o + row * D + d);
+          }
+          float top = M;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= x.parts) p[k] = make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, p[k].x);
+          }
+          if (top == -INFINITY) continue;
+          const float w0 = exp2f(M - top);
+          L *= w0;
+          acc = make_float4(acc.x * w0, acc.y * w0, acc.z * w0, acc.w * w0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (p[k].x == -INFINITY) continue;  // a part that saw no key
+            const float w = exp2f(p[k].x - top);
+            L = fmaf(w, p[k].y, L);
+            acc = make_float4(fmaf(w, v[k].x, acc.x), fmaf(w, v[k].y, acc.y), fmaf(w, v[k].z, acc.z), fmaf(w, v[k].w, acc.w));
+          }
+          M = top;
+        }
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       }
     }
-    if (d < D) store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
 
@@ -304,18 +307,20 @@ int launch(const Args& a, int ctas, cudaStream_t stream) {
 }
 }  // namespace
 
-cudaError_t tree_combine(const tree::Shape& sh, const float* part_o, const float* part_ml, void* out, long out_stride,
-                         int D, int ctas, int dtype, cudaStream_t stream) {
-  const dim3 grid(ctas, (sh.rows_per_tile + 3) / 4);
-  return dtype == DSP_F32
-             ? launch_pdl(tree_combine_kernel<float>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (float*)out, out_stride, D, ctas)
-             : launch_pdl(tree_combine_kernel<bf16>, grid, dim3(128), 0, stream, sh, part_o, part_ml, (bf16*)out, out_stride, D, ctas);
+cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride, int G, int D, int rows_per_tile, int ctas,
+                         int dtype, cudaStream_t stream) {
+  const int sms = dsp_num_sms();
+  const dim3 grid((unsigned)min((long)ctas * rows_per_tile / COMBINE_WARPS, (long)(sms > 0 ? sms : 1) * COMBINE_BLOCKS_PER_SM));
+  return dtype == DSP_F32 ? launch_pdl(tree_combine_kernel<float>, grid, dim3(COMBINE_THREADS), 0, stream, scratch, (float*)out,
+                                       out_stride, G, D, rows_per_tile, ctas)
+                          : launch_pdl(tree_combine_kernel<bf16>, grid, dim3(COMBINE_THREADS), 0, stream, scratch, (bf16*)out,
+                                       out_stride, G, D, rows_per_tile, ctas);
 }
 
 // The same for kernels that live in other libraries.
-extern "C" int dsp_tree_combine(const tree::Shape* sh, const float* part_o, const float* part_ml, void* out, long out_stride,
-                                int D, int ctas, int dtype, cudaStream_t stream) {
-  return tree_combine(*sh, part_o, part_ml, out, out_stride, D, ctas, dtype, stream) == cudaSuccess ? 0 : 1;
+extern "C" int dsp_tree_combine(const TreeScratch* scratch, void* out, long out_stride, int G, int D, int rows_per_tile,
+                                int ctas, int dtype, cudaStream_t stream) {
+  return tree_combine(*scratch, out, out_stride, G, D, rows_per_tile, ctas, dtype, stream) == cudaSuccess ? 0 : 1;
 }
 
 // What the Python side packs, in this order (ops/tree.py).
@@ -356,8 +361,7 @@ extern "C" int dsp_tree_attention(const DspTreeAttention* p, cudaStream_t stream
   a.depth = p->depth;
   a.visible = p->visible;
   a.out = p->out;
-  a.part_o = p->scratch;
-  a.part_ml = p->scratch + 2 * p->ctas * ROWS * p->D;
+  a.scratch = tree_scratch(p->scratch, p->ctas, ROWS, p->D);
   a.q_stride = p->q_stride;
   a.out_stride = p->out_stride;
   a.pt_stride = (int)p->pt_stride;
@@ -370,7 +374,7 @@ extern "C" int dsp_tree_attention(const DspTreeAttention* p, cudaStream_t stream
   DSP_REQUIRE(a.err != nullptr, "dsp_tree_attention: no device error word");
   const int rc = p->dtype == DSP_F32 ? launch<float>(a, (int)p->ctas, stream) : launch<bf16>(a, (int)p->ctas, stream);
   if (rc != 0) return rc;
-  DSP_CUDA(tree_combine(a.sh, a.part_o, a.part_ml, a.out, a.out_stride, a.D, (int)p->ctas, (int)p->dtype, stream));
+  DSP_CUDA(tree_combine(a.scratch, a.out, a.out_stride, a.sh.G, a.D, ROWS, (int)p->ctas, (int)p->dtype, stream));
   DSP_CHECK_LAUNCH("dsp_tree_attention");
   return 0;
 }

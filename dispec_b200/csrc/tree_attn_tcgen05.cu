@@ -10,9 +10,9 @@
 //   warp 10     issues the output products;
 //   warps 2..9  two softmax groups of four warps: group g owns the key tiles g, g + 2, ... of a share with a score buffer,
 //               output accumulator, P, running maximum and sum of its own; thread r of a group owns row r.
-// The whole block meets once a share.  Behind that barrier group 0 merges the two halves and stores the rows (or leaves a
-// partial result) while group 1 brings the next share's queries; warp 0 has worked the next share out and asked for its
-// first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
+// The whole block meets once a share.  Behind that barrier the softmax warps ask for the next share's queries, merge the two
+// halves of the last one and store its rows (or leave a partial result); warp 0 has worked the next share out and asked for
+// its first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
 // its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output
 // product.  Every wait is bounded; one that runs out sets the device error word.
 #include "tcgen05_common.cuh"
@@ -60,7 +60,7 @@ struct Params {
   const int *page_table, *depth;
   const unsigned long long* visible;
   bf16* out;
-  float *part_o, *part_ml;
+  TreeScratch scratch;
   long q_stride, out_stride;
   int pt_stride, words, page_size, num_pages;
   int page_runs;  // the run maps are valid
@@ -125,7 +125,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ __align__(8) uint64_t p_full[2], o_done[2];  // P written, O rescaled, V rows zeroed; the output product is complete
   __shared__ __align__(8) uint64_t q_ready[2];            // the queries of a share with tiles for the group are in tensor memory
   __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
-  __shared__ float merge_m[2][BM], merge_l[2][BM];        // group 1's maximum and sum per row, by share in turn
+  __shared__ float2 merge_ml[2][2][BM];                   // a group's maximum and sum per row, by share in turn
   __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 before the barrier in front of it
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;        // a wait ran out
@@ -146,6 +146,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     if (lane == 0) {
       if (!more) w.at.seq = -1;
       shares[0] = w.at;
+      p.scratch.splits[cta].parts = 0;  // (stays where there is no work, or a wait runs out)
     }
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -167,9 +168,9 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       mbar_init(&p_full[b], 4);
       mbar_init(&o_done[b], 1);
     }
-    mbar_init(&q_ready[0], 4);
-    mbar_init(&q_ready[1], 4);
-    mbar_init(&o_free, 4);
+    mbar_init(&q_ready[0], D == 128 ? 8 : 4);
+    mbar_init(&q_ready[1], D == 128 ? 8 : 4);
+    mbar_init(&o_free, 8);
     failed = 0;
     failed_share = 0x7fffffff;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -299,28 +300,28 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     }
   };
 
-  // The queries of a share, by the warps of group 1: row r of the tile, lane r, two bfloat16 per column (rows past the item
-  // are zero).
-  auto bring_queries = [&](const Share& t) {
+  // The queries of a share: row r of the tile, lane r, two bfloat16 per column (rows past the item are zero).  In heads of 128
+  // each group brings half of the columns, in heads of 64 group 1 brings them all.  Asked for first, put down later.
+  constexpr int Q_PIECES = 8;  // of 16 bytes, a lane
+  auto ask_queries = [&](const Share& t, uint4 (&x)[Q_PIECES]) {
     const int rr = t.row_tile * BM + r;
     const bool valid = rr < t.n * G;
-    const uint4* src = reinterpret_cast<const uint4*>(p.q);
-    if (valid)
-      src = reinterpret_cast<const uint4*>(p.q + (size_t)(t.first + rr / G) * p.q_stride + (size_t)(t.head * G + rr % G) * D);
+    const bf16* src = p.q;
+    if (valid) src += (size_t)(t.first + rr / G) * p.q_stride + (size_t)(t.head * G + rr % G) * D + (D == 128 ? g * 64 : 0);
 #pragma unroll
-    for (int c0 = 0; c0 < D / 2; c0 += 32) {
-      uint32_t x[32];
+    for (int c = 0; c < Q_PIECES; ++c) x[c] = valid ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+  };
+  auto put_queries = [&](const Share& t, const uint4 (&x)[Q_PIECES]) {
+    uint32_t y[32];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint4 v = valid ? __ldg(src + c0 / 4 + c) : make_uint4(0, 0, 0, 0);
-        x[4 * c] = v.x;
-        x[4 * c + 1] = v.y;
-        x[4 * c + 2] = v.z;
-        x[4 * c + 3] = v.w;
-      }
-      __syncwarp();
-      tmem_st32(lane_addr + (uint32_t)(Q_COL + c0), x);
+    for (int c = 0; c < Q_PIECES; ++c) {
+      y[4 * c] = x[c].x;
+      y[4 * c + 1] = x[c].y;
+      y[4 * c + 2] = x[c].z;
+      y[4 * c + 3] = x[c].w;
     }
+    __syncwarp();
+    tmem_st32(lane_addr + (uint32_t)(Q_COL + (D == 128 ? g * 32 : 0)), y);
     tmem_st_wait();
     tc_fence_before();
     __syncwarp();
@@ -330,29 +331,29 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     }
   };
 
-  // By the warps of group 0, behind the barrier of share k: merges the two groups' halves and stores the rows, or the partial
-  // result of the share.
+  // Behind the barrier of share k: merges the two groups' halves and stores the rows, or the partial result of the share; each
+  // group has half of the columns.
   auto finish = [&](int k) {
     const Share& t = shares[k % SHARES];
     const int row0 = t.row_tile * BM, nrows = min(BM, t.n * G - row0), slot = t.slot;
     const bool row_ok = r < nrows;
     const bool two = t.kt_end - t.kt_begin > 1;
-    const float m1 = two ? merge_m[k & 1][r] : -INFINITY, l1 = two ? merge_l[k & 1][r] : 0.f;
-    const float M = fmaxf(m_run, m1);
-    const float w0 = m_run == -INFINITY ? 0.f : ex2(m_run - M);
-    const float w1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-    const float denom = l_run * w0 + l1 * w1;
+    const float2 ml0 = merge_ml[k & 1][0][r], ml1 = two ? merge_ml[k & 1][1][r] : make_float2(-INFINITY, 0.f);
+    const float M = fmaxf(ml0.x, ml1.x);
+    const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - M);
+    const float w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - M);
+    const float denom = ml0.y * w0 + ml1.y * w1;
     const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
       bf16* dst = p.out;
-      float* part = p.part_o;
+      float* part = p.scratch.part_o;
       if (slot >= 0)
         part += ((size_t)slot * BM + r) * D;
       else if (row_ok)
         dst += (size_t)(t.first + (row0 + r) / G) * p.out_stride + (size_t)(t.head * G + (row0 + r) % G) * D;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      for (int c0 = g * (D / 2); c0 < (g + 1) * (D / 2); c0 += 32) {
         uint32_t ov[32], ow[32];
         __syncwarp();
         tmem_ld32(lane_addr + (uint32_t)(O_COL + c0), ov);
@@ -383,7 +384,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         }
         __syncwarp();
       }
-      if (slot >= 0 && row_ok) reinterpret_cast<float2*>(p.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
+      if (g == 0 && slot >= 0 && row_ok) reinterpret_cast<float2*>(p.scratch.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
     }
     tc_fence_before();
     __syncwarp();
@@ -398,9 +399,13 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const int n_kt = t.kt_end - t.kt_begin;
     if (warp == 0) {
       request(t, n_kt, done);
+      const Split split = w.split(sh, cta);
       more = w.next(sh, cta);
       if (lane == 0) {
-        if (!more) w.at.seq = -1;
+        if (!more) {
+          w.at.seq = -1;
+          p.scratch.splits[cta] = split;
+        }
         shares[(share + 1) % SHARES] = w.at;
       }
       asked = 0;
@@ -464,11 +469,14 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       if (!ok) give_up(share);
     } else {
-      // ---- softmax groups: first the end of the last share, or the queries of this one
-      if (g == 1)
-        bring_queries(t);
-      else if (share > 0)
-        finish(share - 1);
+      // ---- softmax groups: first the queries of this share, and the end of the last one while they come
+      {
+        uint4 x[Q_PIECES];
+        const bool brings = D == 128 || g == 1;
+        if (brings) ask_queries(t, x);
+        if (share > 0) finish(share - 1);
+        if (brings) put_queries(t, x);
+      }
       const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
       const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
       const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
@@ -597,10 +605,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       // the group's last product of the share
       if (ok && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) ok = false;
       if (!ok) give_up(share);
-      if (g == 1) {
-        merge_m[share & 1][r] = m_run;
-        merge_l[share & 1][r] = l_run;
-      }
+      merge_ml[share & 1][g][r] = make_float2(m_run, l_run);
     }
     done += n_kt;
     __syncwarp();
@@ -610,7 +615,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     __syncwarp();
   }
   pdl_launch_dependents();
-  if (share > 0 && failed_share >= share && warp >= 2 && warp < 6) finish(share - 1);
+  if (share > 0 && failed_share >= share && warp >= 2 && warp < PV_WARP) finish(share - 1);
 
   tc_fence_before();
   __syncthreads();
@@ -640,7 +645,7 @@ struct DspTreeAttention {
   long q_stride, out_stride, pt_stride, words, S, H, KVH, D, page_size, num_pages, window, dtype, ctas;
   double scale;
 };
-typedef int (*TreeCombine)(const Shape*, const float*, const float*, void*, long, int, int, int, cudaStream_t);
+typedef int (*TreeCombine)(const TreeScratch*, void*, long, int, int, int, int, int, cudaStream_t);
 
 extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTreeAttention* a, void* combine, int* err,
                                                                    cudaStream_t stream) {
@@ -666,8 +671,7 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
   p.depth = a->depth;
   p.visible = a->visible;
   p.out = (bf16*)a->out;
-  p.part_o = a->scratch;
-  p.part_ml = a->scratch + 2 * a->ctas * BM * D;
+  p.scratch = tree_scratch(a->scratch, a->ctas, BM, D);
   p.q_stride = a->q_stride;
   p.out_stride = a->out_stride;
   p.pt_stride = (int)a->pt_stride;
@@ -696,5 +700,5 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
   if (launch_pdl(tree_attn_tcgen05_kernel, dim3((unsigned)a->ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, p, map_k, map_v,
                  runs_k, runs_v) != cudaSuccess)
     return 1;
-  return reinterpret_cast<TreeCombine>(combine)(&p.sh, p.part_o, p.part_ml, p.out, p.out_stride, D, (int)a->ctas, DSP_BF16, stream);
+  return reinterpret_cast<TreeCombine>(combine)(&p.scratch, p.out, p.out_stride, p.sh.G, D, BM, (int)a->ctas, DSP_BF16, stream);
 }

@@ -64,50 +64,71 @@ __device__ __forceinline__ int warp_scan(int v) {
 struct Found {
   int total, chunk;         // all units; units a CTA takes (the same number for all, at least min_units)
   int seq, row_tile, start; // the tree (-1: there is no such unit), the row tile, first unit of that tree in that row tile
+  Tree tree;
 };
-// Called by whole warps.  `pick` names the unit once total and chunk are known.  The trees of up to 32 requests are read once.
+// Called by whole warps.  `pick` names the unit once total and chunk are known.  The trees of up to 64 requests are read once.
 template <typename Pick>
 __device__ __forceinline__ Found find_unit(const Shape& sh, int ctas, Pick pick) {
+  constexpr int HELD = 2;
   const int lane = threadIdx.x & 31;
-  Found f = {0, 0, -1, 0, 0};
-  int mine = 0, held = 0, held_tiles = 0;
-  for (int s = lane; s < sh.S; s += 32) {
-    const Tree t = load_tree(sh, s);
-    held = units_of(sh, t);
-    held_tiles = t.row_tiles;
-    mine += held * held_tiles;
+  Found f = {0, 0, -1, 0, 0, {}};
+  Tree held[HELD];
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    held[k] = {};
+    if (k * 32 + lane < sh.S) held[k] = load_tree(sh, k * 32 + lane);
   }
-  auto units = [&](int s, int tile) -> int {  // of lane's tree s in a row tile
-    if (s >= sh.S) return 0;
-    if (sh.S <= 32) return held_tiles > tile ? held : 0;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) mine += units_of(sh, held[k]) * held[k].row_tiles;
+  for (int s = HELD * 32 + lane; s < sh.S; s += 32) {
     const Tree t = load_tree(sh, s);
-    return t.row_tiles > tile ? units_of(sh, t) : 0;
-  };
+    mine += units_of(sh, t) * t.row_tiles;
+  }
   f.total = warp_sum_int(mine);
   f.chunk = max((f.total + ctas - 1) / ctas, sh.min_units);
   const int u = pick(f);
   if (u >= f.total) return f;
+  // of lane's tree of the k-th 32 in a row tile
+  auto units = [&](const Tree& t, int tile) -> int { return t.row_tiles > tile ? units_of(sh, t) : 0; };
   int before = 0;
   for (int tile = 0;; ++tile) {
     int of_tile = 0;
-    for (int s = lane; s < sh.S; s += 32) of_tile += units(s, tile);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) of_tile += units(held[k], tile);
+    for (int s = HELD * 32 + lane; s < sh.S; s += 32) of_tile += units(load_tree(sh, s), tile);
     of_tile = warp_sum_int(of_tile);
     if (u >= before + of_tile) {
       before += of_tile;
       continue;  // (ends: u is below the total)
     }
-    for (int s0 = 0; s0 < sh.S; s0 += 32) {
-      const int n = units(s0 + lane, tile);
+    auto look = [&](const Tree& t, int s0) -> bool {
+      const int n = units(t, tile);
       const int upto = before + warp_scan(n);
       const uint32_t past = __ballot_sync(0xffffffffu, upto > u);
-      if (past != 0u) {
-        const int who = __ffs(past) - 1;
-        f.seq = s0 + who;
-        f.row_tile = tile;
-        f.start = __shfl_sync(0xffffffffu, upto - n, who);
-        return f;
+      if (past == 0u) {
+        before = __shfl_sync(0xffffffffu, upto, 31);
+        return false;
       }
-      before = __shfl_sync(0xffffffffu, upto, 31);
+      const int who = __ffs(past) - 1;
+      f.seq = s0 + who;
+      f.row_tile = tile;
+      f.start = __shfl_sync(0xffffffffu, upto - n, who);
+      f.tree.first = __shfl_sync(0xffffffffu, t.first, who);
+      f.tree.n = __shfl_sync(0xffffffffu, t.n, who);
+      f.tree.ctx = __shfl_sync(0xffffffffu, t.ctx, who);
+      f.tree.lo_tile = __shfl_sync(0xffffffffu, t.lo_tile, who);
+      f.tree.key_tiles = __shfl_sync(0xffffffffu, t.key_tiles, who);
+      f.tree.row_tiles = __shfl_sync(0xffffffffu, t.row_tiles, who);
+      return true;
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (look(held[k], k * 32)) return f;
+    for (int s0 = HELD * 32; s0 < sh.S; s0 += 32) {
+      Tree t = {};
+      if (s0 + lane < sh.S) t = load_tree(sh, s0 + lane);
+      if (look(t, s0)) return f;
     }
     return f;
   }
@@ -121,9 +142,16 @@ struct Share {
   int slot;                // scratch slot of the partial result, -1: the item is finished here
 };
 
+// The item that begins in a CTA and ends in a later one, for the kernel that merges its partial results: written by that CTA.
+struct Split {
+  int parts;                  // CTAs that have a part (0: there is no such item)
+  int first, row0, rows, head;
+  int unused[3];
+};
+
 // A CTA's walk over its run of units, one item's share at a time.
 struct Walk {
-  int u, end;
+  int u, end, chunk;
   int item_start, key_tiles, lo_tile;
   Share at;
 
@@ -131,11 +159,12 @@ struct Walk {
   __device__ __forceinline__ bool begin(const Shape& sh, int cta, int ctas) {
     const Found f = find_unit(sh, ctas, [&](const Found& g) { return (int)min((long)g.chunk * cta, (long)g.total); });
     if (f.seq < 0) return false;
-    u = f.chunk * cta;
-    end = min(f.total, u + f.chunk);
+    chunk = f.chunk;
+    u = chunk * cta;
+    end = min(f.total, u + chunk);
     at.seq = f.seq;
     at.row_tile = f.row_tile;
-    enter(load_tree(sh, at.seq));
+    enter(f.tree);
     at.head = (u - f.start) / key_tiles;
     item_start = f.start + at.head * key_tiles;
     share(cta);
@@ -153,6 +182,18 @@ struct Walk {
     at.kt_begin = lo_tile + (u - item_start);
     at.kt_end = at.kt_begin + (stop - u);
     at.slot = u == item_start ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
+  }
+  // What the merging kernel has to know of the present share (of the last one of the run, if that is an item's beginning).
+  __device__ __forceinline__ Split split(const Shape& sh, int cta) const {
+    Split x = {};
+    if (at.slot == 2 * cta + 1) {
+      x.parts = (item_start + key_tiles - 1) / chunk - cta + 1;
+      x.first = at.first;
+      x.row0 = at.row_tile * sh.rows_per_tile;
+      x.rows = min(sh.rows_per_tile, at.n * sh.G - x.row0);
+      x.head = at.head;
+    }
+    return x;
   }
   __device__ __forceinline__ bool next(const Shape& sh, int cta) {
     u += at.kt_end - at.kt_begin;
@@ -177,7 +218,20 @@ struct Walk {
 
 }  // namespace tree
 
-// Merges the partial results of the items that several CTAs share (tree_attn.cu).  part_o: [slot][rows_per_tile][D],
-// part_ml: [slot][rows_per_tile] of (maximum in the base-2 domain, sum).
-cudaError_t tree_combine(const tree::Shape& sh, const float* part_o, const float* part_ml, void* out, long out_stride,
-                         int D, int ctas, int dtype, cudaStream_t stream);
+// Scratch of a call: part_o [2 ctas][rows_per_tile][D] floats, part_ml [2 ctas][rows_per_tile] pairs (maximum in the base-2
+// domain, sum), splits [ctas].
+struct TreeScratch {
+  float *part_o, *part_ml;
+  tree::Split* splits;
+};
+inline TreeScratch tree_scratch(float* scratch, long ctas, long rows_per_tile, long D) {
+  TreeScratch s;
+  s.part_o = scratch;
+  s.part_ml = s.part_o + 2 * ctas * rows_per_tile * D;
+  s.splits = reinterpret_cast<tree::Split*>(s.part_ml + 4 * ctas * rows_per_tile);
+  return s;
+}
+
+// Merges the partial results of the items that several CTAs share (tree_attn.cu).
+cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride, int G, int D, int rows_per_tile, int ctas,
+                         int dtype, cudaStream_t stream);

@@ -122,8 +122,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     row_tiles = -(-max_nodes * (heads // kv_heads) // rows)
     if row_tiles < ctas:
         ctas -= ctas % row_tiles
-    # scratch of this call alone (calls on several streams do not meet in it): two partial results for each CTA
-    scratch = node_start.new_empty(2 * ctas * rows * (dim + 2))
+    # scratch of this call alone (calls on several streams do not meet in it): two partial results for each CTA, and what
+    # the merge has to know of it
+    scratch = node_start.new_empty(2 * ctas * rows * (dim + 2) + 8 * ctas)
     args = _ATTENTION.pack(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ctx_len.data_ptr(), node_start.data_ptr(),
         0 if depth is None else depth.data_ptr(), visible.data_ptr(), out.data_ptr(), scratch.data_ptr(), q.stride(0),
