@@ -4,8 +4,8 @@
 // pairs, G heads a node) of one key/value head of one tree; it walks the key tiles from the first key that any of its
 // tree's nodes sees to the tree's last node.  A unit is one key tile of one item.  All units, in the order (row tile, tree,
 // head, key tile), are cut into equal runs, one per CTA, wherever that falls: trees of any lengths load every SM alike, and
-// nothing about lengths is needed on the host.  Where all trees have R row tiles and the number of CTAs is a multiple of R, the
-// CTAs c, c + ctas / R, ... walk the same keys at the same time, which then come from memory once and from the L2
+// nothing about lengths is needed on the host.  Where all trees have R row tiles, each row tile's runs are cut alike and
+// the CTAs c, c + ctas / R, ... walk the same keys at the same time, which then come from memory once and from the L2
 // for the others (64 trees of 320 rows, whose row tiles followed one another in one CTA: 1.28 GB read where
 // the keys and values are 0.42).
 //
@@ -60,35 +60,71 @@ __device__ __forceinline__ int warp_scan(int v) {
   return v;
 }
 
-// Where a unit lies.
+// How the units are cut into runs, one per CTA.
+struct Cut {
+  int total, chunk;   // all units; units of a run (at least min_units)
+  int of_first;       // units of the first row tile
+  int per_row_tile;   // > 0: so many CTAs for each row tile, whose runs begin and end with it
+  __device__ __forceinline__ int begin(int cta) const {
+    if (per_row_tile == 0) return (int)min((long)chunk * cta, (long)total);
+    const int tile = cta / per_row_tile;
+    return min(tile * of_first + (cta - tile * per_row_tile) * chunk, (tile + 1) * of_first);
+  }
+  __device__ __forceinline__ int end(int cta) const {
+    if (per_row_tile == 0) return (int)min((long)chunk * (cta + 1), (long)total);
+    const int tile = cta / per_row_tile;
+    return min(tile * of_first + (cta - tile * per_row_tile + 1) * chunk, (tile + 1) * of_first);
+  }
+  __device__ __forceinline__ int owner(int u) const {
+    if (per_row_tile == 0) return u / chunk;
+    const int tile = u / of_first;
+    return tile * per_row_tile + (u - tile * of_first) / chunk;
+  }
+};
+// Where a CTA's run begins.
 struct Found {
-  int total, chunk;         // all units; units a CTA takes (the same number for all, at least min_units)
-  int seq, row_tile, start; // the tree (-1: there is no such unit), the row tile, first unit of that tree in that row tile
+  Cut cut;
+  int seq, row_tile, start; // the tree (-1: the run is empty), the row tile, first unit of that tree in that row tile
   Tree tree;
 };
-// Called by whole warps.  `pick` names the unit once total and chunk are known.  The trees of up to 64 requests are read once.
-template <typename Pick>
-__device__ __forceinline__ Found find_unit(const Shape& sh, int ctas, Pick pick) {
+// Called by whole warps.  The trees of up to 64 requests are read once.
+__device__ __forceinline__ Found find_run(const Shape& sh, int cta, int ctas) {
   constexpr int HELD = 2;
   const int lane = threadIdx.x & 31;
-  Found f = {0, 0, -1, 0, 0, {}};
+  Found f = {};
+  f.seq = -1;
   Tree held[HELD];
-  int mine = 0;
+  int all = 0, of_first = 0, most = 0;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     held[k] = {};
     if (k * 32 + lane < sh.S) held[k] = load_tree(sh, k * 32 + lane);
   }
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) mine += units_of(sh, held[k]) * held[k].row_tiles;
+  for (int k = 0; k < HELD; ++k) {
+    all += units_of(sh, held[k]) * held[k].row_tiles;
+    of_first += units_of(sh, held[k]);
+    most = max(most, held[k].row_tiles);
+  }
   for (int s = HELD * 32 + lane; s < sh.S; s += 32) {
     const Tree t = load_tree(sh, s);
-    mine += units_of(sh, t) * t.row_tiles;
+    all += units_of(sh, t) * t.row_tiles;
+    of_first += units_of(sh, t);
+    most = max(most, t.row_tiles);
   }
-  f.total = warp_sum_int(mine);
-  f.chunk = max((f.total + ctas - 1) / ctas, sh.min_units);
-  const int u = pick(f);
-  if (u >= f.total) return f;
+  Cut& cut = f.cut;
+  cut.total = warp_sum_int(all);
+  if (cut.total == 0) return f;
+  cut.of_first = warp_sum_int(of_first);
+  // the same number of row tiles in all trees (no tree has more, and their units add up to it): each gets as many CTAs
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  cut.per_row_tile = most > 1 && most <= ctas && (long)most * cut.of_first == cut.total ? ctas / most : 0;
+  cut.chunk = cut.per_row_tile > 0 ? (cut.of_first + cut.per_row_tile - 1) / cut.per_row_tile : (cut.total + ctas - 1) / ctas;
+  cut.chunk = max(cut.chunk, sh.min_units);
+  if (cut.per_row_tile > 0 && cta >= cut.per_row_tile * most) return f;
+  const int u = cut.begin(cta);
+  if (u >= cut.end(cta)) return f;
   // of lane's tree of the k-th 32 in a row tile
   auto units = [&](const Tree& t, int tile) -> int { return t.row_tiles > tile ? units_of(sh, t) : 0; };
   int before = 0;
@@ -151,17 +187,18 @@ struct Split {
 
 // A CTA's walk over its run of units, one item's share at a time.
 struct Walk {
-  int u, end, chunk;
+  int u, end;
+  Cut cut;
   int item_start, key_tiles, lo_tile;
   Share at;
 
   // Called by whole warps.  False: this CTA has no work.
   __device__ __forceinline__ bool begin(const Shape& sh, int cta, int ctas) {
-    const Found f = find_unit(sh, ctas, [&](const Found& g) { return (int)min((long)g.chunk * cta, (long)g.total); });
+    const Found f = find_run(sh, cta, ctas);
     if (f.seq < 0) return false;
-    chunk = f.chunk;
-    u = chunk * cta;
-    end = min(f.total, u + chunk);
+    cut = f.cut;
+    u = cut.begin(cta);
+    end = cut.end(cta);
     at.seq = f.seq;
     at.row_tile = f.row_tile;
     enter(f.tree);
@@ -187,7 +224,7 @@ struct Walk {
   __device__ __forceinline__ Split split(const Shape& sh, int cta) const {
     Split x = {};
     if (at.slot == 2 * cta + 1) {
-      x.parts = (item_start + key_tiles - 1) / chunk - cta + 1;
+      x.parts = cut.owner(item_start + key_tiles - 1) - cta + 1;
       x.first = at.first;
       x.row0 = at.row_tile * sh.rows_per_tile;
       x.rows = min(sh.rows_per_tile, at.n * sh.G - x.row0);
