@@ -100,6 +100,24 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const S
   return stored | drafted;
 }
 
+// a * b + c and a + b of two numbers at once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Multiplies a row's accumulators by alpha.
 __device__ __forceinline__ void rescale(uint32_t o_addr, float alpha) {
 #pragma unroll 1
@@ -531,33 +549,33 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           }
           float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            t0 = fmaxf(t0, __uint_as_float(a[c]));
-            t1 = fmaxf(t1, __uint_as_float(a[c + 1]));
-            t2 = fmaxf(t2, __uint_as_float(b[c]));
-            t3 = fmaxf(t3, __uint_as_float(b[c + 1]));
+          for (int c = 0; c < 32; c += 4) {
+            t0 = fmaxf(t0, fmaxf(__uint_as_float(a[c]), __uint_as_float(a[c + 1])));
+            t1 = fmaxf(t1, fmaxf(__uint_as_float(a[c + 2]), __uint_as_float(a[c + 3])));
+            t2 = fmaxf(t2, fmaxf(__uint_as_float(b[c]), __uint_as_float(b[c + 1])));
+            t3 = fmaxf(t3, fmaxf(__uint_as_float(b[c + 2]), __uint_as_float(b[c + 3])));
           }
           const float tmax = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;  // the scale is positive
           const float m_new = (tmax > m_run + RESCALE_STEP || m_run == -INFINITY) ? fmaxf(tmax, m_run) : m_run;
           const float alpha = m_new == m_run ? 1.f : ex2(m_run - m_new);  // 0 on a row's first visible tile
           m_run = m_new;
           const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
-          float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+          // two scores an instruction where there is one for it
+          const float2 scale2 = make_float2(scale, scale), neg_m2 = make_float2(neg_m, neg_m);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
           uint32_t pk[32];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float e0 = ex2(fmaf(__uint_as_float(a[c]), scale, neg_m));
-            const float e1 = ex2(fmaf(__uint_as_float(a[c + 1]), scale, neg_m));
-            const float e2 = ex2(fmaf(__uint_as_float(b[c]), scale, neg_m));
-            const float e3 = ex2(fmaf(__uint_as_float(b[c + 1]), scale, neg_m));
-            a0 += e0;
-            a1 += e1;
-            a2 += e2;
-            a3 += e3;
-            pk[c / 2] = pack2(e0, e1);
-            pk[16 + c / 2] = pack2(e2, e3);
+            const float2 x = fma2(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), scale2, neg_m2);
+            const float2 y = fma2(make_float2(__uint_as_float(b[c]), __uint_as_float(b[c + 1])), scale2, neg_m2);
+            const float2 ex = make_float2(ex2(x.x), ex2(x.y)), ey = make_float2(ex2(y.x), ex2(y.y));
+            sum0 = add2(sum0, ex);
+            sum1 = add2(sum1, ey);
+            pk[c / 2] = pack2(ex.x, ex.y);
+            pk[16 + c / 2] = pack2(ey.x, ey.y);
           }
-          l_run = l_run * alpha + ((a0 + a1) + (a2 + a3));
+          sum0 = add2(sum0, sum1);
+          l_run = l_run * alpha + (sum0.x + sum0.y);
           // the group's previous O[g] += P V must be complete before O[g] is rescaled and P[g] rewritten
           if (j > 0) {
             if (!__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
