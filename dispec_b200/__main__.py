@@ -10,6 +10,7 @@ tokenizer is not part of the engine.
 
     generate        generate from prompts given as token ids (--model DIR, or --random CONFIG for
                     random weights filled on the device)
+    speculate       the same with drafted trees: several tokens a request checked in one pass
     random          write a model folder with random weights from a config.json and a seed
     replay          feed given token ids step by step and write logits (the program of bin/trace_run)
     throughput      continuous-batching throughput at several concurrency levels
@@ -46,14 +47,18 @@ def _engine_args(ap, random_weights=False):
     ap.add_argument("--device", default="cuda:0")
 
 
-def _make_engine(args):
-    from dispec_b200 import ContinuousBatchingEngine, KVConfig, load_model
+def _make_model(args):
     if getattr(args, "random", None):
         from dispec_b200 import load_model_config, load_random_model
         seed = args.seed if args.weights_seed is None else args.weights_seed
-        model = load_random_model(load_model_config(args.random), seed, args.std, args.dtype, args.device)
-    else:
-        model = load_model(args.model, args.dtype, args.device)
+        return load_random_model(load_model_config(args.random), seed, args.std, args.dtype, args.device)
+    from dispec_b200 import load_model
+    return load_model(args.model, args.dtype, args.device)
+
+
+def _make_engine(args):
+    from dispec_b200 import ContinuousBatchingEngine, KVConfig
+    model = _make_model(args)
     return ContinuousBatchingEngine(model, KVConfig(block_size=args.block_size), num_blocks=args.num_blocks,
                                     max_batch_tokens=args.max_batch_tokens, chunk_size=args.chunk_size,
                                     cuda_graph=not args.no_cuda_graph), model
@@ -96,6 +101,24 @@ def cmd_generate(args) -> int:
     n = sum(len(out[r]) for r in ids)
     print(f"# {n} tokens in {dt:.3f}s ({n / dt:.1f} tok/s), {engine.num_steps} steps, "
           f"{engine.num_preemptions} preemptions", file=sys.stderr)
+    return 0
+
+
+def cmd_speculate(args) -> int:
+    from dispec_b200 import KVConfig, SamplingParams, SpeculativeEngine
+    model = _make_model(args)
+    prompts = _parse_prompts(args, model.spec.vocab_size)
+    engine = SpeculativeEngine(model, KVConfig(block_size=args.block_size), num_blocks=args.num_blocks, max_nodes=args.max_nodes,
+                               max_num_seqs=max(1, len(prompts)))
+    params = [SamplingParams(args.temperature, seed=args.seed + i) for i in range(len(prompts))]
+    t0 = time.perf_counter()
+    out = engine.generate(prompts, args.max_new, params, args.eos_id)
+    dt = time.perf_counter() - t0
+    for i, (p, o) in enumerate(zip(prompts, out)):
+        print(json.dumps({"id": i, "prompt_tokens": len(p), "output_ids": o}))
+    n = sum(len(o) for o in out)
+    print(f"# {n} tokens in {dt:.3f}s ({n / dt:.1f} tok/s), {engine.num_steps} steps over trees of up to {args.max_nodes} nodes, "
+          f"{engine.num_accepted / max(1, engine.num_steps):.2f} tokens a step", file=sys.stderr)
     return 0
 
 
@@ -179,6 +202,18 @@ def main(argv=None) -> int:
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--eos-id", type=int, default=None, help="stop a request after this token")
     g.set_defaults(fn=cmd_generate)
+
+    sp = sub.add_parser("speculate", help="generate with drafts looked up in the request's own tokens")
+    _engine_args(sp, random_weights=True)
+    sp.add_argument("--prompt-ids", action="append", help="one prompt as token ids: '5,17,3' (repeatable)")
+    sp.add_argument("--prompt-file", help="one prompt per line: ids separated by spaces/commas, or a JSON list")
+    sp.add_argument("--random-prompts", type=int, nargs="+", help="lengths of uniform random prompts")
+    sp.add_argument("--max-new", type=int, default=256, help="new tokens per request (max_new_tokens)")
+    sp.add_argument("--max-nodes", type=int, default=16, help="nodes of a drafted tree, the root among them")
+    sp.add_argument("--temperature", type=float, default=0.0, help="0 means greedy")
+    sp.add_argument("--seed", type=int, default=0)
+    sp.add_argument("--eos-id", type=int, default=None, help="stop a request after this token")
+    sp.set_defaults(fn=cmd_speculate)
 
     r = sub.add_parser("random", help="write a model folder with random weights")
     r.add_argument("--config", required=True, help="a config.json (or a folder holding one)")

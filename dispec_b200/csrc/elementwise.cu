@@ -390,11 +390,12 @@ extern "C" int dsp_swiglu(const void* gate_up, void* out, int T, int inter, int 
 //  v head: copied to v_pool[page, kvh, offset, :].
 // The rotation pairs element i with i + rotary_dim/2 (half-split), angle = pos * inv_freq[i]
 // in 32-bit: out[i] = x[i] cos - x[i+h] sin, out[i+h] = x[i+h] cos + x[i] sin.  Elements at
-// and beyond rotary_dim pass through.  rotary_dim == 0 means no rotation at all.
+// and beyond rotary_dim pass through.  rotary_dim == 0 means no rotation at all.  `places`: where each row's key and value
+// lie in its request's cache, where that is not its position (the nodes of a drafted tree).
 // Pool layout: [num_pages, KVH, page_size, D].  page = page_table[seq, pos / page_size].
 template <typename T>
 __global__ void rope_kv_store_kernel(T* __restrict__ qkv, const int* __restrict__ positions,
-                                     const int* __restrict__ seq_of_token,
+                                     const int* __restrict__ places, const int* __restrict__ seq_of_token,
                                      const int* __restrict__ page_table, int pt_stride,
                                      T* __restrict__ k_pool, T* __restrict__ v_pool,
                                      const float* __restrict__ inv_freq, int H, int KVH, int D,
@@ -410,15 +411,15 @@ __global__ void rope_kv_store_kernel(T* __restrict__ qkv, const int* __restrict_
   T* dst = nullptr;
   if (!is_q) {
     if (!write_kv) return;
-    const int seq = seq_of_token[t];
-    const int page = page_table[(size_t)seq * pt_stride + pos / page_size];
+    const int seq = seq_of_token[t], place = places ? places[t] : pos;
+    const int page = page_table[(size_t)seq * pt_stride + place / page_size];
     if (page < 0 || page >= num_pages) {
       if (threadIdx.x == 0) atomicOr(err, DSP_ERR_BAD_PAGE);
       return;
     }
     const int kvh = is_k ? head - H : head - H - KVH;
     T* pool = is_k ? k_pool : v_pool;
-    dst = pool + (((size_t)page * KVH + kvh) * page_size + (pos % page_size)) * D;
+    dst = pool + (((size_t)page * KVH + kvh) * page_size + (place % page_size)) * D;
   }
   if (is_q || is_k) {
     const int half = rotary_dim / 2;
@@ -448,7 +449,7 @@ __global__ void rope_kv_store_kernel(T* __restrict__ qkv, const int* __restrict_
 template <typename T>
 __global__ void __launch_bounds__(256)
 rope_kv_store_token_kernel(T* __restrict__ qkv, const int* __restrict__ positions,
-                           const int* __restrict__ seq_of_token,
+                           const int* __restrict__ places, const int* __restrict__ seq_of_token,
                            const int* __restrict__ page_table, int pt_stride,
                            T* __restrict__ k_pool, T* __restrict__ v_pool,
                            const float* __restrict__ inv_freq, int H, int KVH, int D,
@@ -473,12 +474,12 @@ rope_kv_store_token_kernel(T* __restrict__ qkv, const int* __restrict__ position
   }
   long kv_base = -1;  // element offset of this token's row of kv head 0 in the pools
   if (write_kv && pos >= 0) {
-    const int seq = seq_of_token[t];
-    const int page = page_table[(size_t)seq * pt_stride + pos / page_size];
+    const int seq = seq_of_token[t], place = places ? places[t] : pos;
+    const int page = page_table[(size_t)seq * pt_stride + place / page_size];
     if (page < 0 || page >= num_pages) {
       if (threadIdx.x == 0) atomicOr(err, DSP_ERR_BAD_PAGE);
     } else {
-      kv_base = ((long)page * KVH * page_size + (pos % page_size)) * D;
+      kv_base = ((long)page * KVH * page_size + (place % page_size)) * D;
     }
   }
   pdl_wait();
@@ -544,7 +545,7 @@ rope_kv_store_token_kernel(T* __restrict__ qkv, const int* __restrict__ position
   }
 }
 
-extern "C" int dsp_rope_kv_store(void* qkv, const int* positions, const int* seq_of_token,
+extern "C" int dsp_rope_kv_store_at(void* qkv, const int* positions, const int* places, const int* seq_of_token,
                                  const int* page_table, int pt_stride, void* k_pool, void* v_pool,
                                  const float* inv_freq, int T, int H, int KVH, int D,
                                  int rotary_dim, int page_size, int num_pages, int write_kv, int early,
@@ -564,12 +565,12 @@ extern "C" int dsp_rope_kv_store(void* qkv, const int* positions, const int* seq
     const int threads = (H + KVH) * (rotary_dim / 2 / N) >= 256 ? 256 : 128;
     if (dtype == DSP_F32)
       DSP_CUDA(launch_pdl(rope_kv_store_token_kernel<float>, dim3(T), dim3(threads), smem, stream,
-                          (float*)qkv, positions, seq_of_token, page_table, pt_stride, (float*)k_pool,
+                          (float*)qkv, positions, places, seq_of_token, page_table, pt_stride, (float*)k_pool,
                           (float*)v_pool, inv_freq, H, KVH, D, rotary_dim, page_size, num_pages,
                           write_kv, early, err));
     else
       DSP_CUDA(launch_pdl(rope_kv_store_token_kernel<bf16>, dim3(T), dim3(threads), smem, stream,
-                          (bf16*)qkv, positions, seq_of_token, page_table, pt_stride, (bf16*)k_pool,
+                          (bf16*)qkv, positions, places, seq_of_token, page_table, pt_stride, (bf16*)k_pool,
                           (bf16*)v_pool, inv_freq, H, KVH, D, rotary_dim, page_size, num_pages,
                           write_kv, early, err));
     DSP_CHECK_LAUNCH("dsp_rope_kv_store");
@@ -579,12 +580,21 @@ extern "C" int dsp_rope_kv_store(void* qkv, const int* positions, const int* seq
   const int threads = D / 2 >= 64 ? 64 : 32;
   if (dtype == DSP_F32)
     rope_kv_store_kernel<float><<<grid, threads, 0, stream>>>(
-        (float*)qkv, positions, seq_of_token, page_table, pt_stride, (float*)k_pool, (float*)v_pool,
+        (float*)qkv, positions, places, seq_of_token, page_table, pt_stride, (float*)k_pool, (float*)v_pool,
         inv_freq, H, KVH, D, rotary_dim, page_size, num_pages, write_kv, err);
   else
     rope_kv_store_kernel<bf16><<<grid, threads, 0, stream>>>(
-        (bf16*)qkv, positions, seq_of_token, page_table, pt_stride, (bf16*)k_pool, (bf16*)v_pool,
+        (bf16*)qkv, positions, places, seq_of_token, page_table, pt_stride, (bf16*)k_pool, (bf16*)v_pool,
         inv_freq, H, KVH, D, rotary_dim, page_size, num_pages, write_kv, err);
   DSP_CHECK_LAUNCH("dsp_rope_kv_store");
   return 0;
+}
+
+extern "C" int dsp_rope_kv_store(void* qkv, const int* positions, const int* seq_of_token,
+                                 const int* page_table, int pt_stride, void* k_pool, void* v_pool,
+                                 const float* inv_freq, int T, int H, int KVH, int D,
+                                 int rotary_dim, int page_size, int num_pages, int write_kv, int early,
+                                 int dtype, cudaStream_t stream) {
+  return dsp_rope_kv_store_at(qkv, positions, nullptr, seq_of_token, page_table, pt_stride, k_pool, v_pool, inv_freq, T, H, KVH, D,
+                              rotary_dim, page_size, num_pages, write_kv, early, dtype, stream);
 }

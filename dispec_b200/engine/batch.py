@@ -52,6 +52,29 @@ class LayerStateView:
     slots: torch.Tensor  # [S] int32: state slot of each sequence of the batch
 
 
+@dataclass
+class TreeEntry:
+    """A request's drafted tree: node 0 is the token the last step drew, every other node a draft of the token behind
+    its parent (numbers inside the tree, -1 for node 0), whose number is smaller."""
+    req_id: Any
+    tokens: list
+    parents: list
+    start: int  # position of node 0; equals the request's stored length
+
+
+@dataclass
+class TreeStep:
+    """What the attention of a step of drafted trees reads beside the arrays of every step: node i of tree s is row
+    node_start[s] + i, at position ctx_len[s] + depth, its key and value at place ctx_len[s] + i."""
+    node_start: torch.Tensor  # [S + 1] int32
+    ctx_len: torch.Tensor  # [S] int32: stored tokens in front of each tree
+    visible: torch.Tensor  # [T, words] int64: the nodes a row sees
+    depth: torch.Tensor  # [T] int32
+    places: torch.Tensor  # [T] int32
+    parents: torch.Tensor  # [T] int32
+    max_nodes: int
+
+
 def _align4(n: int) -> int:
     return (n + 3) & ~3
 
@@ -88,6 +111,7 @@ class StepContext:
         self.num_fed = 0  # single tokens whose value comes from the previous step on the device
         self.graph_capture = False  # host-side choices must not depend on the step's values
         self.scratch: dict = {}
+        self.tree = None  # TreeStep: the rows are nodes of drafted trees
         self.layer_trace = None  # a list: the model appends a copy of the stream after every layer run
 
     def cache_view(self, placement, write: bool) -> LayerCacheView:
@@ -315,3 +339,66 @@ def build_context(entries: list, cache, storage, states, staging: HostStaging, d
     ctx = plan.context(dev, storage, states, dtype, device)
     ctx.num_fed = plan.num_fed
     return ctx, plan.row_offsets
+
+
+def build_tree_context(entries: list, cache, storage, staging: HostStaging, dtype, device, vocab_size: int) -> StepContext:
+    """The context of a step whose rows are the nodes of the requests' drafted trees; logits at every node."""
+    from dispec_b200.ops.tree import ancestors
+
+    counts = [len(e.tokens) for e in entries]
+    S, T = len(entries), sum(counts)
+    starts = np.zeros(S + 1, dtype=np.int64)
+    np.cumsum(counts, out=starts[1:])
+    words = -(-max(counts) // 64)
+    pages = [max([len(cache.block_table(e.req_id, g)) for e in entries] + [1]) for g in range(len(cache.groups))]
+    layout, off = {}, 0
+    sizes = {"token_ids": T, "positions": T, "places": T, "depth": T, "parents": T, "seq_of_token": T, "logit_rows": T,
+             "node_start": S + 1, "ctx_len": S, "state_slot": S, "visible": 2 * T * words}
+    sizes.update({f"page_table{g}": S * mp for g, mp in enumerate(pages)})
+    for name, n in sizes.items():  # (every array begins on 16 bytes)
+        layout[name] = (off, n)
+        off += _align4(max(n, 1))
+
+    def fill(buf: np.ndarray) -> None:
+        view = lambda name: buf[layout[name][0]:layout[name][0] + layout[name][1]]
+        tokens, seen = view("token_ids"), view("visible").view(np.int64).reshape(T, words)
+        seen[:] = 0
+        for s, e in enumerate(entries):
+            a, b = int(starts[s]), int(starts[s + 1])
+            bits, depth = ancestors(list(e.parents))
+            tokens[a:b] = np.asarray(e.tokens, dtype=np.int64)
+            view("depth")[a:b] = depth
+            view("positions")[a:b] = e.start + np.asarray(depth)
+            view("places")[a:b] = np.arange(e.start, e.start + (b - a))
+            view("parents")[a:b] = e.parents
+            seen[a:b, :len(bits[0])] = bits
+        if int(tokens.min()) < 0 or int(tokens.max()) >= vocab_size:
+            raise ValueError(f"token id outside [0, {vocab_size})")
+        view("seq_of_token")[:] = np.repeat(np.arange(S), counts)
+        view("logit_rows")[:] = np.arange(T)
+        view("node_start")[:] = starts
+        view("ctx_len")[:] = [e.start for e in entries]
+        view("state_slot")[:] = [cache.state_slot(e.req_id) for e in entries]
+        for g, mp in enumerate(pages):
+            table = view(f"page_table{g}").reshape(S, mp)
+            table[:] = -1
+            for s, e in enumerate(entries):
+                row = cache.block_table(e.req_id, g)
+                table[s, :len(row)] = row
+
+    dev = staging.upload(off, fill)
+    dview = lambda name: dev[layout[name][0]:layout[name][0] + layout[name][1]]
+    ctx = StepContext()
+    ctx.dtype, ctx.device = dtype, device
+    ctx.num_tokens, ctx.num_seqs = T, S
+    ctx.token_ids, ctx.positions, ctx.seq_of_token = dview("token_ids"), dview("positions"), dview("seq_of_token")
+    ctx.q_start, ctx.state_slot = dview("node_start"), dview("state_slot")
+    ctx.logit_rows, ctx.logit_rows_are_all = dview("logit_rows"), True
+    ctx.page_tables = [dview(f"page_table{g}").view(S, mp) for g, mp in enumerate(pages)]
+    ctx.host_q_len, ctx.host_q_start = counts, [int(v) for v in starts]
+    ctx.host_ctx_len = [e.start + n for e, n in zip(entries, counts)]
+    ctx.max_ctx_len = max(ctx.host_ctx_len)
+    ctx.storage, ctx.cache_groups, ctx.page_size = storage, cache.groups, cache.page_size
+    ctx.tree = TreeStep(dview("node_start"), dview("ctx_len"), dview("visible").view(torch.int64).view(T, words),
+                        dview("depth"), dview("places"), dview("parents"), max(counts))
+    return ctx

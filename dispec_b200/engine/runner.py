@@ -15,7 +15,7 @@ import torch
 from dispec_b200 import ops
 from dispec_b200.cache.manager import CacheManager
 from dispec_b200.cache.storage import CacheStorage, StateStorage
-from dispec_b200.engine.batch import HostStaging, SeqEntry, StepPlanLayout, build_context
+from dispec_b200.engine.batch import HostStaging, SeqEntry, StepPlanLayout, TreeEntry, build_context, build_tree_context
 from dispec_b200.ops import library as _library
 from dispec_b200.models.model import DecoderModel
 
@@ -117,6 +117,45 @@ class ModelRunner:
             self._poison(self.cache.commit(e.req_id, e.start + len(e.tokens)))
         self.num_steps += 1
         return logits
+
+    # ------------------------------------------------------------------ drafted trees
+    @torch.inference_mode()
+    def tree_step(self, entries: list[TreeEntry]):
+        """One pass over the requests' drafted trees: the context of the step and the logits behind every node, in
+        float32, tree after tree.  The nodes' keys and values lie behind the stored tokens; nothing is stored for
+        good until ``keep`` has been told which branch was accepted."""
+        if not all(self.model.layers[c.layer].mixer.takes_trees for c in self.model.schedule):
+            raise ValueError("this model has layers that cannot be run on drafted trees")
+        if not entries or len({e.req_id for e in entries}) != len(entries):
+            raise ValueError("a step of drafted trees needs requests, each of them once")
+        for e in entries:
+            if not self.cache.has(e.req_id):
+                raise KeyError(f"request {e.req_id!r} was not admitted")
+            if not e.tokens or len(e.tokens) != len(e.parents):
+                raise ValueError(f"request {e.req_id!r}: {len(e.tokens)} nodes with {len(e.parents)} parents")
+            if e.start != self.cache.num_tokens(e.req_id):
+                raise ValueError(f"request {e.req_id!r}: the tree starts at position {e.start} but "
+                                 f"{self.cache.num_tokens(e.req_id)} tokens are stored")
+        for e in entries:  # may raise OutOfPagesError before anything ran
+            self.cache.extend(e.req_id, e.start + len(e.tokens))
+        ctx = build_tree_context(entries, self.cache, self.storage, self.staging, self.dtype, self.device, self.vocab_size)
+        x, pending = self.model.forward(ctx)
+        logits = self.model.logits(ctx, x, pending, ctx.logit_rows)
+        self.num_steps += 1
+        return ctx, logits
+
+    @torch.inference_mode()
+    def move_accepted(self, ctx, verified) -> None:
+        """Puts the accepted branches' keys and values into line behind the stored tokens, on the device."""
+        for g, named in enumerate(self.storage.pools):
+            ops.keep_path(list(named.values()), ctx.page_tables[g], ctx.tree.ctx_len, verified.path, verified.count)
+
+    def keep(self, entries: list[TreeEntry], counts: list) -> None:
+        """Records that so many tokens of each tree's accepted branch are stored, once they are in line."""
+        for e, n in zip(entries, counts):
+            if not 1 <= n <= len(e.tokens):
+                raise ValueError(f"request {e.req_id!r}: {n} accepted nodes of {len(e.tokens)}")
+            self._poison(self.cache.commit(e.req_id, e.start + n))
 
     # -------------------------------------------------------- captured all-decode steps
     def _context_class(self, entries: list) -> int:

@@ -82,12 +82,15 @@ def swiglu(gate_up: torch.Tensor, out: torch.Tensor | None = None, block: int = 
 def rope_kv_store(qkv: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor,
                   page_table: torch.Tensor, k_pool: torch.Tensor | None, v_pool: torch.Tensor | None,
                   inv_freq: torch.Tensor | None, num_heads: int, num_kv_heads: int, head_dim: int,
-                  rotary_dim: int, write_kv: bool = True) -> None:
+                  rotary_dim: int, write_kv: bool = True, places: torch.Tensor | None = None) -> None:
     """Rotates q and k inside ``qkv`` [T, (H + 2 KVH) D] in place and writes k, v to the pools
     [num_pages, KVH, page_size, D] at page_table[seq, pos // page_size], offset pos % page_size.
-    Rows with a negative position are skipped."""
-    _cuda(qkv, positions, seq_of_token, page_table, k_pool, v_pool, inv_freq)
+    Rows with a negative position are skipped.  ``places`` (int32 [T]): where a row's key and value
+    go, where that is not its position (the nodes of a drafted tree: several may be at one position)."""
+    _cuda(qkv, positions, seq_of_token, page_table, k_pool, v_pool, inv_freq, places)
     T = qkv.shape[0]
+    if places is not None:
+        assert places.dtype == torch.int32 and places.shape == (T,) and places.is_contiguous()
     assert qkv.is_contiguous() and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * head_dim
     assert positions.dtype == torch.int32 and seq_of_token.dtype == torch.int32
     assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.stride(1) == 1
@@ -101,8 +104,8 @@ def rope_kv_store(qkv: torch.Tensor, positions: torch.Tensor, seq_of_token: torc
     if rotary_dim:
         assert inv_freq is not None and inv_freq.dtype == torch.float32
         assert inv_freq.shape[0] >= rotary_dim // 2
-    L.check(L.core().dsp_rope_kv_store(
-        L.ptr(qkv), L.ptr(positions), L.ptr(seq_of_token), L.ptr(page_table), page_table.stride(0),
+    L.check(L.core().dsp_rope_kv_store_at(
+        L.ptr(qkv), L.ptr(positions), L.ptr(places), L.ptr(seq_of_token), L.ptr(page_table), page_table.stride(0),
         L.ptr(k_pool), L.ptr(v_pool), L.ptr(inv_freq), T, num_heads, num_kv_heads, head_dim,
         rotary_dim, page_size, num_pages, int(write_kv), 0, L.dtype_code(qkv.dtype), L.stream_handle()))
 

@@ -99,6 +99,9 @@ class GQAAttention(Mixer):
         scale = self.scale * self.position_encoding.score_scale()
         # single tokens come first in the batch: when their attention kernel rotates q and k itself and
         # stores the new key and value, the rotation kernel runs on the portions of prompts only
+        if ctx.tree is not None:
+            out = self._tree(ctx, qkv, cache, inv_freq, rotary_dim, scale)
+            return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
         n_dec = ctx.num_decode_seqs
         fused = None
         if attn_ops.decode_rope_fusable(ctx, H, KVH, D, rotary_dim, qkv.dtype):
@@ -113,6 +116,18 @@ class GQAAttention(Mixer):
         attn_ops.paged_attention(ctx, qkv, qkv.stride(0), cache, out, H, KVH, D, self.window,
                                  scale, fused_rope=fused)
         return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
+
+    takes_trees = True
+
+    def _tree(self, ctx, qkv, cache, inv_freq, rotary_dim, scale):
+        """A step of drafted trees: several nodes may be at one position, so their keys and values have places of their own."""
+        H, KVH, D, tree = self.num_heads, self.num_kv_heads, self.head_dim, ctx.tree
+        ops.rope_kv_store(qkv, ctx.positions, ctx.seq_of_token, cache.page_table, cache.key_pool if cache.write else None,
+                          cache.value_pool if cache.write else None, inv_freq, H, KVH, D, rotary_dim,
+                          write_kv=cache.write, places=tree.places)
+        return ops.tree_attention(qkv[:, :H * D], cache.key_pool, cache.value_pool, cache.page_table, tree.ctx_len,
+                                  tree.node_start, tree.visible, tree.depth, max_nodes=tree.max_nodes, scale=scale,
+                                  window=self.window)
 
 
 @register_part("mixer", "sink_attention")

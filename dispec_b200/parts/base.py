@@ -103,6 +103,8 @@ class Part:
     # False for a part whose forward decides things on the host from the step's values (such a
     # part cannot be replayed from a captured graph; the runner then runs every step eagerly)
     graph_safe = True
+    # True for a mixer whose forward takes a step of drafted trees (``ctx.tree``, see engine/batch.py)
+    takes_trees = False
 
     def tensor_specs(self) -> dict[str, TensorSpec]:
         return {}
