@@ -151,6 +151,38 @@ def _build(lib_name: str, sources: list[str], defines: list[str], verbose_ptxas:
     return lib
 
 
+def describe_module() -> str:
+    """The Python module that tells C code what a tensor is (host code: built with the C++ compiler against torch's headers)."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    include = os.path.join(root, "include")
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    places = ["-I", HERE, "-I", include, "-I", os.path.join(include, "torch", "csrc", "api", "include"),
+              "-I", sysconfig.get_paths()["include"], "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    key = flags + [torch.__version__, sys.version.split()[0]]
+    out_dir = build_dir()
+    lib = os.path.join(out_dir, f"dispec_b200_describe.{_digest(['describe.cpp'], key)}.so")
+    if not os.path.exists(lib):
+        with _lock:
+            if not os.path.exists(lib):
+                tmp = lib + f".tmp{os.getpid()}"
+                cxx = os.environ.get("CXX") or shutil.which("g++")
+                if not cxx:
+                    raise BuildError("g++ not found (set CXX)")
+                _run([cxx, os.path.join(HERE, "describe.cpp"), "-o", tmp] + flags + places, "c++ describe.cpp")
+                os.replace(tmp, lib)
+                for f in os.listdir(out_dir):  # stale builds
+                    if f.startswith("dispec_b200_describe.") and f.endswith(".so") and f != os.path.basename(lib):
+                        try:
+                            os.remove(os.path.join(out_dir, f))
+                        except OSError:
+                            pass
+    return lib
+
+
 def core_library() -> str:
     return _build("libdispec_b200_core", CORE_SOURCES, [])
 
@@ -162,7 +194,7 @@ def specialised_library(name: str, source: str, defines: dict[str, int]) -> str:
 
 def build_all(head_dims=(16, 32, 64, 128)) -> list[str]:
     """Everything a first call could need, for the head sizes given."""
-    libs = [core_library()]
+    libs = [core_library(), describe_module()]
     for d in head_dims:
         libs.append(attention_library(d))
         if d in (64, 128):

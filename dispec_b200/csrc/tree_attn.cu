@@ -10,6 +10,7 @@
 // (ty, tx) of 16 x 16 owns rows ty, ty + 16 and keys tx + 16 j of the scores, and of the result the same rows and
 // the dimensions 4 tx .. 4 tx + 3 of each 64.  Maximum and sum of a row are exchanged between its 16 threads by
 // shuffles.
+#include "tensor_checks.cuh"
 #include "tree_schedule.cuh"
 
 namespace {
@@ -17,18 +18,7 @@ using namespace tree;
 
 constexpr int ROWS = 32, KEYS = 64, TX = 16, THREADS = 256, RI = ROWS / 16, KJ = KEYS / TX, LP = KEYS + 4;
 
-struct Args {
-  Shape sh;
-  const void *q, *k_pool, *v_pool;
-  const int *page_table, *depth;
-  const unsigned long long* visible;
-  void* out;
-  TreeScratch scratch;
-  long q_stride, out_stride;
-  int pt_stride, words, D, page_size, num_pages;
-  float scale;
-  int* err;
-};
+typedef DspTreeAttention Args;
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 load4(const bf16* p) {
@@ -100,7 +90,7 @@ tree_attn_kernel(const Args a) {
         long at = -1;
         const bool wanted = key < total && (sh.window <= 0 || key > t.ctx - sh.window);
         if (wanted) {
-          const int page = key / a.page_size < a.pt_stride ? table[key / a.page_size] : -1;
+          const int page = key / a.page_size < a.table_width ? table[key / a.page_size] : -1;
           if (page >= 0 && page < a.num_pages)
             at = ((long)page * sh.KVH + t.head) * a.page_size + key % a.page_size;
           else
@@ -296,11 +286,11 @@ tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_str
 }
 
 template <typename T>
-int launch(const Args& a, int ctas, cudaStream_t stream) {
+int launch(const Args& a, cudaStream_t stream) {
   const size_t smem = (size_t)((ROWS + 2 * KEYS) * (a.D + 4) + ROWS * LP) * sizeof(float);
   auto go = [&](auto kernel) -> int {
     DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    DSP_CUDA(launch_plain(kernel, dim3(ctas), dim3(THREADS), smem, stream, a));
+    DSP_CUDA(launch_plain(kernel, dim3((unsigned)a.ctas), dim3(THREADS), smem, stream, a));
     return 0;
   };
   return a.D <= 64 ? go(tree_attn_kernel<T, 1>) : a.D <= 128 ? go(tree_attn_kernel<T, 2>) : go(tree_attn_kernel<T, 4>);
@@ -317,64 +307,96 @@ cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride,
                                        out_stride, G, D, rows_per_tile, ctas);
 }
 
-// The same for kernels that live in other libraries.
-extern "C" int dsp_tree_combine(const TreeScratch* scratch, void* out, long out_stride, int G, int D, int rows_per_tile,
-                                int ctas, int dtype, cudaStream_t stream) {
-  return tree_combine(*scratch, out, out_stride, G, D, rows_per_tile, ctas, dtype, stream) == cudaSuccess ? 0 : 1;
-}
-
-// What the Python side packs, in this order (ops/tree.py).
-struct DspTreeAttention {
-  const void *q, *k_pool, *v_pool;
-  const int *page_table, *ctx_len, *node_start, *depth;
-  const unsigned long long* visible;
-  void* out;
-  float* scratch;
-  long q_stride, out_stride, pt_stride, words, S, H, KVH, D, page_size, num_pages, window, dtype, ctas;
+struct DspTreeOptions {  // as ops/tree.py packs them
+  long max_nodes, window, sms, tensor_cores;
   double scale;
 };
 
-extern "C" int dsp_tree_attention(const DspTreeAttention* p, cudaStream_t stream) {
-  if (p->S == 0) return 0;
-  DSP_REQUIRE(p->S > 0 && p->KVH > 0 && p->H > 0 && p->H % p->KVH == 0, "dsp_tree_attention: %ld heads on %ld key/value heads",
-              p->H, p->KVH);
-  DSP_REQUIRE(p->D % 8 == 0 && p->D >= 8 && p->D <= 256, "dsp_tree_attention: head size %ld (a multiple of 8 up to 256)", p->D);
-  DSP_REQUIRE(p->dtype == DSP_F32 || p->dtype == DSP_BF16, "dsp_tree_attention: unknown dtype %ld", p->dtype);
-  DSP_REQUIRE(p->ctas >= 1 && p->page_size >= 1 && p->num_pages >= 0 && p->words >= 1, "dsp_tree_attention: bad sizes");
-  const uintptr_t bits = (uintptr_t)p->q | (uintptr_t)p->k_pool | (uintptr_t)p->v_pool | (uintptr_t)p->out;
-  DSP_REQUIRE(bits % 16 == 0 && p->q_stride % 8 == 0 && p->out_stride % 8 == 0,
-              "dsp_tree_attention: rows must begin on 16 bytes");
-  Args a = {};
-  a.sh.node_start = p->node_start;
-  a.sh.ctx_len = p->ctx_len;
-  a.sh.S = (int)p->S;
-  a.sh.KVH = (int)p->KVH;
-  a.sh.G = (int)(p->H / p->KVH);
-  a.sh.rows_per_tile = ROWS;
-  a.sh.keys_per_tile = KEYS;
-  a.sh.window = (int)p->window;
-  a.sh.min_units = 1;
-  a.q = p->q;
-  a.k_pool = p->k_pool;
-  a.v_pool = p->v_pool;
-  a.page_table = p->page_table;
-  a.depth = p->depth;
-  a.visible = p->visible;
-  a.out = p->out;
-  a.scratch = tree_scratch(p->scratch, p->ctas, ROWS, p->D);
-  a.q_stride = p->q_stride;
-  a.out_stride = p->out_stride;
-  a.pt_stride = (int)p->pt_stride;
-  a.words = (int)p->words;
-  a.D = (int)p->D;
-  a.page_size = (int)p->page_size;
-  a.num_pages = (int)p->num_pages;
-  a.scale = (float)p->scale;
+// tensors: q, key pool, value pool, page table, ctx_len, node_start, depth (or none), visible, out, scratch.  `tensor_cores`:
+// address of the tensor-core kernel's entry point for this head size, or 0.
+extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, cudaStream_t stream) {
+  const DspTensor &q = t[0], &k = t[1], &v = t[2], &table = t[3], &ctx = t[4], &start = t[5], &depth = t[6], &visible = t[7],
+                  &out = t[8], &scratch = t[9];
+  DSP_REQUIRE(q.device >= 0, "tree_attention: CUDA tensors only (there is no CPU path)");
+  DSP_REQUIRE(q.dims == 2 && k.dims == 4 && v.dims == 4, "tree_attention: q [T, H * D] and two pools [pages, heads, page_size, D] expected");
+  const long T = q.size[0], columns = q.size[1], pages = k.size[0], KVH = k.size[1], page = k.size[2], D = k.size[3];
+  DSP_REQUIRE(q.dtype == DSP_T_F32 || q.dtype == DSP_T_BF16, "tree_attention: kernels exist for float32 and bfloat16");
+  DSP_REQUIRE(k.dtype == q.dtype && v.dtype == q.dtype && k.device == q.device && v.device == q.device && k.contiguous && v.contiguous &&
+                  v.size[0] == pages && v.size[1] == KVH && v.size[2] == page && v.size[3] == D,
+              "tree_attention: the pools must be contiguous, alike, and of the type and on the device of q");
+  DSP_REQUIRE(T <= 1 || q.stride[1] == 1 || columns == 1, "tree_attention: the columns of q must be neighbours");
+  DSP_REQUIRE(D % 8 == 0 && D >= 8 && D <= 256 && KVH > 0 && columns > 0 && columns % D == 0 && columns / D % KVH == 0,
+              "tree_attention: %ld query columns on %ld heads of %ld (a multiple of 8 up to 256)", columns, KVH, D);
+  DSP_REQUIRE(ctx.dims == 1, "tree_attention: ctx_len must be one-dimensional");
+  const long S = ctx.size[0], words = visible.dims == 2 ? visible.size[1] : 0;
+  DSP_REQUIRE(tensor_is(visible, DSP_T_I64, q.device, 2, T, words) && words >= 1 && 64 * words >= o->max_nodes,
+              "tree_attention: visible must be contiguous int64 [%ld, words] with a bit for each of %ld nodes", T, o->max_nodes);
+  DSP_REQUIRE(o->scale > 0. && o->window >= 0 && o->window <= 0x7fffffff && o->max_nodes >= 1,
+              "tree_attention: scale %g must be positive, window %ld not negative, max_nodes %ld at least 1", o->scale, o->window,
+              o->max_nodes);
+  DSP_REQUIRE(tensor_is(ctx, DSP_T_I32, q.device, 1, S) && tensor_is(start, DSP_T_I32, q.device, 1, S + 1),
+              "tree_attention: ctx_len [%ld] and node_start [%ld] must be contiguous int32 on the device of q", S, S + 1);
+  DSP_REQUIRE(is_page_table(table, q.device, S), "tree_attention: page_table must be int32 [%ld, pages], neighbouring pages side by side", S);
+  DSP_REQUIRE(depth.dims < 0 ? o->window == 0 : tensor_is(depth, DSP_T_I32, q.device, 1, T),
+              "tree_attention: depth must be contiguous int32 [%ld]; a window needs it", T);
+  DSP_REQUIRE(out.dtype == q.dtype && out.device == q.device && out.dims == 2 && out.size[0] == T && out.size[1] == columns &&
+                  (T <= 1 || out.stride[1] == 1),
+              "tree_attention: out must be like the queries [%ld, %ld] with neighbouring columns", T, columns);
+  DSP_REQUIRE(T <= 0x7fffffff && S <= 0x7fffffff && pages <= 0x7fffffff && page >= 1 && o->sms >= 1, "tree_attention: sizes out of range");
+  if (T == 0 || S == 0) return 0;
+  const uintptr_t bits = (uintptr_t)q.data | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)out.data;
+  const long piece = q.dtype == DSP_T_F32 ? 4 : 8;  // elements of 16 bytes
+  DSP_REQUIRE(bits % 16 == 0 && (T == 1 || (q.stride[0] % piece == 0 && out.stride[0] % piece == 0)),
+              "tree_attention: rows must begin on 16 bytes");
+  // the tensor-core kernel is built for these page sizes; everything else takes the 32-bit kernel
+  const bool tensor_cores = o->tensor_cores != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
+                            (page == 8 || page == 16 || page == 32 || page == 64) && pages > 0;
+  const long G = columns / D / KVH, rows = tensor_cores ? TREE_TENSOR_CORE_ROWS : ROWS;
+  // a multiple of the row tiles that trees have: then those of one head read its keys at the same time
+  const long row_tiles = (o->max_nodes * G + rows - 1) / rows;
+  const long ctas = row_tiles < o->sms ? o->sms - o->sms % row_tiles : o->sms;
+  DSP_REQUIRE(scratch.contiguous && scratch.device == q.device && scratch.dims == 1 && (uintptr_t)scratch.data % 16 == 0 &&
+                  scratch.size[0] >= 2 * ctas * rows * (D + 2) + 8 * ctas,
+              "tree_attention: scratch is too small");
+  DspTreeAttention a = {};
+  a.sh.node_start = (const int*)start.data;
+  a.sh.ctx_len = (const int*)ctx.data;
+  a.sh.S = (int)S;
+  a.sh.KVH = (int)KVH;
+  a.sh.G = (int)G;
+  a.sh.rows_per_tile = (int)rows;
+  a.sh.window = (int)o->window;
+  a.q = q.data;
+  a.k_pool = k.data;
+  a.v_pool = v.data;
+  a.page_table = (const int*)table.data;
+  a.depth = depth.dims < 0 ? nullptr : (const int*)depth.data;
+  a.visible = (const unsigned long long*)visible.data;
+  a.out = out.data;
+  a.scratch = tree_scratch((float*)scratch.data, ctas, rows, D);
+  a.q_stride = q.stride[0];
+  a.out_stride = out.stride[0];
+  a.pt_stride = (int)table.stride[0];
+  a.table_width = (int)table.size[1];
+  a.words = (int)words;
+  a.D = (int)D;
+  a.page_size = (int)page;
+  a.num_pages = (int)pages;
+  a.ctas = (int)ctas;
+  a.scale = (float)o->scale;
   a.err = dsp_device_error_ptr();
-  DSP_REQUIRE(a.err != nullptr, "dsp_tree_attention: no device error word");
-  const int rc = p->dtype == DSP_F32 ? launch<float>(a, (int)p->ctas, stream) : launch<bf16>(a, (int)p->ctas, stream);
-  if (rc != 0) return rc;
-  DSP_CUDA(tree_combine(a.scratch, a.out, a.out_stride, a.sh.G, a.D, ROWS, (int)p->ctas, (int)p->dtype, stream));
-  DSP_CHECK_LAUNCH("dsp_tree_attention");
+  DSP_REQUIRE(a.err != nullptr, "tree_attention: no device error word");
+  if (tensor_cores) {
+    typedef int (*Kernel)(const DspTreeAttention*, cudaStream_t);
+    const int rc = reinterpret_cast<Kernel>(o->tensor_cores)(&a, stream);
+    DSP_REQUIRE(rc == 0, "tree_attention: %s", rc == 4 ? "shared memory opt-in or tensor map creation failed" : "launch failed");
+  } else {
+    a.sh.keys_per_tile = KEYS;
+    a.sh.min_units = 1;
+    const int rc = q.dtype == DSP_T_F32 ? launch<float>(a, stream) : launch<bf16>(a, stream);
+    if (rc != 0) return rc;
+  }
+  DSP_CUDA(tree_combine(a.scratch, a.out, a.out_stride, a.sh.G, a.D, (int)rows, a.ctas, q.dtype == DSP_T_F32 ? DSP_F32 : DSP_BF16, stream));
+  DSP_CHECK_LAUNCH("tree_attention");
   return 0;
 }

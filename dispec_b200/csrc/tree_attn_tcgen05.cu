@@ -55,17 +55,9 @@ static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
 struct Params {
-  Shape sh;
-  const bf16* q;
-  const int *page_table, *depth;
-  const unsigned long long* visible;
-  bf16* out;
-  TreeScratch scratch;
-  long q_stride, out_stride;
-  int pt_stride, words, page_size, num_pages;
+  DspTreeAttention a;
   int page_runs;  // the run maps are valid
   float scale_log2;
-  int* err;
 };
 
 // Which keys key0 .. key0 + 63 the row of a node sees: stored ones, and nodes of the tree by the row's words.
@@ -74,26 +66,26 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const S
   const int off = key0 - t.ctx;  // number of the first key as a node
   if (off < 0) {
     stored = off <= -64 ? ~0ull : (1ull << -off) - 1ull;
-    if (p.sh.window > 0) {
-      const int hidden = t.ctx + depth - p.sh.window + 1 - key0;  // so many first keys are out of the window
+    if (p.a.sh.window > 0) {
+      const int hidden = t.ctx + depth - p.a.sh.window + 1 - key0;  // so many first keys are out of the window
       if (hidden > 0) stored = hidden >= 64 ? 0ull : stored & ~((1ull << hidden) - 1ull);
     }
   }
   if (off > -64 && off < t.n) {
-    const unsigned long long* w = p.visible + (size_t)row * p.words;
+    const unsigned long long* w = p.a.visible + (size_t)row * p.a.words;
     if (off <= 0) {
       drafted = w[0] << -off;
     } else {
       const int k = off >> 6, sft = off & 63;
-      drafted = k < p.words ? w[k] >> sft : 0ull;
-      if (sft && k + 1 < p.words) drafted |= w[k + 1] << (64 - sft);
+      drafted = k < p.a.words ? w[k] >> sft : 0ull;
+      if (sft && k + 1 < p.a.words) drafted |= w[k + 1] << (64 - sft);
     }
     const int there = t.n - off;  // keys up to the tree's last node
     if (there < 64) drafted &= (1ull << there) - 1ull;
-    if (p.sh.window > 0 && depth >= p.sh.window) {  // a tree deeper than the window
+    if (p.a.sh.window > 0 && depth >= p.a.sh.window) {  // a tree deeper than the window
       for (unsigned long long left = drafted; left != 0ull; left &= left - 1ull) {
         const int c = __ffsll((long long)left) - 1;
-        if (p.depth[t.first + off + c] <= depth - p.sh.window) drafted &= ~(1ull << c);
+        if (p.a.depth[t.first + off + c] <= depth - p.a.sh.window) drafted &= ~(1ull << c);
       }
     }
   }
@@ -151,7 +143,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ uint32_t bad_pages[BAD_SLOTS];  // of key tile n, in slot n % BAD_SLOTS; bit j: page j had no valid id (not loaded)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
-  const Shape& sh = p.sh;
+  const Shape& sh = p.a.sh;
   const int G = sh.G;
   unsigned char* k_s = smem;  // [stage][slice][64 keys][128 bytes]
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
@@ -164,7 +156,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     if (lane == 0) {
       if (!more) w.at.seq = -1;
       shares[0] = w.at;
-      p.scratch.splits[cta].parts = 0;  // (stays where there is no work, or a wait runs out)
+      p.a.scratch.splits[cta].parts = 0;  // (stays where there is no work, or a wait runs out)
     }
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -222,22 +214,22 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 
   // Requests the tiles asked .. upto - 1 of a share, two a turn (`upto` is even or the share's last).
   auto request = [&](const Share& t, int upto, int first_tile) {
-    const int pages_per_tile = BN / p.page_size;
-    const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.page_size * 128u;
-    const int ppt_shift = __ffs(pages_per_tile) - 1, page_shift = __ffs(p.page_size) - 1;  // powers of two here
+    const int pages_per_tile = BN / p.a.page_size;
+    const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.a.page_size * 128u;
+    const int ppt_shift = __ffs(pages_per_tile) - 1, page_shift = __ffs(p.a.page_size) - 1;  // powers of two here
     const int chunk_shift = 5 - ppt_shift, chunk_mask = (1 << chunk_shift) - 1;
     const int page_in_tile = lane & (pages_per_tile - 1);
     const uint32_t tile_lanes = pages_per_tile == 32 ? 0xffffffffu : ((1u << pages_per_tile) - 1u);
     const int n_kt = t.kt_end - t.kt_begin, kt_begin = t.kt_begin, head = t.head;
     const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0, last = t.ctx + t.n - 1;
-    const int* table = p.page_table + (size_t)t.seq * p.pt_stride;
+    const int* table = p.a.page_table + (size_t)t.seq * p.a.pt_stride;
     // Page ids are looked up for a chunk of 32 / pages_per_tile tiles at a time, a chunk ahead.
     auto load_chunk = [&](int c) -> int {
       const int i = (c << chunk_shift) + (lane >> ppt_shift);
-      const int first = (kt_begin + i) * BN + page_in_tile * p.page_size;
-      if (i < n_kt && first <= last && first + p.page_size > lo) {
+      const int first = (kt_begin + i) * BN + page_in_tile * p.a.page_size;
+      if (i < n_kt && first <= last && first + p.a.page_size > lo) {
         const int j = first >> page_shift;
-        return j < p.pt_stride ? table[j] : -1;
+        return j < p.a.table_width ? table[j] : -1;
       }
       return -2;  // not wanted
     };
@@ -247,16 +239,16 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       if (in_chunk == 0) {
         pg = pg_next;
         pg_next = load_chunk((asked >> chunk_shift) + 1);
-        const bool bad = pg != -2 && (pg < 0 || pg >= p.num_pages);  // recorded, not loaded, its keys are hidden
+        const bool bad = pg != -2 && (pg < 0 || pg >= p.a.num_pages);  // recorded, not loaded, its keys are hidden
         if (bad) {
-          atomicOr(p.err, DSP_ERR_BAD_PAGE);
+          atomicOr(p.a.err, DSP_ERR_BAD_PAGE);
           pg = -1;
         }
         bad_mask = __ballot_sync(0xffffffffu, bad);
         live_mask = __ballot_sync(0xffffffffu, pg >= 0);
         const int first_pg = __shfl_sync(0xffffffffu, pg, lane & ~(pages_per_tile - 1));
         run_mask = __ballot_sync(0xffffffffu, pg >= 0 && pg == first_pg + page_in_tile &&
-                                                  first_pg + pages_per_tile <= p.num_pages);
+                                                  first_pg + pages_per_tile <= p.a.num_pages);
       }
       // Two tiles per turn, each with a lane of its own that waits for the tile's ring slots and makes the requests.
       const int second = (lane >> ppt_shift) - in_chunk;  // 0, 1: this lane holds a page of the turn's first, second tile
@@ -287,8 +279,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
             mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
           }
           if (in_run) {  // the tile's pages lie one after the other in the pool: one request per operand
-            tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, head * p.page_size, pg, 0);
-            tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, head * p.page_size, pg, 0);
+            tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, head * p.a.page_size, pg, 0);
+            tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, head * p.a.page_size, pg, 0);
           }
         } else {
           give_up(share);
@@ -296,8 +288,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       if (!__all_sync(0xffffffffu, !mine || in_run)) {
         if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
-          const int row = (pg * sh.KVH + head) * p.page_size;
-          const int dst = page_in_tile * p.page_size * 128;
+          const int row = (pg * sh.KVH + head) * p.a.page_size;
+          const int dst = page_in_tile * p.a.page_size * 128;
 #pragma unroll
           for (int h = 0; h < KD; ++h) {
             tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
@@ -324,8 +316,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   auto ask_queries = [&](const Share& t, uint4 (&x)[Q_PIECES]) {
     const int rr = t.row_tile * BM + r;
     const bool valid = rr < t.n * G;
-    const bf16* src = p.q;
-    if (valid) src += (size_t)(t.first + rr / G) * p.q_stride + (size_t)(t.head * G + rr % G) * D + (D == 128 ? g * 64 : 0);
+    const bf16* src = (const bf16*)p.a.q;
+    if (valid) src += (size_t)(t.first + rr / G) * p.a.q_stride + (size_t)(t.head * G + rr % G) * D + (D == 128 ? g * 64 : 0);
 #pragma unroll
     for (int c = 0; c < Q_PIECES; ++c) x[c] = valid ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
   };
@@ -364,12 +356,12 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
-      bf16* dst = p.out;
-      float* part = p.scratch.part_o;
+      bf16* dst = (bf16*)p.a.out;
+      float* part = p.a.scratch.part_o;
       if (slot >= 0)
         part += ((size_t)slot * BM + r) * D;
       else if (row_ok)
-        dst += (size_t)(t.first + (row0 + r) / G) * p.out_stride + (size_t)(t.head * G + (row0 + r) % G) * D;
+        dst += (size_t)(t.first + (row0 + r) / G) * p.a.out_stride + (size_t)(t.head * G + (row0 + r) % G) * D;
 #pragma unroll 1
       for (int c0 = g * (D / 2); c0 < (g + 1) * (D / 2); c0 += 32) {
         uint32_t ov[32], ow[32];
@@ -402,7 +394,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         }
         __syncwarp();
       }
-      if (g == 0 && slot >= 0 && row_ok) reinterpret_cast<float2*>(p.scratch.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
+      if (g == 0 && slot >= 0 && row_ok) reinterpret_cast<float2*>(p.a.scratch.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
     }
     tc_fence_before();
     __syncwarp();
@@ -422,7 +414,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       if (lane == 0) {
         if (!more) {
           w.at.seq = -1;
-          p.scratch.splits[cta] = split;
+          p.a.scratch.splits[cta] = split;
         }
         shares[(share + 1) % SHARES] = w.at;
       }
@@ -499,13 +491,13 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
       const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
       const float scale = p.scale_log2;
-      const int page_shift = __ffs(p.page_size) - 1;
+      const int page_shift = __ffs(p.a.page_size) - 1;
       const int kt_begin = t.kt_begin, row0 = t.row_tile * BM;
       const int nrows = min(BM, t.n * G - row0);
       const bool row_ok = r < nrows;
       const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
       const int node = row_ok ? t.first + (row0 + r) / G : t.first;
-      const int depth = sh.window > 0 ? p.depth[node] : 0;
+      const int depth = sh.window > 0 ? p.a.depth[node] : 0;
       const int total = t.ctx + t.n;
       const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;  // first key any row sees
       const int lo_r = sh.window > 0 ? t.ctx + depth - sh.window + 1 : 0;
@@ -528,7 +520,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         if (bad != 0u)
           for (int b = 0; b < BN >> page_shift; ++b)
             if ((bad >> b) & 1u)
-              seen &= ~((p.page_size == 64 ? ~0ull : (1ull << p.page_size) - 1ull) << (b << page_shift));
+              seen &= ~((p.a.page_size == 64 ? ~0ull : (1ull << p.a.page_size) - 1ull) << (b << page_shift));
         __syncwarp();
         if (warp_ok) {
           uint32_t a[32], b[32];
@@ -638,7 +630,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (failed) {
-    if (threadIdx.x == 0) atomicOr(p.err, DSP_ERR_WAIT_LIMIT);
+    if (threadIdx.x == 0) atomicOr(p.a.err, DSP_ERR_WAIT_LIMIT);
     // let copies that are still on their way land before the shared memory goes away
     for (int i = 0; i < 2000; ++i) __nanosleep(100);
   }
@@ -651,59 +643,21 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 
 }  // namespace
 
-// As dsp_tree_attention (tree_attn.cu), whose merge of partial results it calls at `combine`.  Returns 0, or: 1 launch
-// failed, 2 unsupported sizes (page sizes are 8, 16, 32 or 64), 3 misaligned rows, 4 the shared-memory opt-in or the tensor
-// maps failed.
-struct DspTreeAttention {
-  const void *q, *k_pool, *v_pool;
-  const int *page_table, *ctx_len, *node_start, *depth;
-  const unsigned long long* visible;
-  void* out;
-  float* scratch;
-  long q_stride, out_stride, pt_stride, words, S, H, KVH, D, page_size, num_pages, window, dtype, ctas;
-  double scale;
-};
-typedef int (*TreeCombine)(const TreeScratch*, void*, long, int, int, int, int, int, cudaStream_t);
-
-extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTreeAttention* a, void* combine, int* err,
-                                                                   cudaStream_t stream) {
-  if (a->S <= 0) return a->S == 0 ? 0 : 2;
-  const int page = (int)a->page_size;
-  if (a->D != D || a->KVH <= 0 || a->H <= 0 || a->H % a->KVH != 0 || a->dtype != DSP_BF16) return 2;
-  if (page != 8 && page != 16 && page != 32 && page != 64) return 2;
-  if (!(a->scale > 0.) || a->ctas < 1 || a->words < 1 || a->num_pages < 1) return 2;
-  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->k_pool | (uintptr_t)a->v_pool | (uintptr_t)a->out;
-  if (bits % 16 != 0 || a->q_stride % 8 != 0 || a->out_stride % 8 != 0) return 3;
+// The arguments come checked from dsp_tree_attention (tree_attn.cu), which also launches the merge.  Returns 0, or: 1 launch
+// failed, 4 the shared-memory opt-in or the tensor maps failed.
+extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTreeAttention* a, cudaStream_t stream) {
+  const int page = a->page_size;
   Params p = {};
-  p.sh.node_start = a->node_start;
-  p.sh.ctx_len = a->ctx_len;
-  p.sh.S = (int)a->S;
-  p.sh.KVH = (int)a->KVH;
-  p.sh.G = (int)(a->H / a->KVH);
-  p.sh.rows_per_tile = BM;
-  p.sh.keys_per_tile = BN;
-  p.sh.window = (int)a->window;
-  p.sh.min_units = 2;  // one tile for each softmax group
-  p.q = (const bf16*)a->q;
-  p.page_table = a->page_table;
-  p.depth = a->depth;
-  p.visible = a->visible;
-  p.out = (bf16*)a->out;
-  p.scratch = tree_scratch(a->scratch, a->ctas, BM, D);
-  p.q_stride = a->q_stride;
-  p.out_stride = a->out_stride;
-  p.pt_stride = (int)a->pt_stride;
-  p.words = (int)a->words;
-  p.page_size = page;
-  p.num_pages = (int)a->num_pages;
-  p.scale_log2 = (float)(a->scale * 1.4426950408889634);
-  p.err = err;
+  p.a = *a;
+  p.a.sh.keys_per_tile = BN;
+  p.a.sh.min_units = 2;  // one tile for each softmax group
+  p.scale_log2 = a->scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v, runs_k, runs_v;
-  const long rows = a->num_pages * a->KVH * page;
+  const long rows = (long)a->num_pages * a->sh.KVH * page;
   if (!make_map(&map_k, a->k_pool, rows, D, D, page) || !make_map(&map_v, a->v_pool, rows, D, D, page)) return 4;
   // a pool of fewer pages than a key tile has gives no map of runs
-  p.page_runs = make_map_page_runs(&runs_k, a->k_pool, a->num_pages, p.sh.KVH, page, D, BN / page) &&
-                make_map_page_runs(&runs_v, a->v_pool, a->num_pages, p.sh.KVH, page, D, BN / page);
+  p.page_runs = make_map_page_runs(&runs_k, a->k_pool, a->num_pages, a->sh.KVH, page, D, BN / page) &&
+                make_map_page_runs(&runs_v, a->v_pool, a->num_pages, a->sh.KVH, page, D, BN / page);
   if (!p.page_runs) {
     runs_k = map_k;
     runs_v = map_v;
@@ -715,8 +669,8 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
       return 4;
     if (device >= 0) allowed[device] = true;
   }
-  if (launch_pdl(tree_attn_tcgen05_kernel, dim3((unsigned)a->ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, p, map_k, map_v,
-                 runs_k, runs_v) != cudaSuccess)
-    return 1;
-  return reinterpret_cast<TreeCombine>(combine)(&p.scratch, p.out, p.out_stride, p.sh.G, D, BM, (int)a->ctas, DSP_BF16, stream);
+  return launch_pdl(tree_attn_tcgen05_kernel, dim3((unsigned)a->ctas), dim3(THREADS), (size_t)SMEM_BYTES, stream, p, map_k, map_v,
+                    runs_k, runs_v) == cudaSuccess
+             ? 0
+             : 1;
 }

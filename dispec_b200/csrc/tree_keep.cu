@@ -6,7 +6,7 @@
 //
 // What bounds it: the bytes for large batches; for small ones the chain count, path -> page table -> row.  A block works
 // that chain out once for several layers, and a thread's loads of up to eight nodes are under way together.
-#include "common.cuh"
+#include "tensor_checks.cuh"
 
 namespace {
 constexpr int MAX_POOLS = 8, THREADS = 256, AHEAD = 8;
@@ -22,7 +22,7 @@ struct Pool {
 struct Args {
   Pool pool[MAX_POOLS];
   const int *page_table, *ctx_len, *path, *count;
-  int pt_stride, path_stride, path_width, page_size;
+  int pt_stride, table_width, path_stride, path_width, page_size;
   int* err;
 };
 
@@ -54,7 +54,7 @@ tree_keep_kernel(const __grid_constant__ Args a) {
         atomicOr(a.err, DSP_ERR_BAD_TREE);
       } else if (node != j) {
         const int k = ctx + node, k2 = ctx + j;
-        const bool inside = ctx >= 0 && k / a.page_size < a.pt_stride;
+        const bool inside = ctx >= 0 && k / a.page_size < a.table_width;
         from = inside ? table[k / a.page_size] : -1;
         const int to = inside ? table[k2 / a.page_size] : -1;
         if (from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages) {
@@ -91,40 +91,47 @@ tree_keep_kernel(const __grid_constant__ Args a) {
 }
 }  // namespace
 
-// What the Python side packs, in this order (ops/tree.py); `pool` holds (address, layers, pages, heads, bytes of a row).
-struct DspTreeKeep {
-  const int *page_table, *ctx_len, *path, *count;
-  long pt_stride, path_stride, path_width, page_size, S, pools;
-  long pool[MAX_POOLS][5];
-};
-
-extern "C" int dsp_tree_keep(const DspTreeKeep* p, cudaStream_t stream) {
-  if (p->S == 0 || p->pools == 0) return 0;
-  DSP_REQUIRE(p->S > 0 && p->S <= 65535 && p->pools > 0 && p->pools <= MAX_POOLS && p->page_size >= 1 && p->path_width >= 1,
-              "dsp_tree_keep: %ld trees, %ld pools", p->S, p->pools);
+// tensors: page table, ctx_len, path, count, and so many pools [layers, pages, heads, page_size, width].
+extern "C" int dsp_tree_keep(const DspTensor* t, int pools, cudaStream_t stream) {
+  const DspTensor &table = t[0], &ctx = t[1], &path = t[2], &count = t[3], *pool = t + 4;
+  DSP_REQUIRE(pools >= 1 && pools <= MAX_POOLS, "keep_path: %d pools (1 to %d)", pools, MAX_POOLS);
+  DSP_REQUIRE(ctx.dims == 1 && path.dims == 2, "keep_path: ctx_len [S] and path [S, n] expected");
+  const long S = ctx.size[0], width = path.size[1], page = pool[0].dims == 5 ? pool[0].size[3] : 0;
+  const int dev = pool[0].device;
+  DSP_REQUIRE(dev >= 0, "keep_path: CUDA tensors only (there is no CPU path)");
+  DSP_REQUIRE(tensor_is(ctx, DSP_T_I32, dev, 1, S) && tensor_is(count, DSP_T_I32, dev, 1, S) && tensor_is(path, DSP_T_I32, dev, 2, S, width),
+              "keep_path: ctx_len [%ld], count [%ld] and path [%ld, n] must be contiguous int32 on the device of the pools", S, S, S);
+  DSP_REQUIRE(is_page_table(table, dev, S), "keep_path: page_table must be int32 [%ld, pages], neighbouring pages side by side", S);
+  DSP_REQUIRE(S <= 65535 && width <= 0x7fffffff, "keep_path: %ld trees (at most 65,535)", S);
   Args a = {};
   long blocks = 0;
-  for (int i = 0; i < p->pools; ++i) {
-    const long* d = p->pool[i];
-    DSP_REQUIRE(d[4] % 16 == 0 && d[0] % 16 == 0 && d[4] > 0, "dsp_tree_keep: rows of %ld bytes (whole 16-byte pieces)", d[4]);
-    if (d[1] == 0 || d[3] == 0) continue;  // (a pool without rows has no blocks)
-    const int row_pieces = (int)(d[3] * d[4] / 16), per = min((int)d[1], max(1, ITEMS * THREADS / row_pieces));
-    a.pool[i] = Pool{(unsigned char*)d[0], (int)d[1], (int)d[3], (int)(d[4] / 16), per, ((int)d[1] + per - 1) / per,
-                     d[2] * d[3] * p->page_size * d[4], (int)d[2]};
-    blocks += a.pool[i].blocks;
+  int used = 0;
+  for (int i = 0; i < pools; ++i) {
+    const DspTensor& p = pool[i];
+    DSP_REQUIRE(p.dims == 5 && p.contiguous && p.device == dev && p.size[3] == page && page >= 1,
+                "keep_path: a pool must be contiguous [layers, pages, heads, %ld, width] on the device of the others", page);
+    DSP_REQUIRE(p.dtype == DSP_T_F32 || p.dtype == DSP_T_BF16, "keep_path: pools are float32 or bfloat16");
+    const long layers = p.size[0], pages = p.size[1], heads = p.size[2], row = p.size[4] * (p.dtype == DSP_T_F32 ? 4 : 2);
+    DSP_REQUIRE(row % 16 == 0 && row > 0 && (uintptr_t)p.data % 16 == 0, "keep_path: rows of %ld bytes (whole 16-byte pieces are moved)", row);
+    if (layers == 0 || heads == 0) continue;  // (a pool without rows has no blocks)
+    const long row_pieces = heads * row / 16, per = min(layers, max(1L, ITEMS * THREADS / row_pieces));
+    a.pool[used++] = Pool{(unsigned char*)p.data, (int)layers, (int)heads, (int)(row / 16), (int)per, (int)((layers + per - 1) / per),
+                          pages * heads * page * row, (int)pages};
+    blocks += (layers + per - 1) / per;
   }
-  if (blocks == 0) return 0;
-  a.page_table = p->page_table;
-  a.ctx_len = p->ctx_len;
-  a.path = p->path;
-  a.count = p->count;
-  a.pt_stride = (int)p->pt_stride;
-  a.path_stride = (int)p->path_stride;
-  a.path_width = (int)p->path_width;
-  a.page_size = (int)p->page_size;
+  if (S == 0 || width == 0 || blocks == 0) return 0;
+  a.page_table = (const int*)table.data;
+  a.ctx_len = (const int*)ctx.data;
+  a.path = (const int*)path.data;
+  a.count = (const int*)count.data;
+  a.pt_stride = (int)table.stride[0];
+  a.table_width = (int)table.size[1];
+  a.path_stride = (int)path.stride[0];
+  a.path_width = (int)width;
+  a.page_size = (int)page;
   a.err = dsp_device_error_ptr();
-  DSP_REQUIRE(a.err != nullptr, "dsp_tree_keep: no device error word");
-  DSP_CUDA(launch_pdl(tree_keep_kernel, dim3((unsigned)blocks, (unsigned)p->S), dim3(THREADS), 0, stream, a));
-  DSP_CHECK_LAUNCH("dsp_tree_keep");
+  DSP_REQUIRE(a.err != nullptr, "keep_path: no device error word");
+  DSP_CUDA(launch_pdl(tree_keep_kernel, dim3((unsigned)blocks, (unsigned)S), dim3(THREADS), 0, stream, a));
+  DSP_CHECK_LAUNCH("keep_path");
   return 0;
 }

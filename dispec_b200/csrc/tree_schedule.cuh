@@ -272,3 +272,18 @@ inline TreeScratch tree_scratch(float* scratch, long ctas, long rows_per_tile, l
 // Merges the partial results of the items that several CTAs share (tree_attn.cu).
 cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride, int G, int D, int rows_per_tile, int ctas,
                          int dtype, cudaStream_t stream);
+
+// The attention's arguments, checked.
+constexpr int TREE_TENSOR_CORE_ROWS = 128;  // rows_per_tile of the tensor-core kernel
+struct DspTreeAttention {
+  tree::Shape sh;
+  const void *q, *k_pool, *v_pool;
+  const int *page_table, *depth;
+  const unsigned long long* visible;
+  void* out;
+  TreeScratch scratch;
+  long q_stride, out_stride;
+  int pt_stride, table_width, words, D, page_size, num_pages, ctas;
+  float scale;
+  int* err;
+};

@@ -20,6 +20,7 @@
 //
 // What bounds it: for a few trees the latencies of a node in a row (the row's arrival, two exchanges, the pass of
 // exponentials, the tests), for many the instructions of the exponentials' pass.
+#include "tensor_checks.cuh"
 #include "tcgen05_common.cuh"  // bounded mbarrier waits, cluster addresses, counted remote stores
 
 namespace {
@@ -479,49 +480,58 @@ int launch(const Args& a, int S, int ctas, cudaStream_t stream) {
 }
 }  // namespace
 
-// What the Python side packs, in this order (ops/tree.py).
-struct DspTreeVerify {
-  const void* logits;
-  const float* draft;
-  const int *tokens, *parents, *node_start;
-  const float *temperature, *uniforms, *draws;
-  int *path, *count, *token;
-  long ld, ldq, S, V, max_nodes, dtype;
-};
-
-extern "C" int dsp_tree_verify(const DspTreeVerify* p, cudaStream_t stream) {
-  if (p->S == 0) return 0;
-  DSP_REQUIRE(p->S > 0 && p->V > 0 && p->V <= MAX_VOCAB, "dsp_tree_verify: a vocabulary of %ld (at most 393,216)", p->V);
-  DSP_REQUIRE(p->max_nodes > 0 && p->max_nodes <= MAX_NODES, "dsp_tree_verify: max_nodes=%ld", p->max_nodes);
-  DSP_REQUIRE(p->dtype == DSP_F32 || p->dtype == DSP_BF16, "dsp_tree_verify: unknown dtype %ld", p->dtype);
+// tensors: logits, draft probabilities (or none), tokens, parents, node_start, temperature, uniforms, draws, path, count, token.
+extern "C" int dsp_tree_verify(const DspTensor* t, const long* options, cudaStream_t stream) {
+  const DspTensor &logits = t[0], &draft = t[1], &tokens = t[2], &parents = t[3], &start = t[4], &temperature = t[5], &uniforms = t[6],
+                  &draws = t[7], &path = t[8], &count = t[9], &token = t[10];
+  const int dev = logits.device;
+  const long max_nodes = options[0];
+  DSP_REQUIRE(dev >= 0, "verify_tree: CUDA tensors only (there is no CPU path)");
+  DSP_REQUIRE(logits.dtype == DSP_T_F32 || logits.dtype == DSP_T_BF16, "verify_tree: kernels exist for float32 and bfloat16 logits");
+  DSP_REQUIRE(logits.dims == 2 && logits.stride[1] == 1 && logits.size[1] >= 1 && logits.size[1] <= MAX_VOCAB,
+              "verify_tree: logits must be [T, V] with neighbouring columns and V up to %d", MAX_VOCAB);
+  DSP_REQUIRE(temperature.dims == 1, "verify_tree: temperature must be one-dimensional");
+  const long T = logits.size[0], V = logits.size[1], S = temperature.size[0];
+  DSP_REQUIRE(tensor_is(tokens, DSP_T_I32, dev, 1, T) && tensor_is(parents, DSP_T_I32, dev, 1, T) && tensor_is(start, DSP_T_I32, dev, 1, S + 1),
+              "verify_tree: tokens [%ld], parents [%ld] and node_start [%ld] must be contiguous int32 on the device of the logits", T, T, S + 1);
+  DSP_REQUIRE(tensor_is(temperature, DSP_T_F32, dev, 1, S) && tensor_is(uniforms, DSP_T_F32, dev, 1, T) && tensor_is(draws, DSP_T_F32, dev, 1, S),
+              "verify_tree: temperature [%ld], uniforms [%ld] and draws [%ld] must be contiguous float32 on the device of the logits", S, T, S);
+  DSP_REQUIRE(draft.dims < 0 || (draft.dtype == DSP_T_F32 && draft.device == dev && draft.dims == 2 && draft.size[0] == T &&
+                                 draft.size[1] == V && draft.stride[1] == 1),
+              "verify_tree: draft_probs must be float32 [%ld, %ld] with neighbouring columns", T, V);
+  DSP_REQUIRE(max_nodes >= 1 && max_nodes <= MAX_NODES, "verify_tree: max_nodes %ld outside 1 .. %d", max_nodes, MAX_NODES);
+  DSP_REQUIRE(tensor_is(path, DSP_T_I32, dev, 2, S, max_nodes) && tensor_is(count, DSP_T_I32, dev, 1, S) && tensor_is(token, DSP_T_I32, dev, 1, S),
+              "verify_tree: results must be contiguous int32");
+  DSP_REQUIRE(T <= 0x7fffffff && S <= 0x7fffffff, "verify_tree: sizes out of range");
+  if (S == 0) return 0;
   Args a = {};
-  a.logits = p->logits;
-  a.draft = p->draft;
-  a.tokens = p->tokens;
-  a.parents = p->parents;
-  a.node_start = p->node_start;
-  a.temperature = p->temperature;
-  a.uniforms = p->uniforms;
-  a.draws = p->draws;
-  a.path = p->path;
-  a.count = p->count;
-  a.token = p->token;
-  a.ld = p->ld;
-  a.ldq = p->ldq;
-  a.V = (int)p->V;
-  a.max_nodes = (int)p->max_nodes;
+  a.logits = logits.data;
+  a.draft = draft.dims < 0 ? nullptr : (const float*)draft.data;
+  a.tokens = (const int*)tokens.data;
+  a.parents = (const int*)parents.data;
+  a.node_start = (const int*)start.data;
+  a.temperature = (const float*)temperature.data;
+  a.uniforms = (const float*)uniforms.data;
+  a.draws = (const float*)draws.data;
+  a.path = (int*)path.data;
+  a.count = (int*)count.data;
+  a.token = (int*)token.data;
+  a.ld = logits.stride[0];
+  a.ldq = draft.dims < 0 ? 0 : draft.stride[0];
+  a.V = (int)V;
+  a.max_nodes = (int)max_nodes;
   a.err = dsp_device_error_ptr();
-  DSP_REQUIRE(a.err != nullptr, "dsp_tree_verify: no device error word");
+  DSP_REQUIRE(a.err != nullptr, "verify_tree: no device error word");
   // CTAs a tree: as many as keep the device's SMs busy with the trees there are, at least 2,048 logits each, and so many
   // that two CTAs' shares fit an SM
   const int sms = dsp_num_sms(), fits = a.draft ? SHARE / 2 : SHARE;
   int ctas = 1;
-  while (ctas < MAX_CTAS && ((p->V + ctas - 1) / ctas > fits || (ctas * 2 * 2048 <= p->V && ctas * 2 * p->S <= 2 * sms))) ctas *= 2;
-  a.share = (int)(((p->V + ctas - 1) / ctas + 7) / 8 * 8);
-  const int S = (int)p->S;
-  const int rc = p->dtype == DSP_F32 ? (a.draft ? launch<float, true>(a, S, ctas, stream) : launch<float, false>(a, S, ctas, stream))
-                                     : (a.draft ? launch<bf16, true>(a, S, ctas, stream) : launch<bf16, false>(a, S, ctas, stream));
+  while (ctas < MAX_CTAS && ((V + ctas - 1) / ctas > fits || (ctas * 2 * 2048 <= V && ctas * 2 * S <= 2 * sms))) ctas *= 2;
+  a.share = (int)(((V + ctas - 1) / ctas + 7) / 8 * 8);
+  const bool f32 = logits.dtype == DSP_T_F32;
+  const int rc = f32 ? (a.draft ? launch<float, true>(a, (int)S, ctas, stream) : launch<float, false>(a, (int)S, ctas, stream))
+                     : (a.draft ? launch<bf16, true>(a, (int)S, ctas, stream) : launch<bf16, false>(a, (int)S, ctas, stream));
   if (rc != 0) return rc;
-  DSP_CHECK_LAUNCH("dsp_tree_verify");
+  DSP_CHECK_LAUNCH("verify_tree");
   return 0;
 }

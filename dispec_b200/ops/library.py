@@ -101,6 +101,26 @@ def mixer_library(name: str) -> ctypes.CDLL:
     return _special[name]
 
 
+_describe = None
+
+
+def describe():
+    """The function that packs what C code has to know of tensors (``csrc/describe.cpp``)."""
+    global _describe
+    if _describe is None:
+        import importlib.machinery
+        import importlib.util
+
+        with _lock:
+            if _describe is None:
+                path = build.describe_module()
+                loader = importlib.machinery.ExtensionFileLoader("dispec_b200_describe", path)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("dispec_b200_describe", loader))
+                loader.exec_module(module)
+                _describe = module.describe
+    return _describe
+
+
 def loaded_libraries() -> list[str]:
     out = [] if _core is None else [_core._name]
     return out + [lib._name for lib in _special.values()]

@@ -8,7 +8,6 @@ keeps its key and value at place ``ctx_len[s] + i`` of its request's cache until
 of the accepted branch."""
 from __future__ import annotations
 
-import ctypes
 import struct
 from dataclasses import dataclass
 
@@ -16,47 +15,24 @@ import torch
 
 from dispec_b200.ops import library as L
 from dispec_b200.ops import tuning
-from dispec_b200.ops.attention import _TCGEN05_ERRORS, _device_error_address
 
-MAX_HEAD_DIM = 256
-TENSOR_CORE_ROWS, FMA_ROWS = 128, 32  # rows of a tile of the two attention kernels
-MAX_POOLS = 8
-MAX_VOCAB = 3 << 17  # of a verified tree: a row is shared by at most 16 CTAs
-MAX_TREE = 1024  # nodes of a tree that is verified
-_ATTENTION = struct.Struct("10q13qd")
-_VERIFY = struct.Struct("11q6q")
-_KEEP = struct.Struct("4q6q40q")
+_ATTENTION = struct.Struct("4qd")
+_VERIFY = struct.Struct("q")
 
 
 def _refuse(what: str, message: str):
     raise L.KernelError(f"{what}: {message}")
 
 
-# A call is made once a layer: the checks below cost a few microseconds of the host together, which is what a call on a small
-# batch takes on the device.
-def _is(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int) -> bool:
-    return t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous()
+# A call is made once a layer, and its checks are part of what it costs: tensors are described to the C entry points as they
+# are (types, devices, sizes, strides), which refuse what they cannot take.
+_tensor_core_calls: dict = {}  # (device, head size) -> address of the tensor-core kernel's entry point
 
 
-def _ints(what: str, name: str, t: torch.Tensor, shape: tuple, device: int) -> None:
-    if not _is(t, torch.int32, shape, device):
-        _refuse(what, f"{name} must be contiguous int32 {list(shape)} on cuda:{device}, not {t.dtype} {list(t.shape)} on {t.device}")
-
-
-def _table(what: str, table: torch.Tensor, seqs: int, device: int) -> None:
-    if table.dtype is not torch.int32 or table.get_device() != device or table.dim() != 2 or table.shape[0] < seqs \
-            or table.stride(1) != 1:
-        _refuse(what, f"page_table must be int32 [{seqs}, pages] on cuda:{device} with neighbouring pages side by side")
-
-
-_tensor_core_calls: dict = {}  # (device, head size) -> entry point, address of the merge, address of the error word
-
-
-def _tensor_core_call(device: int, dim: int):
+def _tensor_core_call(device: int, dim: int) -> int:
     call = _tensor_core_calls.get((device, dim))
     if call is None:
-        call = (getattr(L.tree_attention_library(dim), f"dsp_tree_attention_tcgen05_d{dim}"),
-                ctypes.c_void_p(L.address_of(L.core(), "dsp_tree_combine")), ctypes.c_void_p(_device_error_address(device)))
+        call = L.address_of(L.tree_attention_library(dim), f"dsp_tree_attention_tcgen05_d{dim}")
         _tensor_core_calls[(device, dim)] = call
     return call
 
@@ -82,62 +58,28 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     what = "tree_attention"
     if not q.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")
-    if q.dim() != 2 or k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
-        _refuse(what, f"q [T, H * D] and two pools [pages, heads, page_size, D] expected, got {list(q.shape)}, "
-                      f"{list(k_pool.shape)} and {list(v_pool.shape)}")
-    T, S, dev = q.shape[0], ctx_len.shape[0], q.get_device()
-    num_pages, kv_heads, page_size, dim = k_pool.shape
-    columns, dtype = q.shape[1], q.dtype
-    code = L.dtype_code(dtype)
-    if k_pool.dtype is not dtype or v_pool.dtype is not dtype or k_pool.get_device() != dev or v_pool.get_device() != dev:
-        _refuse(what, f"q ({dtype}) and the pools ({k_pool.dtype}, {v_pool.dtype}) must be of one type on one device")
-    if not (k_pool.is_contiguous() and v_pool.is_contiguous()) or (T > 1 and q.stride(1) != 1):
-        _refuse(what, "the pools must be contiguous and the columns of q neighbours")
-    heads = columns // dim if dim else 0
-    if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM or heads * dim != columns or heads == 0 or heads % kv_heads:
-        _refuse(what, f"{columns} query columns on {kv_heads} heads of {dim} (a multiple of 8 up to {MAX_HEAD_DIM})")
-    words = visible.shape[1] if visible.dim() == 2 else 0
-    if not _is(visible, torch.int64, (T, words), dev) or 64 * words < max_nodes:
-        _refuse(what, f"visible must be contiguous int64 [{T}, words] with a bit for each of {max_nodes} nodes")
-    if not scale > 0.0 or window < 0 or max_nodes < 1:
-        _refuse(what, f"scale {scale} must be positive, window {window} not negative, max_nodes {max_nodes} at least 1")
-    _ints(what, "ctx_len", ctx_len, (S,), dev)
-    _ints(what, "node_start", node_start, (S + 1,), dev)
-    _table(what, page_table, S, dev)
-    if depth is not None:
-        _ints(what, "depth", depth, (T,), dev)
-    elif window:
-        _refuse(what, "a window needs the depths of the nodes")
     if out is None:
-        out = q.new_empty((T, columns))
-    elif out.shape != (T, columns) or out.dtype is not dtype or out.get_device() != dev or (T > 1 and out.stride(1) != 1):
-        _refuse(what, f"out must be {dtype} [{T}, {columns}] with neighbouring columns")
-    if T == 0 or S == 0:
-        return out
-    ctas = tuning._sm_count.get(dev) or tuning.sm_count(dev)
-    # the tensor-core kernel is built for these head and page sizes; bfloat16 in others and float32 take the 32-bit kernel
-    tensor_cores = code == L.BF16 and dim in (64, 128) and page_size in (8, 16, 32, 64) and num_pages > 0
-    rows = TENSOR_CORE_ROWS if tensor_cores else FMA_ROWS
-    # a multiple of the row tiles that trees have: then those of one head read its keys at the same time
-    row_tiles = -(-max_nodes * (heads // kv_heads) // rows)
-    if row_tiles < ctas:
-        ctas -= ctas % row_tiles
-    # scratch of this call alone (calls on several streams do not meet in it): two partial results for each CTA, and what
-    # the merge has to know of it
-    scratch = node_start.new_empty(2 * ctas * rows * (dim + 2) + 8 * ctas)
-    args = _ATTENTION.pack(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), ctx_len.data_ptr(), node_start.data_ptr(),
-        0 if depth is None else depth.data_ptr(), visible.data_ptr(), out.data_ptr(), scratch.data_ptr(), q.stride(0),
-        out.stride(0), page_table.stride(0), words, S, heads, kv_heads, dim, page_size, num_pages, window, code, ctas, scale)
-    if tensor_cores:
-        kernel, combine, error_word = _tensor_core_call(dev, dim)
-        rc = kernel(args, combine, error_word, L.stream_handle())
-        L.LaunchCounter.n += 2
-        if rc != 0:
-            _refuse(what, _TCGEN05_ERRORS.get(rc, str(rc)))
-    else:
-        L.check(L.core().dsp_tree_attention(args, L.stream_handle()), launches=2)
+        out = q.new_empty(q.shape)
+    dev, dim = q.get_device(), k_pool.shape[-1] if k_pool.dim() else 0
+    sms = tuning._sm_count.get(dev) or tuning.sm_count(dev)
+    # the tensor-core kernel is built for these head sizes
+    tensor_cores = _tensor_core_call(dev, dim) if q.dtype is torch.bfloat16 and dim in (64, 128) else 0
+    # scratch of this call alone (calls on several streams do not meet in it): two partial results of 128 rows, or of 32, for
+    # each CTA, and what the merge has to know of it
+    scratch = node_start.new_empty(sms * (2 * (128 if tensor_cores else 32) * (dim + 2) + 8))
+    tensors = (_describe or _load_describe())(q, k_pool, v_pool, page_table, ctx_len, node_start, depth, visible, out, scratch)
+    L.check(L.core().dsp_tree_attention(tensors, _ATTENTION.pack(max_nodes, window, sms, tensor_cores, scale),
+                                        L.stream_handle()), launches=2)
     return out
+
+
+_describe = None
+
+
+def _load_describe():
+    global _describe
+    _describe = L.describe()
+    return _describe
 
 
 def ancestors(parents: list) -> tuple[list, list]:
@@ -181,29 +123,11 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     what = "verify_tree"
     if not logits.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")
-    if logits.dim() != 2 or logits.stride(1) != 1 or not 1 <= logits.shape[1] <= MAX_VOCAB:
-        _refuse(what, f"logits must be [T, V] with neighbouring columns and V up to {MAX_VOCAB}, not {list(logits.shape)}")
-    (T, V), S, dev = logits.shape, temperature.shape[0], logits.get_device()
-    code = L.dtype_code(logits.dtype)
-    _ints(what, "tokens", tokens, (T,), dev)
-    _ints(what, "parents", parents, (T,), dev)
-    _ints(what, "node_start", node_start, (S + 1,), dev)
-    if not (_is(temperature, torch.float32, (S,), dev) and _is(uniforms, torch.float32, (T,), dev)
-            and _is(draws, torch.float32, (S,), dev)):
-        _refuse(what, f"temperature [{S}], uniforms [{T}] and draws [{S}] must be contiguous float32 on cuda:{dev}")
-    if draft_probs is not None and (draft_probs.dtype is not torch.float32 or draft_probs.get_device() != dev
-                                    or draft_probs.shape != (T, V) or draft_probs.stride(1) != 1):
-        _refuse(what, f"draft_probs must be float32 [{T}, {V}] with neighbouring columns on cuda:{dev}")
-    if not 1 <= max_nodes <= MAX_TREE:
-        _refuse(what, f"max_nodes {max_nodes} outside 1 .. {MAX_TREE}")
-    count, path, token = tokens.new_empty(S), tokens.new_empty((S, max_nodes)), tokens.new_empty(S)
-    if S:
-        draft, ldq = (0, 0) if draft_probs is None else (draft_probs.data_ptr(), draft_probs.stride(0))
-        args = _VERIFY.pack(
-            logits.data_ptr(), draft, tokens.data_ptr(), parents.data_ptr(), node_start.data_ptr(), temperature.data_ptr(),
-            uniforms.data_ptr(), draws.data_ptr(), path.data_ptr(), count.data_ptr(), token.data_ptr(), logits.stride(0), ldq,
-            S, V, max_nodes, code)
-        L.check(L.core().dsp_tree_verify(args, L.stream_handle()))
+    S = temperature.shape[0]
+    count, path, token = tokens.new_empty(S), tokens.new_empty((S, max_nodes if max_nodes > 0 else 0)), tokens.new_empty(S)
+    tensors = (_describe or _load_describe())(logits, draft_probs, tokens, parents, node_start, temperature, uniforms, draws,
+                                              path, count, token)
+    L.check(L.core().dsp_tree_verify(tensors, _VERIFY.pack(max_nodes), L.stream_handle()))
     return Verified(count, path, token)
 
 
@@ -215,30 +139,7 @@ def keep_path(pools: list, page_table: torch.Tensor, ctx_len: torch.Tensor, path
     all with the pages of ``page_table`` [S, pages of a request]; ``path`` int32 [S, n] ascends within a tree, as
     ``verify_tree`` gives it (one that does not is left from there on and recorded as a device error)."""
     what = "keep_path"
-    if not pools or len(pools) > MAX_POOLS:
-        _refuse(what, f"{len(pools)} pools (1 to {MAX_POOLS})")
-    if not pools[0].is_cuda:
-        _refuse(what, "CUDA tensors only (there is no CPU path)")
-    dev, S = pools[0].get_device(), ctx_len.shape[0]
-    page_size = pools[0].shape[3] if pools[0].dim() == 5 else 0
-    flat = []
-    for p in pools:
-        if p.dim() != 5 or p.shape[3] != page_size or not p.is_contiguous() or p.get_device() != dev:
-            _refuse(what, f"a pool must be contiguous [layers, pages, heads, {page_size}, width] on cuda:{dev}, not {list(p.shape)}")
-        layers, pages, heads, _, width = p.shape
-        address, row = p.data_ptr(), width * p.element_size()
-        if row % 16 or address % 16:
-            _refuse(what, f"rows of {row} bytes (whole 16-byte pieces are moved)")
-        flat += (address, layers, pages, heads, row)
-    _ints(what, "ctx_len", ctx_len, (S,), dev)
-    _ints(what, "count", count, (S,), dev)
-    _table(what, page_table, S, dev)
-    if path.dim() != 2:
-        _refuse(what, f"path must be [S, n], not {list(path.shape)}")
-    _ints(what, "path", path, (S, path.shape[1]), dev)
-    if S == 0 or path.shape[1] == 0:
-        return
-    flat += [0] * (5 * MAX_POOLS - len(flat))
-    args = _KEEP.pack(page_table.data_ptr(), ctx_len.data_ptr(), path.data_ptr(), count.data_ptr(), page_table.stride(0),
-                      path.stride(0), path.shape[1], page_size, S, len(pools), *flat)
-    L.check(L.core().dsp_tree_keep(args, L.stream_handle()))
+    if not pools or not pools[0].is_cuda:
+        _refuse(what, "CUDA tensors only (there is no CPU path)" if pools else "no pools")
+    tensors = (_describe or _load_describe())(page_table, ctx_len, path, count, *pools)
+    L.check(L.core().dsp_tree_keep(tensors, len(pools), L.stream_handle()))
