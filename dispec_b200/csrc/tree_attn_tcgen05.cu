@@ -142,7 +142,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ int failed_share;  // the first share in which one did: the block leaves together behind that share's barrier
   __shared__ uint32_t bad_pages[BAD_SLOTS];  // of key tile n, in slot n % BAD_SLOTS; bit j: page j had no valid id (not loaded)
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Shape& sh = p.a.sh;
   const int G = sh.G;
   unsigned char* k_s = smem;  // [stage][slice][64 keys][128 bytes]
@@ -152,11 +152,11 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   Walk w;  // warp 0's
   bool more = false;
   if (warp == 0) {
-    more = w.begin(sh, cta, gridDim.x);
+    more = w.begin(sh, blockIdx.x, gridDim.x);
     if (lane == 0) {
       if (!more) w.at.seq = -1;
       shares[0] = w.at;
-      p.a.scratch.splits[cta].parts = 0;  // (stays where there is no work, or a wait runs out)
+      p.a.scratch.splits[w.cta].parts = 0;  // (stays where there is no work, or a wait runs out)
     }
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -409,12 +409,12 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const int n_kt = t.kt_end - t.kt_begin;
     if (warp == 0) {
       request(t, n_kt, done);
-      const Split split = w.split(sh, cta);
-      more = w.next(sh, cta);
+      const Split split = w.split(sh);
+      more = w.next(sh);
       if (lane == 0) {
         if (!more) {
           w.at.seq = -1;
-          p.a.scratch.splits[cta] = split;
+          p.a.scratch.splits[w.cta] = split;
         }
         shares[(share + 1) % SHARES] = w.at;
       }

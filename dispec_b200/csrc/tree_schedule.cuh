@@ -84,14 +84,17 @@ struct Cut {
 // Where a CTA's run begins.
 struct Found {
   Cut cut;
+  int cta;                  // whose run it is
   int seq, row_tile, start; // the tree (-1: the run is empty), the row tile, first unit of that tree in that row tile
   Tree tree;
 };
-// Called by whole warps.  The trees of up to 64 requests are read once.
-__device__ __forceinline__ Found find_run(const Shape& sh, int cta, int ctas) {
+// Called by whole warps.  The trees of up to 64 requests are read once.  Block b has the run of CTA b; with runs per row tile, the
+// blocks take the row tiles in turn, so that where there are fewer units than CTAs the blocks with one lie on as many SMs.
+__device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) {
   constexpr int HELD = 2;
   const int lane = threadIdx.x & 31;
   Found f = {};
+  f.cta = block;
   f.seq = -1;
   Tree held[HELD];
   int all = 0, of_first = 0, most = 0;
@@ -122,7 +125,11 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int cta, int ctas) {
   cut.per_row_tile = most > 1 && most <= ctas && (long)most * cut.of_first == cut.total ? ctas / most : 0;
   cut.chunk = cut.per_row_tile > 0 ? (cut.of_first + cut.per_row_tile - 1) / cut.per_row_tile : (cut.total + ctas - 1) / ctas;
   cut.chunk = max(cut.chunk, sh.min_units);
-  if (cut.per_row_tile > 0 && cta >= cut.per_row_tile * most) return f;
+  if (cut.per_row_tile > 0) {
+    if (block >= cut.per_row_tile * most) return f;
+    f.cta = block % most * cut.per_row_tile + block / most;
+  }
+  const int cta = f.cta;
   const int u = cut.begin(cta);
   if (u >= cut.end(cta)) return f;
   // of lane's tree of the k-th 32 in a row tile
@@ -187,14 +194,16 @@ struct Split {
 
 // A CTA's walk over its run of units, one item's share at a time.
 struct Walk {
+  int cta;
   int u, end;
   Cut cut;
   int item_start, key_tiles, lo_tile;
   Share at;
 
   // Called by whole warps.  False: this CTA has no work.
-  __device__ __forceinline__ bool begin(const Shape& sh, int cta, int ctas) {
-    const Found f = find_run(sh, cta, ctas);
+  __device__ __forceinline__ bool begin(const Shape& sh, int block, int ctas) {
+    const Found f = find_run(sh, block, ctas);
+    cta = f.cta;
     if (f.seq < 0) return false;
     cut = f.cut;
     u = cut.begin(cta);
@@ -204,7 +213,7 @@ struct Walk {
     enter(f.tree);
     at.head = (u - f.start) / key_tiles;
     item_start = f.start + at.head * key_tiles;
-    share(cta);
+    share();
     return true;
   }
   __device__ __forceinline__ void enter(const Tree& t) {
@@ -214,14 +223,14 @@ struct Walk {
     key_tiles = t.key_tiles;
     lo_tile = t.lo_tile;
   }
-  __device__ __forceinline__ void share(int cta) {
+  __device__ __forceinline__ void share() {
     const int item_end = item_start + key_tiles, stop = min(end, item_end);
     at.kt_begin = lo_tile + (u - item_start);
     at.kt_end = at.kt_begin + (stop - u);
     at.slot = u == item_start ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
   }
   // What the merging kernel has to know of the present share (of the last one of the run, if that is an item's beginning).
-  __device__ __forceinline__ Split split(const Shape& sh, int cta) const {
+  __device__ __forceinline__ Split split(const Shape& sh) const {
     Split x = {};
     if (at.slot == 2 * cta + 1) {
       x.parts = cut.owner(item_start + key_tiles - 1) - cta + 1;
@@ -232,7 +241,7 @@ struct Walk {
     }
     return x;
   }
-  __device__ __forceinline__ bool next(const Shape& sh, int cta) {
+  __device__ __forceinline__ bool next(const Shape& sh) {
     u += at.kt_end - at.kt_begin;
     if (u >= end) return false;
     item_start = u;
@@ -248,7 +257,7 @@ struct Walk {
       } while (t.row_tiles <= at.row_tile);
       enter(t);
     }
-    share(cta);
+    share();
     return true;
   }
 };

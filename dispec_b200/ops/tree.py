@@ -64,9 +64,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     sms = tuning._sm_count.get(dev) or tuning.sm_count(dev)
     # the tensor-core kernel is built for these head sizes
     tensor_cores = _tensor_core_call(dev, dim) if q.dtype is torch.bfloat16 and dim in (64, 128) else 0
-    # scratch of this call alone (calls on several streams do not meet in it): two partial results of 128 rows, or of 32, for
-    # each CTA, and what the merge has to know of it
-    scratch = node_start.new_empty(sms * (2 * (128 if tensor_cores else 32) * (dim + 2) + 8))
+    # scratch of this call alone (calls on several streams do not meet in it): two partial results of 128 rows for
+    # each CTA, or of 32 rows where there are two CTAs an SM, and what the merge has to know of it
+    scratch = node_start.new_empty(sms * (2 * (128 if tensor_cores else 64) * (dim + 2) + 16))
     tensors = (_describe or _load_describe())(q, k_pool, v_pool, page_table, ctx_len, node_start, depth, visible, out, scratch)
     L.check(L.core().dsp_tree_attention(tensors, _ATTENTION.pack(max_nodes, window, sms, tensor_cores, scale),
                                         L.stream_handle()), launches=2)
