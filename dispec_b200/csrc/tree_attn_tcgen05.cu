@@ -41,8 +41,13 @@ constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 constexpr int PV_WARP = 10, S1_WARP = 11;
 constexpr int KD = D / 64;
-constexpr int KV_SLICE = BN * 128;
-constexpr int KV_BYTES = KD * KV_SLICE;
+// A tile in shared memory: [group of 8 keys][slice of 64 columns][8 rows of 128 bytes].  So the steps from group to group are
+// equal wherever a page ends (pages are 8 keys or more), and a page's rows, all slices, are one TMA request (a
+// request costs the TMA unit about 145 cycles; by slices, scattered pages of 16 keys were 16 requests a tile: 2 trees behind
+// 32,768 tokens 66 us, now 57).
+constexpr int SLICE = 8 * 128;
+constexpr int GROUP = KD * SLICE;
+constexpr int KV_BYTES = BN / 8 * GROUP;
 constexpr int SMEM_BYTES = (K_STAGES + V_STAGES) * KV_BYTES + 1024;
 // tensor memory, 32-bit columns
 constexpr int S_COLS = BN;
@@ -110,6 +115,36 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// A tile as the B operand: K-major (keys; the leading offset is not used) or N-major (values; slices are the leading offset).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr, uint32_t leading) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);  // start address, 16-byte units
+  d |= (uint64_t)leading << 16;
+  d |= (uint64_t)(GROUP >> 4) << 32;             // between groups of 8 keys
+  d |= (uint64_t)1 << 46;                        // descriptor version of this architecture
+  d |= (uint64_t)2 << 61;                        // layout type: 128-byte swizzle
+  return d;
+}
+__device__ __forceinline__ void load_pages(void* dst, const CUtensorMap* map, uint64_t* bar, int group, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(group), "r"(page)
+      : "memory");
+}
+// A pool [pages][heads][page_size][D] seen as (64 columns, 8 keys, D / 64 slices, groups of 8 keys of a page's heads, pages):
+// a box is one head's rows of `pages_per_box` neighbouring pages.
+inline bool make_map_pages(CUtensorMap* map, const void* base, long num_pages, int heads, int page_size, int pages_per_box) {
+  EncodeTiled fn = encode_fn();
+  if (fn == nullptr || num_pages < pages_per_box) return false;
+  cuuint64_t dims[5] = {64u, 8u, (cuuint64_t)KD, (cuuint64_t)heads * (page_size / 8), (cuuint64_t)num_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)D * 2, 128u, (cuuint64_t)8 * D * 2, (cuuint64_t)heads * page_size * D * 2};
+  cuuint32_t box[5] = {64u, 8u, (cuuint32_t)KD, (cuuint32_t)(page_size / 8), (cuuint32_t)pages_per_box};
+  cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Multiplies a row's accumulators by alpha.
 __device__ __forceinline__ void rescale(uint32_t o_addr, float alpha) {
 #pragma unroll 1
@@ -145,7 +180,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Shape& sh = p.a.sh;
   const int G = sh.G;
-  unsigned char* k_s = smem;  // [stage][slice][64 keys][128 bytes]
+  unsigned char* k_s = smem;  // [stage] tiles
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
   pdl_wait();
@@ -214,7 +249,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 
   // Requests the tiles asked .. upto - 1 of a share, two a turn (`upto` is even or the share's last).
   auto request = [&](const Share& t, int upto, int first_tile) {
-    const int pages_per_tile = BN / p.a.page_size;
+    const int pages_per_tile = BN / p.a.page_size, groups = p.a.page_size >> 3;
     const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.a.page_size * 128u;
     const int ppt_shift = __ffs(pages_per_tile) - 1, page_shift = __ffs(p.a.page_size) - 1;  // powers of two here
     const int chunk_shift = 5 - ppt_shift, chunk_mask = (1 << chunk_shift) - 1;
@@ -279,8 +314,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
             mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
           }
           if (in_run) {  // the tile's pages lie one after the other in the pool: one request per operand
-            tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, head * p.a.page_size, pg, 0);
-            tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, head * p.a.page_size, pg, 0);
+            load_pages(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], head * groups, pg);
+            load_pages(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], head * groups, pg);
           }
         } else {
           give_up(share);
@@ -288,13 +323,9 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       if (!__all_sync(0xffffffffu, !mine || in_run)) {
         if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
-          const int row = (pg * sh.KVH + head) * p.a.page_size;
-          const int dst = page_in_tile * p.a.page_size * 128;
-#pragma unroll
-          for (int h = 0; h < KD; ++h) {
-            tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
-            tma_load_2d(v_s + my_sv * KV_BYTES + dst + h * KV_SLICE, &map_v, &v_full[my_sv], h * 64, row);
-          }
+          const int dst = page_in_tile * groups * GROUP;
+          load_pages(k_s + my_sk * KV_BYTES + dst, &map_k, &k_full[my_sk], head * groups, pg);
+          load_pages(v_s + my_sv * KV_BYTES + dst, &map_v, &v_full[my_sv], head * groups, pg);
         }
       }
       for (int u = 0; u < min(2, n_kt - asked); ++u) {
@@ -424,7 +455,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     } else if (warp == 1 || warp == S1_WARP) {
       // ---- score products of one softmax group
       const uint32_t idesc_s = umma_idesc(BM, BN);
-      const uint64_t k_desc0 = umma_desc(smem_u32(k_s));
+      const uint64_t k_desc0 = tile_desc(smem_u32(k_s), 1u);
       const uint32_t tmem_s = tmem_base + (uint32_t)(g * S_COLS);
       bool ok = true;
       if (g < n_kt) {
@@ -443,7 +474,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (uint32_t)(k >> 2), in = (uint32_t)(k & 3) * 32u;
-            umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * KV_SLICE + in) >> 4), idesc_s, k != 0);
+            umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * SLICE + in) >> 4), idesc_s, k != 0);
           }
           umma_commit(&s_full[g]);
           umma_commit(&k_empty[s]);
@@ -454,7 +485,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     } else if (warp == PV_WARP) {
       // ---- output products: O[g] += P[g] V of the share's tiles in turn
       const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
-      const uint64_t v_desc0 = umma_desc_mn(smem_u32(v_s), KV_SLICE);
+      const uint64_t v_desc0 = tile_desc(smem_u32(v_s), SLICE >> 4);
       bool ok = share == 0 || __all_sync(0xffffffffu, mbar_wait(&o_free, (share - 1) & 1));
       for (int b = 0; b < n_kt && ok; ++b) {
         const int og = b & 1, st = (done + b) % V_STAGES;
@@ -471,7 +502,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
             umma_a_tmem(tmem_base + (uint32_t)(O_COL + og * D), tmem_base + (uint32_t)(P_COL + og * P_COLS + k * 8),
-                        v_desc + (uint64_t)(k * 128), idesc_o, (b >= 2) || k != 0);
+                        v_desc + (uint64_t)(k * (2 * GROUP >> 4)), idesc_o, (b >= 2) || k != 0);
           umma_commit(&v_empty[st]);
           umma_commit(&o_done[og]);
         }
@@ -598,11 +629,12 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           const int key = key0 + key_row;
           const bool dead = key >= total || key < lo || ((bad >> (key_row >> page_shift)) & 1u);
           if (dead) {
-            const uint32_t row_addr = smem_u32(v_s + st * KV_BYTES) + (uint32_t)key_row * 128u + (uint32_t)(r & 1) * 64u;
+            const uint32_t row_addr = smem_u32(v_s + st * KV_BYTES) + (uint32_t)(key_row >> 3) * GROUP +
+                                      (uint32_t)(key_row & 7) * 128u + (uint32_t)(r & 1) * 64u;
 #pragma unroll
             for (int h = 0; h < KD; ++h)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * KV_SLICE + c * 16, make_uint4(0, 0, 0, 0));
+              for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * SLICE + c * 16, make_uint4(0, 0, 0, 0));
           }
           fence_async_smem();
         }
@@ -653,11 +685,12 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
   p.a.sh.min_units = 2;  // one tile for each softmax group
   p.scale_log2 = a->scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v, runs_k, runs_v;
-  const long rows = (long)a->num_pages * a->sh.KVH * page;
-  if (!make_map(&map_k, a->k_pool, rows, D, D, page) || !make_map(&map_v, a->v_pool, rows, D, D, page)) return 4;
+  if (!make_map_pages(&map_k, a->k_pool, a->num_pages, a->sh.KVH, page, 1) ||
+      !make_map_pages(&map_v, a->v_pool, a->num_pages, a->sh.KVH, page, 1))
+    return 4;
   // a pool of fewer pages than a key tile has gives no map of runs
-  p.page_runs = make_map_page_runs(&runs_k, a->k_pool, a->num_pages, a->sh.KVH, page, D, BN / page) &&
-                make_map_page_runs(&runs_v, a->v_pool, a->num_pages, a->sh.KVH, page, D, BN / page);
+  p.page_runs = make_map_pages(&runs_k, a->k_pool, a->num_pages, a->sh.KVH, page, BN / page) &&
+                make_map_pages(&runs_v, a->v_pool, a->num_pages, a->sh.KVH, page, BN / page);
   if (!p.page_runs) {
     runs_k = map_k;
     runs_v = map_v;
