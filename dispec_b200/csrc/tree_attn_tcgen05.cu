@@ -57,6 +57,9 @@ constexpr int P_COL = O_COL + 2 * D;
 constexpr int Q_COL = P_COL + 2 * P_COLS;
 constexpr int TMEM_COLS = 512;
 static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
+// Of eight weights, so many are formed on the multiply-add pipe: 64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128 on 8:
+// 266 us with none, 257 with three; in heads of 64, which have half of the products to a weight, none is as good.
+constexpr int EX2_FMA = D == 128 ? 3 : 0;
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
 struct Params {
@@ -115,6 +118,40 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// 2^x of two numbers up to 2^7 or so on the multiply-add pipe: x = n + f, n whole, |f| <= 1/2; 2^f by a polynomial of degree 3
+// (interpolation at the Chebyshev points of the interval: below 1.1e-4 off, a twentieth of the bfloat16 rounding of a
+// weight), times 2^n from n's bits, which are 0 at x <= -127.  -inf gives 0, NaN stays.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  constexpr float C0 = 0.99992454f, C1 = 0.69313675f, C2 = 0.24263948f, C3 = 0.05583828f;
+  constexpr float WHOLE = 12583039.f;  // 1.5 * 2^23 + 127: the sum's last bits are n + 127
+  x = make_float2(max_nan(x.x, -127.f), max_nan(x.y, -127.f));
+  const float2 t = add2(x, make_float2(WHOLE, WHOLE));
+  const float2 n = add2(t, make_float2(-WHOLE, -WHOLE));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(C3, C3), make_float2(C2, C2));
+  y = fma2(y, f, make_float2(C1, C1));
+  y = fma2(y, f, make_float2(C0, C0));
+  return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
 // A tile as the B operand: K-major (keys; the leading offset is not used) or N-major (values; slices are the leading offset).
 __device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr, uint32_t leading) {
   uint64_t d = 0;
@@ -143,6 +180,27 @@ inline bool make_map_pages(CUtensorMap* map, const void* base, long num_pages, i
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Four lanes' pieces change hands: piece k of the j-th of four neighbouring lanes becomes piece j of the k-th.
+__device__ __forceinline__ void transpose4(uint4 (&x)[4]) {
+#pragma unroll
+  for (int s = 1; s < 4; s <<= 1) {
+    const bool up = threadIdx.x & s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & s) continue;
+      uint4 v = up ? x[i] : x[i | s];
+      v.x = __shfl_xor_sync(0xffffffffu, v.x, s);
+      v.y = __shfl_xor_sync(0xffffffffu, v.y, s);
+      v.z = __shfl_xor_sync(0xffffffffu, v.z, s);
+      v.w = __shfl_xor_sync(0xffffffffu, v.w, s);
+      if (up)
+        x[i] = v;
+      else
+        x[i | s] = v;
+    }
+  }
 }
 
 // Multiplies a row's accumulators by alpha.
@@ -341,25 +399,53 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     }
   };
 
+  // Rows in global memory: a lane holds a row of the tile, but four neighbouring lanes read and write 64 bytes of each of their
+  // rows together (a row a lane, 16 bytes each, an instruction touches 32 lines: 3.5 us from a share's end to the next one's
+  // queries).  Where the four lanes' rows begin in a tensor of rows (node, head); `n` of them are there.
+  const int r4 = r & ~3;
+  struct Rows4 {
+    size_t at[4];
+    int n;
+  };
+  auto rows_of = [&](const Share& t, size_t stride) -> Rows4 {
+    Rows4 x;
+    const int first = t.row_tile * BM + r4;
+    int node = first / G, head = first - node * G;
+    x.n = min(4, t.n * G - first);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x.at[k] = (size_t)(t.first + node) * stride + (size_t)(t.head * G + head) * D;
+      if (++head == G) {
+        head = 0;
+        ++node;
+      }
+    }
+    return x;
+  };
+
   // The queries of a share: row r of the tile, lane r, two bfloat16 per column (rows past the item are zero).  In heads of 128
   // each group brings half of the columns, in heads of 64 group 1 brings them all.  Asked for first, put down later.
   constexpr int Q_PIECES = 8;  // of 16 bytes, a lane
   auto ask_queries = [&](const Share& t, uint4 (&x)[Q_PIECES]) {
-    const int rr = t.row_tile * BM + r;
-    const bool valid = rr < t.n * G;
-    const bf16* src = (const bf16*)p.a.q;
-    if (valid) src += (size_t)(t.first + rr / G) * p.a.q_stride + (size_t)(t.head * G + rr % G) * D + (D == 128 ? g * 64 : 0);
+    const Rows4 rows = rows_of(t, p.a.q_stride);
+    const bf16* q = (const bf16*)p.a.q + (D == 128 ? g * 64 : 0) + (lane & 3) * 8;
 #pragma unroll
-    for (int c = 0; c < Q_PIECES; ++c) x[c] = valid ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < Q_PIECES; ++c)
+      x[c] = c % 4 < rows.n ? __ldg(reinterpret_cast<const uint4*>(q + rows.at[c % 4] + c / 4 * 32)) : make_uint4(0, 0, 0, 0);
   };
   auto put_queries = [&](const Share& t, const uint4 (&x)[Q_PIECES]) {
     uint32_t y[32];
 #pragma unroll
-    for (int c = 0; c < Q_PIECES; ++c) {
-      y[4 * c] = x[c].x;
-      y[4 * c + 1] = x[c].y;
-      y[4 * c + 2] = x[c].z;
-      y[4 * c + 3] = x[c].w;
+    for (int h = 0; h < 2; ++h) {
+      uint4 z[4] = {x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+      transpose4(z);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        y[16 * h + 4 * c] = z[c].x;
+        y[16 * h + 4 * c + 1] = z[c].y;
+        y[16 * h + 4 * c + 2] = z[c].z;
+        y[16 * h + 4 * c + 3] = z[c].w;
+      }
     }
     __syncwarp();
     tmem_st32(lane_addr + (uint32_t)(Q_COL + (D == 128 ? g * 32 : 0)), y);
@@ -387,12 +473,10 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
-      bf16* dst = (bf16*)p.a.out;
-      float* part = p.a.scratch.part_o;
-      if (slot >= 0)
-        part += ((size_t)slot * BM + r) * D;
-      else if (row_ok)
-        dst += (size_t)(t.first + (row0 + r) / G) * p.a.out_stride + (size_t)(t.head * G + (row0 + r) % G) * D;
+      Rows4 rows;
+      if (slot < 0) rows = rows_of(t, p.a.out_stride);
+      bf16* out = (bf16*)p.a.out + (lane & 3) * 8;
+      float* part = p.a.scratch.part_o + ((size_t)slot * BM + r4) * D + (lane & 3) * 4;
 #pragma unroll 1
       for (int c0 = g * (D / 2); c0 < (g + 1) * (D / 2); c0 += 32) {
         uint32_t ov[32], ow[32];
@@ -408,20 +492,31 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 #pragma unroll
           for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * f0);
         }
-        if (row_ok && slot >= 0) {
+        if (slot >= 0) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
-        } else if (row_ok) {
+          for (int h = 0; h < 2; ++h) {
+            uint4 x[4];
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            uint4 x;
-            x.x = pack2(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]));
-            x.y = pack2(__uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3]));
-            x.z = pack2(__uint_as_float(ov[c + 4]), __uint_as_float(ov[c + 5]));
-            x.w = pack2(__uint_as_float(ov[c + 6]), __uint_as_float(ov[c + 7]));
-            *reinterpret_cast<uint4*>(dst + c0 + c) = x;
+            for (int c = 0; c < 4; ++c)
+              x[c] = make_uint4(ov[16 * h + 4 * c], ov[16 * h + 4 * c + 1], ov[16 * h + 4 * c + 2], ov[16 * h + 4 * c + 3]);
+            transpose4(x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (r4 + k < nrows) *reinterpret_cast<uint4*>(part + k * D + c0 + 16 * h) = x[k];
           }
+        } else {
+          uint4 x[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            x[c].x = pack2(__uint_as_float(ov[8 * c]), __uint_as_float(ov[8 * c + 1]));
+            x[c].y = pack2(__uint_as_float(ov[8 * c + 2]), __uint_as_float(ov[8 * c + 3]));
+            x[c].z = pack2(__uint_as_float(ov[8 * c + 4]), __uint_as_float(ov[8 * c + 5]));
+            x[c].w = pack2(__uint_as_float(ov[8 * c + 6]), __uint_as_float(ov[8 * c + 7]));
+          }
+          transpose4(x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < rows.n) *reinterpret_cast<uint4*>(out + rows.at[k] + c0) = x[k];
         }
         __syncwarp();
       }
@@ -573,10 +668,10 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            t0 = fmaxf(t0, fmaxf(__uint_as_float(a[c]), __uint_as_float(a[c + 1])));
-            t1 = fmaxf(t1, fmaxf(__uint_as_float(a[c + 2]), __uint_as_float(a[c + 3])));
-            t2 = fmaxf(t2, fmaxf(__uint_as_float(b[c]), __uint_as_float(b[c + 1])));
-            t3 = fmaxf(t3, fmaxf(__uint_as_float(b[c + 2]), __uint_as_float(b[c + 3])));
+            t0 = max3(t0, __uint_as_float(a[c]), __uint_as_float(a[c + 1]));
+            t1 = max3(t1, __uint_as_float(a[c + 2]), __uint_as_float(a[c + 3]));
+            t2 = max3(t2, __uint_as_float(b[c]), __uint_as_float(b[c + 1]));
+            t3 = max3(t3, __uint_as_float(b[c + 2]), __uint_as_float(b[c + 3]));
           }
           const float tmax = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;  // the scale is positive
           const float m_new = (tmax > m_run + RESCALE_STEP || m_run == -INFINITY) ? fmaxf(tmax, m_run) : m_run;
@@ -591,7 +686,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           for (int c = 0; c < 32; c += 2) {
             const float2 x = fma2(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), scale2, neg_m2);
             const float2 y = fma2(make_float2(__uint_as_float(b[c]), __uint_as_float(b[c + 1])), scale2, neg_m2);
-            const float2 ex = make_float2(ex2(x.x), ex2(x.y)), ey = make_float2(ex2(y.x), ex2(y.y));
+            const float2 ex = make_float2(ex2(x.x), ex2(x.y));
+            const float2 ey = c / 2 % 4 < EX2_FMA ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
             sum0 = add2(sum0, ex);
             sum1 = add2(sum1, ey);
             pk[c / 2] = pack2(ex.x, ex.y);
