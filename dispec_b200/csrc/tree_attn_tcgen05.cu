@@ -10,9 +10,9 @@
 //   warp 10     issues the output products;
 //   warps 2..9  two softmax groups of four warps: group g owns the key tiles g, g + 2, ... of a share with a score buffer,
 //               output accumulator, P, running maximum and sum of its own; thread r of a group owns row r.
-// The whole block meets once a share.  Behind that barrier the softmax warps ask for the next share's queries, merge the two
-// halves of the last one and store its rows (or leave a partial result); warp 0 has worked the next share out and asked for
-// its first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
+// The whole block meets once a share.  Behind that barrier the softmax warps put the share's queries down, which they asked for
+// before it, then merge the two halves of the last one and store its rows (or leave a partial result); warp 0 has worked the
+// share out and asked for its first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
 // its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output
 // product.  Every wait is bounded; one that runs out sets the device error word.
 #include "tcgen05_common.cuh"
@@ -36,7 +36,7 @@ constexpr int BM = 128, BN = 64, THREADS = 384;
 // other's has not) could take the slot's last phase but one for the phase it waits for.
 constexpr int K_STAGES = 6, V_STAGES = 6;
 static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing warp");
-constexpr int SHARES = 4;      // the shares remembered: the next one, the present one and the one whose rows are being stored
+constexpr int SHARES = 4;      // the shares remembered: the next two, the present one and the one whose rows are being stored
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 constexpr int PV_WARP = 10, S1_WARP = 11;
@@ -229,7 +229,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ __align__(8) uint64_t q_ready[2];            // the queries of a share with tiles for the group are in tensor memory
   __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
   __shared__ float2 merge_ml[2][2][BM];                   // a group's maximum and sum per row, by share in turn
-  __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 before the barrier in front of it
+  __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 in share k - 2 or before
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;        // a wait ran out
   __shared__ int failed_share;  // the first share in which one did: the block leaves together behind that share's barrier
@@ -242,15 +242,30 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
   pdl_wait();
-  Walk w;  // warp 0's
+  Walk w;  // warp 0's, a share ahead
   bool more = false;
+  auto step = [&](int share) {  // works that share out, the one behind the last
+    const Split split = w.split(sh);
+    more = w.next(sh);
+    if (lane == 0) {
+      if (!more) {
+        w.at.seq = -1;
+        p.a.scratch.splits[w.cta] = split;
+      }
+      shares[share % SHARES] = w.at;
+    }
+    __syncwarp();
+  };
   if (warp == 0) {
     more = w.begin(sh, blockIdx.x, gridDim.x);
     if (lane == 0) {
-      if (!more) w.at.seq = -1;
+      if (!more) {
+        w.at.seq = -1;
+        p.a.scratch.splits[w.cta].parts = 0;
+      }
       shares[0] = w.at;
-      p.a.scratch.splits[w.cta].parts = 0;  // (stays where there is no work, or a wait runs out)
     }
+    if (more) step(1);
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                  "r"(TMEM_COLS)
@@ -426,12 +441,12 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   // The queries of a share: row r of the tile, lane r, two bfloat16 per column (rows past the item are zero).  In heads of 128
   // each group brings half of the columns, in heads of 64 group 1 brings them all.  Asked for first, put down later.
   constexpr int Q_PIECES = 8;  // of 16 bytes, a lane
-  auto ask_queries = [&](const Share& t, uint4 (&x)[Q_PIECES]) {
+  auto ask_queries = [&](const Share& t, bool wanted, uint4 (&x)[Q_PIECES]) {
     const Rows4 rows = rows_of(t, p.a.q_stride);
     const bf16* q = (const bf16*)p.a.q + (D == 128 ? g * 64 : 0) + (lane & 3) * 8;
 #pragma unroll
     for (int c = 0; c < Q_PIECES; ++c)
-      x[c] = c % 4 < rows.n ? __ldg(reinterpret_cast<const uint4*>(q + rows.at[c % 4] + c / 4 * 32)) : make_uint4(0, 0, 0, 0);
+      x[c] = wanted && c % 4 < rows.n ? __ldg(reinterpret_cast<const uint4*>(q + rows.at[c % 4] + c / 4 * 32)) : make_uint4(0, 0, 0, 0);
   };
   auto put_queries = [&](const Share& t, const uint4 (&x)[Q_PIECES]) {
     uint32_t y[32];
@@ -527,6 +542,10 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     if (lane == 0) mbar_arrive(&o_free);
   };
 
+  uint4 x[Q_PIECES];  // the coming queries
+  const bool brings = D == 128 || g == 1;
+  if (warp >= 2 && warp < PV_WARP) ask_queries(shares[0], brings && shares[0].seq >= 0, x);
+
   // Every wait of a share is for something that happens in that share, or, in warp 0's requests for the coming one, for
   // slots that this share's tiles leave; the whole block passes the barrier at its end.
   for (;; ++share) {
@@ -535,18 +554,11 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const int n_kt = t.kt_end - t.kt_begin;
     if (warp == 0) {
       request(t, n_kt, done);
-      const Split split = w.split(sh);
-      more = w.next(sh);
-      if (lane == 0) {
-        if (!more) {
-          w.at.seq = -1;
-          p.a.scratch.splits[w.cta] = split;
-        }
-        shares[(share + 1) % SHARES] = w.at;
-      }
+      if (more) step(share + 2);
       asked = 0;
       // the coming share's first tiles: as many as slots that this share's tiles are sure to leave
-      if (more) request(w.at, min(K_STAGES - 2, w.at.kt_end - w.at.kt_begin), done + n_kt);
+      const Share& next = shares[(share + 1) % SHARES];
+      if (next.seq >= 0) request(next, min(K_STAGES - 2, next.kt_end - next.kt_begin), done + n_kt);
     } else if (warp == 1 || warp == S1_WARP) {
       // ---- score products of one softmax group
       const uint32_t idesc_s = umma_idesc(BM, BN);
@@ -605,14 +617,9 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       if (!ok) give_up(share);
     } else {
-      // ---- softmax groups: first the queries of this share, and the end of the last one while they come
-      {
-        uint4 x[Q_PIECES];
-        const bool brings = D == 128 || g == 1;
-        if (brings) ask_queries(t, x);
-        if (share > 0) finish(share - 1);
-        if (brings) put_queries(t, x);
-      }
+      // ---- softmax groups: first the queries of this share, asked for before, and the end of the last one while its scores form
+      if (brings) put_queries(t, x);
+      if (share > 0) finish(share - 1);
       const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
       const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
       const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
@@ -740,6 +747,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
+      const Share& next = shares[(share + 1) % SHARES];
+      ask_queries(next, brings && next.seq >= 0, x);
       // the group's last product of the share
       if (ok && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) ok = false;
       if (!ok) give_up(share);
@@ -758,7 +767,10 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (failed) {
-    if (threadIdx.x == 0) atomicOr(p.a.err, DSP_ERR_WAIT_LIMIT);
+    if (threadIdx.x == 0) {
+      atomicOr(p.a.err, DSP_ERR_WAIT_LIMIT);
+      p.a.scratch.splits[w.cta].parts = 0;
+    }
     // let copies that are still on their way land before the shared memory goes away
     for (int i = 0; i < 2000; ++i) __nanosleep(100);
   }
