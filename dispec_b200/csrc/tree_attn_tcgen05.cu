@@ -58,8 +58,8 @@ constexpr int Q_COL = P_COL + 2 * P_COLS;
 constexpr int TMEM_COLS = 512;
 static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 // Of eight weights, so many are formed on the multiply-add pipe: 64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128 on 8:
-// 266 us with none, 257 with three; in heads of 64, which have half of the products to a weight, none is as good.
-constexpr int EX2_FMA = D == 128 ? 3 : 0;
+// 230 us with none, 225 with two, 231 with three.  Heads of 64, with half of the products to a weight: none.
+constexpr int EX2_FMA = D == 128 ? 2 : 0;
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
 struct Params {
@@ -641,10 +641,13 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       for (int i = g; i < n_kt; i += 2, ++j, ++count) {
         const int key0 = (kt_begin + i) * BN;
         // what the row sees of a tile that not every row sees whole, while its scores are being formed
-        const bool some = key0 + BN > t.ctx || __any_sync(0xffffffffu, key0 < lo_r);
+        const bool some = key0 + BN > t.ctx || (sh.window > 0 && __any_sync(0xffffffffu, key0 < lo_r));
         unsigned long long seen = ~0ull;
         if (some && warp_ok) seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[g], count & 1))) {
+        // the tile's scores; and the group's previous O[g] += P V has to be complete before O[g] is rescaled and P[g] rewritten (no
+        // arrival for a tile comes before every warp's for the one before has been counted)
+        if (!__all_sync(0xffffffffu, j == 0 ? mbar_wait(&s_full[g], count & 1)
+                                            : mbar_wait_both(&s_full[g], count & 1, &o_done[g], (count - 1) & 1))) {
           ok = false;
           break;
         }
@@ -702,24 +705,11 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           }
           sum0 = add2(sum0, sum1);
           l_run = l_run * alpha + (sum0.x + sum0.y);
-          // the group's previous O[g] += P V must be complete before O[g] is rescaled and P[g] rewritten
-          if (j > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            if (__any_sync(0xffffffffu, alpha != 1.f)) rescale(o_addr, alpha);
-          }
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) rescale(o_addr, alpha);
           __syncwarp();
           tmem_st32(p_addr, pk);  // 64 bfloat16 in the 32 columns of the group's A operand
         } else {
           if (lane == 0) mbar_arrive(&s_free[g]);
-          // (no arrival for a tile before every warp's for the one before has been counted)
-          if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
-            ok = false;
-            break;
-          }
         }
         // value rows no row of this item may see: zero them (whole 128-byte rows, every slice)
         if (key0 < lo || key0 + BN > total || bad != 0u) {
