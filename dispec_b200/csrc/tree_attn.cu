@@ -288,76 +288,80 @@ tree_attn_kernel(const Args a) {
   } while (more);
 }
 
-// Every block makes out which CTAs began an item that others share (one read of the list, a thread each), and the warps of the
-// whole grid take those items' rows in turn.  A row's partial results are asked for eight at a time, maxima, sums and outputs
-// together: two latencies stand between the wait and the store.
+// Every block makes out which CTAs began an item that others share (one read of the list, a thread each), and the threads of the
+// whole grid take those items' rows in turn, four columns each.  A row's partial results are asked for eight at a time, maxima,
+// sums and outputs together: two latencies stand between the wait and the store.
 constexpr int COMBINE_THREADS = 256, COMBINE_WARPS = COMBINE_THREADS / 32, COMBINE_BLOCKS_PER_SM = 4;
 template <typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_BLOCKS_PER_SM)
 tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_stride, int G, int D, int R, int ctas) {
   __shared__ int items[COMBINE_THREADS];  // CTAs that began one
-  __shared__ int of_warp[COMBINE_WARPS];
+  __shared__ int of_warp[COMBINE_WARPS], rows_of_warp[COMBINE_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   pdl_wait();
   for (int c0 = 0; c0 < ctas; c0 += COMBINE_THREADS) {
     const bool has = c0 + tid < ctas && scratch.splits[c0 + tid].parts > 0;
+    const int most_rows = __reduce_max_sync(0xffffffffu, has ? scratch.splits[c0 + tid].rows : 0);
     // the same list in every block: in the order of the CTAs
     const uint32_t those = __ballot_sync(0xffffffffu, has);
     __syncthreads();
-    if (lane == 0) of_warp[warp] = __popc(those);
+    if (lane == 0) {
+      of_warp[warp] = __popc(those);
+      rows_of_warp[warp] = most_rows;
+    }
     __syncthreads();
-    int before = 0, n_items = 0;
+    int before = 0, n_items = 0, rows = 0;
 #pragma unroll
     for (int w = 0; w < COMBINE_WARPS; ++w) {
       before += w < warp ? of_warp[w] : 0;
       n_items += of_warp[w];
+      rows = max(rows, rows_of_warp[w]);
     }
     if (has) items[before + __popc(those & ((1u << lane) - 1u))] = c0 + tid;
     __syncthreads();
-    for (int i = blockIdx.x * COMBINE_WARPS + warp; i < n_items * R; i += gridDim.x * COMBINE_WARPS) {
-      // neighbouring warps take neighbouring rows
-      const int c = items[i / R], r = i % R;
+    const int quads = D / 4, pieces = n_items * rows * quads;
+    for (int i = blockIdx.x * COMBINE_THREADS + tid; i < pieces; i += gridDim.x * COMBINE_THREADS) {
+      // neighbouring threads take neighbouring columns and rows
+      const int row = i / quads, d = (i - row * quads) * 4, c = items[row / rows], r = row % rows;
       const Split x = scratch.splits[c];
       if (r >= x.rows) continue;
       const float2* ml = reinterpret_cast<const float2*>(scratch.part_ml);
       auto row_of = [&](int k) -> size_t { return (k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * R + r; };  // of the k-th part
       const int rr = x.row0 + r;
       T* dst = out + (size_t)(x.first + rr / G) * out_stride + (size_t)(x.head * G + rr % G) * D;
-      for (int d = lane * 4; d < D; d += 128) {
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < x.parts; k0 += 8) {
-          float4 v[8];
-          float2 p[8];
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < x.parts; k0 += 8) {
+        float4 v[8];
+        float2 p[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const size_t row = row_of(min(k0 + k, x.parts - 1));
-            p[k] = ml[row];
-            v[k] = load4(scratch.part_o + row * D + d);
-          }
-          float top = M;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (k0 + k >= x.parts) p[k] = make_float2(-INFINITY, 0.f);
-            top = fmaxf(top, p[k].x);
-          }
-          if (top == -INFINITY) continue;
-          const float w0 = exp2f(M - top);
-          L *= w0;
-          acc = make_float4(acc.x * w0, acc.y * w0, acc.z * w0, acc.w * w0);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (p[k].x == -INFINITY) continue;  // a part that saw no key
-            const float w = exp2f(p[k].x - top);
-            L = fmaf(w, p[k].y, L);
-            acc = make_float4(fmaf(w, v[k].x, acc.x), fmaf(w, v[k].y, acc.y), fmaf(w, v[k].z, acc.z), fmaf(w, v[k].w, acc.w));
-          }
-          M = top;
+        for (int k = 0; k < 8; ++k) {
+          const size_t at = row_of(min(k0 + k, x.parts - 1));
+          p[k] = ml[at];
+          v[k] = load4(scratch.part_o + at * D + d);
         }
-        const float inv = L > 0.f ? 1.f / L : 0.f;
-        store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k0 + k >= x.parts) p[k] = make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, p[k].x);
+        }
+        if (top == -INFINITY) continue;
+        const float w0 = exp2f(M - top);
+        L *= w0;
+        acc = make_float4(acc.x * w0, acc.y * w0, acc.z * w0, acc.w * w0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (p[k].x == -INFINITY) continue;  // a part that saw no key
+          const float w = exp2f(p[k].x - top);
+          L = fmaf(w, p[k].y, L);
+          acc = make_float4(fmaf(w, v[k].x, acc.x), fmaf(w, v[k].y, acc.y), fmaf(w, v[k].z, acc.z), fmaf(w, v[k].w, acc.w));
+        }
+        M = top;
       }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
   }
 }
