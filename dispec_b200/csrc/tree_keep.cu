@@ -6,12 +6,15 @@
 //
 // What bounds it: the bytes for large batches; for small ones the chain count, path -> page table -> row.  A block works
 // that chain out once for several layers, and a thread's loads of up to eight nodes are under way together.  8 trees of 28
-// layers 3.9 us; 64 trees of 48 layers with rows of 256 bytes 23.8 us, 3.8 TB/s, 0.58 of what a plain copy reaches.
+// layers 2.8 us; 64 trees of 48 layers with rows of 256 bytes 23.8 us, 3.8 TB/s, 0.58 of what a plain copy reaches.
 #include "tensor_checks.cuh"
 
 namespace {
-constexpr int MAX_POOLS = 8, THREADS = 256, AHEAD = 8;
-constexpr int ITEMS = 2;  // pieces of 16 bytes that a thread moves of every node, about: a block takes layers enough for that
+constexpr int MAX_POOLS = 8, THREADS = 128, AHEAD = 8;
+// Pieces of 16 bytes that a thread moves of every node, about: a block takes layers enough for that.  Few, where the SMs have room
+// for all blocks then (six an SM), since a thread takes them one after the other (8 trees of 28 layers: 2.8 us with one, 3.5 with
+// two, 5.4 with four); four otherwise, for the chain's sake (64 trees of 48 layers: 27.5, 24.3, 23.8).
+constexpr int FEW = 1, MANY = 4, BLOCKS_PER_SM = 6;
 
 struct Pool {
   unsigned char* data;  // [layers][pages][heads][page_size][row_bytes]
@@ -115,10 +118,18 @@ extern "C" int dsp_tree_keep(const DspTensor* t, int pools, cudaStream_t stream)
     const long layers = p.size[0], pages = p.size[1], heads = p.size[2], row = p.size[4] * (p.dtype == DSP_T_F32 ? 4 : 2);
     DSP_REQUIRE(row % 16 == 0 && row > 0 && (uintptr_t)p.data % 16 == 0, "keep_path: rows of %ld bytes (whole 16-byte pieces are moved)", row);
     if (layers == 0 || heads == 0) continue;  // (a pool without rows has no blocks)
-    const long row_pieces = heads * row / 16, per = min(layers, max(1L, ITEMS * THREADS / row_pieces));
-    a.pool[used++] = Pool{(unsigned char*)p.data, (int)layers, (int)heads, (int)(row / 16), (int)per, (int)((layers + per - 1) / per),
-                          pages * heads * page * row, (int)pages};
-    blocks += (layers + per - 1) / per;
+    a.pool[used++] = Pool{(unsigned char*)p.data, (int)layers, (int)heads, (int)(row / 16), 0, 0, pages * heads * page * row, (int)pages};
+  }
+  const long places = (long)dsp_num_sms() * BLOCKS_PER_SM;
+  for (int items = FEW; items <= MANY; items *= 2) {
+    blocks = 0;
+    for (int i = 0; i < used; ++i) {
+      Pool& p = a.pool[i];
+      p.layers_per_block = (int)min((long)p.layers, max(1L, (long)items * THREADS / ((long)p.heads * p.pieces)));
+      p.blocks = (p.layers + p.layers_per_block - 1) / p.layers_per_block;
+      blocks += p.blocks;
+    }
+    if (blocks * S <= places) break;
   }
   if (S == 0 || width == 0 || blocks == 0) return 0;
   a.page_table = (const int*)table.data;
