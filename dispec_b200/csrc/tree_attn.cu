@@ -21,7 +21,7 @@
 namespace {
 using namespace tree;
 
-constexpr int ROWS = 32, KEYS = 64, TX = 16, THREADS = 256, RI = ROWS / 16, KJ = KEYS / TX, LP = KEYS + 4;
+constexpr int ROW_SHIFT = 5, ROWS = 1 << ROW_SHIFT, KEYS = KEYS_PER_TILE, TX = 16, THREADS = 256, RI = ROWS / 16, KJ = KEYS / TX, LP = KEYS + 4;
 
 typedef DspTreeAttention Args;
 
@@ -433,7 +433,7 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   // the tensor-core kernel is built for these page sizes; everything else takes the 32-bit kernel
   const bool tensor_cores = o->tensor_cores != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
                             (page == 8 || page == 16 || page == 32 || page == 64) && pages > 0;
-  const long G = columns / D / KVH, rows = tensor_cores ? TREE_TENSOR_CORE_ROWS : ROWS;
+  const long G = columns / D / KVH, rows = tensor_cores ? 1 << ROW_SHIFT_TENSOR_CORES : ROWS;
   // a multiple of the row tiles that trees have: then those of one head read its keys at the same time
   const long row_tiles = (o->max_nodes * G + rows - 1) / rows;
   const long places = o->sms * (tensor_cores || D > 128 ? 1 : 2);  // (by shared memory two CTAs of the 32-bit kernel an SM)
@@ -447,7 +447,7 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   a.sh.S = (int)S;
   a.sh.KVH = (int)KVH;
   a.sh.G = (int)G;
-  a.sh.rows_per_tile = (int)rows;
+  a.sh.row_shift = tensor_cores ? ROW_SHIFT_TENSOR_CORES : ROW_SHIFT;
   a.sh.window = (int)o->window;
   a.q = q.data;
   a.k_pool = k.data;
@@ -474,7 +474,6 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
     const int rc = reinterpret_cast<Kernel>(o->tensor_cores)(&a, stream);
     DSP_REQUIRE(rc == 0, "tree_attention: %s", rc == 4 ? "shared memory opt-in or tensor map creation failed" : "launch failed");
   } else {
-    a.sh.keys_per_tile = KEYS;
     a.sh.min_units = 1;
     const int rc = q.dtype == DSP_T_F32 ? launch<float>(a, stream) : launch<bf16>(a, stream);
     if (rc != 0) return rc;

@@ -37,7 +37,7 @@ using namespace tree;
 
 constexpr int D = DSP_HEAD_DIM;
 static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
-constexpr int BM = 128, BN = 64, THREADS = 384;
+constexpr int BM = 1 << ROW_SHIFT_TENSOR_CORES, BN = KEYS_PER_TILE, THREADS = 384;
 // Key tiles of a share go to two issuing warps in turn, and each waits for its own tiles only.  With an even ring a slot's
 // tiles all belong to one of them; with an odd one a warp that is ahead (its tile landed, an older one of the
 // other's has not) could take the slot's last phase but one for the phase it waits for.
@@ -98,6 +98,7 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const S
     const int there = t.n - off;  // keys up to the tree's last node
     if (there < 64) drafted &= (1ull << there) - 1ull;
     if (p.a.sh.window > 0 && depth >= p.a.sh.window) {  // a tree deeper than the window
+#pragma unroll 1
       for (unsigned long long left = drafted; left != 0ull; left &= left - 1ull) {
         const int c = __ffsll((long long)left) - 1;
         if (p.a.depth[t.first + off + c] <= depth - p.a.sh.window) drafted &= ~(1ull << c);
@@ -349,6 +350,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       return -2;  // not wanted
     };
     if (asked == 0) pg_next = load_chunk(0);
+#pragma unroll 1
     for (; asked < upto; asked += 2) {
       const int in_chunk = asked & chunk_mask;
       if (in_chunk == 0) {
@@ -408,6 +410,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
           load_pages(v_s + my_sv * KV_BYTES + dst, &map_v, &v_full[my_sv], head * groups, pg);
         }
       }
+#pragma unroll 1
       for (int u = 0; u < min(2, n_kt - asked); ++u) {
         if (++sk == K_STAGES) {
           sk = 0;
@@ -555,17 +558,30 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
 
   // Every wait of a share is for something that happens in that share, or, in warp 0's requests for the coming one, for
   // slots that this share's tiles leave; the whole block passes the barrier at its end.
+#pragma unroll 1
   for (;; ++share) {
     const Share& t = shares[share % SHARES];
-    if (failed_share < share || t.seq < 0) break;  // (written before the last barrier; all see the same)
+    const bool sound = failed_share >= share, another = sound && t.seq >= 0;  // (written before the last barrier; all see the same)
+    if (!another) pdl_launch_dependents();
+    if (warp >= 2 && warp < PV_WARP) {
+      // the queries of this share, asked for before, and the end of the last one while its scores form
+      if (another && brings) put_queries(t, x);
+      if (share > 0 && sound) finish(share - 1);
+    }
+    if (!another) break;
     const int n_kt = t.kt_end - t.kt_begin;
     if (warp == 0) {
-      request(t, n_kt, done);
-      if (more) step(share + 2);
-      asked = 0;
-      // the coming share's first tiles: as many as slots that this share's tiles are sure to leave
-      const Share& next = shares[(share + 1) % SHARES];
-      if (next.seq >= 0) request(next, min(K_STAGES - 2, next.kt_end - next.kt_begin), done + n_kt);
+      // this share's tiles, then the coming one's first: as many as slots that this share's tiles are sure to leave
+#pragma unroll 1
+      for (int ahead = 0; ahead < 2; ++ahead) {
+        const Share& of = shares[(share + ahead) % SHARES];
+        if (of.seq < 0) break;
+        const int tiles = of.kt_end - of.kt_begin;
+        request(of, ahead ? min(K_STAGES - 2, tiles) : tiles, ahead ? done + n_kt : done);
+        if (ahead) break;
+        if (more) step(share + 2);
+        asked = 0;
+      }
     } else if (warp == 1 || warp == S1_WARP) {
       // ---- score products of one softmax group
       const uint32_t idesc_s = umma_idesc(BM, BN);
@@ -577,6 +593,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         ++active;
         tc_fence_after();
       }
+#pragma unroll 1
       for (int a = g; a < n_kt && ok; a += 2, ++count0) {
         const int s = (done + a) % K_STAGES, use = (done + a) / K_STAGES;
         ok = __all_sync(0xffffffffu, count0 == 0 ? mbar_wait(&k_full[s], use & 1)
@@ -601,6 +618,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
       const uint64_t v_desc0 = tile_desc(smem_u32(v_s), SLICE >> 4);
       bool ok = share == 0 || __all_sync(0xffffffffu, mbar_wait(&o_free, (share - 1) & 1));
+#pragma unroll 1
       for (int b = 0; b < n_kt && ok; ++b) {
         const int og = b & 1, st = (done + b) % V_STAGES;
         ok = __all_sync(0xffffffffu, mbar_wait_both(&v_full[st], ((done + b) / V_STAGES) & 1, &p_full[og],
@@ -624,9 +642,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       }
       if (!ok) give_up(share);
     } else {
-      // ---- softmax groups: first the queries of this share, asked for before, and the end of the last one while its scores form
-      if (brings) put_queries(t, x);
-      if (share > 0) finish(share - 1);
+      // ---- softmax groups
       const uint32_t s_addr = lane_addr + (uint32_t)(g * S_COLS);
       const uint32_t o_addr = lane_addr + (uint32_t)(O_COL + g * D);
       const uint32_t p_addr = lane_addr + (uint32_t)(P_COL + g * P_COLS);
@@ -645,6 +661,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       l_run = 0.f;
       bool ok = true;
       int j = 0;  // tiles of this group in this share
+#pragma unroll 1
       for (int i = g; i < n_kt; i += 2, ++j, ++count) {
         const int key0 = (kt_begin + i) * BN;
         // what the row sees of a tile that not every row sees whole, while its scores are being formed
@@ -661,6 +678,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         tc_fence_after();
         const uint32_t bad = bad_pages[(done + i) % BAD_SLOTS];
         if (bad != 0u)
+#pragma unroll 1
           for (int b = 0; b < BN >> page_shift; ++b)
             if ((bad >> b) & 1u)
               seen &= ~((p.a.page_size == 64 ? ~0ull : (1ull << p.a.page_size) - 1ull) << (b << page_shift));
@@ -758,9 +776,6 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     tc_fence_after();
     __syncwarp();
   }
-  pdl_launch_dependents();
-  if (share > 0 && failed_share >= share && warp >= 2 && warp < PV_WARP) finish(share - 1);
-
   tc_fence_before();
   __syncthreads();
   if (failed) {
@@ -769,6 +784,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       p.a.scratch.splits[w.cta].parts = 0;
     }
     // let copies that are still on their way land before the shared memory goes away
+#pragma unroll 1
     for (int i = 0; i < 2000; ++i) __nanosleep(100);
   }
   tc_fence_after();
@@ -786,7 +802,6 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
   const int page = a->page_size;
   Params p = {};
   p.a = *a;
-  p.a.sh.keys_per_tile = BN;
   p.a.sh.min_units = 2;  // one tile for each softmax group
   p.scale_log2 = a->scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v, runs_k, runs_v;

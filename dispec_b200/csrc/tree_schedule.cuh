@@ -20,8 +20,13 @@ namespace tree {
 struct Shape {
   const int* node_start;  // [S + 1] first row of each tree's nodes
   const int* ctx_len;     // [S] tokens stored in front of the tree
-  int S, KVH, G, rows_per_tile, keys_per_tile, window, min_units;
+  int S, KVH, G, window, min_units;
+  int row_shift;  // of a tile's query rows
+  __device__ __forceinline__ int rows_per_tile() const { return 1 << row_shift; }
 };
+// Sizes of tiles are powers of two, and shifts: with divisions the search for a CTA's run alone is 3,000 instructions, each of which
+// a CTA fetches to run it once.
+constexpr int KEY_SHIFT = 6, KEYS_PER_TILE = 1 << KEY_SHIFT;
 
 // One tree: sizes in units.
 struct Tree {
@@ -37,9 +42,9 @@ __device__ __forceinline__ Tree load_tree(const Shape& sh, int s) {
   t.ctx = max(0, sh.ctx_len[s]);
   // the root sees furthest back: keys from ctx - window + 1
   const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;
-  t.lo_tile = lo / sh.keys_per_tile;
-  t.key_tiles = t.n > 0 ? (t.ctx + t.n + sh.keys_per_tile - 1) / sh.keys_per_tile - t.lo_tile : 0;
-  t.row_tiles = (t.n * sh.G + sh.rows_per_tile - 1) / sh.rows_per_tile;
+  t.lo_tile = lo >> KEY_SHIFT;
+  t.key_tiles = t.n > 0 ? ((t.ctx + t.n + KEYS_PER_TILE - 1) >> KEY_SHIFT) - t.lo_tile : 0;
+  t.row_tiles = (t.n * sh.G + sh.rows_per_tile() - 1) >> sh.row_shift;
   return t;
 }
 // Units of a tree in one of its row tiles.
@@ -88,10 +93,10 @@ struct Found {
   int seq, row_tile, start; // the tree (-1: the run is empty), the row tile, first unit of that tree in that row tile
   Tree tree;
 };
-// Called by whole warps.  The trees of up to 64 requests are read once.  Block b has the run of CTA b; with runs per row tile, the
+// Called by whole warps.  The trees of up to 32 requests are read once.  Block b has the run of CTA b; with runs per row tile, the
 // blocks take the row tiles in turn, so that where there are fewer units than CTAs the blocks with one lie on as many SMs.
 __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) {
-  constexpr int HELD = 2;
+  constexpr int HELD = 1;
   const int lane = threadIdx.x & 31;
   Found f = {};
   f.cta = block;
@@ -109,6 +114,7 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
     of_first += units_of(sh, held[k]);
     most = max(most, held[k].row_tiles);
   }
+#pragma unroll 1
   for (int s = HELD * 32 + lane; s < sh.S; s += 32) {
     const Tree t = load_tree(sh, s);
     all += units_of(sh, t) * t.row_tiles;
@@ -135,10 +141,12 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
   // of lane's tree of the k-th 32 in a row tile
   auto units = [&](const Tree& t, int tile) -> int { return t.row_tiles > tile ? units_of(sh, t) : 0; };
   int before = 0;
+#pragma unroll 1
   for (int tile = 0;; ++tile) {
     int of_tile = 0;
 #pragma unroll
     for (int k = 0; k < HELD; ++k) of_tile += units(held[k], tile);
+#pragma unroll 1
     for (int s = HELD * 32 + lane; s < sh.S; s += 32) of_tile += units(load_tree(sh, s), tile);
     of_tile = warp_sum_int(of_tile);
     if (u >= before + of_tile) {
@@ -168,6 +176,7 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
       if (look(held[k], k * 32)) return f;
+#pragma unroll 1
     for (int s0 = HELD * 32; s0 < sh.S; s0 += 32) {
       Tree t = {};
       if (s0 + lane < sh.S) t = load_tree(sh, s0 + lane);
@@ -235,8 +244,8 @@ struct Walk {
     if (at.slot == 2 * cta + 1) {
       x.parts = cut.owner(item_start + key_tiles - 1) - cta + 1;
       x.first = at.first;
-      x.row0 = at.row_tile * sh.rows_per_tile;
-      x.rows = min(sh.rows_per_tile, at.n * sh.G - x.row0);
+      x.row0 = at.row_tile << sh.row_shift;
+      x.rows = min(sh.rows_per_tile(), at.n * sh.G - x.row0);
       x.head = at.head;
     }
     return x;
@@ -283,7 +292,7 @@ cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride,
                          int dtype, cudaStream_t stream);
 
 // The attention's arguments, checked.
-constexpr int TREE_TENSOR_CORE_ROWS = 128;  // rows_per_tile of the tensor-core kernel
+constexpr int ROW_SHIFT_TENSOR_CORES = 7;  // 128 rows a tile of the tensor-core kernel
 struct DspTreeAttention {
   tree::Shape sh;
   const void *q, *k_pool, *v_pool;
