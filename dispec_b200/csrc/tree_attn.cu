@@ -361,7 +361,7 @@ tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_str
         }
         M = top;
       }
-      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L == 0.f ? 0.f : 1.f / L;  // (NaN stays)
       store4(dst + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
   }

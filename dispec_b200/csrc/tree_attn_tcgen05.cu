@@ -13,9 +13,10 @@
 // The whole block meets once a share.  Behind that barrier the softmax warps put the share's queries down, which they asked for
 // before it, then merge the two halves of the last one and store its rows (or leave a partial result); warp 0 has worked the
 // share out and asked for its first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
-// its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output
-// product.  Every wait is bounded; one that runs out sets the device error word.  (A value that is not finite at a node hidden
-// from some rows of its tile reaches them as 0 times it: weights of 0 are multiplied like others here.)
+// its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output product, and
+// so are, in tiles that not every row sees whole, values that are not finite, which a weight of 0 would carry to rows that do
+// not see them: a row that does becomes NaN as a whole at the share's end.  Every wait is bounded; one that runs out sets the
+// device error word.
 //
 // What bounds it: not bytes and not the tensor pipe (512 of 1,250 cycles a key tile), but the softmax groups' chain per tile: scores
 // out of tensor memory, maximum, 64 exponentials a thread, weights back.  64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128
@@ -46,6 +47,7 @@ static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing 
 constexpr int SHARES = 4;      // the shares remembered: the next two, the present one and the one whose rows are being stored
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
+constexpr int ODD_SLOTS = 64;  // tiles of a share whose odd keys are told apart
 constexpr int PV_WARP = 10, S1_WARP = 11;
 constexpr int KD = D / 64;
 // A tile in shared memory: [group of 8 keys][slice of 64 columns][8 rows of 128 bytes].  So the steps from group to group are
@@ -68,6 +70,17 @@ static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 // 230 us with none, 225 with two, 231 with three.  Heads of 64, with half of the products to a weight: none.
 constexpr int EX2_FMA = D == 128 ? 2 : 0;
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
+
+// Two bfloat16 values: one that is not finite; the same with 0 in its place.
+__device__ __forceinline__ bool has_odd(uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t without_odd(uint32_t x) {
+  return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 
 struct Params {
   DspTreeAttention a;
@@ -106,6 +119,64 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const S
     }
   }
   return stored | drafted;
+}
+
+// A share's keys whose values are not all finite, in tiles that not every row sees whole.
+struct OddKeys {
+  unsigned long long keys[ODD_SLOTS];  // of the tile beside it (-1: none)
+  int tile[ODD_SLOTS];
+  int any;  // there are some; 2: in more tiles than are told apart
+  __device__ __forceinline__ void forget(int slot) {
+    keys[slot] = 0ull;
+    tile[slot] = -1;
+    if (slot == 0) any = 0;
+  }
+  __device__ __forceinline__ void add(int t, int key) {
+    const int slot = t % ODD_SLOTS, was = atomicCAS(&tile[slot], -1, t);
+    atomicOr(&keys[slot], 1ull << key);
+    atomicMax(&any, was == -1 || was == t ? 1 : 2);
+  }
+};
+
+// Whether a row sees one of them.  (A function of its own: its code stays out of the way.)
+__device__ __noinline__ bool sees_odd_keys(const Params& p, const Share& t, int node, const OddKeys& odd) {
+  if (odd.any == 2) return true;
+  const int depth = p.a.sh.window > 0 ? p.a.depth[node] : 0;
+#pragma unroll 1
+  for (int i = 0; i < ODD_SLOTS; ++i)
+    if (odd.keys[i] != 0ull && (seen_keys(p, t, node, depth, odd.tile[i] * BN) & odd.keys[i]) != 0ull) return true;
+  return false;
+}
+// By the 128 threads of a group, two a key: value rows that no row of the item may see become zeros (whole 128-byte rows, every
+// slice), and so do, in tiles that not every row sees whole, numbers that are not finite.
+__device__ __forceinline__ void clean_values(const Params& p, const Share& t, OddKeys& odd, uint32_t tile_addr, int tile, uint32_t bad, int r) {
+  const int key_row = r >> 1, key = tile * BN + key_row, window = p.a.sh.window;
+  const bool dead = key >= t.ctx + t.n || (window > 0 && key <= t.ctx - window) ||
+                    ((bad >> (key_row >> (__ffs(p.a.page_size) - 1))) & 1u);
+  const uint32_t row_addr = tile_addr + (uint32_t)(key_row >> 3) * GROUP + (uint32_t)(key_row & 7) * 128u + (uint32_t)(r & 1) * 64u;
+  const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll 1
+  for (int h = 0; h < KD; ++h) {
+    const uint32_t at = row_addr + h * SLICE;
+    uint4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = dead ? make_uint4(0, 0, 0, 0) : ld_shared16(at + c * 16);
+    // 0 times a number that is not finite is NaN, and so is every sum with it
+    __nv_bfloat162 sum = zero;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]), zero, sum);
+    }
+    const bool found = has_odd(*reinterpret_cast<const uint32_t*>(&sum));
+    if (!found && !dead) continue;
+    if (found) odd.add(tile, key_row);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      st_shared16(at + c * 16, make_uint4(without_odd(v[c].x), without_odd(v[c].y), without_odd(v[c].z), without_odd(v[c].w)));
+  }
+  fence_async_smem();
 }
 
 // a * b + c and a + b of two numbers at once
@@ -238,6 +309,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
   __shared__ float2 merge_ml[2][2][BM];                   // a group's maximum and sum per row, by share in turn
   __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 in share k - 2 or before
+  __shared__ OddKeys odd_of[3];  // of share k in k % 3
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;        // a wait ran out
   __shared__ int failed_share;  // the first share in which one did: the block leaves together behind that share's barrier
@@ -249,6 +321,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   unsigned char* k_s = smem;  // [stage] tiles
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
+  for (int i = tid; i < 3 * ODD_SLOTS; i += THREADS) odd_of[i / ODD_SLOTS].forget(i % ODD_SLOTS);
   pdl_wait();
   Walk w;  // warp 0's, a share ahead
   bool more = false;
@@ -494,8 +567,10 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const float M = fmaxf(ml0.x, ml1.x);
     const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - M);
     const float w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - M);
-    const float denom = ml0.y * w0 + ml1.y * w1;
-    const float inv = slot >= 0 ? 1.f : denom > 0.f ? 1.f / denom : 0.f;
+    float denom = ml0.y * w0 + ml1.y * w1;
+    if (odd_of[k % 3].any != 0 && row_ok && sees_odd_keys(p, t, t.first + (row0 + r) / G, odd_of[k % 3]))
+      denom = __int_as_float(0x7fc00000);
+    const float inv = slot >= 0 ? 1.f : denom == 0.f ? 0.f : 1.f / denom;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
       Rows4 rows;
@@ -654,18 +729,19 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
       const int node = row_ok ? t.first + (row0 + r) / G : t.first;
       const int depth = sh.window > 0 ? p.a.depth[node] : 0;
-      const int total = t.ctx + t.n;
-      const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;  // first key any row sees
+      // tiles that begin between these are seen whole by every row (no node is deeper than the tree has nodes)
+      const int all_before = t.ctx - BN, some_upto = sh.window > 0 ? t.ctx + t.n - 1 - sh.window : -1;
       const int lo_r = sh.window > 0 ? t.ctx + depth - sh.window + 1 : 0;
       m_run = -INFINITY;
       l_run = 0.f;
       bool ok = true;
       int j = 0;  // tiles of this group in this share
+      if (tid - 64 < ODD_SLOTS) odd_of[(share + 1) % 3].forget(tid - 64);  // (last read at the end of share - 2)
 #pragma unroll 1
       for (int i = g; i < n_kt; i += 2, ++j, ++count) {
         const int key0 = (kt_begin + i) * BN;
         // what the row sees of a tile that not every row sees whole, while its scores are being formed
-        const bool some = key0 + BN > t.ctx || (sh.window > 0 && __any_sync(0xffffffffu, key0 < lo_r));
+        const bool some = key0 > all_before || (sh.window > 0 && __any_sync(0xffffffffu, key0 < lo_r));
         unsigned long long seen = ~0ull;
         if (some && warp_ok) seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
         // the tile's scores; and the group's previous O[g] += P V has to be complete before O[g] is rescaled and P[g] rewritten (no
@@ -736,25 +812,14 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
         } else {
           if (lane == 0) mbar_arrive(&s_free[g]);
         }
-        // value rows no row of this item may see: zero them (whole 128-byte rows, every slice)
-        if (key0 < lo || key0 + BN > total || bad != 0u) {
+        // values that 0 as a weight would not keep out
+        if (key0 > all_before || key0 <= some_upto || bad != 0u) {
           const int st = (done + i) % V_STAGES;
           if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], ((done + i) / V_STAGES) & 1))) {
             ok = false;
             break;
           }
-          const int key_row = r >> 1;  // two threads per key row
-          const int key = key0 + key_row;
-          const bool dead = key >= total || key < lo || ((bad >> (key_row >> page_shift)) & 1u);
-          if (dead) {
-            const uint32_t row_addr = smem_u32(v_s + st * KV_BYTES) + (uint32_t)(key_row >> 3) * GROUP +
-                                      (uint32_t)(key_row & 7) * 128u + (uint32_t)(r & 1) * 64u;
-#pragma unroll
-            for (int h = 0; h < KD; ++h)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * SLICE + c * 16, make_uint4(0, 0, 0, 0));
-          }
-          fence_async_smem();
+          clean_values(p, t, odd_of[share % 3], smem_u32(v_s + st * KV_BYTES), kt_begin + i, bad, r);
         }
         __syncwarp();
         tmem_st_wait();

@@ -102,6 +102,31 @@ def test_attention_hidden_keys_may_be_anything(dtype, bad):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ctx,n,window", [(50, 6, 0), (64, 6, 0), (3000, 70, 0), (200, 9, 3), (1000, 40, 120)])
+def test_attention_hidden_values_may_be_anything(dtype, bad, dim, ctx, n, window):
+    """A value that a row does not see does not reach it, whatever its numbers are; one that it sees does."""
+    case = AttentionCase([(ctx, random_tree(n, random.Random(2))), (90, [-1, 0])], 28, 4, dim, dtype, window=window)
+    want, bound = case.plain()
+    depth = [int(d) for d in case.depth[:n]]
+    inside = lambda i, d: not window or d > depth[i] - window
+    # a node, and another one or a stored token that the deeper nodes do not see
+    last = ctx - window + 2 if window else ctx + n - 1
+    for j in (ctx + 2, last):
+        p, o = int(case.table[0, j // 16]), j % 16
+        case.v[p, :, o] = bad
+    hit = torch.tensor([case.sees(0, i, 2) and inside(i, depth[2]) or
+                        (inside(i, 2 - window) if window else case.sees(0, i, n - 1)) for i in range(n)])
+    assert 0 < int(hit.sum()) < n
+    got = case.run().double().cpu()
+    clear = torch.cat([~hit, torch.ones(2, dtype=torch.bool)])
+    assert ((got - want).abs() <= bound)[clear].all()
+    assert not torch.isfinite(got[:n][hit]).any()
+    no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("scale", [1e-4, 4.0])
 def test_attention_flat_and_sharp_weights(dtype, scale):
     AttentionCase(trees([(400, 9), (31, 4)]), 4, 2, 128, dtype, scale=scale).check()
