@@ -18,9 +18,9 @@
 // not see them: a row that does becomes NaN as a whole at the share's end.  Every wait is bounded; one that runs out sets the
 // device error word.
 //
-// What bounds it: not bytes and not the tensor pipe (512 of 1,250 cycles a key tile), but the softmax groups' chain per tile: scores
+// What bounds it: not bytes and not the tensor pipe (512 of 1,200 cycles a key tile), but the softmax groups' chain per tile: scores
 // out of tensor memory, maximum, 64 exponentials a thread, weights back.  64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128
-// on 8: 225 us, 0.57 PFLOP/s with the rows there are and 2.2 TB/s; 2 trees of 24 behind 32,768, 28 on 4: 52 us, 2.3 TB/s.  Two groups
+// on 8: 231 us, 0.55 PFLOP/s with the rows there are and 2.2 TB/s; 2 trees of 24 behind 32,768, 28 on 4: 52 us, 2.3 TB/s.  Two groups
 // of one row a thread: the accumulators, scores, weights and queries of 128 rows then fill tensor memory; a third group, or
 // key tiles of 128, has no room there.
 #include "tcgen05_common.cuh"
@@ -149,7 +149,8 @@ __device__ __noinline__ bool sees_odd_keys(const Params& p, const Share& t, int 
 }
 // By the 128 threads of a group, two a key: value rows that no row of the item may see become zeros (whole 128-byte rows, every
 // slice), and so do, in tiles that not every row sees whole, numbers that are not finite.
-__device__ __forceinline__ void clean_values(const Params& p, const Share& t, OddKeys& odd, uint32_t tile_addr, int tile, uint32_t bad, int r) {
+__device__ __forceinline__ void clean_values(const Params& p, const Share& t, OddKeys& odd, uint32_t tile_addr, int tile, uint32_t bad,
+                                             int r) {
   const int key_row = r >> 1, key = tile * BN + key_row, window = p.a.sh.window;
   const bool dead = key >= t.ctx + t.n || (window > 0 && key <= t.ctx - window) ||
                     ((bad >> (key_row >> (__ffs(p.a.page_size) - 1))) & 1u);
