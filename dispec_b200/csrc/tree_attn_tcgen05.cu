@@ -67,7 +67,7 @@ constexpr int Q_COL = P_COL + 2 * P_COLS;
 constexpr int TMEM_COLS = 512;
 static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 // Of eight weights, so many are formed on the multiply-add pipe: 64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128 on 8:
-// 230 us with none, 225 with two, 231 with three.  Heads of 64, with half of the products to a weight: none.
+// 241 us with none, 232 with two, 237 with three.  Heads of 64, with half of the products to a weight: no difference, none.
 constexpr int EX2_FMA = D == 128 ? 2 : 0;
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
