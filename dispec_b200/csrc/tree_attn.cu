@@ -406,7 +406,7 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   DSP_REQUIRE(k.dtype == q.dtype && v.dtype == q.dtype && k.device == q.device && v.device == q.device && k.contiguous && v.contiguous &&
                   v.size[0] == pages && v.size[1] == KVH && v.size[2] == page && v.size[3] == D,
               "tree_attention: the pools must be contiguous, alike, and of the type and on the device of q");
-  DSP_REQUIRE(T <= 1 || q.stride[1] == 1 || columns == 1, "tree_attention: the columns of q must be neighbours");
+  DSP_REQUIRE(T == 0 || q.stride[1] == 1 || columns == 1, "tree_attention: the columns of q must be neighbours");
   DSP_REQUIRE(D % 8 == 0 && D >= 8 && D <= 256 && KVH > 0 && columns > 0 && columns % D == 0 && columns / D % KVH == 0,
               "tree_attention: %ld query columns on %ld heads of %ld (a multiple of 8 up to 256)", columns, KVH, D);
   DSP_REQUIRE(ctx.dims == 1, "tree_attention: ctx_len must be one-dimensional");
@@ -422,7 +422,7 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   DSP_REQUIRE(depth.dims < 0 ? o->window == 0 : tensor_is(depth, DSP_T_I32, q.device, 1, T),
               "tree_attention: depth must be contiguous int32 [%ld]; a window needs it", T);
   DSP_REQUIRE(out.dtype == q.dtype && out.device == q.device && out.dims == 2 && out.size[0] == T && out.size[1] == columns &&
-                  (T <= 1 || out.stride[1] == 1),
+                  (T == 0 || out.stride[1] == 1 || columns == 1),
               "tree_attention: out must be like the queries [%ld, %ld] with neighbouring columns", T, columns);
   DSP_REQUIRE(T <= 0x7fffffff && S <= 0x7fffffff && pages <= 0x7fffffff && page >= 1 && o->sms >= 1, "tree_attention: sizes out of range");
   if (T == 0 || S == 0) return 0;
