@@ -347,6 +347,8 @@ tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_str
         for (int k = 0; k < 8; ++k) {
           if (k0 + k >= x.parts) p[k] = make_float2(-INFINITY, 0.f);
           top = fmaxf(top, p[k].x);
+          // a part without a largest score saw no key, and its sum is 0; or scores that are no numbers, and neither is its sum
+          if (p[k].x == -INFINITY) L += p[k].y;
         }
         if (top == -INFINITY) continue;
         const float w0 = exp2f(M - top);
@@ -354,7 +356,7 @@ tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_str
         acc = make_float4(acc.x * w0, acc.y * w0, acc.z * w0, acc.w * w0);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          if (p[k].x == -INFINITY) continue;  // a part that saw no key
+          if (p[k].x == -INFINITY) continue;
           const float w = exp2f(p[k].x - top);
           L = fmaf(w, p[k].y, L);
           acc = make_float4(fmaf(w, v[k].x, acc.x), fmaf(w, v[k].y, acc.y), fmaf(w, v[k].z, acc.z), fmaf(w, v[k].w, acc.w));
