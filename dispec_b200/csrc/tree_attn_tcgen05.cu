@@ -15,7 +15,7 @@
 // share out and asked for its first tiles before.  What a row sees of a tile that holds nodes of the tree is a mask of 64 bits, cut from
 // its words of `visible`.  Value rows that no row of the item may see are zeroed in shared memory before the output product, and
 // so are, in tiles that not every row sees whole, values that are not finite, which a weight of 0 would carry to rows that do
-// not see them: a row that does becomes NaN as a whole at the share's end.  Every wait is bounded; one that runs out sets the
+// not see them: behind the product they are added to the rows that do.  Every wait is bounded; one that runs out sets the
 // device error word.
 //
 // What bounds it: not bytes and not the tensor pipe (512 of 1,200 cycles a key tile), but the softmax groups' chain per tile: scores
@@ -47,7 +47,6 @@ static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing 
 constexpr int SHARES = 4;      // the shares remembered: the next two, the present one and the one whose rows are being stored
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
-constexpr int ODD_SLOTS = 64;  // tiles of a share whose odd keys are told apart
 constexpr int PV_WARP = 10, S1_WARP = 11;
 constexpr int KD = D / 64;
 // A tile in shared memory: [group of 8 keys][slice of 64 columns][8 rows of 128 bytes].  So the steps from group to group are
@@ -121,41 +120,16 @@ __device__ __forceinline__ unsigned long long seen_keys(const Params& p, const S
   return stored | drafted;
 }
 
-// A share's keys whose values are not all finite, in tiles that not every row sees whole.
-struct OddKeys {
-  unsigned long long keys[ODD_SLOTS];  // of the tile beside it (-1: none)
-  int tile[ODD_SLOTS];
-  int any;  // there are some; 2: in more tiles than are told apart
-  __device__ __forceinline__ void forget(int slot) {
-    keys[slot] = 0ull;
-    tile[slot] = -1;
-    if (slot == 0) any = 0;
-  }
-  __device__ __forceinline__ void add(int t, int key) {
-    const int slot = t % ODD_SLOTS, was = atomicCAS(&tile[slot], -1, t);
-    atomicOr(&keys[slot], 1ull << key);
-    atomicMax(&any, was == -1 || was == t ? 1 : 2);
-  }
-};
-
-// Whether a row sees one of them.  (A function of its own: its code stays out of the way.)
-__device__ __noinline__ bool sees_odd_keys(const Params& p, const Share& t, int node, const OddKeys& odd) {
-  if (odd.any == 2) return true;
-  const int depth = p.a.sh.window > 0 ? p.a.depth[node] : 0;
-#pragma unroll 1
-  for (int i = 0; i < ODD_SLOTS; ++i)
-    if (odd.keys[i] != 0ull && (seen_keys(p, t, node, depth, odd.tile[i] * BN) & odd.keys[i]) != 0ull) return true;
-  return false;
-}
 // By the 128 threads of a group, two a key: value rows that no row of the item may see become zeros (whole 128-byte rows, every
-// slice), and so do, in tiles that not every row sees whole, numbers that are not finite.
-__device__ __forceinline__ void clean_values(const Params& p, const Share& t, OddKeys& odd, uint32_t tile_addr, int tile, uint32_t bad,
-                                             int r) {
+// slice), and so do, in tiles that not every row sees whole, numbers that are not finite.  True: there was such a number in this
+// thread's half of a key that some row may see.
+__device__ __forceinline__ bool clean_values(const Params& p, const Share& t, uint32_t tile_addr, int tile, uint32_t bad, int r) {
   const int key_row = r >> 1, key = tile * BN + key_row, window = p.a.sh.window;
   const bool dead = key >= t.ctx + t.n || (window > 0 && key <= t.ctx - window) ||
                     ((bad >> (key_row >> (__ffs(p.a.page_size) - 1))) & 1u);
   const uint32_t row_addr = tile_addr + (uint32_t)(key_row >> 3) * GROUP + (uint32_t)(key_row & 7) * 128u + (uint32_t)(r & 1) * 64u;
   const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+  bool any = false;
 #pragma unroll 1
   for (int h = 0; h < KD; ++h) {
     const uint32_t at = row_addr + h * SLICE;
@@ -172,12 +146,61 @@ __device__ __forceinline__ void clean_values(const Params& p, const Share& t, Od
     }
     const bool found = has_odd(*reinterpret_cast<const uint32_t*>(&sum));
     if (!found && !dead) continue;
-    if (found) odd.add(tile, key_row);
+    any |= found;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       st_shared16(at + c * 16, make_uint4(without_odd(v[c].x), without_odd(v[c].y), without_odd(v[c].z), without_odd(v[c].w)));
   }
   fence_async_smem();
+  return any;
+}
+
+// By a whole warp, behind its group's last output product of a share: the values that clean_values took out of the group's tiles
+// are added to the rows that see their keys, in their own columns (a weight is positive, and changes nothing in what is not
+// finite).  They are read again where they lie, which costs nothing until there are some.  (A function of its own: its code
+// stays out of the way.)
+__device__ __noinline__ void add_odd_values(const Params& p, const Share& t, int g, int node, bool row_ok, uint32_t o_addr) {
+  const Shape& sh = p.a.sh;
+  const int* table = p.a.page_table + (size_t)t.seq * p.a.pt_stride;
+  const int depth = sh.window > 0 ? p.a.depth[node] : 0;
+#pragma unroll 1
+  for (int tile = t.kt_begin + g; tile < t.kt_end; tile += 2) {
+    const int key0 = tile * BN;
+    auto page_of = [&](int key) {
+      const int place = key / p.a.page_size, page = place < p.a.table_width ? table[place] : -1;
+      return page < p.a.num_pages ? page : -1;
+    };
+    // as in the walk: tiles that not every row sees whole, or with a page that is not there
+    bool cleaned = key0 > t.ctx - BN || (sh.window > 0 && key0 <= t.ctx + t.n - 1 - sh.window);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += p.a.page_size) cleaned |= page_of(key0 + c) < 0;
+    if (!cleaned) continue;
+    const unsigned long long seen = row_ok ? seen_keys(p, t, node, depth, key0) : 0ull;
+#pragma unroll 1
+    for (int c = 0; c < BN; ++c) {
+      const bool mine = (seen >> c) & 1ull;
+      const int page = page_of(key0 + c);
+      if (page < 0 || !__any_sync(0xffffffffu, mine)) continue;
+      const bf16* v = (const bf16*)p.a.v_pool + (((size_t)page * sh.KVH + t.head) * p.a.page_size + (key0 + c) % p.a.page_size) * D;
+      bool found = false;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) found |= !isfinite(__bfloat162float(v[c0 + (threadIdx.x & 31)]));
+      if (!__any_sync(0xffffffffu, found)) continue;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t ov[32];
+        tmem_ld32(o_addr + (uint32_t)c0, ov);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float x = __bfloat162float(v[c0 + k]);
+          if (mine && !isfinite(x)) ov[k] = __float_as_uint(__uint_as_float(ov[k]) + x);
+        }
+        __syncwarp();
+        tmem_st32(o_addr + (uint32_t)c0, ov);
+        tmem_st_wait();
+      }
+    }
+  }
 }
 
 // a * b + c and a + b of two numbers at once
@@ -310,7 +333,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   __shared__ __align__(8) uint64_t o_free;                // the last share's accumulators have been read
   __shared__ float2 merge_ml[2][2][BM];                   // a group's maximum and sum per row, by share in turn
   __shared__ Share shares[SHARES];                        // share k in k % SHARES, written by warp 0 in share k - 2 or before
-  __shared__ OddKeys odd_of[3];  // of share k in k % 3
+  __shared__ int odd_share[2];  // the last share in which a group took numbers out of the values
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;        // a wait ran out
   __shared__ int failed_share;  // the first share in which one did: the block leaves together behind that share's barrier
@@ -322,7 +345,6 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
   unsigned char* k_s = smem;  // [stage] tiles
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
-  for (int i = tid; i < 3 * ODD_SLOTS; i += THREADS) odd_of[i / ODD_SLOTS].forget(i % ODD_SLOTS);
   pdl_wait();
   Walk w;  // warp 0's, a share ahead
   bool more = false;
@@ -373,6 +395,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     mbar_init(&o_free, 8);
     failed = 0;
     failed_share = 0x7fffffff;
+    odd_share[0] = odd_share[1] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tc_fence_before();
@@ -568,9 +591,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     const float M = fmaxf(ml0.x, ml1.x);
     const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - M);
     const float w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - M);
-    float denom = ml0.y * w0 + ml1.y * w1;
-    if (odd_of[k % 3].any != 0 && row_ok && sees_odd_keys(p, t, t.first + (row0 + r) / G, odd_of[k % 3]))
-      denom = __int_as_float(0x7fc00000);
+    const float denom = ml0.y * w0 + ml1.y * w1;
     const float inv = slot >= 0 ? 1.f : denom == 0.f ? 0.f : 1.f / denom;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
@@ -737,7 +758,6 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       l_run = 0.f;
       bool ok = true;
       int j = 0;  // tiles of this group in this share
-      if (tid - 64 < ODD_SLOTS) odd_of[(share + 1) % 3].forget(tid - 64);  // (last read at the end of share - 2)
 #pragma unroll 1
       for (int i = g; i < n_kt; i += 2, ++j, ++count) {
         const int key0 = (kt_begin + i) * BN;
@@ -820,7 +840,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
             ok = false;
             break;
           }
-          clean_values(p, t, odd_of[share % 3], smem_u32(v_s + st * KV_BYTES), kt_begin + i, bad, r);
+          if (clean_values(p, t, smem_u32(v_s + st * KV_BYTES), kt_begin + i, bad, r)) odd_share[g] = share;
         }
         __syncwarp();
         tmem_st_wait();
@@ -831,7 +851,18 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
       const Share& next = shares[(share + 1) % SHARES];
       ask_queries(next, brings && next.seq >= 0, x);
       // the group's last product of the share
-      if (ok && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) ok = false;
+      if (ok && j > 0) {
+        if (__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
+          if (odd_share[g] == share && warp_ok) {  // (every warp of the group has arrived for that product)
+            tc_fence_after();
+            add_odd_values(p, t, g, node, row_ok, o_addr);
+            __syncwarp();
+            ask_queries(next, brings && next.seq >= 0, x);  // (asked for again: they need not live through the call)
+          }
+        } else {
+          ok = false;
+        }
+      }
       if (!ok) give_up(share);
       merge_ml[share & 1][g][r] = make_float2(m_run, l_run);
     }
