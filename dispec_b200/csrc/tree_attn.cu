@@ -440,6 +440,10 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   const long row_tiles = (o->max_nodes * G + rows - 1) / rows;
   const long places = o->sms * (tensor_cores || D > 128 ? 1 : 2);  // (by shared memory two CTAs of the 32-bit kernel an SM)
   const long ctas = row_tiles < places ? places - places % row_tiles : places;
+  // Key tiles are counted in 32 bits: those of all trees, each with as many stored tokens as its pages hold.
+  const long most_ctx = min(table.size[1] * page, 1L << 30);
+  DSP_REQUIRE(T * G <= 0x7fffffff && (T * G / rows + S) * KVH <= 0x7fffffff / ((most_ctx + T) / KEYS_PER_TILE + 1),
+              "tree_attention: %ld rows of %ld heads over pages for %ld tokens a request are too many for one call", T, G, most_ctx);
   DSP_REQUIRE(scratch.contiguous && scratch.device == q.device && scratch.dims == 1 && (uintptr_t)scratch.data % 16 == 0 &&
                   scratch.size[0] >= 2 * ctas * rows * (D + 2) + 8 * ctas,
               "tree_attention: scratch is too small");
@@ -451,6 +455,8 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   a.sh.G = (int)G;
   a.sh.row_shift = tensor_cores ? ROW_SHIFT_TENSOR_CORES : ROW_SHIFT;
   a.sh.window = (int)o->window;
+  a.sh.rows = (int)T;
+  a.sh.most_ctx = (int)most_ctx;
   a.q = q.data;
   a.k_pool = k.data;
   a.v_pool = v.data;
@@ -469,7 +475,7 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   a.num_pages = (int)pages;
   a.ctas = (int)ctas;
   a.scale = (float)o->scale;
-  a.err = dsp_device_error_ptr();
+  a.err = a.sh.err = dsp_device_error_ptr();
   DSP_REQUIRE(a.err != nullptr, "tree_attention: no device error word");
   if (tensor_cores) {
     typedef int (*Kernel)(const DspTreeAttention*, cudaStream_t);

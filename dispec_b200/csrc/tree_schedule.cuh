@@ -21,7 +21,10 @@ struct Shape {
   const int* node_start;  // [S + 1] first row of each tree's nodes
   const int* ctx_len;     // [S] tokens stored in front of the tree
   int S, KVH, G, window, min_units;
+  int rows;       // of the queries: a tree that is not inside them is recorded and has no nodes
+  int most_ctx;   // tokens that a request's pages hold: more are not stored (their places have no page, which is recorded there)
   int row_shift;  // of a tile's query rows
+  int* err;
   __device__ __forceinline__ int rows_per_tile() const { return 1 << row_shift; }
 };
 // Sizes of tiles are powers of two, and shifts: with divisions the search for a CTA's run alone is 3,000 instructions, each of which
@@ -37,9 +40,14 @@ struct Tree {
 
 __device__ __forceinline__ Tree load_tree(const Shape& sh, int s) {
   Tree t;
+  const int end = sh.node_start[s + 1];
   t.first = sh.node_start[s];
-  t.n = max(0, sh.node_start[s + 1] - t.first);
-  t.ctx = max(0, sh.ctx_len[s]);
+  t.n = end - t.first;
+  if (t.first < 0 || end < t.first || end > sh.rows) {
+    t.n = 0;
+    atomicOr(sh.err, DSP_ERR_BAD_TREE);
+  }
+  t.ctx = min(max(0, sh.ctx_len[s]), sh.most_ctx);
   // the root sees furthest back: keys from ctx - window + 1
   const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;
   t.lo_tile = lo >> KEY_SHIFT;

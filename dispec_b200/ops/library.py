@@ -147,7 +147,7 @@ def raise_on_device_error(where: str) -> None:
     v = device_error()
     if v:
         names = [n for bit, n in ((1, "page id outside the pool"), (2, "token id outside the vocabulary"),
-                                  (4, "a bounded wait ran out"), (8, "a path through a tree does not ascend")) if v & bit]
+                                  (4, "a bounded wait ran out"), (8, "a tree whose nodes are not among the rows, or a path through one that does not ascend")) if v & bit]
         raise KernelError(f"{where}: device reported: {', '.join(names) or v}")
 
 

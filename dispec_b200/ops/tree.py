@@ -54,7 +54,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     over the keys it sees, zero where there is none.  ``window`` W > 0: a node at depth d (``depth`` int32
     [T], the root at 0) is at position ctx_len + d and sees positions above ctx_len + d - W only; pages that
     no node sees may be gone from the table.  ``max_nodes``: no tree has more nodes, as far as the host knows.
-    32-bit sums and softmax; the result [T, H * D] is rounded once.  Nothing is read back."""
+    32-bit sums and softmax; the result [T, H * D] is rounded once.  Rows of no tree are left as they are; a tree whose rows are not
+    all among the T is recorded as a device error and left out.  Nothing is read back."""
     what = "tree_attention"
     if not q.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")

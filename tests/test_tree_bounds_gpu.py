@@ -1,0 +1,48 @@
+"""Operators on drafted trees whose device lists point outside the arrays: recorded, left out, and everything else as it was."""
+import random
+
+import pytest
+import torch
+
+from tree_util import AttentionCase, random_tree
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+LAST = 2 ** 31 - 1
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda:0")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("starts,whole", [([0, 5, 900], [0]), ([0, 5, LAST], [0]), ([-3, 5, 12], [1]), ([-LAST, 5, 12], [1]), ([0, 5, 3], [0]),
+                                          ([13, 5, 12], [1]), ([LAST, LAST, -LAST], [])])
+def test_attention_trees_outside_the_rows_are_left_out(dtype, starts, whole):
+    from dispec_b200 import ops
+    case = AttentionCase([(70, random_tree(5, random.Random(1))), (30, random_tree(7, random.Random(2)))], 4, 2, 64, dtype)
+    want, bound = case.plain()
+    case.starts = starts
+    wide = torch.full((16, 256), 7.0, dtype=dtype, device="cuda:0")
+    got = case.run(out=wide[2:14]).double().cpu()
+    assert ops.device_error() == 8
+    rows = [slice(0, 5), slice(5, 12)]
+    for s, r in enumerate(rows):
+        if s in whole:
+            assert ((got[r] - want[r]).abs() <= bound[r]).all()
+        else:
+            assert (got[r] == 7).all()
+    assert (wide[:2] == 7).all() and (wide[14:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("ctx", [10 ** 6, LAST, LAST - 40])
+def test_attention_more_stored_tokens_than_pages(dtype, ctx):
+    from dispec_b200 import ops
+    case = AttentionCase([(70, random_tree(5, random.Random(1))), (30, random_tree(7, random.Random(2)))], 4, 2, 64, dtype)
+    case.k, case.v = torch.nan_to_num(case.k), torch.nan_to_num(case.v)
+    want, bound = case.plain()
+    case.ctx = [70, ctx]
+    got = case.run().double().cpu()
+    assert ops.device_error() == 1
+    assert ((got[:5] - want[:5]).abs() <= bound[:5]).all() and torch.isfinite(got[5:]).all()

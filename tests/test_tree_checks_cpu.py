@@ -43,3 +43,9 @@ def test_columns_that_are_not_neighbours_are_refused(T):
     assert "neighbouring columns" in attention(T, out=strided)
     wide = described(F32, (T, 32), (64, 1), contiguous=T == 1)
     assert "scratch" in attention(T, q=wide, out=wide)
+
+
+def test_more_key_tiles_than_are_counted_are_refused():
+    assert "scratch" in attention(1 << 16, table=(1 << 10, 1 << 16), page=4)
+    assert "too many" in attention(1 << 20, table=(1 << 16, 1 << 18), page=4)
+    assert "too many" in attention(0x7fffffff)
