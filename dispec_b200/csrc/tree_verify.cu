@@ -39,7 +39,7 @@ struct Args {
   const float *temperature, *uniforms, *draws;
   int *path, *count, *token;
   long ld, ldq;
-  int V, share, max_nodes;
+  int rows, V, share, max_nodes;
   int* err;
 };
 
@@ -117,7 +117,10 @@ tree_verify_kernel(const Args a) {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   pdl_wait();
   pdl_launch_dependents();
-  const int first = a.node_start[s], n = min(a.node_start[s + 1] - first, a.max_nodes);
+  const int first = a.node_start[s], last = a.node_start[s + 1];
+  const bool inside = first >= 0 && first <= last && last <= a.rows;
+  const int n = inside ? min(last - first, a.max_nodes) : 0;
+  if (!inside && rank == 0 && tid == 0) atomicOr(a.err, DSP_ERR_BAD_TREE);  // (as a tree without nodes)
   const float temp = a.temperature[s];
   const int begin = min(a.V, rank * a.share), end = min(a.V, begin + a.share), mine = end - begin;
   const int per = ((mine + THREADS - 1) / THREADS) | 1;  // logits of a thread: neighbours, and odd, so that banks do not meet
@@ -520,6 +523,7 @@ extern "C" int dsp_tree_verify(const DspTensor* t, const long* options, cudaStre
   a.token = (int*)token.data;
   a.ld = logits.stride[0];
   a.ldq = draft.dims < 0 ? 0 : draft.stride[0];
+  a.rows = (int)T;
   a.V = (int)V;
   a.max_nodes = (int)max_nodes;
   a.err = dsp_device_error_ptr();

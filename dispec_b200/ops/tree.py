@@ -120,7 +120,8 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
 
     Distributions are held in whole numbers (the likeliest token's mass is 2^40), so that no decision depends on the
     order of a sum.  A token id outside the vocabulary is recorded as a device error and never accepted.  A tree without nodes
-    gives count 0 and token -1; nodes beyond ``max_nodes`` are not tried."""
+    gives count 0 and token -1, and so does one whose rows are not all among the T, which is recorded as a device error;
+    nodes beyond ``max_nodes`` are not tried."""
     what = "verify_tree"
     if not logits.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")

@@ -46,3 +46,25 @@ def test_attention_more_stored_tokens_than_pages(dtype, ctx):
     got = case.run().double().cpu()
     assert ops.device_error() == 1
     assert ((got[:5] - want[:5]).abs() <= bound[:5]).all() and torch.isfinite(got[5:]).all()
+
+
+@pytest.mark.parametrize("vocab", [300, 40000])
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("starts,whole", [([0, 4, 900], [0]), ([0, 4, LAST], [0]), ([-3, 4, 9], [1]), ([-LAST, 4, 9], [1]), ([0, 4, 3], [0]),
+                                          ([11, 4, 9], [1]), ([LAST, -LAST, LAST], [])])
+def test_verification_trees_outside_the_rows_have_no_nodes(vocab, drafted, starts, whole):
+    from dispec_b200 import ops
+    gen = torch.Generator().manual_seed(3)
+    parents = [-1, 0, 0, 1, -1, 0, 1, 1, 3]
+    logits = torch.randn(9, vocab, generator=gen).cuda()
+    draft = torch.softmax(torch.randn(9, vocab, generator=gen), -1).cuda() if drafted else None
+    args = (logits, i32(list(range(9))), i32(parents))
+    rest = (torch.tensor([0.9, 0.9]).cuda(), torch.rand(9, generator=gen).cuda(), torch.rand(2, generator=gen).cuda(), draft)
+    good = ops.verify_tree(*args, i32([0, 4, 9]), *rest, max_nodes=5)
+    got = ops.verify_tree(*args, i32(starts), *rest, max_nodes=5)
+    assert ops.device_error() == 8
+    for s in range(2):
+        if s in whole:
+            assert got.count[s] == good.count[s] and got.token[s] == good.token[s] and torch.equal(got.path[s], good.path[s])
+        else:
+            assert got.count[s] == 0 and got.token[s] == -1 and (got.path[s] == -1).all()
