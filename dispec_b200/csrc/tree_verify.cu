@@ -453,6 +453,14 @@ tree_verify_kernel(const Args a) {
     }
     break;
   }
+  // A CTA whose wait ran out is ahead of the others, which may still write to its shared memory: it stays until they have given up
+  // in their turn (waits are bounded) or are gone, and lets what is on its way land.
+  __syncthreads();
+  if (broken && ctas > 1) {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // (for all threads of the cluster that have not exited)
+    for (int i = 0; i < 200; ++i) __nanosleep(100);
+  }
 }
 
 template <typename T, bool DRAFT>
