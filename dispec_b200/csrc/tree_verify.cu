@@ -56,10 +56,10 @@ __device__ __forceinline__ mass_t mass_of(float e) { return (mass_t)(e * 1099511
 //            correctly where nothing over- or underflows (temp and the largest logit are far from that).  A quotient of
 //            -inf comes out as no number, whose exponential is 0 as it should be; one so small that a remainder
 //            is not exact changes no exponential.  Five instructions for a division's ten, and no reciprocal.
-//   GENERAL  a division; the largest logit may be infinite
+//   GENERAL  a division; the largest logit may be infinite, and the temperature too (where both are, their quotient is no number)
 enum Mode { UNIT, PLAIN, GENERAL };
 struct Scale {
-  float temp, inv, top;
+  float temp, inv, largest, top;  // the largest logit, and its quotient
   Mode mode;
   template <Mode M>
   __device__ __forceinline__ float exponential(float l) const {
@@ -71,7 +71,7 @@ struct Scale {
     }
     if (M == GENERAL) x = __fdiv_rn(l, temp);
     const float e = fmaxf(expf(x - top), 0.f);
-    return M == GENERAL && x == top ? 1.f : e;
+    return M == GENERAL && (x == top || l == largest) ? 1.f : e;
   }
   __device__ __forceinline__ float exponential(float l) const {
     return mode == UNIT ? exponential<UNIT>(l) : mode == PLAIN ? exponential<PLAIN>(l) : exponential<GENERAL>(l);
@@ -281,6 +281,7 @@ tree_verify_kernel(const Args a) {
     } else {
       scale.temp = temp;
       scale.inv = __frcp_rn(temp);
+      scale.largest = top;
       scale.top = __fdiv_rn(top, temp);  // (a quotient grows with its numerator, so this is the largest of them)
       scale.mode = !(fabsf(top) < 1.1e18f && temp > 9.3e-10f && temp < 1.1e9f) ? GENERAL : temp == 1.f ? UNIT : PLAIN;
       auto pass = [&](auto exponential) {
