@@ -33,7 +33,7 @@ constexpr int KEY_SHIFT = 6, KEYS_PER_TILE = 1 << KEY_SHIFT;
 
 // One tree: sizes in units.
 struct Tree {
-  int first, n, ctx;      // first row, nodes, stored tokens
+  int first, n, ctx;      // first row, nodes (-1: not inside the rows), stored tokens
   int lo_tile, key_tiles; // first key tile any node sees, key tiles from there
   int row_tiles;
 };
@@ -42,17 +42,13 @@ __device__ __forceinline__ Tree load_tree(const Shape& sh, int s) {
   Tree t;
   const int end = sh.node_start[s + 1];
   t.first = sh.node_start[s];
-  t.n = end - t.first;
-  if (t.first < 0 || end < t.first || end > sh.rows) {
-    t.n = 0;
-    atomicOr(sh.err, DSP_ERR_BAD_TREE);
-  }
+  t.n = t.first >= 0 && end >= t.first && end <= sh.rows ? end - t.first : -1;
   t.ctx = min(max(0, sh.ctx_len[s]), sh.most_ctx);
   // the root sees furthest back: keys from ctx - window + 1
   const int lo = sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0;
   t.lo_tile = lo >> KEY_SHIFT;
   t.key_tiles = t.n > 0 ? ((t.ctx + t.n + KEYS_PER_TILE - 1) >> KEY_SHIFT) - t.lo_tile : 0;
-  t.row_tiles = (t.n * sh.G + sh.rows_per_tile() - 1) >> sh.row_shift;
+  t.row_tiles = (max(t.n, 0) * sh.G + sh.rows_per_tile() - 1) >> sh.row_shift;
   return t;
 }
 // Units of a tree in one of its row tiles.
@@ -111,6 +107,7 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
   f.seq = -1;
   Tree held[HELD];
   int all = 0, of_first = 0, most = 0;
+  bool outside = false;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     held[k] = {};
@@ -121,6 +118,7 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
     all += units_of(sh, held[k]) * held[k].row_tiles;
     of_first += units_of(sh, held[k]);
     most = max(most, held[k].row_tiles);
+    outside |= held[k].n < 0;
   }
 #pragma unroll 1
   for (int s = HELD * 32 + lane; s < sh.S; s += 32) {
@@ -128,7 +126,9 @@ __device__ __forceinline__ Found find_run(const Shape& sh, int block, int ctas) 
     all += units_of(sh, t) * t.row_tiles;
     of_first += units_of(sh, t);
     most = max(most, t.row_tiles);
+    outside |= t.n < 0;
   }
+  if (outside) atomicOr(sh.err, DSP_ERR_BAD_TREE);
   Cut& cut = f.cut;
   cut.total = warp_sum_int(all);
   if (cut.total == 0) return f;
