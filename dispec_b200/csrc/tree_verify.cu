@@ -22,6 +22,8 @@
 // largest logit's exchange 0.55, the pass of exponentials 1.4, the sum's exchange 0.7, the tests 0.45; a refusal against draft
 // probabilities 3.5), for many the instructions of the exponentials' pass.  8 trees with draft probabilities 32 us, 64 trees
 // without 67 us (1.4 TB/s of the rows that are visited).
+#include <float.h>
+
 #include "tensor_checks.cuh"
 #include "tcgen05_common.cuh"  // bounded mbarrier waits, cluster addresses, counted remote stores
 
@@ -56,10 +58,10 @@ __device__ __forceinline__ mass_t mass_of(float e) { return (mass_t)(e * 1099511
 //            correctly where nothing over- or underflows (temp and the largest logit are far from that).  A quotient of
 //            -inf comes out as no number, whose exponential is 0 as it should be; one so small that a remainder
 //            is not exact changes no exponential.  Five instructions for a division's ten, and no reciprocal.
-//   GENERAL  a division; the largest logit may be infinite, and the temperature too (where both are, their quotient is no number)
+//   GENERAL  a division; the largest logit may be infinite
 enum Mode { UNIT, PLAIN, GENERAL };
 struct Scale {
-  float temp, inv, largest, top;  // the largest logit, and its quotient
+  float temp, inv, top;
   Mode mode;
   template <Mode M>
   __device__ __forceinline__ float exponential(float l) const {
@@ -71,7 +73,7 @@ struct Scale {
     }
     if (M == GENERAL) x = __fdiv_rn(l, temp);
     const float e = fmaxf(expf(x - top), 0.f);
-    return M == GENERAL && (x == top || l == largest) ? 1.f : e;
+    return M == GENERAL && x == top ? 1.f : e;
   }
   __device__ __forceinline__ float exponential(float l) const {
     return mode == UNIT ? exponential<UNIT>(l) : mode == PLAIN ? exponential<PLAIN>(l) : exponential<GENERAL>(l);
@@ -121,7 +123,8 @@ tree_verify_kernel(const Args a) {
   const bool inside = first >= 0 && first <= last && last <= a.rows;
   const int n = inside ? min(last - first, a.max_nodes) : 0;
   if (!inside && rank == 0 && tid == 0) atomicOr(a.err, DSP_ERR_BAD_TREE);  // (as a tree without nodes)
-  const float temp = a.temperature[s];
+  // (infinite logits share the mass at any temperature, but by an infinite one they could not be divided)
+  const float given = a.temperature[s], temp = given > FLT_MAX ? FLT_MAX : given;
   const int begin = min(a.V, rank * a.share), end = min(a.V, begin + a.share), mine = end - begin;
   const int per = ((mine + THREADS - 1) / THREADS) | 1;  // logits of a thread: neighbours, and odd, so that banks do not meet
   if (n > 0) near((const T*)a.logits + (size_t)first * a.ld + begin, mine * (int)sizeof(T));
@@ -281,7 +284,6 @@ tree_verify_kernel(const Args a) {
     } else {
       scale.temp = temp;
       scale.inv = __frcp_rn(temp);
-      scale.largest = top;
       scale.top = __fdiv_rn(top, temp);  // (a quotient grows with its numerator, so this is the largest of them)
       scale.mode = !(fabsf(top) < 1.1e18f && temp > 9.3e-10f && temp < 1.1e9f) ? GENERAL : temp == 1.f ? UNIT : PLAIN;
       auto pass = [&](auto exponential) {
@@ -403,6 +405,16 @@ tree_verify_kernel(const Args a) {
       continue;
     }
     // ---- no child was taken: the draw, by the CTA whose part holds the mass it aims at
+    if (broken) {
+      // This CTA is ahead of the others, which may still write to its shared memory: it stays until all their threads have given up in
+      // their turn (waits are bounded) or are gone, and lets what is on its way land.
+      if (rank == 0 && tid == 0) {
+        a.count[s] = 0;
+        a.token[s] = -1;
+      }
+      asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n\tnanosleep.u32 20000;" ::: "memory");
+      return;
+    }
     if (rank == 0 && tid == 0) a.count[s] = count;
     const mass_t R = total, aim = max((mass_t)0, min((mass_t)__fmul_rn(a.draws[s], (float)R), R - 1));
     mass_t before = 0;
@@ -453,14 +465,6 @@ tree_verify_kernel(const Args a) {
       }
     }
     break;
-  }
-  // A CTA whose wait ran out is ahead of the others, which may still write to its shared memory: it stays until they have given up
-  // in their turn (waits are bounded) or are gone, and lets what is on its way land.
-  __syncthreads();
-  if (broken && ctas > 1) {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // (for all threads of the cluster that have not exited)
-    for (int i = 0; i < 200; ++i) __nanosleep(100);
   }
 }
 
