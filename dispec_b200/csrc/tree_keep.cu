@@ -7,6 +7,8 @@
 // What bounds it: the bytes for large batches; for small ones the chain count, path -> page table -> row.  A block works
 // that chain out once for several layers, and a thread's loads of up to eight nodes are under way together.  8 trees of 28
 // layers 2.8 us; 64 trees of 48 layers with rows of 256 bytes 23.8 us, 3.8 TB/s, 0.58 of what a plain copy reaches.
+#include <limits.h>
+
 #include "tensor_checks.cuh"
 
 namespace {
@@ -57,8 +59,9 @@ tree_keep_kernel(const __grid_constant__ Args a) {
         atomicMin(&stop, j);
         atomicOr(a.err, DSP_ERR_BAD_TREE);
       } else if (node != j) {
-        const int k = ctx + node, k2 = ctx + j;
-        const bool inside = ctx >= 0 && k / a.page_size < a.table_width;
+        const bool counted = ctx >= 0 && node <= INT_MAX - ctx;  // (no path has a negative node: it ascends from -1)
+        const int k = counted ? ctx + node : 0, k2 = counted ? ctx + j : 0;
+        const bool inside = counted && k / a.page_size < a.table_width;
         from = inside ? table[k / a.page_size] : -1;
         const int to = inside ? table[k2 / a.page_size] : -1;
         if (from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages) {

@@ -68,3 +68,18 @@ def test_verification_trees_outside_the_rows_have_no_nodes(vocab, drafted, start
             assert got.count[s] == good.count[s] and got.token[s] == good.token[s] and torch.equal(got.path[s], good.path[s])
         else:
             assert got.count[s] == 0 and got.token[s] == -1 and (got.path[s] == -1).all()
+
+
+# The place of a node is ctx + node: with the node 2^31 - 1 behind 5 tokens that sum, in 32 bits, is negative, and
+# divided by the size of a page still below the width of the table.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("ctx,node", [(5, LAST), (1, LAST), (LAST, 2), (LAST, LAST), (-5, 7), (-LAST, LAST), (0, LAST), (8, 0x40000000)])
+def test_keeping_nodes_and_tokens_beyond_what_can_be_counted(dtype, ctx, node):
+    from dispec_b200 import ops
+    pool = torch.randn(3, 6, 2, 4, 16, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    want = pool.clone()
+    table = i32([[3, 0, 4], [1, 2, 5]])
+    want[:, 2, :, 1] = pool[:, 2, :, 3]  # request 1: node 2 behind 4 + 1 tokens goes where node 0 is
+    ops.keep_path([pool], table, i32([ctx, 4]), torch.tensor([[0, node, -1], [0, 3, -1]], dtype=torch.int32).cuda(), i32([2, 2]))
+    assert ops.device_error() == 1
+    assert torch.equal(pool, want)
