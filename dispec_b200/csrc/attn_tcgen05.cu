@@ -50,8 +50,9 @@ static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles
 // warp 0: TMA, warps 1 and 11: issue S = Q K^T for softmax group 0 and 1, warps 2-9: softmax, warp 10: issues O += P V
 constexpr int PV_WARP = 10, S1_WARP = 11;
 constexpr int KD = D / 64;            // 64-wide slices of the head dimension (128-byte rows)
-constexpr int KV_SLICE = BN * 128;    // bytes of one slice of a K or V tile
-constexpr int KV_BYTES = KD * KV_SLICE;
+constexpr int SLICE = KEY_SLICE;      // of 8 keys; tiles lie as the pages are brought (tcgen05_common.cuh)
+constexpr int GROUP = KD * SLICE;     // 8 keys
+constexpr int KV_BYTES = BN / 8 * GROUP;
 constexpr int SMEM_BYTES = (K_STAGES + V_STAGES) * KV_BYTES + 1024;
 static_assert(SMEM_BYTES + 1536 <= 227 * 1024, "dynamic and static shared memory of a CTA");
 // Tensor memory, 32-bit columns: two score buffers, two output accumulators, and the A operands of
@@ -128,7 +129,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
   const int n_kt = kt_end - kt_begin;
   const int* table = p.page_table + (size_t)seq * p.pt_stride;
 
-  unsigned char* k_s = smem;                                  // [stage][slice][64 keys][128 bytes]
+  unsigned char* k_s = smem;                                  // [stage][8 groups of keys][slice][8 keys][128 bytes]
   unsigned char* v_s = k_s + K_STAGES * KV_BYTES;
 
   if (tid == 0) {
@@ -195,7 +196,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
 
   if (warp == 0) {
     // ---- TMA producer of the K tiles and the V tiles, each into a ring of its own
-    const int pages_per_tile = BN / p.page_size;
+    const int pages_per_tile = BN / p.page_size, groups = p.page_size >> 3;  // groups of 8 keys a page
     const uint32_t page_bytes = (uint32_t)KD * (uint32_t)p.page_size * 128u;  // every slice, of K or of V
     // Page ids are looked up for a chunk of 32 / pages_per_tile key tiles at a time, lane l
     // holding page l % pages_per_tile of the chunk's tile l / pages_per_tile, and the chunk after
@@ -271,12 +272,12 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
             mbar_expect_tx(&v_full[my_sv], (uint32_t)__popc(live) * page_bytes);
           }
           // The tile's pages lie one after the other in the pool (what a pool hands out while it
-          // is not fragmented): one request per operand brings them all, where a page of 16
-          // tokens otherwise takes KD requests of 2 KB, and the requests, not the bytes, are what
-          // the TMA unit's time goes to.  Both ways leave the same bytes at the same places.
+          // is not fragmented): one request per operand brings them all, where each page otherwise
+          // takes one of its own, and the requests, not the bytes, are what the TMA unit's time
+          // goes to.  Both ways leave the same bytes at the same places.
           if (in_run) {
-            tma_load_4d(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], 0, kvh * p.page_size, pg, 0);
-            tma_load_4d(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], 0, kvh * p.page_size, pg, 0);
+            load_pages(k_s + my_sk * KV_BYTES, &runs_k, &k_full[my_sk], kvh * groups, pg);
+            load_pages(v_s + my_sv * KV_BYTES, &runs_v, &v_full[my_sv], kvh * groups, pg);
           }
         } else {
           failed = 1;  // nothing more is loaded; the warps that wait for tiles give up in their turn
@@ -286,13 +287,9 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
         // some tile of the turn goes page by page: the bytes were announced above, before any
         // lane's load can count them
         if (mine && !in_run && pg >= 0 && *(volatile int*)&failed == 0) {
-          const int row = (pg * p.KVH + kvh) * p.page_size;
-          const int dst = page_in_tile * p.page_size * 128;
-#pragma unroll
-          for (int h = 0; h < KD; ++h) {
-            tma_load_2d(k_s + my_sk * KV_BYTES + dst + h * KV_SLICE, &map_k, &k_full[my_sk], h * 64, row);
-            tma_load_2d(v_s + my_sv * KV_BYTES + dst + h * KV_SLICE, &map_v, &v_full[my_sv], h * 64, row);
-          }
+          const int dst = page_in_tile * groups * GROUP;
+          load_pages(k_s + my_sk * KV_BYTES + dst, &map_k, &k_full[my_sk], kvh * groups, pg);
+          load_pages(v_s + my_sv * KV_BYTES + dst, &map_v, &v_full[my_sv], kvh * groups, pg);
         }
       }
       for (int u = 0; u < 2; ++u) {
@@ -313,7 +310,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
       const bool leader = elect_one();
       const uint32_t idesc_s = umma_idesc(BM, BN);
       // descriptors are linear in the address: the tile's base once, a constant per k step
-      const uint64_t k_desc0 = umma_desc(smem_u32(k_s));
+      const uint64_t k_desc0 = key_desc(smem_u32(k_s), GROUP);
       auto issue_scores = [&](int i) {
         const int s = i % K_STAGES;
         tc_fence_after();
@@ -323,7 +320,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (uint32_t)(k >> 2), in = (uint32_t)(k & 3) * 32u;
-            umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * KV_SLICE + in) >> 4), idesc_s, k != 0);
+            umma_a_tmem(tmem_s, tmem_base + (uint32_t)(Q_COL + k * 8), k_desc + ((off * SLICE + in) >> 4), idesc_s, k != 0);
           }
           umma_commit(&s_full[i & 1]);
           umma_commit(&k_empty[s]);
@@ -345,7 +342,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
     {
       const bool leader = elect_one();
       const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
-      const uint64_t v_desc0 = umma_desc_mn(smem_u32(v_s), KV_SLICE);
+      const uint64_t v_desc0 = value_desc(smem_u32(v_s), GROUP);
       bool ok = true;
       for (int b = 0; b < n_kt && ok; ++b) {
         const int g = b & 1, st = b % V_STAGES;
@@ -357,7 +354,7 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
 #pragma unroll
           for (int k = 0; k < BN / 16; ++k)
             umma_a_tmem(tmem_base + (uint32_t)(O_COL + g * D), tmem_base + (uint32_t)(P_COL + g * P_COLS + k * 8),
-                        v_desc + (uint64_t)(k * 128), idesc_o, (b >= 2) || k != 0);
+                        v_desc + (uint64_t)(k * (2 * GROUP >> 4)), idesc_o, (b >= 2) || k != 0);
           umma_commit(&v_empty[st]);
           umma_commit(&o_done[g]);
         }
@@ -479,12 +476,12 @@ attn_tcgen05_kernel(const Params p, int tile_offset, const __grid_constant__ CUt
           dead = pg < 0 || pg >= p.num_pages;
         }
         if (dead) {
-          const uint32_t row_addr = smem_u32(v_s + (i % V_STAGES) * KV_BYTES) + (uint32_t)key_row * 128u +
-                                    (uint32_t)(r & 1) * 64u;
+          const uint32_t row_addr = smem_u32(v_s + (i % V_STAGES) * KV_BYTES) + (uint32_t)(key_row >> 3) * GROUP +
+                                    (uint32_t)(key_row & 7) * 128u + (uint32_t)(r & 1) * 64u;
 #pragma unroll
           for (int h = 0; h < KD; ++h)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * KV_SLICE + c * 16, make_uint4(0, 0, 0, 0));
+            for (int c = 0; c < 4; ++c) st_shared16(row_addr + h * SLICE + c * 16, make_uint4(0, 0, 0, 0));
         }
         fence_async_smem();
       }
@@ -594,8 +591,8 @@ bool pool_map(const void* base, long num_pages, int heads, int page_size, CUtens
   k.num_pages = num_pages;
   k.heads = heads;
   k.page_size = page_size;
-  if (!make_map(&k.map, base, num_pages * heads * page_size, D, D, page_size)) return false;
-  k.has_runs = make_map_page_runs(&k.runs, base, num_pages, heads, page_size, D, BN / page_size);
+  if (!make_map_pages(&k.map, base, num_pages, heads, page_size, D, 1)) return false;
+  k.has_runs = make_map_pages(&k.runs, base, num_pages, heads, page_size, D, BN / page_size);
   if (!k.has_runs) k.runs = k.map;
   if (used < SLOTS) cache[used++] = k;
   *out = k.map;

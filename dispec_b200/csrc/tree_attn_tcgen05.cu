@@ -49,11 +49,9 @@ constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 constexpr int PV_WARP = 10, S1_WARP = 11;
 constexpr int KD = D / 64;
-// A tile in shared memory: [group of 8 keys][slice of 64 columns][8 rows of 128 bytes].  So the steps from group to group are
-// equal wherever a page ends (pages are 8 keys or more), and a page's rows, all slices, are one TMA request (a
-// request costs the TMA unit about 145 cycles; by slices, scattered pages of 16 keys were 16 requests a tile: 2 trees behind
-// 32,768 tokens 66 us, now 57).
-constexpr int SLICE = 8 * 128;
+// A tile in shared memory lies as the pages are brought (tcgen05_common.cuh): [group of 8 keys][slice of 64 columns][8 rows of 128
+// bytes], a page's rows in one TMA request.
+constexpr int SLICE = KEY_SLICE;
 constexpr int GROUP = KD * SLICE;
 constexpr int KV_BYTES = BN / 8 * GROUP;
 constexpr int SMEM_BYTES = (K_STAGES + V_STAGES) * KV_BYTES + 1024;
@@ -253,36 +251,6 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
   y = fma2(y, f, make_float2(C1, C1));
   y = fma2(y, f, make_float2(C0, C0));
   return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
-}
-
-// A tile as the B operand: K-major (keys; the leading offset is not used) or N-major (values; slices are the leading offset).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr, uint32_t leading) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);  // start address, 16-byte units
-  d |= (uint64_t)leading << 16;
-  d |= (uint64_t)(GROUP >> 4) << 32;             // between groups of 8 keys
-  d |= (uint64_t)1 << 46;                        // descriptor version of this architecture
-  d |= (uint64_t)2 << 61;                        // layout type: 128-byte swizzle
-  return d;
-}
-__device__ __forceinline__ void load_pages(void* dst, const CUtensorMap* map, uint64_t* bar, int group, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4, %5}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(group), "r"(page)
-      : "memory");
-}
-// A pool [pages][heads][page_size][D] seen as (64 columns, 8 keys, D / 64 slices, groups of 8 keys of a page's heads, pages):
-// a box is one head's rows of `pages_per_box` neighbouring pages.
-inline bool make_map_pages(CUtensorMap* map, const void* base, long num_pages, int heads, int page_size, int pages_per_box) {
-  EncodeTiled fn = encode_fn();
-  if (fn == nullptr || num_pages < pages_per_box) return false;
-  cuuint64_t dims[5] = {64u, 8u, (cuuint64_t)KD, (cuuint64_t)heads * (page_size / 8), (cuuint64_t)num_pages};
-  cuuint64_t strides[4] = {(cuuint64_t)D * 2, 128u, (cuuint64_t)8 * D * 2, (cuuint64_t)heads * page_size * D * 2};
-  cuuint32_t box[5] = {64u, 8u, (cuuint32_t)KD, (cuuint32_t)(page_size / 8), (cuuint32_t)pages_per_box};
-  cuuint32_t elem[5] = {1, 1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Four lanes' pieces change hands: piece k of the j-th of four neighbouring lanes becomes piece j of the k-th.
@@ -682,7 +650,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     } else if (warp == 1 || warp == S1_WARP) {
       // ---- score products of one softmax group
       const uint32_t idesc_s = umma_idesc(BM, BN);
-      const uint64_t k_desc0 = tile_desc(smem_u32(k_s), 1u);
+      const uint64_t k_desc0 = key_desc(smem_u32(k_s), GROUP);
       const uint32_t tmem_s = tmem_base + (uint32_t)(g * S_COLS);
       bool ok = true;
       if (g < n_kt) {
@@ -713,7 +681,7 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
     } else if (warp == PV_WARP) {
       // ---- output products: O[g] += P[g] V of the share's tiles in turn
       const uint32_t idesc_o = umma_idesc(BM, D) | (1u << 16);  // B (values) is N-major
-      const uint64_t v_desc0 = tile_desc(smem_u32(v_s), SLICE >> 4);
+      const uint64_t v_desc0 = value_desc(smem_u32(v_s), GROUP);
       bool ok = share == 0 || __all_sync(0xffffffffu, mbar_wait(&o_free, (share - 1) & 1));
 #pragma unroll 1
       for (int b = 0; b < n_kt && ok; ++b) {
@@ -902,12 +870,12 @@ extern "C" int DSP_CAT(dsp_tree_attention_tcgen05_d, DSP_HEAD_DIM)(const DspTree
   p.a.sh.min_units = 2;  // one tile for each softmax group
   p.scale_log2 = a->scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v, runs_k, runs_v;
-  if (!make_map_pages(&map_k, a->k_pool, a->num_pages, a->sh.KVH, page, 1) ||
-      !make_map_pages(&map_v, a->v_pool, a->num_pages, a->sh.KVH, page, 1))
+  if (!make_map_pages(&map_k, a->k_pool, a->num_pages, a->sh.KVH, page, D, 1) ||
+      !make_map_pages(&map_v, a->v_pool, a->num_pages, a->sh.KVH, page, D, 1))
     return 4;
   // a pool of fewer pages than a key tile has gives no map of runs
-  p.page_runs = make_map_pages(&runs_k, a->k_pool, a->num_pages, a->sh.KVH, page, BN / page) &&
-                make_map_pages(&runs_v, a->v_pool, a->num_pages, a->sh.KVH, page, BN / page);
+  p.page_runs = make_map_pages(&runs_k, a->k_pool, a->num_pages, a->sh.KVH, page, D, BN / page) &&
+                make_map_pages(&runs_v, a->v_pool, a->num_pages, a->sh.KVH, page, D, BN / page);
   if (!p.page_runs) {
     runs_k = map_k;
     runs_v = map_v;
