@@ -24,18 +24,19 @@ from dispec_b200.sampling.sampler import _BELOW_ONE, Sampler, SamplingParams, ma
 def look_up(tokens: list, max_nodes: int, longest: int = 3, branches: int = 3) -> tuple[list, list]:
     """Drafts by looking the last tokens up: (tokens, parents) of a tree whose node 0 is the last token.  What followed
     earlier occurrences of the last ``longest`` tokens (then of fewer) is drafted, the latest occurrences
-    first, at most ``branches`` of them; continuations that begin alike share their nodes."""
+    first, at most ``branches`` of them, each once however many of the last tokens it shares; continuations that begin
+    alike share their nodes."""
     nodes, parents = [tokens[-1]], [-1]
     children: list[dict] = [{}]
-    found = 0
+    found = set()  # places in ``tokens`` where a continuation begins
     for n in range(min(longest, len(tokens) - 1), 0, -1):
         tail = tokens[-n:]
         for at in range(len(tokens) - n - 1, -1, -1):
-            if found >= branches or len(nodes) >= max_nodes:
+            if len(found) >= branches or len(nodes) >= max_nodes:
                 return nodes, parents
-            if tokens[at:at + n] != tail:
+            if tokens[at:at + n] != tail or at + n in found:
                 continue
-            found += 1
+            found.add(at + n)
             node = 0
             for t in tokens[at + n:at + n + max(1, (max_nodes - 1) // branches)]:
                 nxt = children[node].get(t)
