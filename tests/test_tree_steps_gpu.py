@@ -93,7 +93,7 @@ def test_sampled_tokens_follow_the_models_distribution(tmp_path):
     same tokens.  Five standard deviations."""
     from dispec_b200 import SamplingParams, SpeculativeEngine, load_model
     config, weights, _ = model_folder(str(tmp_path), "b", "float32")
-    vocab, T, N, prompt = config["vocab_size"], 0.6, 500, [5, 17, 3, 8]
+    vocab, T, N, prompt = config["vocab_size"], 2.0, 500, [5, 17, 3, 8]
     known = {}
 
     def p_behind(tokens):
