@@ -29,7 +29,10 @@
 
 namespace {
 constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_CTAS = 16, MAX_NODES = 1024;
-constexpr int SHARE = 24 * 1024;      // logits of a row in a CTA's shared memory, two CTAs an SM
+// Logits of a row that a CTA should have at most, without and with draft probabilities beside them.  Two CTAs fit an SM up to some 23,600
+// and 11,300.  With draft probabilities it stays with that (32 trees of 95,000 logits: 67 us on 16 CTAs each, 78 on eight, which
+// do not fit twice); without, eight CTAs alone on their SMs are better than 16 in pairs (64 trees of 188,000 logits: 64 and 78 us).
+constexpr int SHARE = 24 * 1024, SHARE_DRAFT = 11 * 1024;
 constexpr int MAX_VOCAB = 3 << 17;    // 24,576 logits in each of 16 CTAs
 typedef long long mass_t;
 constexpr mass_t ONE = (mass_t)1 << 40;
@@ -541,9 +544,9 @@ extern "C" int dsp_tree_verify(const DspTensor* t, const long* options, cudaStre
   a.max_nodes = (int)max_nodes;
   a.err = dsp_device_error_ptr();
   DSP_REQUIRE(a.err != nullptr, "verify_tree: no device error word");
-  // CTAs a tree: as many as keep the device's SMs busy with the trees there are, at least 2,048 logits each, and so many
-  // that two CTAs' shares fit an SM
-  const int sms = dsp_num_sms(), fits = a.draft ? SHARE / 2 : SHARE;
+  // CTAs a tree: as many as keep the device's SMs busy with the trees there are, at least 2,048 logits each, and so many that no
+  // share is larger than it should be (beyond 16 CTAs of that it is)
+  const int sms = dsp_num_sms(), fits = a.draft ? SHARE_DRAFT : SHARE;
   int ctas = 1;
   while (ctas < MAX_CTAS && ((V + ctas - 1) / ctas > fits || (ctas * 2 * 2048 <= V && ctas * 2 * S <= 2 * sms))) ctas *= 2;
   a.share = (int)(((V + ctas - 1) / ctas + 7) / 8 * 8);

@@ -63,3 +63,21 @@ def test_what_is_no_temperature_takes_the_largest_logit(temperature):
     logits[:, 7] = 1.0
     case = VerifyCase([[-1, 0]], [0, 7], logits, [temperature], [0.999] * 2, [0.999])
     assert case.run() == ([2], [[0, 1]], [7])
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+@pytest.mark.parametrize("vocab", [95000, 188000, 262144, 393216])
+@pytest.mark.parametrize("trees", [1, 24])
+def test_shares_of_every_size(drafted, vocab, trees):
+    """Vocabularies whose shares fit an SM twice, once, and up to the largest."""
+    spec = [3] * trees
+    case = verify_case(spec, vocab, 0.9, drafted, seed=vocab + trees)
+    follows(case, spec)
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+def test_a_vocabulary_beyond_the_largest_is_refused(drafted):
+    from dispec_b200 import ops
+    case = verify_case([2], 393217, 0.9, drafted, seed=1)
+    with pytest.raises(ops.KernelError, match="393216"):
+        case.run()
