@@ -20,9 +20,10 @@
 //
 // What bounds it: not bytes and not the tensor pipe (512 of 1,200 cycles a key tile), but the softmax groups' chain per tile: scores
 // out of tensor memory, maximum, 64 exponentials a thread, weights back.  64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128
-// on 8: 231 us, 0.55 PFLOP/s with the rows there are and 2.2 TB/s; 2 trees of 24 behind 32,768, 28 on 4: 52 us, 2.3 TB/s.  Two groups
-// of one row a thread: the accumulators, scores, weights and queries of 128 rows then fill tensor memory; a third group, or
-// key tiles of 128, has no room there.
+// on 8: 232 us, 0.55 PFLOP/s with the rows there are and 2.2 TB/s; 2 trees of 24 behind 32,768, 28 on 4: 52 us, 2.3 TB/s.  Two groups
+// of one row a thread: the accumulators, scores, weights and queries of 128 rows then fill tensor memory, and a third group, or
+// key tiles of 128, has no room beside them (queries in shared memory and weights in the place of their scores would make
+// some; that was not tried).
 #include "tcgen05_common.cuh"
 #include "tree_schedule.cuh"
 
@@ -39,11 +40,13 @@ using namespace tree;
 constexpr int D = DSP_HEAD_DIM;
 static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
 constexpr int BM = 1 << ROW_SHIFT_TENSOR_CORES, BN = KEYS_PER_TILE, THREADS = 384;
-// Key tiles of a share go to two issuing warps in turn, and each waits for its own tiles only.  With an even ring a slot's
-// tiles all belong to one of them; with an odd one a warp that is ahead (its tile landed, an older one of the
-// other's has not) could take the slot's last phase but one for the phase it waits for.
+// Key tiles of a share go to two issuing warps in turn, and each waits for its own tiles only.  With an even ring the tiles of a
+// share in one slot all belong to one of them; with an odd one a warp that is ahead (its tile landed, an older one of the
+// other's has not) could take the slot's last phase but one for the phase it waits for.  From share to share a slot may change
+// hands (behind an odd number of tiles): the block meets in between, when every tile of the last share has landed and been
+// used, and that barrier is needed for it.
 constexpr int K_STAGES = 6, V_STAGES = 6;
-static_assert(K_STAGES % 2 == 0, "a slot of the key ring belongs to one issuing warp");
+static_assert(K_STAGES % 2 == 0, "in a share, a slot of the key ring belongs to one issuing warp");
 constexpr int SHARES = 4;      // the shares remembered: the next two, the present one and the one whose rows are being stored
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
@@ -64,7 +67,9 @@ constexpr int Q_COL = P_COL + 2 * P_COLS;
 constexpr int TMEM_COLS = 512;
 static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 // Of eight weights, so many are formed on the multiply-add pipe: 64 trees of 64 nodes behind 2,050 tokens, 40 heads of 128 on 8:
-// 241 us with none, 232 with two, 237 with three.  Heads of 64, with half of the products to a weight: no difference, none.
+// 240 us with none, 232 with two, 237 with three; 2 trees of 24 behind 32,768 on scattered pages 50.7 with none and 52.0 with two,
+// 8 trees of 16 the same with both.  The larger call decides.  The result's error is the same to four digits (2.305e-3 of its size
+// against 64 bits, 2.342e-3 behind 32,768).  Heads of 64, with half of the products to a weight: no difference, none.
 constexpr int EX2_FMA = D == 128 ? 2 : 0;
 constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
@@ -788,6 +793,8 @@ tree_attn_tcgen05_kernel(const __grid_constant__ Params p, const __grid_constant
             const float2 y = fma2(make_float2(__uint_as_float(b[c]), __uint_as_float(b[c + 1])), scale2, neg_m2);
             const float2 ex = make_float2(ex2(x.x), ex2(x.y));
             const float2 ey = c / 2 % 4 < EX2_FMA ? ex2_fma(y) : make_float2(ex2(y.x), ex2(y.y));
+            // the second product takes weights of eight bits, as it takes values (their sum is of the 32-bit ones): with both the
+            // result is off by 2.3e-3 of its size, and by 1.65e-3 from its own rounding alone
             sum0 = add2(sum0, ex);
             sum1 = add2(sum1, ey);
             pk[c / 2] = pack2(ex.x, ex.y);

@@ -27,8 +27,8 @@ struct Shape {
   int* err;
   __device__ __forceinline__ int rows_per_tile() const { return 1 << row_shift; }
 };
-// Sizes of tiles are powers of two, and shifts: with divisions the search for a CTA's run alone is 3,000 instructions, each of which
-// a CTA fetches to run it once.
+// Sizes of tiles are powers of two, and shifts: a CTA runs the search for its run once, and fetches every instruction of a division
+// for it.
 constexpr int KEY_SHIFT = 6, KEYS_PER_TILE = 1 << KEY_SHIFT;
 
 // One tree: sizes in units.

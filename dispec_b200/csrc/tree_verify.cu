@@ -21,7 +21,8 @@
 // What bounds it: for a few trees the latencies of a node in a row (with 151,936 logits on 16 CTAs the row's arrival 1.05 us, the
 // largest logit's exchange 0.55, the pass of exponentials 1.4, the sum's exchange 0.7, the tests 0.45; a refusal against draft
 // probabilities 3.5), for many the instructions of the exponentials' pass.  8 trees with draft probabilities 32 us, 64 trees
-// without 67 us (1.4 TB/s of the rows that are visited).
+// without 67 us (1.4 TB/s of the rows that are visited).  A refusal against draft probabilities goes through the masses again, with all
+// of the node's refusals: c of them at one node take c (c + 1) / 2 passes.
 #include <float.h>
 
 #include "tensor_checks.cuh"
