@@ -125,6 +125,8 @@ class SpeculativeEngine:
         for r in live:
             # (no more drafts than the request may still emit beside the drawn token)
             nodes, parents = self.draft(r.tokens, max(1, min(self.max_nodes, max_new_tokens - len(r.out))))
+            if not nodes or nodes[0] != r.tokens[-1]:
+                raise ValueError(f"a draft begins with {nodes[:1]}, not with the request's last token {r.tokens[-1]}")
             entries.append(TreeEntry(r.req_id, nodes, parents, len(r.tokens) - 1))
             uniforms += [min(r.rng.random(), _BELOW_ONE) for _ in nodes]
         draws = [min(r.rng.random(), _BELOW_ONE) for r in live]

@@ -124,3 +124,15 @@ def test_sampled_tokens_follow_the_models_distribution(tmp_path):
             expected += each
             variance += each * (1 - each)
     assert ((counts - expected).abs() <= 5 * variance.sqrt()).all(), (counts, expected, variance.sqrt())
+
+
+@pytest.mark.parametrize("draft", [lambda tokens, n: ([tokens[-1] + 1], [-1]), lambda tokens, n: ([], []),
+                                   lambda tokens, n: ([tokens[0]], [-1]) if len(tokens) > 5 else ([tokens[-1]], [-1])])
+def test_drafts_of_another_root_are_refused(draft, tmp_path):
+    """What the model would run on is not what the request holds."""
+    from dispec_b200 import SpeculativeEngine, load_model
+    model_folder(str(tmp_path), "b", "float32")
+    engine = SpeculativeEngine(load_model(str(tmp_path), "float32", "cuda:0"), num_blocks=16, draft=draft)
+    with pytest.raises(ValueError, match="last token"):
+        engine.generate([[5, 17, 3, 300]], 8)
+    assert not engine.runner.cache.live_requests()
