@@ -39,6 +39,9 @@ CORE_SOURCES = [
     "tree_attn.cu",
     "tree_keep.cu",
     "tree_verify.cu",
+    "shared_attn.cu",
+    "beam_select.cu",
+    "reorder_slots.cu",
     "random_fill.cu",
     "selftest.cu",
 ]
@@ -200,6 +203,7 @@ def build_all(head_dims=(16, 32, 64, 128)) -> list[str]:
         if d in (64, 128):
             libs.append(prefill_attention_library(d))
             libs.append(tree_attention_library(d))
+            libs.append(shared_attention_library(d))
     libs += [mixer_library(name) for name in MIXER_LIBRARIES]
     # the attention with widths of their own for keys and values is compiled per pair of widths
     libs += [sink_attention_library(dk, dv) for dk, dv in ((64, 64), (128, 64), (128, 128))]
@@ -218,6 +222,11 @@ def prefill_attention_library(head_dim: int) -> str:
 def tree_attention_library(head_dim: int) -> str:
     """The attention of drafted trees on the tensor cores."""
     return specialised_library(f"tree_attn_tcgen05_d{head_dim}", "tree_attn_tcgen05.cu", {"DSP_HEAD_DIM": head_dim})
+
+
+def shared_attention_library(head_dim: int) -> str:
+    """The attention of sequences with a shared beginning on the tensor cores."""
+    return specialised_library(f"shared_attn_tcgen05_d{head_dim}", "shared_attn_tcgen05.cu", {"DSP_HEAD_DIM": head_dim})
 
 
 def sink_attention_library(key_dim: int, value_dim: int) -> str:

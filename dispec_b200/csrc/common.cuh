@@ -18,6 +18,7 @@ enum DspDeviceError {
   DSP_ERR_BAD_TOKEN = 2,   // token id outside the vocabulary
   DSP_ERR_WAIT_LIMIT = 4,  // a bounded wait on a barrier ran out
   DSP_ERR_BAD_TREE = 8,    // a drafted tree's nodes are not among the rows, or the nodes of a path through it do not ascend
+  DSP_ERR_BAD_GROUP = 16,  // a group whose rows are not among those there are, or slots that do not ascend or lie outside their pool
 };
 
 extern "C" const char* dsp_last_error();

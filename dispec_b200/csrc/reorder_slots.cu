@@ -1,0 +1,132 @@
+// Slots of pools follow a choice: in every pool [layers, slots, ...]
+//     pool[:, dst[i]] = pool[:, src[i]]   for all i, as though all were read before any is written.
+//
+// Bytes of different columns have nothing to do with each other.  So a block takes some columns of one layer of one pool for
+// ALL i: it holds them in registers, eight pieces a thread, meets, and writes them.  A slot may be read by several and
+// written by another in one call, in place and without a copy of anything, and no block waits for another.
+//
+// dst ascends, so that no slot is written twice; what does not ascend, or names a slot that is not there, is left from there on
+// and recorded.
+#include "tensor_checks.cuh"
+
+namespace {
+constexpr int MAX_POOLS = 64, EACH = 8;
+
+struct Pool {
+  char* data;
+  long row_bytes;  // of a slot in one layer
+  int slots, first_block;
+  int chunks;      // blocks of a layer
+};
+struct Args {
+  Pool pools[MAX_POOLS];
+  const int *src, *dst;
+  int count, pools_n, chunk_shift;  // pieces of an entry in a block: 1 << chunk_shift
+  int* err;
+};
+
+template <typename Piece, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+reorder_kernel(const __grid_constant__ Args a) {
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = a.count;
+  int p = 0;  // the last pool whose first block is not behind this one
+  for (int step = MAX_POOLS / 2; step > 0; step >>= 1)
+    if (p + step < a.pools_n && a.pools[p + step].first_block <= (int)blockIdx.x) p += step;
+  const Pool& pool = a.pools[p];
+  const int block = blockIdx.x - pool.first_block, layer = block / pool.chunks, chunk = block - layer * pool.chunks;
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  for (int i = tid; i < a.count; i += THREADS) {
+    const int s = a.src[i], d = a.dst[i];
+    if (s < 0 || s >= pool.slots || d < 0 || d >= pool.slots || (i > 0 && d <= a.dst[i - 1])) atomicMin(&bad, i);
+  }
+  __syncthreads();
+  const int count = bad;
+  if (count < a.count && tid == 0) atomicOr(a.err, DSP_ERR_BAD_GROUP);
+  const long in_row = pool.row_bytes / (long)sizeof(Piece);
+  Piece* base = reinterpret_cast<Piece*>(pool.data) + (size_t)layer * pool.slots * in_row;
+  const long column0 = (long)chunk << a.chunk_shift;
+  const int mask = (1 << a.chunk_shift) - 1;
+  Piece x[EACH];
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int q = tid + k * THREADS, i = q >> a.chunk_shift;
+    const long column = column0 + (q & mask);
+    if (i < count && column < in_row) x[k] = base[(size_t)a.src[i] * in_row + column];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int q = tid + k * THREADS, i = q >> a.chunk_shift;
+    const long column = column0 + (q & mask);
+    if (i < count && column < in_row) base[(size_t)a.dst[i] * in_row + column] = x[k];
+  }
+}
+}  // namespace
+
+// tensors: src, dst, pools ...
+extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t stream) {
+  const DspTensor &src = t[0], &dst = t[1];
+#define REORDER_REQUIRE(cond, ...) DSP_REQUIRE(cond, "reorder_slots: " __VA_ARGS__)
+  REORDER_REQUIRE(src.device >= 0, "CUDA tensors only (there is no CPU path)");
+  REORDER_REQUIRE(pools >= 1 && pools <= MAX_POOLS, "%ld pools, 1 to %d expected", pools, MAX_POOLS);
+  REORDER_REQUIRE(src.dims == 1, "src must be one-dimensional");
+  const long n = src.size[0];
+  REORDER_REQUIRE(tensor_is(src, DSP_T_I32, src.device, 1, n) && tensor_is(dst, DSP_T_I32, src.device, 1, n),
+                  "src and dst must be contiguous int32 of one length on one device");
+  Args a = {};
+  uintptr_t bits = 0;
+  const DspTensor& first = t[2];
+  for (long p = 0; p < pools; ++p) {
+    const DspTensor& x = t[2 + p];
+    REORDER_REQUIRE(x.dims >= 3 && x.dims <= DSP_T_DIMS && x.contiguous && x.device == src.device && x.dtype != DSP_T_OTHER,
+                    "pool %ld must be a contiguous tensor [layers, slots, ...] of three to five dimensions, float32, bfloat16, int32 or int64, on the device of src", p);
+    REORDER_REQUIRE(x.size[1] == first.size[1], "pool %ld has %ld slots, the first one %ld", p, x.size[1], first.size[1]);
+    long elements = 1;
+    for (int k = 2; k < x.dims; ++k) elements *= x.size[k];
+    a.pools[p].data = (char*)x.data;
+    a.pools[p].row_bytes = elements * (x.dtype == DSP_T_BF16 ? 2 : x.dtype == DSP_T_I64 ? 8 : 4);
+    a.pools[p].slots = (int)x.size[1];
+    REORDER_REQUIRE(x.size[1] <= 0x7fffffff, "pool %ld has too many slots", p);
+    bits |= (uintptr_t)x.data | (uintptr_t)a.pools[p].row_bytes;
+    for (long o = 0; o < p; ++o)
+      REORDER_REQUIRE(a.pools[o].data != a.pools[p].data || a.pools[p].row_bytes == 0, "pools %ld and %ld are the same memory", o, p);
+  }
+  if (n == 0) return 0;
+  // the widest pieces that all rows consist of; as many of an entry in a block as its threads can hold
+  const long piece = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+  const int threads = n <= 512 ? 256 : 1024;  // (rows of 64 bytes at least up to 2,048 entries)
+  REORDER_REQUIRE(n <= (long)threads * EACH, "%ld slots to be copied, at most %d", n, 1024 * EACH);
+  while ((n << (a.chunk_shift + 1)) <= (long)threads * EACH) ++a.chunk_shift;
+  long blocks = 0;
+  for (long p = 0; p < pools; ++p) {
+    Pool& x = a.pools[p];
+    const long in_row = x.row_bytes / piece, chunks = (in_row + (1L << a.chunk_shift) - 1) >> a.chunk_shift;
+    x.chunks = (int)max(chunks, 1L);
+    x.first_block = (int)blocks;
+    blocks += chunks * t[2 + p].size[0];
+    REORDER_REQUIRE(blocks <= 0x7fffffff && chunks <= 0x7fffffff, "the pools are too large for one call");
+  }
+  if (blocks == 0) return 0;
+  REORDER_REQUIRE(current_device() == src.device, "the tensors are on device %d, the current device is %d", src.device, current_device());
+  a.src = (const int*)src.data;
+  a.dst = (const int*)dst.data;
+  a.count = (int)n;
+  a.pools_n = (int)pools;
+  a.err = dsp_device_error_ptr();
+  REORDER_REQUIRE(a.err != nullptr, "no device error word");
+  auto go = [&](auto kernel) -> int {
+    DSP_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, a));
+    return 0;
+  };
+  const int rc = threads == 256 ? (piece == 16 ? go(reorder_kernel<uint4, 256>) : piece == 4 ? go(reorder_kernel<uint32_t, 256>)
+                                                                                             : go(reorder_kernel<uint16_t, 256>))
+                                : (piece == 16 ? go(reorder_kernel<uint4, 1024>) : piece == 4 ? go(reorder_kernel<uint32_t, 1024>)
+                                                                                              : go(reorder_kernel<uint16_t, 1024>));
+  if (rc != 0) return rc;
+  DSP_CHECK_LAUNCH("reorder_slots");
+  return 0;
+}

@@ -1,0 +1,177 @@
+// Attention of sequences with a shared beginning over the paged key/value cache: one query row a sequence, the merge of partial
+// results, and the entry point.
+//
+// Sequence r of group g has n_r stored tokens, its own among them.  Its key and value j lie at place j of the pages of the group's
+// first sequence where j < P_g, else of its own.  Head h of its row:
+//     o = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale q . k_j),   max(0, n_r - W) <= j < n_r   (W: the window, if there is one)
+// A sum over keys may be taken in parts: with m the largest score of a part, l = sum exp(s_j - m) and a = sum exp(s_j - m) v_j, parts
+// join as  M = max m,  o = sum a exp(m - M) / sum l exp(m - M).  So the shared keys are read once for all sequences of a group,
+// whose rows fill the tiles of a matrix product, and each sequence's own keys once for its G rows.  A row that sees nothing gives 0.
+// The work is cut as shared_schedule.cuh says; the kernels: rows_attn_tcgen05.cuh, rows_attn.cuh.
+#include "merge_parts.cuh"
+#include "rows_attn.cuh"
+#include "shared_schedule.cuh"
+#include "tensor_checks.cuh"
+
+namespace {
+using namespace shared;
+
+// Threads take the rows of all sequences in turn, four columns each.
+constexpr int COMBINE_THREADS = 256, COMBINE_BLOCKS_PER_SM = 4;
+template <typename T>
+__global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_BLOCKS_PER_SM)
+shared_combine_kernel(const Shape sh, const SharedScratch scratch, T* __restrict__ out, long out_stride, int D, int ctas) {
+  __shared__ int start[MAX_GROUPS + 1];
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int g = threadIdx.x; g <= sh.groups; g += COMBINE_THREADS) start[g] = sh.group_start[g];
+  __syncthreads();
+  const int H = sh.KVH * sh.G, quads = D / 4;
+  const long pieces = (long)sh.rows * H * quads;
+  const float2 *part_ml = reinterpret_cast<const float2*>(scratch.part_ml), *rows_ml = reinterpret_cast<const float2*>(scratch.rows_ml);
+  for (long i = (long)blockIdx.x * COMBINE_THREADS + threadIdx.x; i < pieces; i += (long)gridDim.x * COMBINE_THREADS) {
+    const int row_head = (int)(i / quads), d = (int)(i - (long)row_head * quads) * 4, row = row_head / H, h = row_head - row * H;
+    const int head = h / sh.G, of_head = h - head * sh.G;
+    const int g = group_of(start, sh.groups, sh.rows, row);
+    if (g < 0) continue;  // in no group: left as it is
+    const int length = sh.length(row), first = start[g];
+    const bool several = start[g + 1] - first > 1;
+    const int prefix = several ? min(max(0, sh.prefix_len[g]), sh.most_ctx) : 0, lo = sh.window > 0 ? max(0, length - sh.window) : 0;
+    // an item of which the row sees a key is there, and has a record
+    int of_tile[2];
+    Record rec[2];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const bool sees = part == 0 ? lo < min(prefix, length) : max(prefix, lo) < length;
+      const int rr = (part == 0 ? (row - first) * sh.G : 0) + of_head;
+      of_tile[part] = rr & (sh.rows_per_tile() - 1);
+      rec[part] = {0, 0};
+      if (sees) rec[part] = scratch.records[sh.item(part, g, part == 0 ? first : row, rr >> sh.row_shift, head)];
+      // (a record that a CTA whose wait ran out did not write is none)
+      if (rec[part].cta < 0 || rec[part].parts < 0 || rec[part].parts > ctas - rec[part].cta) rec[part] = {0, 0};
+    }
+    const float4 v = merge_parts(rec[0].parts + rec[1].parts, [&](int k, float2& ml, float4& o) {
+      const int part = k >= rec[0].parts;
+      if (part) k -= rec[0].parts;
+      if (rec[part].parts == 1) {
+        const size_t at = ((size_t)part * sh.rows + row) * H + h;
+        ml = rows_ml[at];
+        o = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
+      } else {
+        const size_t at = ((size_t)2 * (rec[part].cta + k) + (k == 0)) * sh.rows_per_tile() + of_tile[part];
+        ml = part_ml[at];
+        o = *reinterpret_cast<const float4*>(scratch.part_o + at * D + d);
+      }
+    });
+    store4(out + (size_t)row * out_stride + (size_t)h * D + d, v);
+  }
+}
+
+long scratch_floats(const Shape& sh, long ctas, long D) {
+  const long rows = sh.rows_per_tile(), H = (long)sh.KVH * sh.G;
+  return 2 * ctas * rows * (D + 2) + 2 * (long)sh.rows * H * (D + 2) + 2 * sh.items();
+}
+}  // namespace
+
+struct DspSharedOptions {  // as ops/beams.py packs them
+  long window, sms, tensor_cores;
+  double scale;
+};
+
+// tensors: q, key pool, value pool, page table, ctx_len, group_start, prefix_len, out, scratch.  `tensor_cores`: address of the
+// tensor-core kernel's entry point for this head size, or 0.
+extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* o, cudaStream_t stream) {
+  const DspTensor &q = t[0], &k = t[1], &v = t[2], &table = t[3], &ctx = t[4], &start = t[5], &prefix = t[6], &out = t[7], &scratch = t[8];
+#define SHARED_REQUIRE(cond, ...) DSP_REQUIRE(cond, "shared_prefix_attention: " __VA_ARGS__)
+  SHARED_REQUIRE(q.device >= 0, "CUDA tensors only (there is no CPU path)");
+  SHARED_REQUIRE(q.dims == 2 && k.dims == 4 && v.dims == 4, "q [R, H * D] and two pools [pages, heads, page_size, D] expected");
+  const long R = q.size[0], columns = q.size[1], pages = k.size[0], KVH = k.size[1], page = k.size[2], D = k.size[3];
+  SHARED_REQUIRE(q.dtype == DSP_T_F32 || q.dtype == DSP_T_BF16, "kernels exist for float32 and bfloat16");
+  SHARED_REQUIRE(k.dtype == q.dtype && v.dtype == q.dtype && k.device == q.device && v.device == q.device && k.contiguous && v.contiguous &&
+                     v.size[0] == pages && v.size[1] == KVH && v.size[2] == page && v.size[3] == D,
+                 "the pools must be contiguous, alike, and of the type and on the device of q");
+  SHARED_REQUIRE(R == 0 || q.stride[1] == 1 || columns == 1, "the columns of q must be neighbours");
+  SHARED_REQUIRE(D % 8 == 0 && D >= 8 && D <= 256 && KVH > 0 && columns > 0 && columns % D == 0 && columns / D % KVH == 0,
+                 "%ld query columns on %ld heads of %ld (a multiple of 8 up to 256)", columns, KVH, D);
+  SHARED_REQUIRE(o->scale > 0. && o->scale <= 3e38 && o->window >= 0 && o->window <= 0x7fffffff,
+                 "scale %g must be positive, window %ld not negative", o->scale, o->window);
+  SHARED_REQUIRE(prefix.dims == 1 && prefix.size[0] <= MAX_GROUPS, "prefix_len must be one-dimensional, of at most %d groups", MAX_GROUPS);
+  const long groups = prefix.size[0];
+  SHARED_REQUIRE(tensor_is(ctx, DSP_T_I32, q.device, 1, R) && tensor_is(start, DSP_T_I32, q.device, 1, groups + 1) &&
+                     tensor_is(prefix, DSP_T_I32, q.device, 1, groups),
+                 "ctx_len [%ld], group_start [%ld] and prefix_len [%ld] must be contiguous int32 on the device of q", R, groups + 1, groups);
+  SHARED_REQUIRE(is_page_table(table, q.device, R), "page_table must be int32 [%ld, pages], neighbouring pages side by side", R);
+  SHARED_REQUIRE(out.dtype == q.dtype && out.device == q.device && out.dims == 2 && out.size[0] == R && out.size[1] == columns &&
+                     (R == 0 || out.stride[1] == 1 || columns == 1),
+                 "out must be like the queries [%ld, %ld] with neighbouring columns", R, columns);
+  SHARED_REQUIRE(R <= 0x7fffffff && pages <= 0x7fffffff && page >= 1 && page <= 0x7fffffff && o->sms >= 1 && table.stride[0] <= 0x7fffffff,
+                 "sizes out of range");
+  if (R == 0 || groups == 0) return 0;
+  const uintptr_t bits = (uintptr_t)q.data | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)out.data;
+  const long piece = q.dtype == DSP_T_F32 ? 4 : 8;  // elements of 16 bytes
+  SHARED_REQUIRE(bits % 16 == 0 && (R == 1 || (q.stride[0] % piece == 0 && out.stride[0] % piece == 0)), "rows must begin on 16 bytes");
+  // the tensor-core kernel is built for these page sizes; everything else takes the 32-bit kernel
+  const bool tensor_cores = o->tensor_cores != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
+                            (page == 8 || page == 16 || page == 32 || page == 64) && pages > 0;
+  const long ctas = o->sms * (tensor_cores || D > 128 ? 1 : 2);  // (by shared memory two CTAs of the 32-bit kernel an SM)
+  DspSharedAttention a = {};
+  a.sh.group_start = (const int*)start.data;
+  a.sh.prefix_len = (const int*)prefix.data;
+  a.sh.ctx_len = (const int*)ctx.data;
+  a.sh.groups = (int)groups;
+  a.sh.KVH = (int)KVH;
+  a.sh.G = (int)(columns / D / KVH);
+  a.sh.window = (int)o->window;
+  a.sh.rows = (int)R;
+  a.sh.row_shift = tensor_cores ? ROW_SHIFT_TENSOR_CORES : ROW_SHIFT_32BIT;
+  // places are counted in 32 bits, a tile of keys beyond the last among them
+  a.sh.most_ctx = (int)min(table.size[1] * page, 1L << 30);
+  // Units are counted in 32 bits: those of all items, each over as many tokens as a sequence's pages hold.
+  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (a.sh.most_ctx / KEYS_PER_TILE + 1),
+                 "%ld rows of %ld heads over pages for %d tokens a sequence are too many for one call", R, columns / D, a.sh.most_ctx);
+  SHARED_REQUIRE(scratch.contiguous && scratch.device == q.device && scratch.dims == 1 && (uintptr_t)scratch.data % 16 == 0 &&
+                     scratch.size[0] >= scratch_floats(a.sh, ctas, D),
+                 "scratch is too small");
+  SHARED_REQUIRE(current_device() == q.device, "the tensors are on device %d, the current device is %d", q.device, current_device());
+  const long rows = a.sh.rows_per_tile(), of_rows = 2 * R * columns / D;
+  a.scratch.part_o = (float*)scratch.data;
+  a.scratch.rows_o = a.scratch.part_o + 2 * ctas * rows * D;
+  a.scratch.part_ml = a.scratch.rows_o + of_rows * D;
+  a.scratch.rows_ml = a.scratch.part_ml + 4 * ctas * rows;
+  a.scratch.records = reinterpret_cast<Record*>(a.scratch.rows_ml + 2 * of_rows);
+  a.q = q.data;
+  a.k_pool = k.data;
+  a.v_pool = v.data;
+  a.page_table = (const int*)table.data;
+  a.out = out.data;
+  a.q_stride = q.stride[0];
+  a.out_stride = out.stride[0];
+  a.pt_stride = (int)table.stride[0];
+  a.table_width = (int)min(table.size[1], 0x7fffffffL);
+  a.D = (int)D;
+  a.page_size = (int)page;
+  a.num_pages = (int)pages;
+  a.ctas = (int)ctas;
+  a.scale = (float)o->scale;
+  a.err = a.sh.err = dsp_device_error_ptr();
+  SHARED_REQUIRE(a.err != nullptr, "no device error word");
+  if (tensor_cores) {
+    typedef int (*Kernel)(const DspSharedAttention*, cudaStream_t);
+    const int rc = reinterpret_cast<Kernel>(o->tensor_cores)(&a, stream);
+    SHARED_REQUIRE(rc == 0, "%s", rc == 4 ? "shared memory opt-in or tensor map creation failed" : "launch failed");
+  } else {
+    a.sh.min_units = 1;
+    const int rc = q.dtype == DSP_T_F32 ? launch_rows_attn<SharedWork, float>(a, stream) : launch_rows_attn<SharedWork, bf16>(a, stream);
+    if (rc != 0) return rc;
+  }
+  const long pieces = R * columns / 4;
+  const dim3 grid((unsigned)min((pieces + COMBINE_THREADS - 1) / COMBINE_THREADS, o->sms * COMBINE_BLOCKS_PER_SM));
+  if (q.dtype == DSP_T_F32)
+    DSP_CUDA(launch_pdl(shared_combine_kernel<float>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, a.scratch, (float*)a.out, a.out_stride,
+                        a.D, a.ctas));
+  else
+    DSP_CUDA(launch_pdl(shared_combine_kernel<bf16>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, a.scratch, (bf16*)a.out, a.out_stride,
+                        a.D, a.ctas));
+  DSP_CHECK_LAUNCH("shared_prefix_attention");
+  return 0;
+}

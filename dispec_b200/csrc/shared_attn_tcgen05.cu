@@ -1,0 +1,10 @@
+// Attention of sequences with a shared beginning on the tensor cores (the formula: shared_attn.cu; the kernel:
+// rows_attn_tcgen05.cuh; how the work is cut and what a row sees: shared_schedule.cuh).  Compiled once per head size
+// (-DDSP_HEAD_DIM=64 or 128).
+#include "shared_schedule.cuh"
+#include "rows_attn_tcgen05.cuh"
+
+// The arguments come checked from dsp_shared_attention (shared_attn.cu), which also launches the merge.
+extern "C" int DSP_CAT(dsp_shared_attention_tcgen05_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
+  return launch_rows_attn_tcgen05<SharedWork>(*a, stream);
+}

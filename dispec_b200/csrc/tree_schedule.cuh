@@ -13,7 +13,7 @@
 // not divided yet, running maximum, sum of weights) per CTA in scratch: slot 2 c + 1 for the item that begins in CTA c,
 // slot 2 c for the one that began before; tree_combine_kernel merges them in the order of the CTAs.
 #pragma once
-#include "common.cuh"
+#include "rows_schedule.cuh"
 
 namespace tree {
 
@@ -27,9 +27,6 @@ struct Shape {
   int* err;
   __device__ __forceinline__ int rows_per_tile() const { return 1 << row_shift; }
 };
-// Sizes of tiles are powers of two, and shifts: a CTA runs the search for its run once, and fetches every instruction of a division
-// for it.
-constexpr int KEY_SHIFT = 6, KEYS_PER_TILE = 1 << KEY_SHIFT;
 
 // One tree: sizes in units.
 struct Tree {
@@ -53,21 +50,6 @@ __device__ __forceinline__ Tree load_tree(const Shape& sh, int s) {
 }
 // Units of a tree in one of its row tiles.
 __device__ __forceinline__ int units_of(const Shape& sh, const Tree& t) { return t.key_tiles * sh.KVH; }
-
-__device__ __forceinline__ int warp_sum_int(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ int warp_scan(int v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += up;
-  }
-  return v;
-}
 
 // How the units are cut into runs, one per CTA.
 struct Cut {
@@ -218,7 +200,7 @@ struct Walk {
   Share at;
 
   // Called by whole warps.  False: this CTA has no work.
-  __device__ __forceinline__ bool begin(const Shape& sh, int block, int ctas) {
+  __device__ __forceinline__ bool begin(const Shape& sh, const NoPlan&, int block, int ctas) {
     const Found f = find_run(sh, block, ctas);
     cta = f.cta;
     if (f.seq < 0) return false;
@@ -258,7 +240,7 @@ struct Walk {
     }
     return x;
   }
-  __device__ __forceinline__ bool next(const Shape& sh) {
+  __device__ __forceinline__ bool next(const Shape& sh, const NoPlan&) {
     u += at.kt_end - at.kt_begin;
     if (u >= end) return false;
     item_start = u;
@@ -300,7 +282,6 @@ cudaError_t tree_combine(const TreeScratch& scratch, void* out, long out_stride,
                          int dtype, cudaStream_t stream);
 
 // The attention's arguments, checked.
-constexpr int ROW_SHIFT_TENSOR_CORES = 7;  // 128 rows a tile of the tensor-core kernel
 struct DspTreeAttention {
   tree::Shape sh;
   const void *q, *k_pool, *v_pool;
@@ -312,4 +293,76 @@ struct DspTreeAttention {
   int pt_stride, table_width, words, D, page_size, num_pages, ctas;
   float scale;
   int* err;
+};
+
+// What the kernels over rows have to know of drafted trees: a share's rows are nodes, its keys the stored tokens and the nodes.
+struct TreeWork {
+  typedef DspTreeAttention Args;
+  typedef tree::Shape Shape;
+  typedef tree::Share Share;
+  typedef tree::Walk Walk;
+  typedef NoPlan Plan;
+  static constexpr bool ROW_PARTS = false;  // items that are finished where they began are stored as results
+  struct Row {
+    int node, depth;
+  };
+  static __device__ __forceinline__ void make_plan(const Shape&, Plan&, int, int) {}
+  static __device__ __forceinline__ void note(const Args& a, int cta, const tree::Split& split, bool more) {
+    if (!more) a.scratch.splits[cta] = split;
+  }
+  static __device__ __forceinline__ void note_none(const Args& a, int cta) { a.scratch.splits[cta].parts = 0; }
+  // the keys that some row of the share may see
+  static __device__ __forceinline__ int key_begin(const Shape& sh, const Share& t) { return sh.window > 0 ? max(0, t.ctx - sh.window + 1) : 0; }
+  static __device__ __forceinline__ int key_end(const Share& t) { return t.ctx + t.n; }
+  // every row sees every key of the tile that begins with key0 (no node is deeper than the tree has nodes)
+  static __device__ __forceinline__ bool whole(const Shape& sh, const Share& t, int key0) {
+    return key0 <= t.ctx - KEYS_PER_TILE && (sh.window <= 0 || key0 > t.ctx + t.n - 1 - sh.window);
+  }
+  static __device__ __forceinline__ Row row(const Args& a, const Share&, int node) { return {node, a.sh.window > 0 ? a.depth[node] : 0}; }
+  // by a whole warp: a row of it may not see every key of the tile
+  static __device__ __forceinline__ bool any_hidden(const Shape& sh, const Share& t, const Row& row, int key0) {
+    return key0 > t.ctx - KEYS_PER_TILE || (sh.window > 0 && __any_sync(0xffffffffu, key0 < t.ctx + row.depth - sh.window + 1));
+  }
+  // Which keys key0 .. key0 + 63 a row sees: stored ones, and nodes of the tree by the row's words.
+  static __device__ __forceinline__ unsigned long long seen_keys(const Args& a, const Share& t, const Row& row, int key0) {
+    unsigned long long stored = 0ull, drafted = 0ull;
+    const int off = key0 - t.ctx;  // number of the first key as a node
+    if (off < 0) {
+      stored = off <= -64 ? ~0ull : (1ull << -off) - 1ull;
+      if (a.sh.window > 0) {
+        const int hidden = t.ctx + row.depth - a.sh.window + 1 - key0;  // so many first keys are out of the window
+        if (hidden > 0) stored = hidden >= 64 ? 0ull : stored & ~((1ull << hidden) - 1ull);
+      }
+    }
+    if (off > -64 && off < t.n) {
+      const unsigned long long* w = a.visible + (size_t)row.node * a.words;
+      if (off <= 0) {
+        drafted = w[0] << -off;
+      } else {
+        const int k = off >> 6, sft = off & 63;
+        drafted = k < a.words ? w[k] >> sft : 0ull;
+        if (sft && k + 1 < a.words) drafted |= w[k + 1] << (64 - sft);
+      }
+      const int there = t.n - off;  // keys up to the tree's last node
+      if (there < 64) drafted &= (1ull << there) - 1ull;
+      if (a.sh.window > 0 && row.depth >= a.sh.window) {  // a tree deeper than the window
+#pragma unroll 1
+        for (unsigned long long left = drafted; left != 0ull; left &= left - 1ull) {
+          const int c = __ffsll((long long)left) - 1;
+          if (a.depth[t.first + off + c] <= row.depth - a.sh.window) drafted &= ~(1ull << c);
+        }
+      }
+    }
+    return stored | drafted;
+  }
+  // the same of one key below key_end
+  static __device__ __forceinline__ bool sees(const Args& a, const Share& t, const Row& row, int key) {
+    int depth_of_key = key - t.ctx;
+    if (key >= t.ctx) {
+      const int k = key - t.ctx;
+      if (k >= 64 * a.words || !((a.visible[(size_t)row.node * a.words + (k >> 6)] >> (k & 63)) & 1ull)) return false;
+      if (a.sh.window > 0) depth_of_key = a.depth[t.first + k];
+    }
+    return a.sh.window <= 0 || depth_of_key > row.depth - a.sh.window;
+  }
 };

@@ -71,6 +71,16 @@ def tree_attention_library(head_dim: int) -> ctypes.CDLL:
     return _special[key]
 
 
+def shared_attention_library(head_dim: int) -> ctypes.CDLL:
+    key = f"shared_attn_tcgen05_d{head_dim}"
+    if key not in _special:
+        core()
+        with _lock:
+            if key not in _special:
+                _special[key] = ctypes.CDLL(build.shared_attention_library(head_dim))
+    return _special[key]
+
+
 def sink_attention_library(key_dim: int, value_dim: int) -> ctypes.CDLL:
     key = f"attn_sink_mma_k{key_dim}_v{value_dim}"
     if key not in _special:
@@ -147,7 +157,8 @@ def raise_on_device_error(where: str) -> None:
     v = device_error()
     if v:
         names = [n for bit, n in ((1, "page id outside the pool"), (2, "token id outside the vocabulary"),
-                                  (4, "a bounded wait ran out"), (8, "a tree whose nodes are not among the rows, or a path through one that does not ascend")) if v & bit]
+                                  (4, "a bounded wait ran out"), (8, "a tree whose nodes are not among the rows, or a path through one that does not ascend"),
+                                  (16, "a group whose rows are not among those there are, or slots that do not ascend or lie outside their pool")) if v & bit]
         raise KernelError(f"{where}: device reported: {', '.join(names) or v}")
 
 
