@@ -60,6 +60,12 @@ __device__ __forceinline__ K warp_kth(K x, int k) {
   return __shfl_sync(0xffffffffu, x, k);
 }
 
+__device__ __forceinline__ float ex2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct Args {
   const void* logits;
   const float* scores;
@@ -127,12 +133,14 @@ beam_pieces_kernel(const Args a) {
       x[k] = at < there ? to_f32(src[at]) : -INFINITY;
     }
   }
-  float top = -INFINITY;
+  // (fmaxf leaves NaN out)
+  float tops4[EACH / 4], top = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    x[k] = x[k] != x[k] ? -INFINITY : x[k];
-    top = fmaxf(top, x[k]);
+  for (int k = 0; k < EACH / 4; ++k) {
+    tops4[k] = fmaxf(fmaxf(x[4 * k], x[4 * k + 1]), fmaxf(x[4 * k + 2], x[4 * k + 3]));
+    top = fmaxf(top, tops4[k]);
   }
+  top = fmaxf(top, -INFINITY);
   const float mine = top;
   const uint32_t kth = warp_kth(ordered(top), (n + WARPS - 1) / WARPS - 1);
   const uint32_t warp_top = __reduce_max_sync(0xffffffffu, ordered(top));
@@ -148,25 +156,31 @@ beam_pieces_kernel(const Args a) {
     bound = min(bound, bounds[w]);
   }
   top = unordered(all_top);
-  // what reaches the bound
+  // what reaches the bound (NaN does not)
   const float limit = unordered(max(bound, NOTHING));
   if (mine >= limit && mine > -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      if (x[k] >= limit && x[k] > -INFINITY) {
-        const int at = atomicAdd(&found, 1);
-        const uint32_t column = first + WIDE * (tid + k / WIDE * THREADS) + k % WIDE;
-        if (at < CAP) list[at] = (unsigned long long)ordered(x[k]) << 32 | ~column;
+    for (int k = 0; k < EACH / 4; ++k) {
+      if (!(tops4[k] >= limit)) continue;
+#pragma unroll
+      for (int j = 4 * k; j < 4 * k + 4; ++j) {
+        if (x[j] >= limit && x[j] > -INFINITY) {
+          const int at = atomicAdd(&found, 1);
+          const uint32_t column = first + WIDE * (tid + j / WIDE * THREADS) + j % WIDE;
+          if (at < CAP) list[at] = (unsigned long long)ordered(x[j]) << 32 | ~column;
+        }
       }
     }
   }
   // exponentials: the difference is exact or nearly so, and the error of a product with log2 e shrinks with the term
   float sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[k] - top) * 1.4426950408889634f));
-    sum += x[k] == top ? (top == -INFINITY ? 0.f : 1.f) : e;
+  for (int k = 0; k < EACH; ++k) sum += ex2_of((x[k] - top) * 1.4426950408889634f);
+  if (!(sum < INFINITY)) {  // there is a NaN, or an infinity less itself: NaN counts as -inf, and infinities share the mass
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (x[k] == x[k] && x[k] > -INFINITY) sum += x[k] == top ? 1.f : ex2_of((x[k] - top) * 1.4426950408889634f);
   }
   double all = sum;
 #pragma unroll
@@ -189,7 +203,7 @@ beam_pieces_kernel(const Args a) {
     }
     int above = 0;
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) above += ordered(x[k]) > lo;
+    for (int k = 0; k < EACH; ++k) above += ordered(x[k]) > lo && x[k] > -INFINITY;
     const int equal = n - block_sum(above, of_warp);  // so many of the equals are taken, by column
     int c0 = 0, c1 = PIECE - 1;                       // the last of their columns, counted from `first`
     while (c0 < c1) {
@@ -244,8 +258,10 @@ struct Candidate {
 __global__ void __launch_bounds__(THREADS)
 beam_groups_kernel(const Args a) {
   __shared__ Candidate list[CAP];
-  __shared__ unsigned long long bounds[WARPS];
-  __shared__ int found;
+  __shared__ uint4 heads[THREADS / 4];
+  __shared__ int open[CAP];  // lists whose first entry reaches the bound
+  __shared__ uint32_t bound;
+  __shared__ int found, opened;
   __shared__ Candidate best_of_warp[WARPS], taken;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, group = blockIdx.x;
   pdl_launch_dependents();
@@ -261,7 +277,10 @@ beam_groups_kernel(const Args a) {
     parent[i] = token[i] = -1;
     score[i] = -INFINITY;
   }
-  if (tid == 0) found = 0;
+  if (tid == 0) {
+    found = opened = 0;
+    bound = (uint32_t)(NOTHING64 >> 32);
+  }
   // the rows' largest logits and sums: a warp a row
   for (int r = warp; r < rows; r += WARPS) {
     const Stat* stats = a.stats + (size_t)(first + r) * a.pieces;
@@ -296,7 +315,7 @@ beam_groups_kernel(const Args a) {
     const double away = x == of_row.x ? 0. : (double)x - (double)of_row.x;
     return {ordered((double)a.scores[first + r] + away - (double)of_row.y), (uint32_t)r, ~(uint32_t)e};
   };
-  // a lower bound of the n-th best key: a candidate a thread, or the best of a thread's lists
+  // A lower bound of the n-th best key, in its first 32 bits: the n-th of 256, a candidate a thread or the best of a thread's lists.
   unsigned long long mine = NOTHING64;
   if (lists >= THREADS) {
     for (int l = tid; l < lists; l += THREADS)
@@ -305,24 +324,37 @@ beam_groups_kernel(const Args a) {
     const int l = tid % lists, depth = tid / lists;
     if (depth < entries(l)) mine = candidate(l, depth).key;
   }
-  const unsigned long long kth = warp_kth(mine, (n + WARPS - 1) / WARPS - 1);
-  if (lane == 0) bounds[warp] = kth;
+  const uint32_t head = (uint32_t)(mine >> 32);
+  reinterpret_cast<uint32_t*>(heads)[tid] = head;
   __syncthreads();
-  unsigned long long bound = ~0ull;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) bound = min(bound, bounds[w]);
-  for (int l = tid; l < lists; l += THREADS) {
-    const int upto = entries(l);
-    for (int depth = 0; depth < upto; ++depth) {
-      const Candidate c = candidate(l, depth);
-      if (c.key < bound || c.key <= NOTHING64) break;
-      const int at = atomicAdd(&found, 1);
-      if (at >= CAP) break;
-      list[at] = c;
+  int larger = 0;
+  for (int j = 0; j < THREADS / 4; ++j) {
+    const uint4 x = heads[j];
+    // (equals in the order of the threads: one of them is the n-th)
+    larger += (x.x > head || (x.x == head && 4 * j < tid)) + (x.y > head || (x.y == head && 4 * j + 1 < tid)) +
+              (x.z > head || (x.z == head && 4 * j + 2 < tid)) + (x.w > head || (x.w == head && 4 * j + 3 < tid));
+  }
+  if (larger == n - 1) bound = head;
+  __syncthreads();
+  const uint32_t limit = bound;
+  auto reaches = [&](const Candidate& c) { return (uint32_t)(c.key >> 32) >= limit && c.key > NOTHING64; };
+  for (int l = tid; l < lists; l += THREADS)
+    if (entries(l) > 0 && reaches(candidate(l, 0))) {
+      const int at = atomicAdd(&opened, 1);
+      if (at < CAP) open[at] = l;
     }
+  __syncthreads();
+  // the entries of those lists, side by side
+  for (int i = tid; i < min(opened, CAP) * n; i += THREADS) {
+    const int l = open[i / n], depth = i % n;
+    if (depth >= entries(l)) continue;
+    const Candidate c = candidate(l, depth);
+    if (!reaches(c)) continue;
+    const int at = atomicAdd(&found, 1);
+    if (at < CAP) list[at] = c;
   }
   __syncthreads();
-  if (found <= CAP) {
+  if (found <= CAP && opened <= CAP) {
     const int count = found;
     for (int i = tid; i < count; i += THREADS) {
       const Candidate c = list[i];

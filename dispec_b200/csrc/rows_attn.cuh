@@ -97,10 +97,10 @@ rows_attn_kernel(const typename Work::Args a) {
   const auto& sh = a.sh;
   __shared__ typename Work::Plan plan;
   typename Work::Walk w;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: what comes next may look at the inputs before it waits)
   Work::make_plan(sh, plan, blockIdx.x, gridDim.x);
-  if (!w.begin(sh, plan, blockIdx.x, gridDim.x)) {
+  if (!Work::begin(w, sh, plan, blockIdx.x, gridDim.x)) {
     if (tid == 0) Work::note_none(a, w.cta);
     return;
   }
@@ -280,7 +280,7 @@ rows_attn_kernel(const typename Work::Args a) {
       }
     }
     const auto split = w.split(sh);
-    more = w.next(sh, plan);
+    more = w.next(sh);
     if (tid == 0) Work::note(a, w.cta, split, more);
   } while (more);
 }

@@ -297,7 +297,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
   bool more = false;
   auto step = [&](int share) {  // works that share out, the one behind the last
     const auto split = w.split(sh);
-    more = w.next(sh, plan);
+    more = w.next(sh);
     if (lane == 0) {
       if (!more) w.at.seq = -1;
       Work::note(p.a, w.cta, split, more);
@@ -306,7 +306,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
     __syncwarp();
   };
   if (warp == 0) {
-    more = w.begin(sh, plan, blockIdx.x, gridDim.x);
+    more = Work::begin(w, sh, plan, blockIdx.x, gridDim.x);
     if (lane == 0) {
       if (!more) {
         w.at.seq = -1;
@@ -856,7 +856,7 @@ int launch_rows_attn_tcgen05(const typename Work::Args& a, cudaStream_t stream) 
   const int page = a.page_size;
   Params<Work> p = {};
   p.a = a;
-  p.a.sh.min_units = 2;  // one tile for each softmax group
+  p.a.sh.min_units = max(a.sh.min_units, 2);  // one tile for each softmax group
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap map_k, map_v, runs_k, runs_v;
   if (!make_map_pages(&map_k, a.k_pool, a.num_pages, a.sh.KVH, page, D, 1) ||

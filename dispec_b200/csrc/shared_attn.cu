@@ -7,7 +7,8 @@
 // A sum over keys may be taken in parts: with m the largest score of a part, l = sum exp(s_j - m) and a = sum exp(s_j - m) v_j, parts
 // join as  M = max m,  o = sum a exp(m - M) / sum l exp(m - M).  So the shared keys are read once for all sequences of a group,
 // whose rows fill the tiles of a matrix product, and each sequence's own keys once for its G rows.  A row that sees nothing gives 0.
-// The work is cut as shared_schedule.cuh says; the kernels: rows_attn_tcgen05.cuh, rows_attn.cuh.
+// The work is cut as shared_schedule.cuh says; the kernels: shared_attn_few.cuh, rows_attn_tcgen05.cuh where many rows share keys,
+// rows_attn.cuh in 32-bit arithmetic.
 #include "merge_parts.cuh"
 #include "rows_attn.cuh"
 #include "shared_schedule.cuh"
@@ -16,39 +17,55 @@
 namespace {
 using namespace shared;
 
-// Threads take the rows of all sequences in turn, four columns each.
-constexpr int COMBINE_THREADS = 256, COMBINE_BLOCKS_PER_SM = 4;
+constexpr int FEW_CTAS = 2;                                 // an SM (shared_attn_few.cuh)
+constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
+// What an item's beginning and end cost, in key tiles, and the fewest key tiles of a run.
+constexpr int EXTRA_FEW = 1, MIN_TILES_FEW = 1, EXTRA_MANY = 5;
+
+// A thread has four columns of a row and head.  Groups and lengths were there before the kernels in front began, and are looked at
+// before their results are waited for; then two latencies are left, the records' and the partial results'.
+constexpr int COMBINE_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(COMBINE_THREADS, COMBINE_BLOCKS_PER_SM)
-shared_combine_kernel(const Shape sh, const SharedScratch scratch, T* __restrict__ out, long out_stride, int D, int ctas) {
-  __shared__ int start[MAX_GROUPS + 1];
+__global__ void __launch_bounds__(COMBINE_THREADS, 3)
+shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch scratch, const SharedScratch scratch_many,
+                      T* __restrict__ out, long out_stride, int D, int ctas, int ctas_many) {
+  const int H = sh.KVH * sh.G, quads = D / 4;
+  const long i = (long)blockIdx.x * COMBINE_THREADS + threadIdx.x;
+  const float2* rows_ml = reinterpret_cast<const float2*>(scratch.rows_ml);
+  const int row_head = (int)min(i / quads, (long)sh.rows * H), d = (int)(i % quads) * 4, row = row_head / H, h = row_head - row * H;
+  const int head = h / sh.G, of_head = h - head * sh.G;
+  const int g = row < sh.rows ? group_of(sh.group_start, sh.groups, sh.rows, row) : -1;
+  bool many = false, sees[2] = {false, false};  // the shared part was the other kernel's
+  int of_tile[2] = {0, 0};
+  long item[2] = {0, 0};
+  if (g >= 0) {
+    const int length = sh.length(row), first = sh.group_start[g], n = sh.group_start[g + 1] - first;
+    const int prefix = n > 1 ? min(max(0, sh.prefix_len[g]), sh.most_ctx) : 0, lo = sh.window > 0 ? max(0, length - sh.window) : 0;
+    many = (long)n * sh.G > sh.many;
+    // an item of which the row sees a key is there, and has a record
+    sees[0] = lo < min(prefix, length);
+    sees[1] = max(prefix, lo) < length;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const Shape& of = part == 0 && many ? sh_many : sh;
+      const int rr = (part == 0 ? (row - first) * sh.G : 0) + of_head;
+      of_tile[part] = rr & (of.rows_per_tile() - 1);
+      item[part] = of.item(part, g, part == 0 ? first : row, rr >> of.row_shift, head);
+    }
+  }
   pdl_launch_dependents();
   pdl_wait();
-  for (int g = threadIdx.x; g <= sh.groups; g += COMBINE_THREADS) start[g] = sh.group_start[g];
-  __syncthreads();
-  const int H = sh.KVH * sh.G, quads = D / 4;
-  const long pieces = (long)sh.rows * H * quads;
-  const float2 *part_ml = reinterpret_cast<const float2*>(scratch.part_ml), *rows_ml = reinterpret_cast<const float2*>(scratch.rows_ml);
-  for (long i = (long)blockIdx.x * COMBINE_THREADS + threadIdx.x; i < pieces; i += (long)gridDim.x * COMBINE_THREADS) {
-    const int row_head = (int)(i / quads), d = (int)(i - (long)row_head * quads) * 4, row = row_head / H, h = row_head - row * H;
-    const int head = h / sh.G, of_head = h - head * sh.G;
-    const int g = group_of(start, sh.groups, sh.rows, row);
-    if (g < 0) continue;  // in no group: left as it is
-    const int length = sh.length(row), first = start[g];
-    const bool several = start[g + 1] - first > 1;
-    const int prefix = several ? min(max(0, sh.prefix_len[g]), sh.most_ctx) : 0, lo = sh.window > 0 ? max(0, length - sh.window) : 0;
-    // an item of which the row sees a key is there, and has a record
-    int of_tile[2];
+  if (g >= 0) {  // (a row in no group is left as it is)
     Record rec[2];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      const bool sees = part == 0 ? lo < min(prefix, length) : max(prefix, lo) < length;
-      const int rr = (part == 0 ? (row - first) * sh.G : 0) + of_head;
-      of_tile[part] = rr & (sh.rows_per_tile() - 1);
-      rec[part] = {0, 0};
-      if (sees) rec[part] = scratch.records[sh.item(part, g, part == 0 ? first : row, rr >> sh.row_shift, head)];
+      const bool of_many = part == 0 && many;
+      Record x = {0, 0, 1};
+      if (sees[part]) x = (of_many ? scratch_many : scratch).records[item[part]];
       // (a record that a CTA whose wait ran out did not write is none)
-      if (rec[part].cta < 0 || rec[part].parts < 0 || rec[part].parts > ctas - rec[part].cta) rec[part] = {0, 0};
+      if (x.cta < 0 || x.parts < 0 || x.stride < 1 || (x.parts > 0 && x.cta + (x.parts - 1) * x.stride >= (of_many ? ctas_many : ctas)))
+        x = {0, 0, 1};
+      rec[part] = x;
     }
     const float4 v = merge_parts(rec[0].parts + rec[1].parts, [&](int k, float2& ml, float4& o) {
       const int part = k >= rec[0].parts;
@@ -58,28 +75,35 @@ shared_combine_kernel(const Shape sh, const SharedScratch scratch, T* __restrict
         ml = rows_ml[at];
         o = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
       } else {
-        const size_t at = ((size_t)2 * (rec[part].cta + k) + (k == 0)) * sh.rows_per_tile() + of_tile[part];
-        ml = part_ml[at];
-        o = *reinterpret_cast<const float4*>(scratch.part_o + at * D + d);
+        const bool of_many = part == 0 && many;
+        const SharedScratch& of = of_many ? scratch_many : scratch;
+        const size_t slot = 2 * (size_t)(rec[part].cta + k * rec[part].stride) + (k == 0);
+        const size_t at = slot * (of_many ? sh_many : sh).rows_per_tile() + of_tile[part];
+        ml = reinterpret_cast<const float2*>(of.part_ml)[at];
+        o = *reinterpret_cast<const float4*>(of.part_o + at * D + d);
       }
     });
     store4(out + (size_t)row * out_stride + (size_t)h * D + d, v);
   }
 }
 
-long scratch_floats(const Shape& sh, long ctas, long D) {
-  const long rows = sh.rows_per_tile(), H = (long)sh.KVH * sh.G;
-  return 2 * ctas * rows * (D + 2) + 2 * (long)sh.rows * H * (D + 2) + 2 * sh.items();
+// A kernel's scratch of its own, laid out from `at` on.
+long layout(SharedScratch& x, float* at, const Shape& sh, long ctas, long D) {
+  const long rows = sh.rows_per_tile();
+  x.part_o = at;
+  x.part_ml = x.part_o + 2 * ctas * rows * D;
+  x.records = reinterpret_cast<Record*>(x.part_ml + 4 * ctas * rows);
+  return 2 * ctas * rows * (D + 2) + 2 * ((sh.items() + 1) / 2 * 2);
 }
 }  // namespace
 
 struct DspSharedOptions {  // as ops/beams.py packs them
-  long window, sms, tensor_cores;
+  long window, sms, few, many;
   double scale;
 };
 
-// tensors: q, key pool, value pool, page table, ctx_len, group_start, prefix_len, out, scratch.  `tensor_cores`: address of the
-// tensor-core kernel's entry point for this head size, or 0.
+// Addresses of the tensor-core kernels' entry points for this head size, or 0: `few`, `many`.
+// tensors: q, key pool, value pool, page table, ctx_len, group_start, prefix_len, out, scratch.
 extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* o, cudaStream_t stream) {
   const DspTensor &q = t[0], &k = t[1], &v = t[2], &table = t[3], &ctx = t[4], &start = t[5], &prefix = t[6], &out = t[7], &scratch = t[8];
 #define SHARED_REQUIRE(cond, ...) DSP_REQUIRE(cond, "shared_prefix_attention: " __VA_ARGS__)
@@ -110,10 +134,10 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   const uintptr_t bits = (uintptr_t)q.data | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)out.data;
   const long piece = q.dtype == DSP_T_F32 ? 4 : 8;  // elements of 16 bytes
   SHARED_REQUIRE(bits % 16 == 0 && (R == 1 || (q.stride[0] % piece == 0 && out.stride[0] % piece == 0)), "rows must begin on 16 bytes");
-  // the tensor-core kernel is built for these page sizes; everything else takes the 32-bit kernel
-  const bool tensor_cores = o->tensor_cores != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
+  // the tensor-core kernels are built for these page sizes; everything else takes the 32-bit kernel
+  const bool tensor_cores = o->few != 0 && o->many != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
                             (page == 8 || page == 16 || page == 32 || page == 64) && pages > 0;
-  const long ctas = o->sms * (tensor_cores || D > 128 ? 1 : 2);  // (by shared memory two CTAs of the 32-bit kernel an SM)
+  const long ctas = o->sms * (tensor_cores ? FEW_CTAS : D > 128 ? 1 : 2);  // (by shared memory two CTAs an SM)
   DspSharedAttention a = {};
   a.sh.group_start = (const int*)start.data;
   a.sh.prefix_len = (const int*)prefix.data;
@@ -123,22 +147,35 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   a.sh.G = (int)(columns / D / KVH);
   a.sh.window = (int)o->window;
   a.sh.rows = (int)R;
-  a.sh.row_shift = tensor_cores ? ROW_SHIFT_TENSOR_CORES : ROW_SHIFT_32BIT;
+  a.sh.row_shift = tensor_cores ? ROW_SHIFT_FEW : ROW_SHIFT_32BIT;
+  a.sh.extra = EXTRA_FEW;
+  a.sh.min_units = MIN_TILES_FEW + EXTRA_FEW;
+  // where groups have more rows a head than a tile of the kernel for few on average, the shared parts of those that do are the
+  // other one's
+  const bool use_many = tensor_cores && R * a.sh.G > groups * FEW_ROWS_OF_A_TILE;
+  a.sh.many = use_many ? FEW_ROWS_OF_A_TILE : 0x7fffffff;
   // places are counted in 32 bits, a tile of keys beyond the last among them
   a.sh.most_ctx = (int)min(table.size[1] * page, 1L << 30);
   // Units are counted in 32 bits: those of all items, each over as many tokens as a sequence's pages hold.
-  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (a.sh.most_ctx / KEYS_PER_TILE + 1),
+  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (a.sh.most_ctx / KEYS_PER_TILE + 1 + EXTRA_MANY),
                  "%ld rows of %ld heads over pages for %d tokens a sequence are too many for one call", R, columns / D, a.sh.most_ctx);
+  DspSharedAttention many = a;
+  many.sh.is_many = 1;
+  many.sh.row_shift = ROW_SHIFT_TENSOR_CORES;
+  many.sh.extra = EXTRA_MANY;
+  many.sh.min_units = 2 + EXTRA_MANY;
+  a.ctas = (int)ctas;
+  many.ctas = use_many ? (int)o->sms : 0;
+  const long of_rows = 2 * R * columns / D;
+  a.scratch.rows_o = many.scratch.rows_o = (float*)scratch.data;
+  a.scratch.rows_ml = many.scratch.rows_ml = a.scratch.rows_o + of_rows * D;
+  long floats = of_rows * (D + 2);
+  floats += layout(a.scratch, (float*)scratch.data + floats, a.sh, a.ctas, D);
+  if (use_many) floats += layout(many.scratch, (float*)scratch.data + floats, many.sh, many.ctas, D);
   SHARED_REQUIRE(scratch.contiguous && scratch.device == q.device && scratch.dims == 1 && (uintptr_t)scratch.data % 16 == 0 &&
-                     scratch.size[0] >= scratch_floats(a.sh, ctas, D),
-                 "scratch is too small");
+                     scratch.size[0] >= floats,
+                 "scratch is too small: %ld of %ld", scratch.size[0], floats);
   SHARED_REQUIRE(current_device() == q.device, "the tensors are on device %d, the current device is %d", q.device, current_device());
-  const long rows = a.sh.rows_per_tile(), of_rows = 2 * R * columns / D;
-  a.scratch.part_o = (float*)scratch.data;
-  a.scratch.rows_o = a.scratch.part_o + 2 * ctas * rows * D;
-  a.scratch.part_ml = a.scratch.rows_o + of_rows * D;
-  a.scratch.rows_ml = a.scratch.part_ml + 4 * ctas * rows;
-  a.scratch.records = reinterpret_cast<Record*>(a.scratch.rows_ml + 2 * of_rows);
   a.q = q.data;
   a.k_pool = k.data;
   a.v_pool = v.data;
@@ -151,27 +188,33 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   a.D = (int)D;
   a.page_size = (int)page;
   a.num_pages = (int)pages;
-  a.ctas = (int)ctas;
   a.scale = (float)o->scale;
   a.err = a.sh.err = dsp_device_error_ptr();
   SHARED_REQUIRE(a.err != nullptr, "no device error word");
   if (tensor_cores) {
     typedef int (*Kernel)(const DspSharedAttention*, cudaStream_t);
-    const int rc = reinterpret_cast<Kernel>(o->tensor_cores)(&a, stream);
+    int rc = 0;
+    if (use_many) {
+      DspSharedAttention x = a;
+      x.sh = many.sh;
+      x.scratch = many.scratch;
+      x.ctas = many.ctas;
+      x.sh.err = a.err;
+      rc = reinterpret_cast<Kernel>(o->many)(&x, stream);
+    }
+    if (rc == 0) rc = reinterpret_cast<Kernel>(o->few)(&a, stream);
     SHARED_REQUIRE(rc == 0, "%s", rc == 4 ? "shared memory opt-in or tensor map creation failed" : "launch failed");
   } else {
-    a.sh.min_units = 1;
     const int rc = q.dtype == DSP_T_F32 ? launch_rows_attn<SharedWork, float>(a, stream) : launch_rows_attn<SharedWork, bf16>(a, stream);
     if (rc != 0) return rc;
   }
-  const long pieces = R * columns / 4;
-  const dim3 grid((unsigned)min((pieces + COMBINE_THREADS - 1) / COMBINE_THREADS, o->sms * COMBINE_BLOCKS_PER_SM));
+  const dim3 grid((unsigned)((R * columns / 4 + COMBINE_THREADS - 1) / COMBINE_THREADS));
   if (q.dtype == DSP_T_F32)
-    DSP_CUDA(launch_pdl(shared_combine_kernel<float>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, a.scratch, (float*)a.out, a.out_stride,
-                        a.D, a.ctas));
+    DSP_CUDA(launch_pdl(shared_combine_kernel<float>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, many.sh, a.scratch, many.scratch,
+                        (float*)a.out, a.out_stride, a.D, a.ctas, many.ctas));
   else
-    DSP_CUDA(launch_pdl(shared_combine_kernel<bf16>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, a.scratch, (bf16*)a.out, a.out_stride,
-                        a.D, a.ctas));
+    DSP_CUDA(launch_pdl(shared_combine_kernel<bf16>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, many.sh, a.scratch, many.scratch,
+                        (bf16*)a.out, a.out_stride, a.D, a.ctas, many.ctas));
   DSP_CHECK_LAUNCH("shared_prefix_attention");
   return 0;
 }

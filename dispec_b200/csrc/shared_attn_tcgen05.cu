@@ -1,10 +1,13 @@
-// Attention of sequences with a shared beginning on the tensor cores (the formula: shared_attn.cu; the kernel:
-// rows_attn_tcgen05.cuh; how the work is cut and what a row sees: shared_schedule.cuh).  Compiled once per head size
-// (-DDSP_HEAD_DIM=64 or 128).
+// Attention of sequences with a shared beginning on the tensor cores (the formula: shared_attn.cu; how the work is cut and what a
+// row sees: shared_schedule.cuh).  Compiled once per head size (-DDSP_HEAD_DIM=64 or 128).
 #include "shared_schedule.cuh"
 #include "rows_attn_tcgen05.cuh"
+#include "shared_attn_few.cuh"
 
 // The arguments come checked from dsp_shared_attention (shared_attn.cu), which also launches the merge.
-extern "C" int DSP_CAT(dsp_shared_attention_tcgen05_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
+extern "C" int DSP_CAT(dsp_shared_attention_few_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
+  return launch_shared_few(*a, stream);
+}
+extern "C" int DSP_CAT(dsp_shared_attention_many_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
   return launch_rows_attn_tcgen05<SharedWork>(*a, stream);
 }

@@ -4,9 +4,14 @@
 // P_g = prefix_len[g] tokens are the same for all of them and are read through the pages of its first sequence.  A segment is
 // either such a beginning with the rows of all the group's sequences, or one sequence's keys behind it with its own G rows (a
 // group of one has no shared part: all its keys are one segment).  An item is one tile of query rows of one key/value head of
-// one segment; it walks the key tiles of 64 that any of its rows sees.  A unit is one key tile of one item.  All units, in the order
-// (shared parts, sequences; row tile, head, key tile), are cut into equal runs, one per CTA, wherever that falls, so that few long
-// beginnings load every SM as well as many short sequences, and nothing about lengths is needed on the host.
+// one segment; it walks the key tiles of 64 that any of its rows sees, and is counted as so many units and `extra` more, which
+// stand for its beginning and end.  All units, in the order (shared parts, sequences; row tile, head, key tile), are cut into equal
+// runs, one per CTA, wherever that falls, so that few long beginnings load every SM as well as many short sequences, and nothing
+// about lengths is needed on the host.
+//
+// Two kernels may share the work: beginnings with more than `many` rows a head go to one whose tiles have 128 rows, the rest to
+// one with smaller tiles.  Where all beginnings of the first have R row tiles, teams of R CTAs walk the same keys with one row
+// tile each, which then come from memory once and from the L2 for the others.
 //
 // Every item leaves a partial result (32-bit sums that are not divided yet, running maximum, sum of weights): in the place of its
 // rows, `rows_o`, where one CTA had all of it, else one in each CTA's scratch slots (2 c + 1 for the item that begins in CTA c,
@@ -16,20 +21,24 @@
 
 namespace shared {
 
-constexpr int MAX_GROUPS = 1024;  // of a call: a CTA holds what it has to know of all of them
+constexpr int MAX_GROUPS = 1024;  // of a call: a CTA holds what it has to know of all of them while it finds its run
 
 struct Shape {
   const int *group_start, *prefix_len, *ctx_len;
-  int groups, KVH, G, window, min_units;
+  int groups, KVH, G, window, min_units, extra;
   int rows;       // sequences: a group that is not inside them is recorded and left out
   int most_ctx;   // tokens that a sequence's pages hold
   int row_shift;  // of a tile's query rows
+  int many;       // shared parts of more rows a head are for the kernel of many rows
+  int is_many;    // that kernel's shape
   int* err;
   __host__ __device__ __forceinline__ int rows_per_tile() const { return 1 << row_shift; }
   // items are numbered by row tiles: those of shared parts by their group's first row, then those of sequences
   __host__ __device__ __forceinline__ long shared_tiles() const { return ((long)rows * G >> row_shift) + groups + 1; }
   __host__ __device__ __forceinline__ int tiles_of_sequence() const { return (G + rows_per_tile() - 1) >> row_shift; }
-  __host__ __device__ __forceinline__ long items() const { return (shared_tiles() + (long)rows * tiles_of_sequence()) * KVH; }
+  __host__ __device__ __forceinline__ long items() const {
+    return (shared_tiles() + (is_many ? 0 : (long)rows * tiles_of_sequence())) * KVH;
+  }
   __device__ __forceinline__ long item(int part, int group, int first, int row_tile, int head) const {
     const long tile = part == 0 ? ((long)first * G >> row_shift) + group + row_tile
                                 : shared_tiles() + (long)first * tiles_of_sequence() + row_tile;
@@ -51,107 +60,163 @@ __device__ __forceinline__ int group_of(const int* start, int groups, int rows, 
   return start[lo] <= row && row < start[lo + 1] && start[lo] >= 0 && start[lo + 1] <= rows ? lo : -1;
 }
 
-// What a CTA has to know of the groups, in shared memory, and where its run begins.
-struct Plan {
+// What a CTA has to know of the groups while it finds its run.
+struct Groups {
   int start[MAX_GROUPS + 1], prefix[MAX_GROUPS], shortest[MAX_GROUPS], longest[MAX_GROUPS];
-  int of_warp[32];
-  int total, chunk;               // all units; units of a run
-  int segment, segment_start;     // of the CTA's first unit
+  int of_warp[32], most_tiles[32], least_tiles[32];
 };
-
 struct Segment {
-  int seq, group, part, first, n;  // sequence whose pages are read; first row and number of rows
-  int from, begin, end;            // first key of the segment; the keys that any of its rows sees
-  int all_begin, all_end;          // the keys that all of them see
+  int group, part, first, n;   // first row and number of rows; the first one's pages are read
+  int from, begin, end;        // first key of the segment; the keys that any of its rows sees
+  int all_begin, all_end;      // the keys that all of them see
   int lo_tile, key_tiles, row_tiles;
 };
 
-__device__ __forceinline__ Segment segment(const Shape& sh, const Plan& plan, int s) {
+// The shared part of group g, whose sequences have between `shortest` and `longest` tokens.
+__device__ __forceinline__ Segment shared_part(const Shape& sh, int g, int first, int end, int prefix, int shortest, int longest) {
   Segment x = {};
-  const int row = s - sh.groups;
-  if (row < 0) {
-    x.group = s;
-    x.part = 0;
-    x.first = plan.start[s];
-    x.n = plan.start[s + 1] - x.first;
-    if (x.first < 0 || plan.start[s + 1] > sh.rows || x.n < 2) return x;
-    x.end = min(plan.prefix[s], plan.longest[s]);
-    x.all_end = min(plan.prefix[s], plan.shortest[s]);
-    if (sh.window > 0) {
-      x.begin = max(0, plan.shortest[s] - sh.window);
-      x.all_begin = max(0, plan.longest[s] - sh.window);
-    }
-  } else {
-    x.group = group_of(plan.start, sh.groups, sh.rows, row);
-    x.part = 1;
-    x.first = row;
-    x.n = 1;
-    if (x.group < 0) return x;
-    const int length = sh.length(row);
-    x.from = plan.start[x.group + 1] - plan.start[x.group] > 1 ? plan.prefix[x.group] : 0;
-    x.begin = x.all_begin = max(x.from, sh.window > 0 ? length - sh.window : 0);
-    x.end = x.all_end = length;
+  x.group = g;
+  x.first = first;
+  x.n = end - first;
+  if (first < 0 || end > sh.rows || x.n < 2 || ((long)x.n * sh.G > sh.many) != (sh.is_many != 0)) return x;
+  x.end = min(prefix, longest);
+  x.all_end = min(prefix, shortest);
+  if (sh.window > 0) {
+    x.begin = max(0, shortest - sh.window);
+    x.all_begin = max(0, longest - sh.window);
   }
-  x.seq = x.first;
   x.lo_tile = x.begin >> KEY_SHIFT;
   x.key_tiles = x.end > x.begin ? ((x.end + KEYS_PER_TILE - 1) >> KEY_SHIFT) - x.lo_tile : 0;
   x.row_tiles = (x.n * sh.G + sh.rows_per_tile() - 1) >> sh.row_shift;
   return x;
 }
-__device__ __forceinline__ int units_of(const Shape& sh, const Segment& x) { return x.key_tiles * x.row_tiles * sh.KVH; }
+// The own part of a row of group g (first .. end - 1), -1: of none.
+__device__ __forceinline__ Segment own_part(const Shape& sh, int row, int g, int first, int end, int prefix) {
+  Segment x = {};
+  x.group = g;
+  x.part = 1;
+  x.first = row;
+  x.n = 1;
+  if (g < 0 || sh.is_many) return x;
+  const int length = sh.length(row);
+  x.from = end - first > 1 ? prefix : 0;
+  x.begin = x.all_begin = max(x.from, sh.window > 0 ? length - sh.window : 0);
+  x.end = x.all_end = length;
+  x.lo_tile = x.begin >> KEY_SHIFT;
+  x.key_tiles = x.end > x.begin ? ((x.end + KEYS_PER_TILE - 1) >> KEY_SHIFT) - x.lo_tile : 0;
+  x.row_tiles = sh.tiles_of_sequence();
+  return x;
+}
+// `near`: a group that the row may be in, looked at first.
+__device__ __forceinline__ Segment segment(const Shape& sh, const Groups& groups, int s, int near = -1) {
+  const int row = s - sh.groups;
+  if (row < 0)
+    return shared_part(sh, s, groups.start[s], groups.start[s + 1], groups.prefix[s], groups.shortest[s], groups.longest[s]);
+  if (near < 0 || row < groups.start[near] || row >= groups.start[near + 1] || groups.start[near + 1] > sh.rows)
+    near = group_of(groups.start, sh.groups, sh.rows, row);
+  const int at = max(near, 0);
+  return own_part(sh, row, near, groups.start[at], groups.start[at + 1], groups.prefix[at]);
+}
+__device__ __forceinline__ int units_of(const Shape& sh, const Segment& x, int row_tiles) {
+  return x.key_tiles > 0 ? (x.key_tiles + sh.extra) * row_tiles * sh.KVH : 0;
+}
+
+// Where a CTA's run begins.
+constexpr int AHEAD = 24;  // segments from there on that are worked out while all groups are at hand
+struct Run {
+  int total, chunk;            // all units (of one row tile, with teams); units of a run
+  int teams;                   // CTAs that walk the same keys
+  int segment, segment_start;  // of the CTA's first unit (-1: there is none)
+  Segment ahead[AHEAD];
+};
+struct Plan {
+  Groups groups;
+  Run run;
+};
 
 // By the whole block.
-__device__ __forceinline__ void make_plan(const Shape& sh, Plan& plan, int cta, int ctas) {
+__device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& run, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  const int own_length = tid < sh.rows ? sh.length(tid) : 0;  // (asked for with the groups)
   for (int g = tid; g <= sh.groups; g += threads) {
-    plan.start[g] = sh.group_start[g];
+    groups.start[g] = sh.group_start[g];
     if (g == sh.groups) break;
-    plan.prefix[g] = min(max(0, sh.prefix_len[g]), sh.most_ctx);
-    plan.shortest[g] = 0x7fffffff;
-    plan.longest[g] = 0;
+    groups.prefix[g] = min(max(0, sh.prefix_len[g]), sh.most_ctx);
+    groups.shortest[g] = 0x7fffffff;
+    groups.longest[g] = 0;
   }
-  if (tid == 0) plan.segment = -1;
+  if (tid == 0) run.segment = -1;
   __syncthreads();
   for (int g = tid; g < sh.groups; g += threads)
-    if (plan.start[g] < 0 || plan.start[g + 1] < plan.start[g] || plan.start[g + 1] > sh.rows) atomicOr(sh.err, DSP_ERR_BAD_GROUP);
+    if (groups.start[g] < 0 || groups.start[g + 1] < groups.start[g] || groups.start[g + 1] > sh.rows) atomicOr(sh.err, DSP_ERR_BAD_GROUP);
   for (int row = tid; row < sh.rows; row += threads) {
-    const int length = sh.length(row), g = group_of(plan.start, sh.groups, sh.rows, row);
+    const int length = row == tid ? own_length : sh.length(row), g = group_of(groups.start, sh.groups, sh.rows, row);
     if (g < 0) continue;
-    atomicMin(&plan.shortest[g], length);
-    atomicMax(&plan.longest[g], length);
+    atomicMin(&groups.shortest[g], length);
+    atomicMax(&groups.longest[g], length);
   }
   __syncthreads();
   // a thread has neighbouring segments
-  const int segments = sh.groups + sh.rows, each = (segments + threads - 1) / threads;
+  const int segments = sh.groups + (sh.is_many ? 0 : sh.rows), each = (segments + threads - 1) / threads;
   const int s0 = min(tid * each, segments), s1 = min(s0 + each, segments);
-  int mine = 0;
-  for (int s = s0; s < s1; ++s) mine += units_of(sh, segment(sh, plan, s));
+  int mine = 0, of_first = 0, most = 0, least = 0x7fffffff, near = -1;
+  for (int s = s0; s < s1; ++s) {
+    const Segment x = segment(sh, groups, s, near);
+    near = x.part ? x.group : -1;
+    mine += units_of(sh, x, x.row_tiles);
+    of_first += units_of(sh, x, 1);
+    if (x.key_tiles > 0) {
+      most = max(most, x.row_tiles);
+      least = min(least, x.row_tiles);
+    }
+  }
+  bool teams = false;
+  if (sh.is_many) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) {
+      groups.most_tiles[warp] = most;
+      groups.least_tiles[warp] = least;
+    }
+    __syncthreads();
+    for (int w = 0; w < threads >> 5; ++w) {
+      most = max(most, groups.most_tiles[w]);
+      least = min(least, groups.least_tiles[w]);
+    }
+    teams = most == least && most > 1 && most <= ctas;
+  }
+  const int team_size = teams ? most : 1;
+  if (teams) mine = of_first;
   int upto = warp_scan(mine);
-  if (lane == 31) plan.of_warp[warp] = upto;
+  if (lane == 31) groups.of_warp[warp] = upto;
   __syncthreads();
   int total = 0;
   for (int w = 0; w < threads >> 5; ++w) {
-    if (w < warp) upto += plan.of_warp[w];
-    total += plan.of_warp[w];
+    if (w < warp) upto += groups.of_warp[w];
+    total += groups.of_warp[w];
   }
-  const int chunk = max((total + ctas - 1) / ctas, sh.min_units);
-  const long u = (long)chunk * cta;
-  if (u < total && u < upto && u >= upto - mine) {
+  const int runs = ctas / team_size, chunk = max((total + runs - 1) / runs, sh.min_units);
+  const long u = (long)chunk * (cta / team_size);
+  if (cta / team_size < runs && u < total && u < upto && u >= upto - mine) {
     int at = upto - mine;
     for (int s = s0; s < s1; ++s) {
-      const int n = units_of(sh, segment(sh, plan, s));
+      const Segment x = segment(sh, groups, s, near);
+      const int n = units_of(sh, x, teams ? 1 : x.row_tiles);
       if (u < at + n) {
-        plan.segment = s;
-        plan.segment_start = at;
+        run.segment = s;
+        run.segment_start = at;
         break;
       }
       at += n;
     }
   }
   if (tid == 0) {
-    plan.total = total;
-    plan.chunk = chunk;
+    run.total = total;
+    run.chunk = chunk;
+    run.teams = team_size;
   }
+  __syncthreads();
+  if (tid < AHEAD && run.segment >= 0 && run.segment + tid < segments) run.ahead[tid] = segment(sh, groups, run.segment + tid);
   __syncthreads();
 }
 
@@ -165,43 +230,66 @@ struct Share {
   int slot;                // scratch slot of the partial result, -1: in the place of its rows
 };
 
-// Where an item's partial results are: in `parts` CTAs from `cta` on (one: in the place of its rows).
+// Where an item's partial results are: in `parts` CTAs, cta, cta + stride, ... (one: in the place of its rows).
 struct Record {
-  int cta, parts;
+  int cta;
+  short parts, stride;
 };
 struct Note {
   long item;  // -1: the share does not begin its item
   Record record;
 };
 
-// A CTA's walk over its run of units, one item's share at a time.
+// A CTA's walk over its run of units, one item's share at a time.  Called by whole warps.
 struct Walk {
-  int cta;
+  int cta, teams;
   int u, end, chunk, segment_at;
   int item_start, key_tiles, lo_tile, row_tiles;
+  bool begins;             // the share has its item's first key tile
+  const Run* run_;
   Share at;
 
-  __device__ __forceinline__ bool begin(const Shape& sh, const Plan& plan, int block, int) {
+  __device__ __forceinline__ bool begin(const Shape& sh, const Run& run, int block) {
     cta = block;
+    run_ = &run;
     at.seq = -1;
-    if (plan.segment < 0) return false;
-    chunk = plan.chunk;
-    u = chunk * cta;
-    end = (int)min((long)u + chunk, (long)plan.total);
-    segment_at = plan.segment;
-    enter(segment(sh, plan, segment_at));
-    const int item = (u - plan.segment_start) / key_tiles;
-    item_start = plan.segment_start + item * key_tiles;
-    at.row_tile = item / sh.KVH;
-    at.head = item - at.row_tile * sh.KVH;
-    share();
-    return true;
+    if (run.segment < 0) return false;
+    teams = run.teams;
+    chunk = run.chunk;
+    u = chunk * (cta / teams);
+    end = (int)min((long)u + chunk, (long)run.total);
+    segment_at = run.segment;
+    enter(sh);
+    const int cost = key_tiles + sh.extra, item = (u - run.segment_start) / cost;
+    item_start = run.segment_start + item * cost;
+    at.row_tile = teams > 1 ? cta % teams : item / sh.KVH;
+    at.head = item % sh.KVH;
+    return share(sh) || next(sh);
   }
-  __device__ __forceinline__ void enter(const Segment& x) {
-    at.seq = x.seq;
+  // what has to be known of segment `segment_at`; false: it has no keys
+  __device__ __forceinline__ bool enter(const Shape& sh) {
+    Segment x;
+    const int row = segment_at - sh.groups;
+    if (segment_at - run_->segment < AHEAD) {
+      x = run_->ahead[segment_at - run_->segment];
+    } else if (row < 0) {
+      const int g = segment_at, first = sh.group_start[g], last = sh.group_start[g + 1];
+      int shortest = 0x7fffffff, longest = 0;
+      if (first >= 0 && last <= sh.rows)
+        for (int r = first + (int)(threadIdx.x & 31); r < last; r += 32) {
+          const int length = sh.length(r);
+          shortest = min(shortest, length);
+          longest = max(longest, length);
+        }
+      x = shared_part(sh, g, first, last, min(max(0, sh.prefix_len[g]), sh.most_ctx), __reduce_min_sync(0xffffffffu, shortest),
+                      __reduce_max_sync(0xffffffffu, longest));
+    } else {
+      const int g = group_of(sh.group_start, sh.groups, sh.rows, row), at = max(g, 0);
+      x = own_part(sh, row, g, sh.group_start[at], sh.group_start[at + 1], min(max(0, sh.prefix_len[at]), sh.most_ctx));
+    }
+    at.seq = at.first = x.first;
     at.part = x.part;
     at.group = x.group;
-    at.first = x.first;
     at.n = x.n;
     at.from = x.from;
     at.begin = x.begin;
@@ -210,46 +298,48 @@ struct Walk {
     at.all_end = x.all_end;
     key_tiles = x.key_tiles;
     lo_tile = x.lo_tile;
-    row_tiles = x.row_tiles;
+    row_tiles = teams > 1 ? 1 : x.row_tiles;
+    return key_tiles > 0;
   }
-  __device__ __forceinline__ void share() {
-    const int item_end = item_start + key_tiles, stop = min(end, item_end);
-    at.kt_begin = lo_tile + (u - item_start);
-    at.kt_end = at.kt_begin + (stop - u);
-    at.slot = u == item_start ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
+  // the run's part of the present item; false: it has no key tile
+  __device__ __forceinline__ bool share(const Shape& sh) {
+    const int first_tile = item_start + sh.extra, item_end = first_tile + key_tiles, stop = min(end, item_end);
+    begins = u <= first_tile;
+    at.kt_begin = lo_tile + max(u - first_tile, 0);
+    at.kt_end = lo_tile + (stop - first_tile);
+    at.slot = begins ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
+    u = stop;
+    return at.kt_end > at.kt_begin;
   }
   __device__ __forceinline__ Note split(const Shape& sh) const {
-    Note x = {-1, {cta, 1}};
-    if (u == item_start) {
+    Note x = {-1, {cta, 1, (short)teams}};
+    if (begins) {
       x.item = sh.item(at.part, at.group, at.first, at.row_tile, at.head);
-      x.record.parts = (item_start + key_tiles - 1) / chunk - cta + 1;
+      x.record.parts = (short)((item_start + sh.extra + key_tiles - 1) / chunk - cta / teams + 1);
     }
     return x;
   }
-  __device__ __forceinline__ bool next(const Shape& sh, const Plan& plan) {
-    u += at.kt_end - at.kt_begin;
-    if (u >= end) return false;
-    item_start = u;
-    if (++at.head == sh.KVH) {
-      at.head = 0;
-      if (++at.row_tile == row_tiles) {
-        at.row_tile = 0;
-        Segment x;
-        do {  // (there is such a segment: units are left)
-          x = segment(sh, plan, ++segment_at);
-        } while (x.key_tiles == 0);
-        enter(x);
+  __device__ __forceinline__ bool next(const Shape& sh) {
+    do {
+      if (u >= end) return false;
+      item_start = u;
+      if (++at.head == sh.KVH) {
+        at.head = 0;
+        if (teams > 1 || ++at.row_tile == row_tiles) {
+          if (teams == 1) at.row_tile = 0;
+          do ++segment_at;
+          while (!enter(sh));  // (there is such a segment: units are left)
+        }
       }
-    }
-    share();
+    } while (!share(sh));
     return true;
   }
 };
 
 }  // namespace shared
 
-// Scratch of a call: part_o [2 ctas][rows of a tile][D] floats, part_ml [2 ctas][rows of a tile] pairs (maximum in the base-2
-// domain, sum), rows_o [2][rows H][D], rows_ml [2][rows H] pairs, records [items].
+// Scratch of a kernel: part_o [2 ctas][rows of a tile][D] floats, part_ml [2 ctas][rows of a tile] pairs (maximum in the base-2
+// domain, sum), records [items]; and of both, for items that were not cut: rows_o [2][rows H][D], rows_ml [2][rows H] pairs.
 struct SharedScratch {
   float *part_o, *part_ml, *rows_o, *rows_ml;
   shared::Record* records;
@@ -279,7 +369,8 @@ struct SharedWork {
   struct Row {
     int lo, hi;
   };
-  static __device__ __forceinline__ void make_plan(const Shape& sh, Plan& plan, int cta, int ctas) { shared::make_plan(sh, plan, cta, ctas); }
+  static __device__ __forceinline__ void make_plan(const Shape& sh, Plan& plan, int cta, int ctas) { shared::make_plan(sh, plan.groups, plan.run, cta, ctas); }
+  static __device__ __forceinline__ bool begin(Walk& w, const Shape& sh, const Plan& plan, int block, int) { return w.begin(sh, plan.run, block); }
   static __device__ __forceinline__ void note(const Args& a, int, const shared::Note& x, bool) {
     if (x.item >= 0) a.scratch.records[x.item] = x.record;
   }

@@ -200,7 +200,7 @@ struct Walk {
   Share at;
 
   // Called by whole warps.  False: this CTA has no work.
-  __device__ __forceinline__ bool begin(const Shape& sh, const NoPlan&, int block, int ctas) {
+  __device__ __forceinline__ bool begin(const Shape& sh, int block, int ctas) {
     const Found f = find_run(sh, block, ctas);
     cta = f.cta;
     if (f.seq < 0) return false;
@@ -240,7 +240,7 @@ struct Walk {
     }
     return x;
   }
-  __device__ __forceinline__ bool next(const Shape& sh, const NoPlan&) {
+  __device__ __forceinline__ bool next(const Shape& sh) {
     u += at.kt_end - at.kt_begin;
     if (u >= end) return false;
     item_start = u;
@@ -307,6 +307,7 @@ struct TreeWork {
     int node, depth;
   };
   static __device__ __forceinline__ void make_plan(const Shape&, Plan&, int, int) {}
+  static __device__ __forceinline__ bool begin(Walk& w, const Shape& sh, const Plan&, int block, int ctas) { return w.begin(sh, block, ctas); }
   static __device__ __forceinline__ void note(const Args& a, int cta, const tree::Split& split, bool more) {
     if (!more) a.scratch.splits[cta] = split;
   }

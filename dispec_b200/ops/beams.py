@@ -12,7 +12,7 @@ import torch
 from dispec_b200.ops import library as L
 from dispec_b200.ops import tuning
 
-_ATTENTION = struct.Struct("3qd")
+_ATTENTION = struct.Struct("4qd")
 _PIECE, _STAT = 8192, 16  # logits that a block holds, bytes of what it leaves of them (csrc/beam_select.cu)
 
 
@@ -29,15 +29,16 @@ def _load_describe():
     return _describe
 
 
-_tensor_core_calls: dict = {}  # head size -> address of the tensor-core kernel's entry point
+_tensor_core_calls: dict = {}  # head size -> addresses of the tensor-core kernels' entry points
 
 
-def _tensor_core_call(dim: int) -> int:
-    call = _tensor_core_calls.get(dim)
-    if call is None:
-        call = L.address_of(L.shared_attention_library(dim), f"dsp_shared_attention_tcgen05_d{dim}")
-        _tensor_core_calls[dim] = call
-    return call
+def _tensor_core_call(dim: int) -> tuple:
+    calls = _tensor_core_calls.get(dim)
+    if calls is None:
+        lib = L.shared_attention_library(dim)
+        calls = tuple(L.address_of(lib, f"dsp_shared_attention_{rows}_d{dim}") for rows in ("few", "many"))
+        _tensor_core_calls[dim] = calls
+    return calls
 
 
 def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -67,17 +68,22 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     dev = q.get_device()
     (rows, columns), (_, kv_heads, page, dim) = q.shape, k_pool.shape
     sms = tuning._sm_count.get(dev) or tuning.sm_count(dev)
-    # the tensor-core kernel is built for these head sizes and pages
+    # the tensor-core kernels are built for these head sizes and pages
     tensor_cores = q.dtype is torch.bfloat16 and dim in (64, 128) and page in (8, 16, 32, 64)
-    # scratch of this call alone (calls on several streams do not meet in it): two partial results of a tile of rows for each
-    # CTA, two for each row, and what the merge has to know of every item (csrc/shared_schedule.cuh)
-    tile, ctas = (128, sms) if tensor_cores else (32, sms * (1 if dim > 128 else 2))
-    share = columns // max(1, kv_heads * dim)
-    items = (rows * share // tile + prefix_len.numel() + 1 + rows * -(-share // tile)) * kv_heads
-    scratch = prefix_len.new_empty(2 * (ctas * tile + rows * kv_heads * share) * (dim + 2) + 2 * items)
+    # scratch of this call alone (calls on several streams do not meet in it): two partial results for each row, and for each
+    # kernel two of a tile of rows for each CTA and what the merge has to know of every item (csrc/shared_schedule.cuh)
+    share, groups = columns // max(1, kv_heads * dim), prefix_len.numel()
+    tile, ctas = (64, 2 * sms) if tensor_cores else (32, sms * (1 if dim > 128 else 2))
+    items = (rows * share // tile + groups + 1 + rows * -(-share // tile)) * kv_heads + 1
+    rest = ctas * tile * (dim + 2) + items
+    many = tensor_cores and rows * share > 64 * groups
+    if many:
+        rest += sms * 128 * (dim + 2) + (rows * share // 128 + groups + 1) * kv_heads + 1
+    scratch = prefix_len.new_empty(2 * (rows * kv_heads * share * (dim + 2) + rest))
     tensors = (_describe or _load_describe())(q, k_pool, v_pool, page_table, ctx_len, group_start, prefix_len, out, scratch)
-    L.check(L.core().dsp_shared_attention(tensors, _ATTENTION.pack(window, sms, _tensor_core_call(dim) if tensor_cores else 0, scale),
-                                          L.stream_handle()), launches=2)
+    few_call, many_call = _tensor_core_call(dim) if tensor_cores else (0, 0)
+    L.check(L.core().dsp_shared_attention(tensors, _ATTENTION.pack(window, sms, few_call, many_call, scale), L.stream_handle()),
+            launches=3 if many else 2)
     return out
 
 

@@ -6,7 +6,7 @@ import pytest
 from dispec_b200.ops import library as L
 from test_tree_checks_cpu import BF16, F32, I32, I64, NONE, described
 
-OPTIONS = struct.Struct("3qd")  # window, sms, tensor_cores, scale
+OPTIONS = struct.Struct("4qd")  # window, sms, the tensor-core kernels, scale
 
 
 def refused(call):
@@ -22,7 +22,7 @@ def attention(R=3, scratch=0, table=None, scale=1.0, window=0, groups=1, page=4,
              prefix=described(I32, (groups,)), out=described(F32, (R, 4 * dim)), scratch=described(I32, (scratch,)))
     t.update(change)
     names = ("q", "k", "v", "table", "ctx", "start", "prefix", "out", "scratch")
-    return refused(lambda: L.core().dsp_shared_attention(b"".join(t[n] for n in names), OPTIONS.pack(window, 148, 0, scale), None))
+    return refused(lambda: L.core().dsp_shared_attention(b"".join(t[n] for n in names), OPTIONS.pack(window, 148, 0, 0, scale), None))
 
 
 @pytest.mark.parametrize("R", [1, 2, 9])

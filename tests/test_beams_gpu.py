@@ -49,6 +49,25 @@ def test_attention_many_shares_a_cta(dim, kv_heads, window):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("groups", [[(300, [301 + j % 5 for j in range(70)])], [(130, [131] * 40), (700, [701] * 40), (64, [90] * 40)],
+                                    [(900, [905] * 60), (200, [201, 210]), (70, [80] * 33), (5, [300])],
+                                    [(90, [100] * 17 + [0, 40] * 9)] * 2])
+@pytest.mark.parametrize("dim,window", [(128, 0), (64, 0), (128, 60), (64, 130)])
+def test_attention_many_rows_a_key(dtype, groups, dim, window):
+    """Shared parts of more than 64 rows a head, alike in their row tiles and not, beside smaller ones."""
+    SharedCase(groups, 8, 2, dim, dtype, window=window).check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 1), (16, 1), (17, 1), (32, 1), (33, 1), (64, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_rows_of_a_tile(heads, kv_heads, dim):
+    """A tile's rows in one, two and four tiles of sixteen, whole and not."""
+    SharedCase([(200, [230, 201]), (90, [91, 140, 95]), (0, [333])], heads, kv_heads, dim, BF16).check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("page_size", [1, 8, 16, 24, 32, 64, 128])
 @pytest.mark.parametrize("scatter", [False, True])
 def test_attention_pages(dtype, page_size, scatter):
