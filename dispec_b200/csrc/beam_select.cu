@@ -15,6 +15,7 @@
 // bisected.  A block a group then merges the sums of its rows' pieces and picks n of the pieces' lists in the same way.
 //
 // Loads bound it.
+#include "packed2.cuh"
 #include "tensor_checks.cuh"
 
 namespace {
@@ -49,6 +50,15 @@ constexpr unsigned long long NOTHING64 = 0x000fffffffffffffull;
 template <typename K>
 __device__ __forceinline__ K warp_kth(K x, int k) {
   const int lane = threadIdx.x & 31;
+  if constexpr (sizeof(K) == 4) {
+    if (k < 4) {  // one after the other is quicker
+      for (int i = 0; i < k; ++i) {
+        const uint32_t those = __ballot_sync(0xffffffffu, x == __reduce_max_sync(0xffffffffu, x));
+        if (lane == __ffs(those) - 1) x = 0;
+      }
+      return __reduce_max_sync(0xffffffffu, x);
+    }
+  }
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -92,6 +102,53 @@ __device__ __forceinline__ int block_sum(int mine, int* of_warp) {
   return all;
 }
 
+// Where more logits reach the lower bound than can be put in order: the n-th largest by bisection, and where its equals are more
+// than wanted, the last column taken.  By the whole block; how many are in the list then.
+template <int WIDE>
+__device__ __noinline__ int exact_bound(const float* x, uint32_t bound, uint32_t all_top, int n, int first, unsigned long long* list,
+                                        int* found, int* of_warp) {
+  const int tid = threadIdx.x;
+  uint32_t lo = bound, hi = all_top;  // at least n are >= lo (or all that there are); the answer is in lo .. hi
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int c = 0;
+#pragma unroll 1
+    for (int k = 0; k < EACH; ++k) c += ordered(x[k]) >= mid && x[k] > -INFINITY;
+    if (block_sum(c, of_warp) >= n)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  int above = 0;
+#pragma unroll 1
+  for (int k = 0; k < EACH; ++k) above += ordered(x[k]) > lo && x[k] > -INFINITY;
+  const int equal = n - block_sum(above, of_warp);  // so many of the equals are taken, by column
+  int c0 = 0, c1 = PIECE - 1;                       // the last of their columns, counted from `first`
+  while (c0 < c1) {
+    const int mid = (c0 + c1) / 2;
+    int c = 0;
+#pragma unroll 1
+    for (int k = 0; k < EACH; ++k) c += ordered(x[k]) == lo && WIDE * (tid + k / WIDE * THREADS) + k % WIDE <= mid;
+    if (block_sum(c, of_warp) >= equal)
+      c1 = mid;
+    else
+      c0 = mid + 1;
+  }
+  if (tid == 0) *found = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < EACH; ++k) {
+    const int column = WIDE * (tid + k / WIDE * THREADS) + k % WIDE;
+    const uint32_t o = ordered(x[k]);
+    if ((o > lo || (o == lo && column <= c0)) && x[k] > -INFINITY) {
+      const int at = atomicAdd(found, 1);
+      if (at < CAP) list[at] = (unsigned long long)o << 32 | ~(uint32_t)(first + column);
+    }
+  }
+  __syncthreads();
+  return min(*found, CAP);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4)
 beam_pieces_kernel(const Args a) {
@@ -102,8 +159,8 @@ beam_pieces_kernel(const Args a) {
   constexpr int WIDE = 16 / sizeof(T);  // logits of a load
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
   const int row = blockIdx.y, first = blockIdx.x * PIECE;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: the next kernel looks at the groups before it waits)
   if (tid == 0) found = 0;
   // Thread t has the columns first + WIDE (t + 256 k) .. + WIDE - 1, however the row lies in memory: equal rows give equal sums.
   const T* src = (const T*)a.logits + (size_t)row * a.stride + first;
@@ -137,10 +194,9 @@ beam_pieces_kernel(const Args a) {
   float tops4[EACH / 4], top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < EACH / 4; ++k) {
-    tops4[k] = fmaxf(fmaxf(x[4 * k], x[4 * k + 1]), fmaxf(x[4 * k + 2], x[4 * k + 3]));
+    tops4[k] = fmaxf(max3(x[4 * k], x[4 * k + 1], x[4 * k + 2]), x[4 * k + 3]);
     top = fmaxf(top, tops4[k]);
   }
-  top = fmaxf(top, -INFINITY);
   const float mine = top;
   const uint32_t kth = warp_kth(ordered(top), (n + WARPS - 1) / WARPS - 1);
   const uint32_t warp_top = __reduce_max_sync(0xffffffffu, ordered(top));
@@ -173,9 +229,14 @@ beam_pieces_kernel(const Args a) {
     }
   }
   // exponentials: the difference is exact or nearly so, and the error of a product with log2 e shrinks with the term
-  float sum = 0.f;
+  float2 sums2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int k = 0; k < EACH; ++k) sum += ex2_of((x[k] - top) * 1.4426950408889634f);
+  for (int k = 0; k < EACH; k += 2) {
+    const float2 y = mul2(add2(make_float2(x[k], x[k + 1]), make_float2(-top, -top)), make_float2(1.4426950408889634f, 1.4426950408889634f));
+    sums2[k / 2 % 2] = add2(sums2[k / 2 % 2], make_float2(ex2_of(y.x), ex2_of(y.y)));
+  }
+  sums2[0] = add2(sums2[0], sums2[1]);
+  float sum = sums2[0].x + sums2[0].y;
   if (!(sum < INFINITY)) {  // there is a NaN, or an infinity less itself: NaN counts as -inf, and infinities share the mass
     sum = 0.f;
 #pragma unroll
@@ -189,46 +250,10 @@ beam_pieces_kernel(const Args a) {
   __syncthreads();
   int count = found;
   if (count > CAP) {
-    // too many reach it: the n-th largest logit by bisection, and where its equals are more than wanted, the last column taken
-    uint32_t lo = bound, hi = all_top;  // at least n are >= lo (or all that there are); the answer is in lo .. hi
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      int c = 0;
+    float copy[EACH];  // (so that the usual way keeps its registers)
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) c += ordered(x[k]) >= mid && x[k] > -INFINITY;
-      if (block_sum(c, of_warp) >= n)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    int above = 0;
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) above += ordered(x[k]) > lo && x[k] > -INFINITY;
-    const int equal = n - block_sum(above, of_warp);  // so many of the equals are taken, by column
-    int c0 = 0, c1 = PIECE - 1;                       // the last of their columns, counted from `first`
-    while (c0 < c1) {
-      const int mid = (c0 + c1) / 2;
-      int c = 0;
-#pragma unroll
-      for (int k = 0; k < EACH; ++k) c += ordered(x[k]) == lo && WIDE * (tid + k / WIDE * THREADS) + k % WIDE <= mid;
-      if (block_sum(c, of_warp) >= equal)
-        c1 = mid;
-      else
-        c0 = mid + 1;
-    }
-    if (tid == 0) found = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const int column = WIDE * (tid + k / WIDE * THREADS) + k % WIDE;
-      const uint32_t o = ordered(x[k]);
-      if ((o > lo || (o == lo && column <= c0)) && x[k] > -INFINITY) {
-        const int at = atomicAdd(&found, 1);
-        if (at < CAP) list[at] = (unsigned long long)o << 32 | ~(uint32_t)(first + column);
-      }
-    }
-    __syncthreads();
-    count = min(found, CAP);
+    for (int k = 0; k < EACH; ++k) copy[k] = x[k];
+    count = exact_bound<WIDE>(copy, bound, all_top, n, first, list, &found, of_warp);
   }
   const size_t piece = (size_t)row * a.pieces + blockIdx.x;
   unsigned long long* out = a.lists + piece * n;
@@ -264,8 +289,6 @@ beam_groups_kernel(const Args a) {
   __shared__ int found, opened;
   __shared__ Candidate best_of_warp[WARPS], taken;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, group = blockIdx.x;
-  pdl_launch_dependents();
-  pdl_wait();
   const int first = a.group_start[group], end = a.group_start[group + 1];
   int* parent = a.parent + (size_t)group * n;
   int* token = a.token + (size_t)group * n;
@@ -281,6 +304,8 @@ beam_groups_kernel(const Args a) {
     found = opened = 0;
     bound = (uint32_t)(NOTHING64 >> 32);
   }
+  pdl_launch_dependents();
+  pdl_wait();
   // the rows' largest logits and sums: a warp a row
   for (int r = warp; r < rows; r += WARPS) {
     const Stat* stats = a.stats + (size_t)(first + r) * a.pieces;

@@ -7,6 +7,7 @@
 //
 // dst ascends, so that no slot is written twice; what does not ascend, or names a slot that is not there, is left from there on
 // and recorded.
+#include "tcgen05_common.cuh"
 #include "tensor_checks.cuh"
 
 namespace {
@@ -21,31 +22,85 @@ struct Pool {
 struct Args {
   Pool pools[MAX_POOLS];
   const int *src, *dst;
-  int count, pools_n, chunk_shift;  // pieces of an entry in a block: 1 << chunk_shift
+  int count, pools_n;
+  int chunk_shift, chunk_bytes;  // of an entry in a block: 1 << chunk_shift pieces; of bulk copies
   int* err;
 };
+
+// The pool of a block: the last one whose first block is not behind it.
+__device__ __forceinline__ const Pool& pool_of(const Args& a) {
+  int p = 0;
+  for (int step = MAX_POOLS / 2; step > 0; step >>= 1)
+    if (p + step < a.pools_n && a.pools[p + step].first_block <= (int)blockIdx.x) p += step;
+  return a.pools[p];
+}
+// How many entries are copied, by the whole block.
+__device__ __forceinline__ int sound_entries(const Args& a, const Pool& pool, int* bad) {
+  if (threadIdx.x == 0) *bad = a.count;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.count; i += blockDim.x) {
+    const int s = a.src[i], d = a.dst[i], before = i > 0 ? a.dst[i - 1] : -1;
+    if (s < 0 || s >= pool.slots || d < 0 || d >= pool.slots || d <= before) atomicMin(bad, i);
+  }
+  __syncthreads();
+  if (*bad < a.count && threadIdx.x == 0) atomicOr(a.err, DSP_ERR_BAD_GROUP);
+  return *bad;
+}
+
+// Rows of whole 16-byte pieces and up to BULK_ENTRIES entries: the columns of an entry are one bulk copy into shared memory and one
+// back.
+constexpr int BULK_THREADS = 128, BULK_ENTRIES = 512, BULK_BYTES = 48 * 1024;
+__global__ void __launch_bounds__(BULK_THREADS)
+reorder_bulk_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(128) unsigned char stage[];
+  __shared__ int bad;
+  __shared__ __align__(8) uint64_t landed;
+  const int tid = threadIdx.x;
+  const Pool& pool = pool_of(a);
+  const int block = blockIdx.x - pool.first_block, layer = block / pool.chunks, chunk = block - layer * pool.chunks;
+  const long column = (long)chunk * a.chunk_bytes;
+  const uint32_t bytes = (uint32_t)min((long)a.chunk_bytes, pool.row_bytes - column);
+  char* base = pool.data + (size_t)layer * pool.slots * pool.row_bytes + column;
+  if (tid == 0) {
+    tc::mbar_init(&landed, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  const int count = sound_entries(a, pool, &bad);
+  if (count == 0) return;
+  if (tid == 0) tc::mbar_expect_tx(&landed, bytes * (uint32_t)count);
+  __syncthreads();
+  for (int i = tid; i < count; i += BULK_THREADS)
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     tc::smem_u32(stage + (size_t)i * a.chunk_bytes)),
+                 "l"(base + (size_t)a.src[i] * pool.row_bytes), "r"(bytes), "r"(tc::smem_u32(&landed))
+                 : "memory");
+  if (!tc::mbar_wait(&landed, 0)) {
+    atomicOr(a.err, DSP_ERR_WAIT_LIMIT);
+    // let copies that are still on their way land before the shared memory goes away
+#pragma unroll 1
+    for (int i = 0; i < 2000; ++i) __nanosleep(100);
+    return;
+  }
+  for (int i = tid; i < count; i += BULK_THREADS)
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + (size_t)a.dst[i] * pool.row_bytes),
+                 "r"(tc::smem_u32(stage + (size_t)i * a.chunk_bytes)), "r"(bytes)
+                 : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 
 template <typename Piece, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 reorder_kernel(const __grid_constant__ Args a) {
   __shared__ int bad;
   const int tid = threadIdx.x;
-  if (tid == 0) bad = a.count;
-  int p = 0;  // the last pool whose first block is not behind this one
-  for (int step = MAX_POOLS / 2; step > 0; step >>= 1)
-    if (p + step < a.pools_n && a.pools[p + step].first_block <= (int)blockIdx.x) p += step;
-  const Pool& pool = a.pools[p];
+  const Pool& pool = pool_of(a);
   const int block = blockIdx.x - pool.first_block, layer = block / pool.chunks, chunk = block - layer * pool.chunks;
   pdl_launch_dependents();
   pdl_wait();
-  __syncthreads();
-  for (int i = tid; i < a.count; i += THREADS) {
-    const int s = a.src[i], d = a.dst[i];
-    if (s < 0 || s >= pool.slots || d < 0 || d >= pool.slots || (i > 0 && d <= a.dst[i - 1])) atomicMin(&bad, i);
-  }
-  __syncthreads();
-  const int count = bad;
-  if (count < a.count && tid == 0) atomicOr(a.err, DSP_ERR_BAD_GROUP);
+  const int count = sound_entries(a, pool, &bad);
   const long in_row = pool.row_bytes / (long)sizeof(Piece);
   Piece* base = reinterpret_cast<Piece*>(pool.data) + (size_t)layer * pool.slots * in_row;
   const long column0 = (long)chunk << a.chunk_shift;
@@ -96,15 +151,18 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
       REORDER_REQUIRE(a.pools[o].data != a.pools[p].data || a.pools[p].row_bytes == 0, "pools %ld and %ld are the same memory", o, p);
   }
   if (n == 0) return 0;
-  // the widest pieces that all rows consist of; as many of an entry in a block as its threads can hold
+  // the widest pieces that all rows consist of; as much of an entry in a block as it can hold
   const long piece = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+  const bool bulk = piece == 16 && n <= BULK_ENTRIES;
   const int threads = n <= 512 ? 256 : 1024;  // (rows of 64 bytes at least up to 2,048 entries)
   REORDER_REQUIRE(n <= (long)threads * EACH, "%ld slots to be copied, at most %d", n, 1024 * EACH);
   while ((n << (a.chunk_shift + 1)) <= (long)threads * EACH) ++a.chunk_shift;
+  const long chunk_bytes = bulk ? BULK_BYTES / n / 16 * 16 : piece << a.chunk_shift;
+  a.chunk_bytes = (int)chunk_bytes;
   long blocks = 0;
   for (long p = 0; p < pools; ++p) {
     Pool& x = a.pools[p];
-    const long in_row = x.row_bytes / piece, chunks = (in_row + (1L << a.chunk_shift) - 1) >> a.chunk_shift;
+    const long chunks = (x.row_bytes + chunk_bytes - 1) / chunk_bytes;
     x.chunks = (int)max(chunks, 1L);
     x.first_block = (int)blocks;
     blocks += chunks * t[2 + p].size[0];
@@ -118,15 +176,21 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
   a.pools_n = (int)pools;
   a.err = dsp_device_error_ptr();
   REORDER_REQUIRE(a.err != nullptr, "no device error word");
-  auto go = [&](auto kernel) -> int {
-    DSP_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, a));
+  auto go = [&](auto kernel, int threads_of, size_t smem) -> int {
+    DSP_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(threads_of), smem, stream, a));
     return 0;
   };
-  const int rc = threads == 256 ? (piece == 16 ? go(reorder_kernel<uint4, 256>) : piece == 4 ? go(reorder_kernel<uint32_t, 256>)
-                                                                                             : go(reorder_kernel<uint16_t, 256>))
-                                : (piece == 16 ? go(reorder_kernel<uint4, 1024>) : piece == 4 ? go(reorder_kernel<uint32_t, 1024>)
-                                                                                              : go(reorder_kernel<uint16_t, 1024>));
-  if (rc != 0) return rc;
+  if (bulk) {
+    DSP_CUDA(cudaFuncSetAttribute(reorder_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BULK_BYTES));
+    const int rc = go(reorder_bulk_kernel, BULK_THREADS, BULK_BYTES);
+    if (rc != 0) return rc;
+  } else {
+    const int rc = threads == 256 ? (piece == 16 ? go(reorder_kernel<uint4, 256>, 256, 0) : piece == 4 ? go(reorder_kernel<uint32_t, 256>, 256, 0)
+                                                                                                       : go(reorder_kernel<uint16_t, 256>, 256, 0))
+                                  : (piece == 16 ? go(reorder_kernel<uint4, 1024>, 1024, 0) : piece == 4 ? go(reorder_kernel<uint32_t, 1024>, 1024, 0)
+                                                                                                         : go(reorder_kernel<uint16_t, 1024>, 1024, 0));
+    if (rc != 0) return rc;
+  }
   DSP_CHECK_LAUNCH("reorder_slots");
   return 0;
 }
