@@ -7,28 +7,29 @@
 // largest keys in descending order, ties to the lowest row, then the lowest v.  NaN counts as -inf; what is -inf is no
 // candidate; a row whose score is not finite has none; where infinities are the largest logits, they share the mass.
 //
-// Within a row the order of keys is that of logits, so the n best of a piece of a row can be told before its sum is known.
-// One pass over the logits: a block holds 8,192 of a row in registers, 32 a thread, and leaves their maximum, their sum of
-// exponentials and their n best in order.  A lower bound of the n-th best, which few others reach, costs no
-// search: of each of the 8 warps the ceil(n / 8)-th largest of its lanes' maxima, of these the smallest: at least n logits are as
-// large.  What reaches it (some 2 n) is put in order by counting.  Where too many do (many equal logits), the exact bound is
-// bisected.  A block a group then merges the sums of its rows' pieces and picks n of the pieces' lists in the same way.
+// Within a row the order of keys is that of logits, so the n best of a part of a row can be told before its sum is known.
+// One pass over the logits: the rows' pieces of 8,192 are dealt out to the CTAs in runs, and a CTA goes through its run with the
+// next two pieces on their way into shared memory (bulk copies, where rows begin on 16 bytes).  Of its part of a row it leaves the
+// n best in order; and of every piece each warp leaves the maximum and the sum of exponentials of its 1,024 logits, so that sums do
+// not depend on how rows are dealt out.
+// What does not exceed the n-th best so far is left alone; what does is put aside, and now and then the list is put in order anew by
+// counting.  Of a part's first piece a lower bound of the n-th best, which few others reach, costs no search: of each of the 8 warps
+// the ceil(n / 8)-th largest of its lanes' maxima, of these the smallest: at least n logits are as large.  Where too many reach it
+// (many equal logits), the piece's exact bound is bisected.  A block a group then merges the sums of its rows' parts and picks n
+// of their lists.
 //
 // Loads bound it.
 #include "packed2.cuh"
+#include "tcgen05_common.cuh"
 #include "tensor_checks.cuh"
 
 namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 32, PIECE = THREADS * EACH;
 constexpr int MAX_COUNT = 8 * 32;  // each warp vouches for an eighth of the wanted
-constexpr int CAP = 1024;          // candidates that are put in order by counting
-
-// Statistics of a piece of a row and how many entries its list has.
-struct Stat {
-  double sum;  // of exp(x - top)
-  float top;
-  int count;
-};
+constexpr int CAP = 1024;          // candidates of a group that are put in order by counting
+constexpr int ASIDE = 32;          // logits that are put aside before a part's list is put in order
+constexpr int LIST_CAP = 2 * MAX_COUNT + 2 * ASIDE;
+constexpr int SAMPLES = 4 * THREADS;
 
 // Numbers in the order of floats; -inf gives the smallest of those that are numbers.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -82,11 +83,15 @@ struct Args {
   const int* group_start;
   int *parent, *token;
   float* score;
-  Stat* stats;                  // [rows][pieces]
-  unsigned long long* lists;    // [rows][pieces][n]: logit in order and its column's complement
+  float2* stats;                // [rows][pieces][WARPS] largest logit and sum of exponentials
+  // CTA c's part of row r is number c + r (one behind it is left out where both end together, and has no entries)
+  uint32_t* parts;              // [rows + ctas] the row, and how many entries the list has
+  unsigned long long* lists;    // [rows + ctas][n]: logit in order and its column's complement
   float2* of_rows;              // [rows] largest logit and logarithm of the sum
   long stride;                  // of a row of logits
   int rows, groups, vocab, pieces, n;
+  int run;                      // pieces of a CTA
+  int bulk;                     // rows begin and end on 16 bytes
   int* err;
 };
 
@@ -102,13 +107,13 @@ __device__ __forceinline__ int block_sum(int mine, int* of_warp) {
   return all;
 }
 
-// Where more logits reach the lower bound than can be put in order: the n-th largest by bisection, and where its equals are more
-// than wanted, the last column taken.  By the whole block; how many are in the list then.
+// Where more logits of a piece reach a bound than can be put in order: the n-th largest by bisection, and where its equals are more
+// than wanted, the last column taken.  By the whole block; the n go to list[aside] and on.
 template <int WIDE>
-__device__ __noinline__ int exact_bound(const float* x, uint32_t bound, uint32_t all_top, int n, int first, unsigned long long* list,
-                                        int* found, int* of_warp) {
+__device__ __noinline__ void exact_bound(const float* x, uint32_t limit, int n, int first, unsigned long long* list,
+                                         int aside, int* found, int* of_warp) {
   const int tid = threadIdx.x;
-  uint32_t lo = bound, hi = all_top;  // at least n are >= lo (or all that there are); the answer is in lo .. hi
+  uint32_t lo = limit, hi = ordered(INFINITY);  // more than n exceed the limit; the answer is above it
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
     int c = 0;
@@ -134,7 +139,7 @@ __device__ __noinline__ int exact_bound(const float* x, uint32_t bound, uint32_t
     else
       c0 = mid + 1;
   }
-  if (tid == 0) *found = 0;
+  if (tid == 0) *found = aside;
   __syncthreads();
 #pragma unroll 1
   for (int k = 0; k < EACH; ++k) {
@@ -142,132 +147,197 @@ __device__ __noinline__ int exact_bound(const float* x, uint32_t bound, uint32_t
     const uint32_t o = ordered(x[k]);
     if ((o > lo || (o == lo && column <= c0)) && x[k] > -INFINITY) {
       const int at = atomicAdd(found, 1);
-      if (at < CAP) list[at] = (unsigned long long)o << 32 | ~(uint32_t)(first + column);
+      if (at < LIST_CAP) list[at] = (unsigned long long)o << 32 | ~(uint32_t)(first + column);
     }
   }
   __syncthreads();
-  return min(*found, CAP);
 }
 
+constexpr int PIECES_CTAS = 3, STAGES = 2;  // CTAs an SM
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS, PIECES_CTAS)
 beam_pieces_kernel(const Args a) {
-  __shared__ unsigned long long list[CAP];
-  __shared__ double sums[WARPS];
-  __shared__ uint32_t tops[WARPS], bounds[WARPS];
+  extern __shared__ __align__(128) unsigned char stage_bytes[];  // [STAGES][PIECE] logits
+  __shared__ unsigned long long lists[2][LIST_CAP];  // the n best so far in order, what was put aside behind them; and in turn
+  __shared__ uint32_t bounds[WARPS];
+  __shared__ __align__(8) uint64_t landed[STAGES];
   __shared__ int of_warp[WARPS], found;
   constexpr int WIDE = 16 / sizeof(T);  // logits of a load
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
-  const int row = blockIdx.y, first = blockIdx.x * PIECE;
+  if (tid == 0) {
+    for (int k = 0; k < STAGES; ++k) tc::mbar_init(&landed[k], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: the next kernel looks at the groups before it waits)
-  if (tid == 0) found = 0;
-  // Thread t has the columns first + WIDE (t + 256 k) .. + WIDE - 1, however the row lies in memory: equal rows give equal sums.
-  const T* src = (const T*)a.logits + (size_t)row * a.stride + first;
-  float x[EACH];
-  const int there = a.vocab - first;  // columns from this block's first on
-  if (there >= PIECE && (uintptr_t)src % 16 == 0) {
-    uint4 raw[EACH / WIDE];
+  __syncthreads();
+  const int begin = blockIdx.x * a.run, end = min(begin + a.run, a.rows * a.pieces);
+  auto ask = [&](int p, int k) {  // by one thread: piece p into stage k
+    if (p >= end || !a.bulk) return;
+    const int row = p / a.pieces, first = (p - row * a.pieces) * PIECE;
+    const uint32_t bytes = (uint32_t)min(PIECE, a.vocab - first) * (uint32_t)sizeof(T);
+    tc::mbar_expect_tx(&landed[k], bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     tc::smem_u32(stage_bytes + (size_t)k * PIECE * sizeof(T))),
+                 "l"((const T*)a.logits + (size_t)row * a.stride + first), "r"(bytes), "r"(tc::smem_u32(&landed[k]))
+                 : "memory");
+  };
+  if (tid == 0)
+    for (int k = 0; k < STAGES; ++k) ask(begin + k, k);
+  int row = begin / a.pieces, in_row = begin - row * a.pieces;
+  bool fresh = true;  // the first piece of a part
+  unsigned long long* list = lists[0];
+  uint32_t limit = NOTHING;  // the n-th best so far
+  int aside = n;             // entries of the list in front of this piece's
+#pragma unroll 1
+  for (int turn = 0, p = begin; p < end; ++turn, ++p) {
+    const int first = in_row * PIECE, there = a.vocab - first;  // columns from the piece's first on
+    // Thread t has the columns first + WIDE (t + 256 k) .. + WIDE - 1, however the row lies in memory: equal rows of equal parts
+    // give equal sums.
+    float x[EACH];
+    bool ok = true;
+    if (a.bulk) {
+      ok = tc::mbar_wait(&landed[turn % STAGES], (turn / STAGES) & 1);
+      const uint4* src = reinterpret_cast<const uint4*>(stage_bytes + (size_t)(turn % STAGES) * PIECE * sizeof(T)) + tid;
 #pragma unroll
-    for (int k = 0; k < EACH / WIDE; ++k) raw[k] = __ldcs(reinterpret_cast<const uint4*>(src) + tid + k * THREADS);
+      for (int k = 0; k < EACH / WIDE; ++k) {
+        const uint4 raw = src[k * THREADS];
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int k = 0; k < EACH / WIDE; ++k) {
-      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (WIDE == 4) {
-          x[4 * k + j] = __uint_as_float(w[j]);
-        } else {
-          x[8 * k + 2 * j] = __uint_as_float(w[j] << 16);
-          x[8 * k + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (WIDE == 4) {
+            x[4 * k + j] = __uint_as_float(w[j]);
+          } else {
+            x[8 * k + 2 * j] = __uint_as_float(w[j] << 16);
+            x[8 * k + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+          }
         }
       }
+      if (there < PIECE) {  // (whole pieces of 16 bytes are there)
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+          if (WIDE * (tid + k / WIDE * THREADS) >= there) x[k] = -INFINITY;
+      }
+    } else {
+      const T* src = (const T*)a.logits + (size_t)row * a.stride + first;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int at = WIDE * (tid + k / WIDE * THREADS) + k % WIDE;
+        x[k] = at < there ? to_f32(src[at]) : -INFINITY;
+      }
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      const int at = WIDE * (tid + k / WIDE * THREADS) + k % WIDE;
-      x[k] = at < there ? to_f32(src[at]) : -INFINITY;
-    }
-  }
-  // (fmaxf leaves NaN out)
-  float tops4[EACH / 4], top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < EACH / 4; ++k) {
-    tops4[k] = fmaxf(max3(x[4 * k], x[4 * k + 1], x[4 * k + 2]), x[4 * k + 3]);
-    top = fmaxf(top, tops4[k]);
-  }
-  const float mine = top;
-  const uint32_t kth = warp_kth(ordered(top), (n + WARPS - 1) / WARPS - 1);
-  const uint32_t warp_top = __reduce_max_sync(0xffffffffu, ordered(top));
-  if (lane == 0) {
-    tops[warp] = warp_top;
-    bounds[warp] = kth;
-  }
-  __syncthreads();
-  uint32_t all_top = 0, bound = 0xffffffffu;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    all_top = max(all_top, tops[w]);
-    bound = min(bound, bounds[w]);
-  }
-  top = unordered(all_top);
-  // what reaches the bound (NaN does not)
-  const float limit = unordered(max(bound, NOTHING));
-  if (mine >= limit && mine > -INFINITY) {
+    // (fmaxf leaves NaN out)
+    float tops4[EACH / 4], mine = -INFINITY;
 #pragma unroll
     for (int k = 0; k < EACH / 4; ++k) {
-      if (!(tops4[k] >= limit)) continue;
+      tops4[k] = fmaxf(max3(x[4 * k], x[4 * k + 1], x[4 * k + 2]), x[4 * k + 3]);
+      mine = fmaxf(mine, tops4[k]);
+    }
+    const float top = unordered(__reduce_max_sync(0xffffffffu, ordered(mine)));  // of the warp
+    // exponentials: the difference is exact or nearly so, and the error of a product with log2 e shrinks with the term
+    float2 sums2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int j = 4 * k; j < 4 * k + 4; ++j) {
-        if (x[j] >= limit && x[j] > -INFINITY) {
-          const int at = atomicAdd(&found, 1);
-          const uint32_t column = first + WIDE * (tid + j / WIDE * THREADS) + j % WIDE;
-          if (at < CAP) list[at] = (unsigned long long)ordered(x[j]) << 32 | ~column;
+    for (int k = 0; k < EACH; k += 2) {
+      const float2 y = mul2(add2(make_float2(x[k], x[k + 1]), make_float2(-top, -top)), make_float2(1.4426950408889634f, 1.4426950408889634f));
+      sums2[k / 2 % 2] = add2(sums2[k / 2 % 2], make_float2(ex2_of(y.x), ex2_of(y.y)));
+    }
+    sums2[0] = add2(sums2[0], sums2[1]);
+    float sum = sums2[0].x + sums2[0].y;
+    if (!(sum < INFINITY)) {  // there is a NaN, or an infinity less itself: NaN counts as -inf, and infinities share the mass
+      sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k)
+        if (x[k] == x[k] && x[k] > -INFINITY) sum += x[k] == top ? 1.f : ex2_of((x[k] - top) * 1.4426950408889634f);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) a.stats[(size_t)p * WARPS + warp] = make_float2(top, sum);
+    if (fresh) {
+      const uint32_t kth = warp_kth(ordered(mine), (n + WARPS - 1) / WARPS - 1);
+      if (lane == 0) bounds[warp] = kth;
+      for (int i = tid; i < n; i += THREADS) list[i] = 0;
+      if (tid == 0) found = n;
+      aside = n;
+      __syncthreads();
+      limit = 0xffffffffu;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) limit = min(limit, bounds[w]);
+      // what reaches the bound exceeds the number below it (that is not -0, which is none below 0); -inf does not
+      limit = max(limit, NOTHING + 1) - 1;
+      if (limit == 0x7fffffffu) --limit;
+    }
+    // what exceeds the limit (NaN does not); of equals the first column counts, and that was there before
+    const float above = unordered(limit);
+    if (mine > above) {
+#pragma unroll
+      for (int k = 0; k < EACH / 4; ++k) {
+        if (!(tops4[k] > above)) continue;
+#pragma unroll
+        for (int j = 4 * k; j < 4 * k + 4; ++j) {
+          if (x[j] > above) {
+            const int at = atomicAdd(&found, 1);
+            const uint32_t column = first + WIDE * (tid + j / WIDE * THREADS) + j % WIDE;
+            if (at < LIST_CAP) list[at] = (unsigned long long)ordered(x[j]) << 32 | ~column;
+          }
         }
       }
     }
-  }
-  // exponentials: the difference is exact or nearly so, and the error of a product with log2 e shrinks with the term
-  float2 sums2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    if (__syncthreads_or(!ok)) {  // a copy did not arrive: the block leaves together
+      if (tid == 0) atomicOr(a.err, DSP_ERR_WAIT_LIMIT);
+      // let copies that are still on their way land before the shared memory goes away
+#pragma unroll 1
+      for (int i = 0; i < 2000; ++i) __nanosleep(100);
+      return;
+    }
+    if (tid == 0) ask(p + STAGES, turn % STAGES);  // (everybody has this stage in registers)
+    const bool last = ++in_row == a.pieces || p + 1 == end;
+    int count = found;
+    __syncthreads();  // (nobody puts anything aside before all have read that)
+    if (count > LIST_CAP) {
+      float copy[EACH];  // (so that the usual way keeps its registers)
 #pragma unroll
-  for (int k = 0; k < EACH; k += 2) {
-    const float2 y = mul2(add2(make_float2(x[k], x[k + 1]), make_float2(-top, -top)), make_float2(1.4426950408889634f, 1.4426950408889634f));
-    sums2[k / 2 % 2] = add2(sums2[k / 2 % 2], make_float2(ex2_of(y.x), ex2_of(y.y)));
-  }
-  sums2[0] = add2(sums2[0], sums2[1]);
-  float sum = sums2[0].x + sums2[0].y;
-  if (!(sum < INFINITY)) {  // there is a NaN, or an infinity less itself: NaN counts as -inf, and infinities share the mass
-    sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (x[k] == x[k] && x[k] > -INFINITY) sum += x[k] == top ? 1.f : ex2_of((x[k] - top) * 1.4426950408889634f);
-  }
-  double all = sum;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  if (lane == 0) sums[warp] = all;
-  __syncthreads();
-  int count = found;
-  if (count > CAP) {
-    float copy[EACH];  // (so that the usual way keeps its registers)
-#pragma unroll
-    for (int k = 0; k < EACH; ++k) copy[k] = x[k];
-    count = exact_bound<WIDE>(copy, bound, all_top, n, first, list, &found, of_warp);
-  }
-  const size_t piece = (size_t)row * a.pieces + blockIdx.x;
-  unsigned long long* out = a.lists + piece * n;
-  for (int i = tid; i < count; i += THREADS) {
-    const unsigned long long key = list[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += list[j] > key;  // (no two are equal: columns differ)
-    if (rank < n) out[rank] = key;
-  }
-  if (tid == 0) {
-    double total = 0.;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += sums[w];
-    a.stats[piece] = {total, top, min(count, n)};
+      for (int k = 0; k < EACH; ++k) copy[k] = x[k];
+      exact_bound<WIDE>(copy, limit, n, first, list, aside, &found, of_warp);
+      count = found;
+      __syncthreads();
+    }
+    aside = count;
+    if (fresh || last || count > n + ASIDE) {
+      unsigned long long* next = list == lists[0] ? lists[1] : lists[0];
+      for (int i = tid; i < n; i += THREADS) next[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < count; i += THREADS) {
+        const unsigned long long key = list[i];
+        if (key == 0) continue;
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += list[j] > key;  // (no two are equal: columns differ)
+        if (rank < n) next[rank] = key;
+      }
+      if (tid == 0) found = n;
+      aside = n;
+      list = next;
+      __syncthreads();
+      limit = max((uint32_t)(list[n - 1] >> 32), NOTHING);
+    }
+    fresh = false;
+    if (last) {
+      int entries = 0;
+      const int part = blockIdx.x + row;
+      for (int i = tid; i < n; i += THREADS) {
+        a.lists[(size_t)part * n + i] = list[i];
+        entries += list[i] != 0;
+      }
+      entries = block_sum(entries, of_warp);
+      if (tid == 0) {
+        a.parts[part] = (uint32_t)row << 16 | (uint32_t)entries;
+        if (in_row == a.pieces && p + 1 == end) a.parts[part + 1] = (uint32_t)row << 16;
+      }
+      if (in_row == a.pieces) {
+        in_row = 0;
+        ++row;
+      }
+      fresh = true;
+    }
   }
 }
 
@@ -283,9 +353,9 @@ struct Candidate {
 __global__ void __launch_bounds__(THREADS)
 beam_groups_kernel(const Args a) {
   __shared__ Candidate list[CAP];
-  __shared__ uint4 heads[THREADS / 4];
+  __shared__ uint2 range[WARPS];
+  __shared__ int reached[2][WARPS];
   __shared__ int open[CAP];  // lists whose first entry reaches the bound
-  __shared__ uint32_t bound;
   __shared__ int found, opened;
   __shared__ Candidate best_of_warp[WARPS], taken;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, group = blockIdx.x;
@@ -300,68 +370,108 @@ beam_groups_kernel(const Args a) {
     parent[i] = token[i] = -1;
     score[i] = -INFINITY;
   }
-  if (tid == 0) {
-    found = opened = 0;
-    bound = (uint32_t)(NOTHING64 >> 32);
-  }
+  if (tid == 0) found = opened = 0;
   pdl_launch_dependents();
   pdl_wait();
   // the rows' largest logits and sums: a warp a row
+  const int per_row = a.pieces * WARPS;
   for (int r = warp; r < rows; r += WARPS) {
-    const Stat* stats = a.stats + (size_t)(first + r) * a.pieces;
+    const float2* stats = a.stats + (size_t)(first + r) * per_row;
     float top = -INFINITY;
-    for (int p = lane; p < a.pieces; p += 32) top = fmaxf(top, stats[p].top);
+    for (int i = lane; i < per_row; i += 32) top = fmaxf(top, stats[i].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     double sum = 0.;
-    for (int p = lane; p < a.pieces; p += 32) {
-      const float of = stats[p].top;
-      if (of == top)
-        sum += stats[p].sum;
-      else if (of > -INFINITY && top < INFINITY)
-        sum += stats[p].sum * exp((double)of - (double)top);
+    for (int i = lane; i < per_row; i += 32) {
+      const float2 of = stats[i];
+      if (of.x == top)
+        sum += (double)of.y;
+      else if (of.x > -INFINITY && top < INFINITY)
+        sum += (double)of.y * exp((double)of.x - (double)top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) a.of_rows[first + r] = make_float2(top, (float)log(sum));
   }
   __syncthreads();
-  const int lists = rows * a.pieces;
+  auto first_cta = [&](int r) { return r * a.pieces / a.run; };
+  auto last_cta = [&](int r) { return (r * a.pieces + a.pieces - 1) / a.run; };
+  // the parts of the group's rows follow one another
+  const int part0 = rows > 0 ? first_cta(first) + first : 0, lists = rows > 0 ? last_cta(end - 1) + end - part0 : 0;
   auto entries = [&](int l) -> int {
-    const int r = first + l / a.pieces;
-    const float s = a.scores[r];
-    return isfinite(s) ? a.stats[(size_t)first * a.pieces + l].count : 0;
+    const uint32_t row_count = a.parts[part0 + l];
+    return isfinite(a.scores[row_count >> 16]) ? (int)(row_count & 0xffffu) : 0;
   };
   auto candidate = [&](int l, int depth) -> Candidate {
-    const int r = l / a.pieces;
-    const unsigned long long e = a.lists[((size_t)first * a.pieces + l) * n + depth];
+    const int row = (int)(a.parts[part0 + l] >> 16);
+    const unsigned long long e = a.lists[(size_t)(part0 + l) * n + depth];
     const float x = unordered((uint32_t)(e >> 32));
-    const float2 of_row = a.of_rows[first + r];
+    const float2 of_row = a.of_rows[row];
     const double away = x == of_row.x ? 0. : (double)x - (double)of_row.x;
-    return {ordered((double)a.scores[first + r] + away - (double)of_row.y), (uint32_t)r, ~(uint32_t)e};
+    return {ordered((double)a.scores[row] + away - (double)of_row.y), (uint32_t)(row - first), ~(uint32_t)e};
   };
-  // A lower bound of the n-th best key, in its first 32 bits: the n-th of 256, a candidate a thread or the best of a thread's lists.
-  unsigned long long mine = NOTHING64;
-  if (lists >= THREADS) {
-    for (int l = tid; l < lists; l += THREADS)
-      if (entries(l) > 0) mine = max(mine, candidate(l, 0).key);
-  } else if (lists > 0) {
-    const int l = tid % lists, depth = tid / lists;
-    if (depth < entries(l)) mine = candidate(l, depth).key;
+  // A lower bound of the n-th best key, in its first 32 bits.  Of each list (they are in order) every `each`-th entry is looked at,
+  // some 1,024 in all, four a thread; an entry that is at least t stands for `each` that are, so that ceil(n / each) of them
+  // vouch for n.  The largest such t is bisected to a 4,096th of what lies between the best and the worst.
+  const int each = min(n, (lists * n + SAMPLES - 1) / SAMPLES), per_list = each > 0 ? n / each : 0;
+  uint32_t sample[SAMPLES / THREADS];
+#pragma unroll
+  for (int k = 0; k < SAMPLES / THREADS; ++k) {
+    sample[k] = (uint32_t)(NOTHING64 >> 32);
+    if (lists <= SAMPLES) {
+      const int i = tid + k * THREADS, l = i / max(per_list, 1), depth = (i - l * per_list + 1) * each - 1;
+      if (l < lists && depth < entries(l)) sample[k] = (uint32_t)(candidate(l, depth).key >> 32);
+    } else {  // the best of several lists' first entries
+      for (int l = tid + k * THREADS; l < lists; l += SAMPLES)
+        if (entries(l) > 0) sample[k] = max(sample[k], (uint32_t)(candidate(l, 0).key >> 32));
+    }
   }
-  const uint32_t head = (uint32_t)(mine >> 32);
-  reinterpret_cast<uint32_t*>(heads)[tid] = head;
-  __syncthreads();
-  int larger = 0;
-  for (int j = 0; j < THREADS / 4; ++j) {
-    const uint4 x = heads[j];
-    // (equals in the order of the threads: one of them is the n-th)
-    larger += (x.x > head || (x.x == head && 4 * j < tid)) + (x.y > head || (x.y == head && 4 * j + 1 < tid)) +
-              (x.z > head || (x.z == head && 4 * j + 2 < tid)) + (x.w > head || (x.w == head && 4 * j + 3 < tid));
+  const int wanted = lists <= SAMPLES ? (n + max(each, 1) - 1) / max(each, 1) : n;
+  constexpr uint32_t NONE = (uint32_t)(NOTHING64 >> 32);
+  uint32_t lo = 0xffffffffu, hi = NONE;
+  int there = 0;
+#pragma unroll
+  for (int k = 0; k < SAMPLES / THREADS; ++k) {
+    if (sample[k] > NONE) {
+      ++there;
+      lo = min(lo, sample[k]);
+    }
+    hi = max(hi, sample[k]);
   }
-  if (larger == n - 1) bound = head;
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  there = __reduce_add_sync(0xffffffffu, there);
+  if (lane == 0) {
+    range[warp] = make_uint2(lo, hi);
+    reached[1][warp] = there;
+  }
   __syncthreads();
-  const uint32_t limit = bound;
+  there = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    lo = min(lo, range[w].x);
+    hi = max(hi, range[w].y);
+    there += reached[1][w];
+  }
+  if (there < wanted) lo = hi = NONE;  // everything is let through
+#pragma unroll 1
+  for (int step = 0; step < 12 && lo < hi; ++step) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < SAMPLES / THREADS; ++k) c += sample[k] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) reached[step & 1][warp] = c;
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) c += reached[step & 1][w];
+    if (c >= wanted)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const uint32_t limit = lo;
   auto reaches = [&](const Candidate& c) { return (uint32_t)(c.key >> 32) >= limit && c.key > NOTHING64; };
   for (int l = tid; l < lists; l += THREADS)
     if (entries(l) > 0 && reaches(candidate(l, 0))) {
@@ -433,8 +543,13 @@ beam_groups_kernel(const Args a) {
   }
 }
 
-long scratch_bytes(long rows, long pieces, long n) {
-  return rows * pieces * (long)(sizeof(Stat) + 8 * n) + rows * (long)sizeof(float2);
+// Floats of scratch, and where its arrays begin.
+long layout(Args& a, float* at, long rows, long pieces, long ctas, long n) {
+  a.lists = reinterpret_cast<unsigned long long*>(at);
+  a.stats = reinterpret_cast<float2*>(a.lists + (rows + ctas) * n);
+  a.of_rows = a.stats + rows * pieces * WARPS;
+  a.parts = reinterpret_cast<uint32_t*>(a.of_rows + rows);
+  return (rows + ctas) * (2 * n + 1) + 2 * rows * (pieces * WARPS + 1);
 }
 }  // namespace
 
@@ -458,35 +573,48 @@ extern "C" int dsp_beam_select(const DspTensor* t, cudaStream_t stream) {
   if (groups == 0) return 0;
   SELECT_REQUIRE((uintptr_t)logits.data % (logits.dtype == DSP_T_F32 ? 4 : 2) == 0, "logits must be aligned to their size");
   SELECT_REQUIRE(current_device() == logits.device, "the tensors are on device %d, the current device is %d", logits.device, current_device());
-  const long pieces = (V + PIECE - 1) / PIECE;
+  const int sms = dsp_num_sms();
+  const long pieces = (V + PIECE - 1) / PIECE, most_ctas = (sms > 0 ? sms : 1) * PIECES_CTAS;
+  const long run = max((R * pieces + most_ctas - 1) / most_ctas, 1L), ctas = (R * pieces + run - 1) / run;
   SELECT_REQUIRE(R * pieces <= 0x7fffffff, "%ld rows of %ld logits are too many for one call", R, V);
-  SELECT_REQUIRE(scratch.contiguous && scratch.device == logits.device && scratch.dims == 1 && scratch.dtype == DSP_T_F32 &&
-                     (uintptr_t)scratch.data % 16 == 0 && scratch.size[0] * 4 >= scratch_bytes(R, pieces, n),
-                 "scratch is too small");
   Args a = {};
+  const long need = layout(a, (float*)scratch.data, R, pieces, ctas, n);
+  SELECT_REQUIRE(scratch.contiguous && scratch.device == logits.device && scratch.dims == 1 && scratch.dtype == DSP_T_F32 &&
+                     (uintptr_t)scratch.data % 16 == 0 && scratch.size[0] >= need,
+                 "scratch is too small");
   a.logits = logits.data;
   a.scores = (const float*)scores.data;
   a.group_start = (const int*)start.data;
   a.parent = (int*)parent.data;
   a.token = (int*)token.data;
   a.score = (float*)score.data;
-  a.stats = reinterpret_cast<Stat*>(scratch.data);
-  a.lists = reinterpret_cast<unsigned long long*>(a.stats + R * pieces);
-  a.of_rows = reinterpret_cast<float2*>(a.lists + R * pieces * n);
   a.stride = R > 1 ? logits.stride[0] : 0;
   a.rows = (int)R;
   a.groups = (int)groups;
   a.vocab = (int)V;
   a.pieces = (int)pieces;
+  a.run = (int)run;
   a.n = (int)n;
   a.err = dsp_device_error_ptr();
   SELECT_REQUIRE(a.err != nullptr, "no device error word");
   if (R > 0) {
-    const dim3 grid((unsigned)pieces, (unsigned)R);
-    if (logits.dtype == DSP_T_F32)
-      DSP_CUDA(launch_pdl(beam_pieces_kernel<float>, grid, dim3(THREADS), 0, stream, a));
-    else
-      DSP_CUDA(launch_pdl(beam_pieces_kernel<bf16>, grid, dim3(THREADS), 0, stream, a));
+    const bool f32 = logits.dtype == DSP_T_F32;
+    const long size = f32 ? 4 : 2;
+    a.bulk = (uintptr_t)logits.data % 16 == 0 && a.stride * size % 16 == 0 && V * size % 16 == 0;
+    const size_t smem = a.bulk ? STAGES * PIECE * size : 0;
+    const dim3 grid((unsigned)ctas);
+    auto go = [&](auto kernel) -> int {
+      static bool allowed[2][MAX_DEVICES] = {};  // asked for once a device and type
+      const int device = current_device();
+      if (device < 0 || !allowed[f32][device]) {
+        DSP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(STAGES * PIECE * size)));
+        if (device >= 0) allowed[f32][device] = true;
+      }
+      DSP_CUDA(launch_pdl(kernel, grid, dim3(THREADS), smem, stream, a));
+      return 0;
+    };
+    const int rc = f32 ? go(beam_pieces_kernel<float>) : go(beam_pieces_kernel<bf16>);
+    if (rc != 0) return rc;
   }
   DSP_CUDA(launch_pdl(beam_groups_kernel, dim3((unsigned)groups), dim3(THREADS), 0, stream, a));
   DSP_CHECK_LAUNCH("beam_select");

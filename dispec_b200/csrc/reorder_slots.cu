@@ -181,7 +181,12 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
     return 0;
   };
   if (bulk) {
-    DSP_CUDA(cudaFuncSetAttribute(reorder_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BULK_BYTES));
+    static bool allowed[MAX_DEVICES] = {};  // asked for once a device
+    const int device = current_device();
+    if (device < 0 || !allowed[device]) {
+      DSP_CUDA(cudaFuncSetAttribute(reorder_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BULK_BYTES));
+      if (device >= 0) allowed[device] = true;
+    }
     const int rc = go(reorder_bulk_kernel, BULK_THREADS, BULK_BYTES);
     if (rc != 0) return rc;
   } else {

@@ -13,7 +13,7 @@ from dispec_b200.ops import library as L
 from dispec_b200.ops import tuning
 
 _ATTENTION = struct.Struct("4qd")
-_PIECE, _STAT = 8192, 16  # logits that a block holds, bytes of what it leaves of them (csrc/beam_select.cu)
+_PIECE = 8192  # logits of a piece of a row (csrc/beam_select.cu)
 
 
 def _refuse(what: str, message: str):
@@ -113,8 +113,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, group_start: torch.T
     (rows, vocab), groups = logits.shape, max(0, group_start.shape[0] - 1)
     parent, token = group_start.new_empty((groups, count)), group_start.new_empty((groups, count))
     score = scores.new_empty((groups, count))
-    # scratch of this call alone: what the pieces of every row leave (csrc/beam_select.cu)
-    scratch = scores.new_empty(rows * -(-vocab // _PIECE) * (_STAT // 4 + 2 * count) + 2 * rows)
+    # scratch of this call alone: what the CTAs leave of their parts of rows, and of every piece (csrc/beam_select.cu)
+    dev = logits.get_device()
+    pieces = -(-vocab // _PIECE)
+    parts = rows + min(rows * pieces, 3 * (tuning._sm_count.get(dev) or tuning.sm_count(dev)))
+    scratch = scores.new_empty(parts * (2 * count + 1) + 2 * rows * (8 * pieces + 1))
     tensors = (_describe or _load_describe())(logits, scores, group_start, parent, token, score, scratch)
     L.check(L.core().dsp_beam_select(tensors, L.stream_handle()), launches=2)
     return Selected(parent, token, score)
