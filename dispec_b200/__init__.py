@@ -16,7 +16,8 @@ def __getattr__(name):
     if name in ("load_model", "build_model", "write_random_model", "load_random_model"):
         import dispec_b200.weights as w
         return getattr(w, name)
-    if name in ("LLMEngine", "ContinuousBatchingEngine", "ModelRunner", "SeqEntry", "Scheduler", "SpeculativeEngine", "TreeEntry"):
+    if name in ("LLMEngine", "ContinuousBatchingEngine", "ModelRunner", "SeqEntry", "Scheduler", "SpeculativeEngine", "TreeEntry",
+                "BeamSearchEngine"):
         import dispec_b200.engine as e
         return getattr(e, name)
     if name in ("SamplingParams", "sample"):

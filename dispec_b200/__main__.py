@@ -11,6 +11,7 @@ tokenizer is not part of the engine.
     generate        generate from prompts given as token ids (--model DIR, or --random CONFIG for
                     random weights filled on the device)
     speculate       the same with drafted trees: several tokens a request checked in one pass
+    beam            the same by beam search: the likeliest continuations of every prompt
     random          write a model folder with random weights from a config.json and a seed
     replay          feed given token ids step by step and write logits (the program of bin/trace_run)
     throughput      continuous-batching throughput at several concurrency levels
@@ -122,6 +123,22 @@ def cmd_speculate(args) -> int:
     return 0
 
 
+def cmd_beam(args) -> int:
+    from dispec_b200 import BeamSearchEngine, KVConfig
+    model = _make_model(args)
+    prompts = _parse_prompts(args, model.spec.vocab_size)
+    engine = BeamSearchEngine(model, KVConfig(block_size=args.block_size), num_blocks=args.num_blocks, beam_width=args.width,
+                              max_num_seqs=max(args.width, args.width * min(len(prompts), 64)))
+    t0 = time.perf_counter()
+    out = engine.generate(prompts, args.max_new, length_penalty=args.length_penalty, eos_token_id=args.eos_id, num_return=args.num_return)
+    dt = time.perf_counter() - t0
+    for i, (p, found) in enumerate(zip(prompts, out)):
+        for h in found:
+            print(json.dumps({"id": i, "prompt_tokens": len(p), "score": h.score, "output_ids": h.tokens}))
+    print(f"# {len(prompts)} prompts in {dt:.3f}s, {engine.num_steps} steps of up to {args.width} beams a prompt", file=sys.stderr)
+    return 0
+
+
 def cmd_random(args) -> int:
     from dispec_b200 import load_model_config, write_random_model
     cfg = load_model_config(args.config)
@@ -214,6 +231,19 @@ def main(argv=None) -> int:
     sp.add_argument("--seed", type=int, default=0)
     sp.add_argument("--eos-id", type=int, default=None, help="stop a request after this token")
     sp.set_defaults(fn=cmd_speculate)
+
+    bm = sub.add_parser("beam", help="generate by beam search")
+    _engine_args(bm, random_weights=True)
+    bm.add_argument("--prompt-ids", action="append", help="one prompt as token ids: '5,17,3' (repeatable)")
+    bm.add_argument("--prompt-file", help="one prompt per line: ids separated by spaces/commas, or a JSON list")
+    bm.add_argument("--random-prompts", type=int, nargs="+", help="lengths of uniform random prompts")
+    bm.add_argument("--max-new", type=int, default=64, help="new tokens per continuation (max_new_tokens)")
+    bm.add_argument("--width", type=int, default=4, help="beams of a prompt")
+    bm.add_argument("--num-return", type=int, default=1, help="continuations printed of each prompt, the best first")
+    bm.add_argument("--length-penalty", type=float, default=1.0, help="a continuation of n tokens is ranked by its log-probability / n^this")
+    bm.add_argument("--seed", type=int, default=0)
+    bm.add_argument("--eos-id", type=int, default=None, help="a continuation ends with this token")
+    bm.set_defaults(fn=cmd_beam)
 
     r = sub.add_parser("random", help="write a model folder with random weights")
     r.add_argument("--config", required=True, help="a config.json (or a folder holding one)")

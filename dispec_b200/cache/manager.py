@@ -10,7 +10,7 @@ a page given back leaves -1 behind, which the kernels never index.
 Reference: puneethgv/DiSpec dispec/kv/block_manager.py (one group, tables at :22-31, allocate
 :66-86, append_token :98-106, free :143-152).  Differences: several groups, window release,
 reservations made at admission (a request admitted by the scheduler can always finish its
-prompt), state slots.
+prompt), state slots, requests that fork and share their filled pages.
 """
 from __future__ import annotations
 
@@ -227,13 +227,53 @@ class CacheManager:
                 j = r.first_live[g]
                 page = table[j]
                 table[j] = -1
-                self.pools[g].release(page)
+                if self.pools[g].release(page):  # (no other request reads it)
+                    released.append((g, page))
                 if r.renew[g]:
                     self.pools[g].reserve(1)
                     r.reserved[g] += 1
-                released.append((g, page))
                 r.first_live[g] += 1
         return released
+
+    def fork(self, req_id, new_id) -> tuple[int, list[tuple[int, int, int]]]:
+        """Registers ``new_id`` as a copy of a request: the pages that its stored tokens fill are shared, and the one they
+        fill partly gets a copy of its own, since both will write there.  Returns the new state slot and (group, page, copy)
+        of every page to be copied; the state slot's contents are to be copied too.  Takes nothing where it raises.  The request has
+        no promises (``prompt_len`` 0 at its admission)."""
+        if new_id in self._requests:
+            raise ValueError(f"request {new_id!r} is already live")
+        r = self._requests[req_id]
+        if any(r.reserved) or any(r.renew):
+            raise ValueError(f"request {req_id!r} holds promises of pages and cannot fork")
+        if not self._free_slots:
+            raise OutOfSlotsError(f"all {self.max_num_seqs} request slots are taken")
+        full, rest = divmod(r.num_tokens, self.page_size)
+        if rest:
+            for pool in self.pools:
+                if pool.available < 1:
+                    raise OutOfPagesError("a fork needs a page in every group")
+        tables, copies = [], []
+        for g, (table, pool) in enumerate(zip(r.tables, self.pools)):
+            mine = table[:full]
+            for page in mine:
+                if page >= 0:
+                    pool.add_ref(page)
+            if rest:
+                mine.append(pool.alloc())
+                copies.append((g, table[full], mine[-1]))
+            tables.append(mine)
+        slot = self._free_slots.pop()
+        self._requests[new_id] = _Request(state_slot=slot, num_tokens=r.num_tokens, tables=tables, first_live=list(r.first_live),
+                                          reserved=[0] * len(self.groups), renew=[False] * len(self.groups))
+        return slot, copies
+
+    def shared_pages(self, req_ids: list, group: int = 0, known: int = 0) -> int:
+        """How many first pages all these requests share (``known``: so many do, as the caller knows)."""
+        tables = [self._requests[r].tables[group] for r in req_ids]
+        n = min(len(t) for t in tables)
+        while known < n and all(t[known] == tables[0][known] for t in tables):
+            known += 1
+        return min(known, n)
 
     def free(self, req_id) -> list[tuple[int, int]]:
         """Ends a request: every page, promise and its state slot go back."""
@@ -243,8 +283,7 @@ class CacheManager:
         released = []
         for g, table in enumerate(r.tables):
             for page in table:
-                if page >= 0:
-                    self.pools[g].release(page)
+                if page >= 0 and self.pools[g].release(page):
                     released.append((g, page))
             if r.reserved[g]:
                 self.pools[g].unreserve(r.reserved[g])
@@ -253,22 +292,25 @@ class CacheManager:
 
     # --------------------------------------------------------------------- invariants
     def check(self) -> None:
-        """No page lost, held twice or free while held; promises add up; slots unique."""
+        """No page lost, held by more requests than it counts, held twice by one, or free while held; promises add up; slots
+        unique."""
         for g, pool in enumerate(self.pools):
             held = []
             promised = 0
             for r in self._requests.values():
-                held += [p for p in r.tables[g] if p >= 0]
+                of_one = [p for p in r.tables[g] if p >= 0]
+                assert len(of_one) == len(set(of_one)), f"group {g}: a page is held twice"
+                held += of_one
                 promised += r.reserved[g]
-            assert len(held) == len(set(held)), f"group {g}: a page is held twice"
+            holders = {p: held.count(p) for p in set(held)} if len(held) != len(set(held)) else dict.fromkeys(held, 1)
             free = set(pool._free)
             assert len(free) == len(pool._free), f"group {g}: a page is on the free list twice"
             assert not (free & set(held)), f"group {g}: a held page is on the free list"
-            assert len(free) + len(held) == pool.num_pages, f"group {g}: a page is lost"
+            assert len(free) + len(holders) == pool.num_pages, f"group {g}: a page is lost"
             assert promised == pool.reserved, f"group {g}: promises {promised} != {pool.reserved}"
             assert pool.reserved <= len(free), f"group {g}: more promised than free"
-            for p in held:
-                assert pool.ref_count(p) == 1
+            for p, n in holders.items():
+                assert pool.ref_count(p) == n, f"group {g}: a page is held twice"
         slots = [r.state_slot for r in self._requests.values()]
         assert len(slots) == len(set(slots)) and not (set(slots) & set(self._free_slots))
         assert len(slots) + len(self._free_slots) == self.max_num_seqs

@@ -1,4 +1,5 @@
 from dispec_b200.engine.batch import SeqEntry, StepContext, TreeEntry
+from dispec_b200.engine.beam import BeamSearchEngine, Hypothesis
 from dispec_b200.engine.llm_engine import LLMEngine
 from dispec_b200.engine.runner import ModelRunner
 from dispec_b200.engine.scheduler import (ContinuousBatchingEngine, Request, Scheduler, State,
@@ -6,4 +7,5 @@ from dispec_b200.engine.scheduler import (ContinuousBatchingEngine, Request, Sch
 from dispec_b200.engine.speculative import SpeculativeEngine
 
 __all__ = ["SeqEntry", "StepContext", "LLMEngine", "ModelRunner", "ContinuousBatchingEngine",
-           "Request", "Scheduler", "State", "StepPlan", "SpeculativeEngine", "TreeEntry"]
+           "Request", "Scheduler", "State", "StepPlan", "SpeculativeEngine", "TreeEntry",
+           "BeamSearchEngine", "Hypothesis"]

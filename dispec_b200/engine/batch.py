@@ -75,6 +75,14 @@ class TreeStep:
     max_nodes: int
 
 
+@dataclass
+class SharedStep:
+    """What the attention of a step of beams reads beside the arrays of every step: the sequences come in groups whose first tokens
+    lie in the same pages."""
+    group_start: torch.Tensor  # [groups + 1] int32: sequences of each group
+    prefix_len: list  # per cache group [groups] int32: so many first tokens
+
+
 def _align4(n: int) -> int:
     return (n + 3) & ~3
 
@@ -112,6 +120,7 @@ class StepContext:
         self.graph_capture = False  # host-side choices must not depend on the step's values
         self.scratch: dict = {}
         self.tree = None  # TreeStep: the rows are nodes of drafted trees
+        self.shared = None  # SharedStep: single tokens of sequences that share their beginnings
         self.layer_trace = None  # a list: the model appends a copy of the stream after every layer run
 
     def cache_view(self, placement, write: bool) -> LayerCacheView:

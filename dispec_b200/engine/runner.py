@@ -15,7 +15,8 @@ import torch
 from dispec_b200 import ops
 from dispec_b200.cache.manager import CacheManager
 from dispec_b200.cache.storage import CacheStorage, StateStorage
-from dispec_b200.engine.batch import HostStaging, SeqEntry, StepPlanLayout, TreeEntry, build_context, build_tree_context
+from dispec_b200.engine.batch import (HostStaging, SeqEntry, SharedStep, StepPlanLayout, TreeEntry, build_context,
+                                      build_tree_context)
 from dispec_b200.ops import library as _library
 from dispec_b200.models.model import DecoderModel
 
@@ -156,6 +157,70 @@ class ModelRunner:
             if not 1 <= n <= len(e.tokens):
                 raise ValueError(f"request {e.req_id!r}: {n} accepted nodes of {len(e.tokens)}")
             self._poison(self.cache.commit(e.req_id, e.start + n))
+
+    # ------------------------------------------------------------------------- beams
+    @torch.inference_mode()
+    def beam_step(self, groups: list[list[SeqEntry]], shared: list[list[int]]):
+        """One token for every sequence of every group: the logits behind them in float32, group after group, and the first
+        sequence of each group on the device ([groups + 1] int32).  ``shared``: per group and cache group, so many first pages
+        are known to be the same for the group's sequences; counted on in place.  They are read once a group by mixers that
+        can (``takes_shared``)."""
+        entries = [e for of in groups for e in of]
+        if not entries or not all(groups) or len({e.req_id for e in entries}) != len(entries):
+            raise ValueError("a step of beams needs groups of requests, each of them once")
+        for e in entries:
+            if not self.cache.has(e.req_id):
+                raise KeyError(f"request {e.req_id!r} was not admitted")
+            if len(e.tokens) != 1:
+                raise ValueError(f"request {e.req_id!r}: a step of beams takes one token each")
+            if e.start != self.cache.num_tokens(e.req_id):
+                raise ValueError(f"request {e.req_id!r}: its token is at position {e.start} but {self.cache.num_tokens(e.req_id)} "
+                                 "tokens are stored")
+        for e in entries:  # may raise OutOfPagesError before anything ran
+            self.cache.extend(e.req_id, e.start + 1)
+        ctx, _ = build_context([SeqEntry(e.req_id, e.tokens, e.start, [0]) for e in entries], self.cache, self.storage, self.states,
+                               self.staging, self.dtype, self.device, self.model.attention_tile_tokens, self.vocab_size)
+        n, starts, prefixes = len(groups), [0], []
+        for of in groups:
+            starts.append(starts[-1] + len(of))
+        for c in range(len(self.cache.groups)):
+            for of, known in zip(groups, shared):
+                if len(of) > 1:
+                    known[c] = self.cache.shared_pages([e.req_id for e in of], c, known[c])
+                prefixes.append(known[c] * self.page_size if len(of) > 1 else 0)
+        numbers = torch.tensor(starts + prefixes, dtype=torch.int32).to(self.device)
+        if any(prefixes):
+            ctx.shared = SharedStep(numbers[:n + 1], [numbers[n + 1 + c * n:n + 1 + (c + 1) * n] for c in range(len(self.cache.groups))])
+        x, pending = self.model.forward(ctx)
+        logits = self.model.logits(ctx, x, pending, ctx.logit_rows)
+        for e in entries:
+            self._poison(self.cache.commit(e.req_id, e.start + 1))
+        self.num_steps += 1
+        return logits, numbers[:n + 1]
+
+    @torch.inference_mode()
+    def fork(self, pairs: list) -> None:
+        """For each (request, new one): the new one goes on from where the request is, with pages in common and a copy of the
+        page that both will write to and of the states."""
+        pages = [[] for _ in self.cache.groups]
+        slots = []
+        for req_id, new_id in pairs:
+            slot, copies = self.cache.fork(req_id, new_id)
+            slots.append((slot, self.cache.state_slot(req_id)))
+            for g, page, copy in copies:
+                pages[g].append((copy, page))
+        for named, moves in zip(self.storage.pools, pages):
+            self._copy_slots(list(named.values()), moves)
+        self._copy_slots([b.view(1, b.shape[0], -1) for b in self.states.buffers], slots)
+
+    def _copy_slots(self, pools: list, moves: list) -> None:
+        """(destination, source) pairs, in pools [layers, slots, ...]."""
+        if not pools or not moves:
+            return
+        moves = sorted(moves)
+        numbers = torch.tensor([d for d, _ in moves] + [s for _, s in moves], dtype=torch.int32).to(self.device)
+        for i in range(0, len(pools), 64):
+            ops.reorder_slots(pools[i:i + 64], numbers[len(moves):], numbers[:len(moves)])
 
     # -------------------------------------------------------- captured all-decode steps
     def _context_class(self, entries: list) -> int:

@@ -102,6 +102,9 @@ class GQAAttention(Mixer):
         if ctx.tree is not None:
             out = self._tree(ctx, qkv, cache, inv_freq, rotary_dim, scale)
             return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
+        if ctx.shared is not None:
+            out = self._shared(ctx, qkv, cache, inv_freq, rotary_dim, scale)
+            return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
         n_dec = ctx.num_decode_seqs
         fused = None
         if attn_ops.decode_rope_fusable(ctx, H, KVH, D, rotary_dim, qkv.dtype):
@@ -117,7 +120,16 @@ class GQAAttention(Mixer):
                                  scale, fused_rope=fused)
         return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
 
-    takes_trees = True
+    takes_trees = takes_shared = True
+
+    def _shared(self, ctx, qkv, cache, inv_freq, rotary_dim, scale):
+        """A step of beams: single tokens, whose sequences share pages group by group."""
+        H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
+        ops.rope_kv_store(qkv, ctx.positions, ctx.seq_of_token, cache.page_table, cache.key_pool if cache.write else None,
+                          cache.value_pool if cache.write else None, inv_freq, H, KVH, D, rotary_dim, write_kv=cache.write)
+        return ops.shared_prefix_attention(qkv[:, :H * D], cache.key_pool, cache.value_pool, cache.page_table, ctx.ctx_len,
+                                           ctx.shared.group_start, ctx.shared.prefix_len[cache.group], scale=scale,
+                                           window=self.window)
 
     def _tree(self, ctx, qkv, cache, inv_freq, rotary_dim, scale):
         """A step of drafted trees: several nodes may be at one position, so their keys and values have places of their own."""

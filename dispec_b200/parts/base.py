@@ -105,6 +105,8 @@ class Part:
     graph_safe = True
     # True for a mixer whose forward takes a step of drafted trees (``ctx.tree``, see engine/batch.py)
     takes_trees = False
+    # True for a mixer that reads pages which sequences share once for all of them (``ctx.shared``); others read them for each
+    takes_shared = False
 
     def tensor_specs(self) -> dict[str, TensorSpec]:
         return {}
