@@ -34,12 +34,16 @@ shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch s
   const float2* rows_ml = reinterpret_cast<const float2*>(scratch.rows_ml);
   const int row_head = (int)min(i / quads, (long)sh.rows * H), d = (int)(i % quads) * 4, row = row_head / H, h = row_head - row * H;
   const int head = h / sh.G, of_head = h - head * sh.G;
-  const int g = row < sh.rows ? group_of(sh.group_start, sh.groups, sh.rows, row) : -1;
+  __shared__ int start[MAX_GROUPS + 1];
+  for (int k = threadIdx.x; k <= sh.groups; k += COMBINE_THREADS) start[k] = sh.group_start[k];
+  const int length = row < sh.rows ? sh.length(row) : 0;  // (asked for with the groups)
+  __syncthreads();
+  const int g = row < sh.rows ? group_of(start, sh.groups, sh.rows, row) : -1;
   bool many = false, sees[2] = {false, false};  // the shared part was the other kernel's
   int of_tile[2] = {0, 0};
   long item[2] = {0, 0};
   if (g >= 0) {
-    const int length = sh.length(row), first = sh.group_start[g], n = sh.group_start[g + 1] - first;
+    const int first = start[g], n = start[g + 1] - first;
     const int prefix = n > 1 ? min(max(0, sh.prefix_len[g]), sh.most_ctx) : 0, lo = sh.window > 0 ? max(0, length - sh.window) : 0;
     many = (long)n * sh.G > sh.many;
     // an item of which the row sees a key is there, and has a record
@@ -56,33 +60,55 @@ shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch s
   pdl_launch_dependents();
   pdl_wait();
   if (g >= 0) {  // (a row in no group is left as it is)
+    // asked for with the records, which say whether they are wanted
     Record rec[2];
+    float2 ml[2];
+    float4 o[2];
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       const bool of_many = part == 0 && many;
-      Record x = {0, 0, 1};
-      if (sees[part]) x = (of_many ? scratch_many : scratch).records[item[part]];
+      const size_t at = ((size_t)part * sh.rows + row) * H + h;
+      rec[part] = {0, 0, 1};
+      ml[part] = make_float2(-INFINITY, 0.f);
+      o[part] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (sees[part]) {
+        rec[part] = (of_many ? scratch_many : scratch).records[item[part]];
+        ml[part] = rows_ml[at];
+        o[part] = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const bool of_many = part == 0 && many;
+      const Record x = rec[part];
       // (a record that a CTA whose wait ran out did not write is none)
       if (x.cta < 0 || x.parts < 0 || x.stride < 1 || (x.parts > 0 && x.cta + (x.parts - 1) * x.stride >= (of_many ? ctas_many : ctas)))
-        x = {0, 0, 1};
-      rec[part] = x;
+        rec[part] = {0, 0, 1};
     }
-    const float4 v = merge_parts(rec[0].parts + rec[1].parts, [&](int k, float2& ml, float4& o) {
-      const int part = k >= rec[0].parts;
-      if (part) k -= rec[0].parts;
-      if (rec[part].parts == 1) {
-        const size_t at = ((size_t)part * sh.rows + row) * H + h;
-        ml = rows_ml[at];
-        o = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
-      } else {
-        const bool of_many = part == 0 && many;
-        const SharedScratch& of = of_many ? scratch_many : scratch;
-        const size_t slot = 2 * (size_t)(rec[part].cta + k * rec[part].stride) + (k == 0);
-        const size_t at = slot * (of_many ? sh_many : sh).rows_per_tile() + of_tile[part];
-        ml = reinterpret_cast<const float2*>(of.part_ml)[at];
-        o = *reinterpret_cast<const float4*>(of.part_o + at * D + d);
-      }
-    });
+    float4 v;
+    if (rec[0].parts <= 1 && rec[1].parts <= 1) {
+      v = merge_parts<2>(2, [&](int k, float2& a, float4& b) {
+        a = (k ? rec[1] : rec[0]).parts ? (k ? ml[1] : ml[0]) : make_float2(-INFINITY, 0.f);
+        b = k ? o[1] : o[0];
+      });
+    } else {
+      v = merge_parts<8>(rec[0].parts + rec[1].parts, [&](int k, float2& a, float4& b) {
+        const int part = k >= rec[0].parts;
+        if (part) k -= rec[0].parts;
+        const Record x = part ? rec[1] : rec[0];
+        if (x.parts == 1) {
+          a = part ? ml[1] : ml[0];
+          b = part ? o[1] : o[0];
+        } else {
+          const bool of_many = part == 0 && many;
+          const SharedScratch& of = of_many ? scratch_many : scratch;
+          const size_t slot = 2 * (size_t)(x.cta + k * x.stride) + (k == 0);
+          const size_t at = (slot << (of_many ? sh_many.row_shift : sh.row_shift)) + (part ? of_tile[1] : of_tile[0]);
+          a = reinterpret_cast<const float2*>(of.part_ml)[at];
+          b = *reinterpret_cast<const float4*>(of.part_o + at * D + d);
+        }
+      });
+    }
     store4(out + (size_t)row * out_stride + (size_t)h * D + d, v);
   }
 }

@@ -65,6 +65,166 @@ __device__ __forceinline__ uint32_t key_mask(uint32_t alive, int at) {
   return ((alive >> at) & 1u ? 0xffffu : 0u) | ((alive >> (at + 1)) & 1u ? 0xffff0000u : 0u);
 }
 
+// A key tile in shared memory.
+struct Tile {
+  uint32_t k_s, v_s;
+  int key0;
+  uint32_t bad;  // bit j: page j is not there
+  bool ragged;   // not every row sees all of it
+};
+
+// By a warp: its sixteen rows over NB blocks of sixteen keys of a tile, from block `block` on.
+template <int NB>
+__device__ __forceinline__ void few_step(const Tile& tl, const shared::Share& t, int block, int page_shift, float scale,
+                                         const uint32_t (&q)[D / 16][4], const int (&lo)[2], const int (&hi)[2], float (&o)[D / 8][4],
+                                         float (&m)[2], float (&l)[2]) {
+  const int lane = threadIdx.x & 31, tq = lane & 3, m8 = lane >> 3, l8 = lane & 7;
+  const int c0 = block * 16, key0 = tl.key0;
+  if (key0 + c0 >= t.end || key0 + c0 + 16 * NB <= t.begin) return;
+  float sc[2 * NB][4] = {};
+  {
+    // (two chains of products for each eight keys where there is one block only)
+    float odd[NB == 1 ? 2 : 1][4] = {};
+#pragma unroll
+    for (int k0 = 0; k0 < D / 16; k0 += 4 / NB) {
+      uint32_t b[NB][4 / NB][4];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int row = c0 + n * 16 + (m8 >> 1) * 8 + l8;
+        const uint32_t base = tl.k_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
+#pragma unroll
+        for (int k = 0; k < 4 / NB; ++k) {
+          const int chunk = (k0 + k) * 2 + (m8 & 1);
+          ldmatrix4(b[n][k], base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4 / NB; ++k)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          mma16(NB == 1 && (k & 1) ? odd[0] : sc[2 * n], q[k0 + k], b[n][k][0], b[n][k][1]);
+          mma16(NB == 1 && (k & 1) ? odd[NB == 1 ? 1 : 0] : sc[2 * n + 1], q[k0 + k], b[n][k][2], b[n][k][3]);
+        }
+    }
+    if (NB == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[0][j] += odd[0][j];
+        sc[1][j] += odd[NB == 1 ? 1 : 0][j];
+      }
+    }
+  }
+  uint32_t alive = 0xffffffffu;  // keys of the blocks that some row may see
+  if (tl.ragged) {
+#pragma unroll
+    for (int c = 0; c < 2 * NB; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = c0 + c * 8 + tq * 2 + (j & 1), key = key0 + at, i = j >> 1;
+        const bool seen = key >= lo[i] && key < hi[i] && !((tl.bad >> (at >> page_shift)) & 1u);
+        sc[c][j] = seen ? sc[c][j] : -INFINITY;
+      }
+    const int at = c0 + lane;
+    alive = __ballot_sync(0xffffffffu, lane < 16 * NB && key0 + at >= t.begin && key0 + at < t.end && !((tl.bad >> (at >> page_shift)) & 1u));
+  }
+  float alpha[2];
+  uint32_t pk[NB][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float top = fmaxf(sc[0][2 * i], sc[0][2 * i + 1]);
+#pragma unroll
+    for (int c = 1; c < 2 * NB; ++c) top = max3(top, sc[c][2 * i], sc[c][2 * i + 1]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale;  // the scale is positive
+    const float m_new = top > m[i] + RESCALE_STEP || m[i] == -INFINITY ? fmaxf(top, m[i]) : m[i];
+    alpha[i] = m_new == m[i] ? 1.f : ex2(m[i] - m_new);
+    m[i] = m_new;
+    const float neg = m_new == -INFINITY ? 0.f : -m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2 * NB; ++c) {
+      const float e0 = ex2(fmaf(sc[c][2 * i], scale, neg)), e1 = ex2(fmaf(sc[c][2 * i + 1], scale, neg));
+      sum += e0 + e1;
+      // the second product takes weights of eight bits, as it takes values (their sum is of the 32-bit ones)
+      pk[c >> 1][i + 2 * (c & 1)] = pack2(e0, e1);
+    }
+    l[i] = l[i] * alpha[i] + sum;
+  }
+  if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      o[n][0] *= alpha[0];
+      o[n][1] *= alpha[0];
+      o[n][2] *= alpha[1];
+      o[n][3] *= alpha[1];
+    }
+  }
+  // Values of keys that no row sees are left out.  So are, where some rows see a key and others do not, numbers that are not finite,
+  // which a weight of 0 would carry to rows that do not see them; the rows that see them get them behind the product.
+  const bool mixed = tl.ragged && (t.begin != t.all_begin || t.end != t.all_end);
+  bool odd = false;
+#pragma unroll
+  for (int c = 0; c < NB; ++c) {
+    const int row = c0 + c * 16 + (m8 & 1) * 8 + l8;
+    const uint32_t base = tl.v_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
+    if (!tl.ragged) {
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        const int chunk = n * 2 + (m8 >> 1);
+        uint32_t b[4];
+        ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+        mma16(o[2 * n], pk[c], b[0], b[1]);
+        mma16(o[2 * n + 1], pk[c], b[2], b[3]);
+      }
+    } else {
+      const uint32_t mask0 = key_mask(alive, c * 16 + tq * 2), mask1 = key_mask(alive, c * 16 + tq * 2 + 8);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        const int chunk = n * 2 + (m8 >> 1);
+        uint32_t b[4];
+        ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] &= j & 1 ? mask1 : mask0;
+        if (mixed) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            odd |= has_odd(b[j]);
+            b[j] = without_odd(b[j]);
+          }
+        }
+        mma16(o[2 * n], pk[c], b[0], b[1]);
+        mma16(o[2 * n + 1], pk[c], b[2], b[3]);
+      }
+    }
+  }
+  if (mixed && __any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+    for (int c = 0; c < 16 * NB; ++c) {
+      if (!((alive >> c) & 1u)) continue;
+      const int key = key0 + c0 + c, at = c0 + c;
+      const bool sees0 = key >= lo[0] && key < hi[0], sees1 = key >= lo[1] && key < hi[1];
+      const uint32_t line = tl.v_s + (uint32_t)(at >> 3) * GROUP + (uint32_t)(at & 7) * 128u + (uint32_t)tq * 4u;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        uint32_t x;
+        asm volatile("ld.shared.u32 %0, [%1];"
+                     : "=r"(x)
+                     : "r"(line + (uint32_t)(n >> 3) * SLICE + (uint32_t)(((n & 7) ^ (at & 7)) << 4))
+                     : "memory");
+        const float x0 = __uint_as_float(x << 16), x1 = __uint_as_float(x & 0xffff0000u);
+        if (!isfinite(x0)) {
+          o[n][0] += sees0 ? x0 : 0.f;
+          o[n][2] += sees1 ? x0 : 0.f;
+        }
+        if (!isfinite(x1)) {
+          o[n][1] += sees0 ? x1 : 0.f;
+          o[n][3] += sees1 ? x1 : 0.f;
+        }
+      }
+    }
+  }
+}
+
 // Joins the 4 / MT warps of each of the share's MT row tiles, by all working warps, and puts the rows down: `out` and `out_ml` are
 // those of row tid / 4 of the tile, or null.
 template <int MT>
@@ -244,7 +404,7 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
   }
 
   // ---- work
-  const int gid = lane >> 2, tq = lane & 3, m8 = lane >> 3, l8 = lane & 7;
+  const int gid = lane >> 2, tq = lane & 3;
   const float scale = p.scale_log2;
   int tile = 0;
 #pragma unroll 1
@@ -284,139 +444,13 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
         const uint32_t k_s = smem_u32(ring + s * 2 * KV_BYTES), v_s = k_s + KV_BYTES;
         const uint32_t bad = bad_pages[s];
         const bool ragged = bad != 0u || !SharedWork::whole(sh, t, key0);
+        const Tile tl = {k_s, v_s, key0, bad, ragged};
+        if (MT == 1)
+          few_step<1>(tl, t, part, page_shift, scale, q, lo, hi, o, m, l);
+        else
 #pragma unroll 1
-        for (int block = part * MT; block < (part + 1) * MT; ++block) {
-          const int c0 = block * 16;  // of the tile's keys
-          if (key0 + c0 >= t.end || key0 + c0 + 16 <= t.begin) continue;
-          float sc[2][4] = {};
-          {
-            const int row = c0 + (m8 >> 1) * 8 + l8;
-            const uint32_t base = k_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
-            float odd[2][4] = {};  // (two chains of products for each eight keys)
-#pragma unroll
-            for (int k0 = 0; k0 < D / 16; k0 += 4) {
-              uint32_t b[4][4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int chunk = (k0 + k) * 2 + (m8 & 1);
-                ldmatrix4(b[k], base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
-              }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                mma16(k & 1 ? odd[0] : sc[0], q[k0 + k], b[k][0], b[k][1]);
-                mma16(k & 1 ? odd[1] : sc[1], q[k0 + k], b[k][2], b[k][3]);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              sc[0][j] += odd[0][j];
-              sc[1][j] += odd[1][j];
-            }
-          }
-          uint32_t alive = 0xffffu;  // keys of the block that some row may see
-          if (ragged) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int at = c0 + c * 8 + tq * 2 + (j & 1), key = key0 + at, i = j >> 1;
-                const bool seen = key >= lo[i] && key < hi[i] && !((bad >> (at >> page_shift)) & 1u);
-                sc[c][j] = seen ? sc[c][j] : -INFINITY;
-              }
-            alive = __ballot_sync(0xffffffffu, lane < 16 && key0 + c0 + lane >= t.begin && key0 + c0 + lane < t.end &&
-                                                   !((bad >> ((c0 + lane) >> page_shift)) & 1u));
-          }
-          float alpha[2], sum[2];
-          uint32_t pk[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale;  // the scale is positive
-            const float m_new = top > m[i] + RESCALE_STEP || m[i] == -INFINITY ? fmaxf(top, m[i]) : m[i];
-            alpha[i] = m_new == m[i] ? 1.f : ex2(m[i] - m_new);
-            m[i] = m_new;
-            const float neg = m_new == -INFINITY ? 0.f : -m_new;
-            const float e0 = ex2(fmaf(sc[0][2 * i], scale, neg)), e1 = ex2(fmaf(sc[0][2 * i + 1], scale, neg));
-            const float e2 = ex2(fmaf(sc[1][2 * i], scale, neg)), e3 = ex2(fmaf(sc[1][2 * i + 1], scale, neg));
-            sum[i] = (e0 + e1) + (e2 + e3);
-            l[i] = l[i] * alpha[i] + sum[i];
-            // the second product takes weights of eight bits, as it takes values (their sum is of the 32-bit ones)
-            pk[i] = pack2(e0, e1);
-            pk[2 + i] = pack2(e2, e3);
-          }
-          if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              o[n][0] *= alpha[0];
-              o[n][1] *= alpha[0];
-              o[n][2] *= alpha[1];
-              o[n][3] *= alpha[1];
-            }
-          }
-          const int row = c0 + (m8 & 1) * 8 + l8;
-          const uint32_t base = v_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
-          if (!ragged) {
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-              const int chunk = n * 2 + (m8 >> 1);
-              uint32_t b[4];
-              ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
-              mma16(o[2 * n], pk, b[0], b[1]);
-              mma16(o[2 * n + 1], pk, b[2], b[3]);
-            }
-          } else {
-            // Values of keys that no row sees are left out.  So are, where some rows see a key and others do not, numbers that are
-            // not finite, which a weight of 0 would carry to rows that do not see them; the rows that see them get them behind
-            // the product.
-            const uint32_t mask0 = key_mask(alive, tq * 2), mask1 = key_mask(alive, tq * 2 + 8);
-            const bool mixed = t.begin != t.all_begin || t.end != t.all_end;
-            bool odd = false;
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-              const int chunk = n * 2 + (m8 >> 1);
-              uint32_t b[4];
-              ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) b[j] &= j & 1 ? mask1 : mask0;
-              if (mixed) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  odd |= has_odd(b[j]);
-                  b[j] = without_odd(b[j]);
-                }
-              }
-              mma16(o[2 * n], pk, b[0], b[1]);
-              mma16(o[2 * n + 1], pk, b[2], b[3]);
-            }
-            if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-              for (int c = 0; c < 16; ++c) {
-                if (!((alive >> c) & 1u)) continue;
-                const int key = key0 + c0 + c, at = c0 + c;
-                const bool sees0 = key >= lo[0] && key < hi[0], sees1 = key >= lo[1] && key < hi[1];
-                const uint32_t line = v_s + (uint32_t)(at >> 3) * GROUP + (uint32_t)(at & 7) * 128u + (uint32_t)tq * 4u;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                  uint32_t x;
-                  asm volatile("ld.shared.u32 %0, [%1];"
-                               : "=r"(x)
-                               : "r"(line + (uint32_t)(n >> 3) * SLICE + (uint32_t)(((n & 7) ^ (at & 7)) << 4))
-                               : "memory");
-                  const float x0 = __uint_as_float(x << 16), x1 = __uint_as_float(x & 0xffff0000u);
-                  if (!isfinite(x0)) {
-                    o[n][0] += sees0 ? x0 : 0.f;
-                    o[n][2] += sees1 ? x0 : 0.f;
-                  }
-                  if (!isfinite(x1)) {
-                    o[n][1] += sees0 ? x1 : 0.f;
-                    o[n][3] += sees1 ? x1 : 0.f;
-                  }
-                }
-              }
-            }
-          }
-        }
+          for (int block = part * MT; block < (part + 1) * MT; block += 2)
+            few_step<2>(tl, t, block, page_shift, scale, q, lo, hi, o, m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }

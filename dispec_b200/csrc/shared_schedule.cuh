@@ -160,8 +160,9 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
   const int segments = sh.groups + (sh.is_many ? 0 : sh.rows), each = (segments + threads - 1) / threads;
   const int s0 = min(tid * each, segments), s1 = min(s0 + each, segments);
   int mine = 0, of_first = 0, most = 0, least = 0x7fffffff, near = -1;
+  Segment x = {};
   for (int s = s0; s < s1; ++s) {
-    const Segment x = segment(sh, groups, s, near);
+    x = segment(sh, groups, s, near);
     near = x.part ? x.group : -1;
     mine += units_of(sh, x, x.row_tiles);
     of_first += units_of(sh, x, 1);
@@ -200,7 +201,7 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
   if (cta / team_size < runs && u < total && u < upto && u >= upto - mine) {
     int at = upto - mine;
     for (int s = s0; s < s1; ++s) {
-      const Segment x = segment(sh, groups, s, near);
+      if (each > 1) x = segment(sh, groups, s, near);
       const int n = units_of(sh, x, teams ? 1 : x.row_tiles);
       if (u < at + n) {
         run.segment = s;
@@ -216,7 +217,13 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
     run.teams = team_size;
   }
   __syncthreads();
-  if (tid < AHEAD && run.segment >= 0 && run.segment + tid < segments) run.ahead[tid] = segment(sh, groups, run.segment + tid);
+  if (run.segment >= 0) {
+    if (each == 1) {  // (a thread still has its segment)
+      if (tid >= run.segment && tid < min(run.segment + AHEAD, segments)) run.ahead[tid - run.segment] = x;
+    } else if (tid < AHEAD && run.segment + tid < segments) {
+      run.ahead[tid] = segment(sh, groups, run.segment + tid);
+    }
+  }
   __syncthreads();
 }
 
