@@ -133,12 +133,13 @@ __device__ __forceinline__ bool clean_values(const Params<Work>& p, const typena
 // finite).  They are read again where they lie, which costs nothing until there are some.  (A function of its own: its code
 // stays out of the way.)
 template <typename Work>
-__device__ __noinline__ void add_odd_values(const Params<Work>& p, const typename Work::Share& t, int g, typename Work::Row row, bool row_ok,
+__device__ __noinline__ void add_odd_values(const Params<Work>& p, const typename Work::Share& t, int first, int step,
+                                            typename Work::Row row, bool row_ok,
                                             uint32_t o_addr) {
   const auto& sh = p.a.sh;
   const int* table = p.a.page_table + (size_t)t.seq * p.a.pt_stride;
 #pragma unroll 1
-  for (int tile = t.kt_begin + g; tile < t.kt_end; tile += 2) {
+  for (int tile = t.kt_begin + first; tile < t.kt_end; tile += step) {
     const int key0 = tile * BN;
     auto page_of = [&](int key) {
       const int place = key / p.a.page_size, page = place < p.a.table_width ? table[place] : -1;
@@ -679,7 +680,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
       const bool row_ok = r < nrows;
       const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
       const int node = row_ok ? t.first + (row0 + r) / G : t.first;
-      const typename Work::Row row = Work::row(p.a, t, node);
+      const auto row = Work::keep_row(p.a, t, node);
       m_run = -INFINITY;
       l_run = 0.f;
       bool ok = true;
@@ -690,7 +691,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
         // what the row sees of a tile that not every row sees whole, while its scores are being formed
         const bool some = Work::any_hidden(sh, t, row, key0);
         unsigned long long seen = ~0ull;
-        if (some && warp_ok) seen = row_ok ? Work::seen_keys(p.a, t, row, key0) : 0ull;
+        if (some && warp_ok) seen = row_ok ? Work::seen_keys(p.a, t, Work::row_of(p.a, t, row), key0) : 0ull;
         // the tile's scores; and the group's previous O[g] += P V has to be complete before O[g] is rescaled and P[g] rewritten (no
         // arrival for a tile comes before every warp's for the one before has been counted)
         if (!__all_sync(0xffffffffu, j == 0 ? mbar_wait(&s_full[g], count & 1)
@@ -783,7 +784,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
         if (__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
           if (odd_share[g] == share && warp_ok) {  // (every warp of the group has arrived for that product)
             tc_fence_after();
-            add_odd_values(p, t, g, row, row_ok, o_addr);
+            add_odd_values(p, t, g, 2, Work::row_of(p.a, t, row), row_ok, o_addr);
             __syncwarp();
             ask_queries(next, brings && next.seq >= 0, x);  // (asked for again: they need not live through the call)
           }

@@ -6,6 +6,7 @@
 // for it.
 constexpr int KEY_SHIFT = 6, KEYS_PER_TILE = 1 << KEY_SHIFT;
 constexpr int ROW_SHIFT_TENSOR_CORES = 7;  // 128 rows a tile of the tensor-core kernel
+constexpr int ROW_SHIFT_MANY = 8;          // 256 of the one for shared beginnings that many rows see
 constexpr int ROW_SHIFT_FEW = 6;           // 64 of the one for sequences whose keys few rows see
 constexpr int ROW_SHIFT_32BIT = 5;         // 32 of the 32-bit kernel
 

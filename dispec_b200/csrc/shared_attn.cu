@@ -187,7 +187,7 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
                  "%ld rows of %ld heads over pages for %d tokens a sequence are too many for one call", R, columns / D, a.sh.most_ctx);
   DspSharedAttention many = a;
   many.sh.is_many = 1;
-  many.sh.row_shift = ROW_SHIFT_TENSOR_CORES;
+  many.sh.row_shift = ROW_SHIFT_MANY;
   many.sh.extra = EXTRA_MANY;
   many.sh.min_units = 2 + EXTRA_MANY;
   a.ctas = (int)ctas;

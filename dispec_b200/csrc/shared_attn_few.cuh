@@ -327,7 +327,7 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
       const int tile = kt + (lane >> ppt_shift), first = tile * BN + page_in_tile * page_size;
       if (tile >= t.kt_end || first >= t.end || first + page_size <= t.begin) return -2;
       const int j = first >> page_shift;
-      return j < p.a.table_width ? p.a.page_table[(size_t)t.seq * p.a.pt_stride + j] : -1;
+      return j < p.a.table_width ? max(p.a.page_table[(size_t)t.seq * p.a.pt_stride + j], -1) : -1;
     };
     int share = 0, tile = 0, pg_first = more ? load_chunk(w.at, w.at.kt_begin) : -2;
     while (more && ok) {

@@ -3,11 +3,12 @@
 #include "shared_schedule.cuh"
 #include "rows_attn_tcgen05.cuh"
 #include "shared_attn_few.cuh"
+#include "shared_attn_many.cuh"
 
 // The arguments come checked from dsp_shared_attention (shared_attn.cu), which also launches the merge.
 extern "C" int DSP_CAT(dsp_shared_attention_few_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
   return launch_shared_few(*a, stream);
 }
 extern "C" int DSP_CAT(dsp_shared_attention_many_d, DSP_HEAD_DIM)(const DspSharedAttention* a, cudaStream_t stream) {
-  return launch_rows_attn_tcgen05<SharedWork>(*a, stream);
+  return launch_shared_many(*a, stream);
 }

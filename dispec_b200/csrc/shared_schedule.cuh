@@ -391,9 +391,10 @@ struct SharedWork {
     const int length = a.sh.length(node);
     return {max(t.from, a.sh.window > 0 ? length - a.sh.window : 0), min(t.end, length)};
   }
-  static __device__ __forceinline__ bool any_hidden(const Shape&, const Share&, const Row& row, int key0) {
-    return __any_sync(0xffffffffu, key0 < row.lo || key0 + KEYS_PER_TILE > row.hi);
-  }
+  // what a softmax thread keeps of its row through a share: few tiles are not seen whole, and its length is read again for them
+  static __device__ __forceinline__ int keep_row(const Args&, const Share&, int node) { return node; }
+  static __device__ __forceinline__ Row row_of(const Args& a, const Share& t, int node) { return row(a, t, node); }
+  static __device__ __forceinline__ bool any_hidden(const Shape& sh, const Share& t, int, int key0) { return !whole(sh, t, key0); }
   static __device__ __forceinline__ unsigned long long seen_keys(const Args&, const Share&, const Row& row, int key0) {
     const int lo = max(row.lo - key0, 0), n = min(row.hi - key0, KEYS_PER_TILE) - lo;  // bits lo .. lo + n - 1
     return n <= 0 ? 0ull : n >= 64 ? ~0ull : ((1ull << n) - 1ull) << lo;

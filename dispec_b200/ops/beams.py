@@ -78,7 +78,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     rest = ctas * tile * (dim + 2) + items
     many = tensor_cores and rows * share > 64 * groups
     if many:
-        rest += sms * 128 * (dim + 2) + (rows * share // 128 + groups + 1) * kv_heads + 1
+        rest += sms * 256 * (dim + 2) + (rows * share // 256 + groups + 1) * kv_heads + 1
     scratch = prefix_len.new_empty(2 * (rows * kv_heads * share * (dim + 2) + rest))
     tensors = (_describe or _load_describe())(q, k_pool, v_pool, page_table, ctx_len, group_start, prefix_len, out, scratch)
     few_call, many_call = _tensor_core_call(dim) if tensor_cores else (0, 0)
