@@ -19,8 +19,15 @@ using namespace shared;
 
 constexpr int FEW_CTAS = 2;                                 // an SM (shared_attn_few.cuh)
 constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
-// What an item's beginning and end cost, in key tiles, and the fewest key tiles of a run.
-constexpr int EXTRA_FEW = 1, MIN_TILES_FEW = 1, EXTRA_MANY = 5;
+// What an item's beginning and end cost, in key tiles; rows of a tile that takes twice as long (64 rows 2.5 us a key tile and CTA
+// where 16 take 1.3).  (256 sequences behind shared parts of 2,050, 28 heads of 128 on 4: 105.7, 103.7, 100.4 and 100.8 us with 0 to 3 for
+// the kernel for few rows; 8 groups of 5 behind 4,101: 39.7, 33.9, 31.1, 32.0.  In 32 bits a key tile takes 8 us, and nothing is
+// small beside it: 2 groups of 5 behind 701, 12 heads on 2: 21.6, 25.2, 32.2.)
+// A kernel more is some 17 us more: one group of 224 rows a head of 128, 4 heads, shared parts of 4,000, 8,000 and 32,000 tokens: 48, 50
+// and 70 us with both kernels, 38, 51 and 119 with the one for few alone; of 112 rows 8,000 and 32,000: 46 and 63, 43 and 80; of
+// 320 rows, 8 heads, 4,000, 8,000 and 32,768: 74, 78 and 121, 64, 84 and 213.
+constexpr long MANY_UNITS = 16;
+constexpr int EXTRA_FEW = 2, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
 
 // A thread has four columns of a row and head.  Groups and lengths were there before the kernels in front began, and are looked at
 // before their results are waited for; then two latencies are left, the records' and the partial results'.
@@ -174,20 +181,23 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   a.sh.window = (int)o->window;
   a.sh.rows = (int)R;
   a.sh.row_shift = tensor_cores ? ROW_SHIFT_FEW : ROW_SHIFT_32BIT;
-  a.sh.extra = EXTRA_FEW;
-  a.sh.min_units = MIN_TILES_FEW + EXTRA_FEW;
-  // where groups have more rows a head than a tile of the kernel for few on average, the shared parts of those that do are the
-  // other one's
-  const bool use_many = tensor_cores && R * a.sh.G > groups * FEW_ROWS_OF_A_TILE;
+  a.sh.extra = tensor_cores ? EXTRA_FEW : EXTRA_32BIT;
+  a.sh.heavy = tensor_cores ? HEAVY_FEW : 0x7fffffff;
+  a.sh.min_units = 1 + a.sh.extra;
+  // Where groups have more rows a head on average than a tile of the kernel for few, and their shared parts may be so long (as long
+  // as their pages) that each SM has MANY_UNITS of its tiles or more, the shared parts of those that do are the other kernel's.
+  const long units = (R * a.sh.G + FEW_ROWS_OF_A_TILE - 1) / FEW_ROWS_OF_A_TILE * KVH * (table.size[1] * page / KEYS_PER_TILE + 1);
+  const bool use_many = tensor_cores && R * a.sh.G > groups * FEW_ROWS_OF_A_TILE && units > MANY_UNITS * o->sms;
   a.sh.many = use_many ? FEW_ROWS_OF_A_TILE : 0x7fffffff;
   // places are counted in 32 bits, a tile of keys beyond the last among them
   a.sh.most_ctx = (int)min(table.size[1] * page, 1L << 30);
   // Units are counted in 32 bits: those of all items, each over as many tokens as a sequence's pages hold.
-  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (a.sh.most_ctx / KEYS_PER_TILE + 1 + EXTRA_MANY),
+  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (2 * (a.sh.most_ctx / KEYS_PER_TILE + 1) + EXTRA_MANY),
                  "%ld rows of %ld heads over pages for %d tokens a sequence are too many for one call", R, columns / D, a.sh.most_ctx);
   DspSharedAttention many = a;
   many.sh.is_many = 1;
   many.sh.row_shift = ROW_SHIFT_MANY;
+  many.sh.heavy = 0x7fffffff;
   many.sh.extra = EXTRA_MANY;
   many.sh.min_units = 2 + EXTRA_MANY;
   a.ctas = (int)ctas;

@@ -4,8 +4,8 @@
 // P_g = prefix_len[g] tokens are the same for all of them and are read through the pages of its first sequence.  A segment is
 // either such a beginning with the rows of all the group's sequences, or one sequence's keys behind it with its own G rows (a
 // group of one has no shared part: all its keys are one segment).  An item is one tile of query rows of one key/value head of
-// one segment; it walks the key tiles of 64 that any of its rows sees, and is counted as so many units and `extra` more, which
-// stand for its beginning and end.  All units, in the order (shared parts, sequences; row tile, head, key tile), are cut into equal
+// one segment; it walks the key tiles of 64 that any of its rows sees, and is counted as so many units, twice as many where a tile
+// has more than `heavy` rows, and `extra` more, which stand for its beginning and end.  All units, in the order (shared parts, sequences; row tile, head, key tile), are cut into equal
 // runs, one per CTA, wherever that falls, so that few long beginnings load every SM as well as many short sequences, and nothing
 // about lengths is needed on the host.
 //
@@ -29,6 +29,7 @@ struct Shape {
   int rows;       // sequences: a group that is not inside them is recorded and left out
   int most_ctx;   // tokens that a sequence's pages hold
   int row_shift;  // of a tile's query rows
+  int heavy;      // a row tile of more rows takes two units a key tile
   int many;       // shared parts of more rows a head are for the kernel of many rows
   int is_many;    // that kernel's shape
   int* err;
@@ -70,8 +71,13 @@ struct Segment {
   int from, begin, end;        // first key of the segment; the keys that any of its rows sees
   int all_begin, all_end;      // the keys that all of them see
   int lo_tile, key_tiles, row_tiles;
+  int weight, last_weight;     // units a key tile of a whole row tile, and of the last one
 };
 
+__device__ __forceinline__ void set_weights(const Shape& sh, Segment& x) {
+  x.weight = sh.rows_per_tile() > sh.heavy ? 2 : 1;
+  x.last_weight = x.n * sh.G - ((x.row_tiles - 1) << sh.row_shift) > sh.heavy ? 2 : 1;
+}
 // The shared part of group g, whose sequences have between `shortest` and `longest` tokens.
 __device__ __forceinline__ Segment shared_part(const Shape& sh, int g, int first, int end, int prefix, int shortest, int longest) {
   Segment x = {};
@@ -88,6 +94,7 @@ __device__ __forceinline__ Segment shared_part(const Shape& sh, int g, int first
   x.lo_tile = x.begin >> KEY_SHIFT;
   x.key_tiles = x.end > x.begin ? ((x.end + KEYS_PER_TILE - 1) >> KEY_SHIFT) - x.lo_tile : 0;
   x.row_tiles = (x.n * sh.G + sh.rows_per_tile() - 1) >> sh.row_shift;
+  set_weights(sh, x);
   return x;
 }
 // The own part of a row of group g (first .. end - 1), -1: of none.
@@ -105,6 +112,7 @@ __device__ __forceinline__ Segment own_part(const Shape& sh, int row, int g, int
   x.lo_tile = x.begin >> KEY_SHIFT;
   x.key_tiles = x.end > x.begin ? ((x.end + KEYS_PER_TILE - 1) >> KEY_SHIFT) - x.lo_tile : 0;
   x.row_tiles = sh.tiles_of_sequence();
+  set_weights(sh, x);
   return x;
 }
 // `near`: a group that the row may be in, looked at first.
@@ -117,8 +125,10 @@ __device__ __forceinline__ Segment segment(const Shape& sh, const Groups& groups
   const int at = max(near, 0);
   return own_part(sh, row, near, groups.start[at], groups.start[at + 1], groups.prefix[at]);
 }
-__device__ __forceinline__ int units_of(const Shape& sh, const Segment& x, int row_tiles) {
-  return x.key_tiles > 0 ? (x.key_tiles + sh.extra) * row_tiles * sh.KVH : 0;
+// Units of a segment, or with teams of one of its row tiles (which all weigh the same then).
+__device__ __forceinline__ int units_of(const Shape& sh, const Segment& x, bool teams) {
+  if (x.key_tiles <= 0) return 0;
+  return sh.KVH * ((teams ? 0 : (x.row_tiles - 1) * (x.key_tiles * x.weight + sh.extra)) + x.key_tiles * (teams ? 1 : x.last_weight) + sh.extra);
 }
 
 // Where a CTA's run begins.
@@ -164,8 +174,8 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
   for (int s = s0; s < s1; ++s) {
     x = segment(sh, groups, s, near);
     near = x.part ? x.group : -1;
-    mine += units_of(sh, x, x.row_tiles);
-    of_first += units_of(sh, x, 1);
+    mine += units_of(sh, x, false);
+    of_first += units_of(sh, x, true);
     if (x.key_tiles > 0) {
       most = max(most, x.row_tiles);
       least = min(least, x.row_tiles);
@@ -202,7 +212,7 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
     int at = upto - mine;
     for (int s = s0; s < s1; ++s) {
       if (each > 1) x = segment(sh, groups, s, near);
-      const int n = units_of(sh, x, teams ? 1 : x.row_tiles);
+      const int n = units_of(sh, x, teams);
       if (u < at + n) {
         run.segment = s;
         run.segment_start = at;
@@ -252,6 +262,7 @@ struct Walk {
   int cta, teams;
   int u, end, chunk, segment_at;
   int item_start, key_tiles, lo_tile, row_tiles;
+  int weights[2];          // units a key tile of a whole row tile, and of the last one
   bool begins;             // the share has its item's first key tile
   const Run* run_;
   Share at;
@@ -267,12 +278,21 @@ struct Walk {
     end = (int)min((long)u + chunk, (long)run.total);
     segment_at = run.segment;
     enter(sh);
-    const int cost = key_tiles + sh.extra, item = (u - run.segment_start) / cost;
-    item_start = run.segment_start + item * cost;
-    at.row_tile = teams > 1 ? cta % teams : item / sh.KVH;
-    at.head = item % sh.KVH;
+    at.row_tile = 0;
+    item_start = run.segment_start;
+    if (teams > 1) {
+      at.row_tile = cta % teams;
+    } else {
+      const int whole = sh.KVH * (key_tiles * weights[0] + sh.extra);
+      at.row_tile = min((u - item_start) / whole, row_tiles - 1);
+      item_start += at.row_tile * whole;
+    }
+    const int cost = key_tiles * weight() + sh.extra;
+    at.head = (u - item_start) / cost;
+    item_start += at.head * cost;
     return share(sh) || next(sh);
   }
+  __device__ __forceinline__ int weight() const { return teams > 1 ? 1 : at.row_tile + 1 < row_tiles ? weights[0] : weights[1]; }
   // what has to be known of segment `segment_at`; false: it has no keys
   __device__ __forceinline__ bool enter(const Shape& sh) {
     Segment x;
@@ -306,23 +326,27 @@ struct Walk {
     key_tiles = x.key_tiles;
     lo_tile = x.lo_tile;
     row_tiles = teams > 1 ? 1 : x.row_tiles;
+    weights[0] = x.weight;
+    weights[1] = x.last_weight;
     return key_tiles > 0;
   }
   // the run's part of the present item; false: it has no key tile
   __device__ __forceinline__ bool share(const Shape& sh) {
-    const int first_tile = item_start + sh.extra, item_end = first_tile + key_tiles, stop = min(end, item_end);
-    begins = u <= first_tile;
-    at.kt_begin = lo_tile + max(u - first_tile, 0);
-    at.kt_end = lo_tile + (stop - first_tile);
+    // (so many key tiles lie in front of a unit of the item)
+    const int w = weight(), first_tile = item_start + sh.extra, item_end = first_tile + key_tiles * w, stop = min(end, item_end);
+    const int before = max(u - first_tile, 0) >> (w - 1), upto = max(stop - first_tile, 0) >> (w - 1);
+    begins = before == 0;
+    at.kt_begin = lo_tile + before;
+    at.kt_end = lo_tile + upto;
     at.slot = begins ? (stop == item_end ? -1 : 2 * cta + 1) : 2 * cta;
     u = stop;
-    return at.kt_end > at.kt_begin;
+    return upto > before;
   }
   __device__ __forceinline__ Note split(const Shape& sh) const {
     Note x = {-1, {cta, 1, (short)teams}};
     if (begins) {
       x.item = sh.item(at.part, at.group, at.first, at.row_tile, at.head);
-      x.record.parts = (short)((item_start + sh.extra + key_tiles - 1) / chunk - cta / teams + 1);
+      x.record.parts = (short)((item_start + sh.extra + key_tiles * weight() - 1) / chunk - cta / teams + 1);
     }
     return x;
   }

@@ -76,7 +76,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     tile, ctas = (64, 2 * sms) if tensor_cores else (32, sms * (1 if dim > 128 else 2))
     items = (rows * share // tile + groups + 1 + rows * -(-share // tile)) * kv_heads + 1
     rest = ctas * tile * (dim + 2) + items
-    many = tensor_cores and rows * share > 64 * groups
+    many = tensor_cores and rows * share > 64 * groups  # (it may be)
     if many:
         rest += sms * 256 * (dim + 2) + (rows * share // 256 + groups + 1) * kv_heads + 1
     scratch = prefix_len.new_empty(2 * (rows * kv_heads * share * (dim + 2) + rest))
