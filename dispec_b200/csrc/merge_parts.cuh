@@ -4,8 +4,12 @@
 #pragma once
 #include "common.cuh"
 
+struct Merged {
+  float4 sum;        // of weights times values, four columns
+  float top, total;  // the largest score (base-2 domain) and the sum of weights, both relative to it
+};
 template <int AT_ONCE = 8, typename Load>
-__device__ __forceinline__ float4 merge_parts(int parts, Load load) {
+__device__ __forceinline__ Merged merge_parts(int parts, Load load) {
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = 0; k0 < parts; k0 += AT_ONCE) {
@@ -34,6 +38,9 @@ __device__ __forceinline__ float4 merge_parts(int parts, Load load) {
     }
     M = top;
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;  // (NaN stays)
-  return make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  return {acc, M, L};
+}
+__device__ __forceinline__ float4 merged(const Merged& x) {
+  const float inv = x.total == 0.f ? 0.f : 1.f / x.total;  // (NaN stays)
+  return make_float4(x.sum.x * inv, x.sum.y * inv, x.sum.z * inv, x.sum.w * inv);
 }

@@ -29,20 +29,26 @@ constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
 constexpr long MANY_UNITS = 16;
 constexpr int EXTRA_FEW = 2, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
 
-// A thread has four columns of a row and head.  Groups and lengths were there before the kernels in front began, and are looked at
-// before their results are waited for; then two latencies are left, the records' and the partial results'.
+// Joins a row's partial results: `quads` neighbouring threads have four columns each of a row and head, and where rows are few, so many
+// threads more (`share`) divide the partial results of a row among them, up to one for each CTA (8 rows behind 16,384 tokens, 12 heads
+// of 128 on 2: 150 parts; a layer of a step 41 us where one thread a row took 75).
+// Groups and lengths were there before the kernels in front began, and are looked at before their results are waited for; then two
+// latencies are left, the records' and the partial results'.
 constexpr int COMBINE_THREADS = 256;
 template <typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS, 3)
 shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch scratch, const SharedScratch scratch_many,
-                      T* __restrict__ out, long out_stride, int D, int ctas, int ctas_many) {
-  const int H = sh.KVH * sh.G, quads = D / 4;
-  const long i = (long)blockIdx.x * COMBINE_THREADS + threadIdx.x;
-  const float2* rows_ml = reinterpret_cast<const float2*>(scratch.rows_ml);
-  const int row_head = (int)min(i / quads, (long)sh.rows * H), d = (int)(i % quads) * 4, row = row_head / H, h = row_head - row * H;
-  const int head = h / sh.G, of_head = h - head * sh.G;
+                      T* __restrict__ out, long out_stride, int D, int ctas, int ctas_many, int share) {
   __shared__ int start[MAX_GROUPS + 1];
-  for (int k = threadIdx.x; k <= sh.groups; k += COMBINE_THREADS) start[k] = sh.group_start[k];
+  __shared__ float4 sums[COMBINE_THREADS];
+  __shared__ float2 mls[COMBINE_THREADS];
+  const int H = sh.KVH * sh.G, quads = D / 4, per_row = quads * share, tid = threadIdx.x;
+  const int of_block = COMBINE_THREADS / per_row, in_block = tid / per_row, in_row = tid - in_block * per_row;
+  const long row_head = (long)blockIdx.x * of_block + in_block;
+  const int mine = in_row / quads, d = (in_row - mine * quads) * 4;  // which of the row's parts; its columns
+  const int row = in_block < of_block ? (int)min(row_head / H, (long)sh.rows) : sh.rows, h = (int)(row_head % H);
+  const int head = h / sh.G, of_head = h - head * sh.G;
+  for (int k = tid; k <= sh.groups; k += COMBINE_THREADS) start[k] = sh.group_start[k];
   const int length = row < sh.rows ? sh.length(row) : 0;  // (asked for with the groups)
   __syncthreads();
   const int g = row < sh.rows ? group_of(start, sh.groups, sh.rows, row) : -1;
@@ -66,58 +72,59 @@ shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch s
   }
   pdl_launch_dependents();
   pdl_wait();
-  if (g >= 0) {  // (a row in no group is left as it is)
-    // asked for with the records, which say whether they are wanted
-    Record rec[2];
-    float2 ml[2];
-    float4 o[2];
+  // asked for with the records, which say whether they are wanted
+  Record rec[2];
+  float2 ml[2];
+  float4 o[2];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const bool of_many = part == 0 && many;
-      const size_t at = ((size_t)part * sh.rows + row) * H + h;
+  for (int part = 0; part < 2; ++part) {
+    const bool of_many = part == 0 && many;
+    const size_t at = ((size_t)part * sh.rows + row) * H + h;
+    rec[part] = {0, 0, 1};
+    ml[part] = make_float2(-INFINITY, 0.f);
+    o[part] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (sees[part]) {
+      rec[part] = (of_many ? scratch_many : scratch).records[item[part]];
+      ml[part] = reinterpret_cast<const float2*>(scratch.rows_ml)[at];
+      o[part] = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
+    }
+    // (a record that a CTA whose wait ran out did not write is none)
+    const Record x = rec[part];
+    if (x.cta < 0 || x.parts < 0 || x.stride < 1 || (x.parts > 0 && x.cta + (x.parts - 1) * x.stride >= (of_many ? ctas_many : ctas)))
       rec[part] = {0, 0, 1};
-      ml[part] = make_float2(-INFINITY, 0.f);
-      o[part] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (sees[part]) {
-        rec[part] = (of_many ? scratch_many : scratch).records[item[part]];
-        ml[part] = rows_ml[at];
-        o[part] = *reinterpret_cast<const float4*>(scratch.rows_o + at * D + d);
-      }
-    }
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const bool of_many = part == 0 && many;
-      const Record x = rec[part];
-      // (a record that a CTA whose wait ran out did not write is none)
-      if (x.cta < 0 || x.parts < 0 || x.stride < 1 || (x.parts > 0 && x.cta + (x.parts - 1) * x.stride >= (of_many ? ctas_many : ctas)))
-        rec[part] = {0, 0, 1};
-    }
-    float4 v;
-    if (rec[0].parts <= 1 && rec[1].parts <= 1) {
-      v = merge_parts<2>(2, [&](int k, float2& a, float4& b) {
-        a = (k ? rec[1] : rec[0]).parts ? (k ? ml[1] : ml[0]) : make_float2(-INFINITY, 0.f);
-        b = k ? o[1] : o[0];
-      });
-    } else {
-      v = merge_parts<8>(rec[0].parts + rec[1].parts, [&](int k, float2& a, float4& b) {
-        const int part = k >= rec[0].parts;
-        if (part) k -= rec[0].parts;
-        const Record x = part ? rec[1] : rec[0];
-        if (x.parts == 1) {
-          a = part ? ml[1] : ml[0];
-          b = part ? o[1] : o[0];
-        } else {
-          const bool of_many = part == 0 && many;
-          const SharedScratch& of = of_many ? scratch_many : scratch;
-          const size_t slot = 2 * (size_t)(x.cta + k * x.stride) + (k == 0);
-          const size_t at = (slot << (of_many ? sh_many.row_shift : sh.row_shift)) + (part ? of_tile[1] : of_tile[0]);
-          a = reinterpret_cast<const float2*>(of.part_ml)[at];
-          b = *reinterpret_cast<const float4*>(of.part_o + at * D + d);
-        }
-      });
-    }
-    store4(out + (size_t)row * out_stride + (size_t)h * D + d, v);
   }
+  auto load = [&](int k, float2& a, float4& b) {
+    const int part = k >= rec[0].parts;
+    if (part) k -= rec[0].parts;
+    const Record x = part ? rec[1] : rec[0];
+    if (x.parts <= 1) {
+      a = part ? ml[1] : ml[0];
+      b = part ? o[1] : o[0];
+    } else {
+      const bool of_many = part == 0 && many;
+      const SharedScratch& of = of_many ? scratch_many : scratch;
+      const size_t slot = 2 * (size_t)(x.cta + k * x.stride) + (k == 0);
+      const size_t at = (slot << (of_many ? sh_many.row_shift : sh.row_shift)) + (part ? of_tile[1] : of_tile[0]);
+      a = reinterpret_cast<const float2*>(of.part_ml)[at];
+      b = *reinterpret_cast<const float4*>(of.part_o + at * D + d);
+    }
+  };
+  const int parts = rec[0].parts + rec[1].parts;
+  // thread `mine` has the parts mine, mine + share, ...
+  const int own = parts > mine ? (parts - mine + share - 1) / share : 0;
+  const Merged x = merge_parts<4>(own, [&](int k, float2& a, float4& b) { load(mine + k * share, a, b); });
+  float4 v = merged(x);
+  if (share > 1) {
+    sums[tid] = x.sum;
+    mls[tid] = make_float2(x.top, x.total);
+    __syncthreads();
+    if (mine > 0) return;
+    v = merged(merge_parts<2>(min(parts, share), [&](int k, float2& a, float4& b) {
+      a = mls[tid + k * quads];
+      b = sums[tid + k * quads];
+    }));
+  }
+  if (g >= 0) store4(out + (size_t)row * out_stride + (size_t)h * D + d, v);  // (a row in no group is left as it is)
 }
 
 // A kernel's scratch of its own, laid out from `at` on.
@@ -244,13 +251,19 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
     const int rc = q.dtype == DSP_T_F32 ? launch_rows_attn<SharedWork, float>(a, stream) : launch_rows_attn<SharedWork, bf16>(a, stream);
     if (rc != 0) return rc;
   }
-  const dim3 grid((unsigned)((R * columns / 4 + COMBINE_THREADS - 1) / COMBINE_THREADS));
+  // threads that share a row and head: one for eight of the parts that a shared part's item may have, by the CTAs that there are for
+  // each and by its key tiles
+  const long quads = D / 4, row_heads = R * columns / D, parts = min(ctas / min(groups * KVH, ctas), (long)a.sh.most_ctx / KEYS_PER_TILE);
+  int share = 1;
+  while (quads * share * 2 <= COMBINE_THREADS && share * 16 <= parts) share *= 2;
+  const long of_block = COMBINE_THREADS / (quads * share);
+  const dim3 grid((unsigned)((row_heads + of_block - 1) / of_block));
   if (q.dtype == DSP_T_F32)
     DSP_CUDA(launch_pdl(shared_combine_kernel<float>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, many.sh, a.scratch, many.scratch,
-                        (float*)a.out, a.out_stride, a.D, a.ctas, many.ctas));
+                        (float*)a.out, a.out_stride, a.D, a.ctas, many.ctas, share));
   else
     DSP_CUDA(launch_pdl(shared_combine_kernel<bf16>, grid, dim3(COMBINE_THREADS), 0, stream, a.sh, many.sh, a.scratch, many.scratch,
-                        (bf16*)a.out, a.out_stride, a.D, a.ctas, many.ctas));
+                        (bf16*)a.out, a.out_stride, a.D, a.ctas, many.ctas, share));
   DSP_CHECK_LAUNCH("shared_prefix_attention");
   return 0;
 }

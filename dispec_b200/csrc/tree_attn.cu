@@ -56,11 +56,11 @@ tree_combine_kernel(const TreeScratch scratch, T* __restrict__ out, long out_str
       auto row_of = [&](int k) -> size_t { return (k == 0 ? 2 * (size_t)c + 1 : 2 * (size_t)(c + k)) * R + r; };  // of the k-th part
       const int rr = x.row0 + r;
       T* dst = out + (size_t)(x.first + rr / G) * out_stride + (size_t)(x.head * G + rr % G) * D;
-      store4(dst + d, merge_parts(x.parts, [&](int k, float2& m, float4& v) {
+      store4(dst + d, merged(merge_parts(x.parts, [&](int k, float2& m, float4& v) {
         const size_t at = row_of(k);
         m = ml[at];
         v = load4(scratch.part_o + at * D + d);
-      }));
+      })));
     }
   }
 }

@@ -80,7 +80,7 @@ class SharedStep:
     """What the attention of a step of beams reads beside the arrays of every step: the sequences come in groups whose first tokens
     lie in the same pages."""
     group_start: torch.Tensor  # [groups + 1] int32: sequences of each group
-    prefix_len: list  # per cache group [groups] int32: so many first tokens
+    prefix_len: list  # per cache group [groups] int32: so many first tokens; None: they are not worth an attention of their own
 
 
 def _align4(n: int) -> int:

@@ -26,6 +26,16 @@ from dispec_b200.models.model import DecoderModel
 GRAPH_CONTEXT_CLASSES = (2048, 8192, 32768, 131072, 524288)
 
 
+# Bytes of keys and values that reading shared pages once has to save in a layer.  The attention of shared pages is three launches
+# where that of single tokens is one: some 10 us, in which 100 MB come from the L2 and the memory.  A layer of a step, heads of 128,
+# shared and each its own: 8 beams behind 4,096 tokens, 28 heads on 4 (59 MB) 42 and 37 us, 4 behind 16,384 (101 MB) 46 and 50, 8 behind
+# 16,384 (235 MB) 53 and 73, 32 behind 16,384 (1 GB) 76 and 191; 8 behind 16,384, 12 heads on 2 (117 MB) 41 and 40.  In 32 bits the
+# attention of single tokens is bound by its arithmetic, and the products of shared pages are of tiles of rows: 2 beams behind
+# 64 tokens, 12 heads on 2 (0.1 MB) 60 and 57 us, behind 256 (0.5 MB) 61 and 70, behind 16,384 86 and 1,260.
+SHARED_BYTES = {torch.bfloat16: 100_000_000, torch.float32: 500_000}
+MAX_SHARED_GROUPS = 1024  # of a call (ops/beams.py)
+
+
 class ModelRunner:
     def __init__(self, model: DecoderModel, page_size: int = 16, num_pages=4096,
                  max_num_seqs: int = 256, poison: bool = False, cuda_graph: bool = False,
@@ -180,17 +190,21 @@ class ModelRunner:
             self.cache.extend(e.req_id, e.start + 1)
         ctx, _ = build_context([SeqEntry(e.req_id, e.tokens, e.start, [0]) for e in entries], self.cache, self.storage, self.states,
                                self.staging, self.dtype, self.device, self.model.attention_tile_tokens, self.vocab_size)
-        n, starts, prefixes = len(groups), [0], []
+        n, starts, prefixes, worth = len(groups), [0], [], []
         for of in groups:
             starts.append(starts[-1] + len(of))
-        for c in range(len(self.cache.groups)):
+        for c, spec in enumerate(self.cache.groups):
+            saved = 0  # bytes that need not be read in a layer
             for of, known in zip(groups, shared):
                 if len(of) > 1:
                     known[c] = self.cache.shared_pages([e.req_id for e in of], c, known[c])
                 prefixes.append(known[c] * self.page_size if len(of) > 1 else 0)
+                of_window = prefixes[-1] if spec.window <= 0 else max(0, min(prefixes[-1], prefixes[-1] + spec.window - of[0].start - 1))
+                saved += (len(of) - 1) * of_window * sum(t.num_heads * t.width for t in spec.tensors) * self.dtype.itemsize
+            worth.append(n <= MAX_SHARED_GROUPS and saved >= SHARED_BYTES[self.dtype])
         numbers = torch.tensor(starts + prefixes, dtype=torch.int32).to(self.device)
-        if any(prefixes):
-            ctx.shared = SharedStep(numbers[:n + 1], [numbers[n + 1 + c * n:n + 1 + (c + 1) * n] for c in range(len(self.cache.groups))])
+        if any(worth):
+            ctx.shared = SharedStep(numbers[:n + 1], [numbers[n + 1 + c * n:n + 1 + (c + 1) * n] if w else None for c, w in enumerate(worth)])
         x, pending = self.model.forward(ctx)
         logits = self.model.logits(ctx, x, pending, ctx.logit_rows)
         for e in entries:

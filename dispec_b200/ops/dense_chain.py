@@ -58,7 +58,8 @@ def run_layers(model, ctx, x: torch.Tensor) -> bool:
     """Runs the layers on the rows ``x`` in place; False (nothing has run) where this step is not for it.  A step that
     is being captured is not: its launches are replayed from the graph, whoever made them, and one row a step was
     1.5 % slower on this function's buffers (950 us against 935) than on those of the parts."""
-    if ctx.graph_capture or getattr(ctx, "tree", None) is not None:  # (a step of drafted trees has an attention of its own)
+    # (steps of drafted trees and of sequences that share pages have attentions of their own)
+    if ctx.graph_capture or getattr(ctx, "tree", None) is not None or getattr(ctx, "shared", None) is not None:
         return False
     block = model.layers[model.schedule[0].layer]
     mixer, ff = block.mixer, block.feed_forward

@@ -102,7 +102,7 @@ class GQAAttention(Mixer):
         if ctx.tree is not None:
             out = self._tree(ctx, qkv, cache, inv_freq, rotary_dim, scale)
             return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
-        if ctx.shared is not None:
+        if ctx.shared is not None and ctx.shared.prefix_len[cache.group] is not None:
             out = self._shared(ctx, qkv, cache, inv_freq, rotary_dim, scale)
             return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
         n_dec = ctx.num_decode_seqs

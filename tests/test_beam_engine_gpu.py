@@ -70,9 +70,16 @@ def engine_for(folder, dtype, page_size, width, **kw):
     return engine
 
 
+@pytest.fixture
+def always_shared(monkeypatch):
+    """The attention of shared pages wherever there are some, however few."""
+    from dispec_b200.engine import runner
+    monkeypatch.setattr(runner, "SHARED_BYTES", {torch.bfloat16: 1, torch.float32: 1})
+
+
 @pytest.mark.parametrize("name", ["a", "b", "c", "d", "e"])
 @pytest.mark.parametrize("width,penalty,eos", [(1, 1.0, None), (4, 1.0, None), (3, 0.6, 7), (5, 0.0, None)])
-def test_the_found_continuations_are_those_of_the_plain_search(name, width, penalty, eos):
+def test_the_found_continuations_are_those_of_the_plain_search(name, width, penalty, eos, always_shared):
     with tempfile.TemporaryDirectory() as td:
         config, weights = ru.make_model_folder(td, name, dtype="float32")
         engine = engine_for(td, "float32", ru.TINY[name]["page_size"], width)
@@ -95,7 +102,7 @@ def test_an_end_token_that_is_likely():
 
 
 @pytest.mark.parametrize("family", FAMILIES)
-def test_other_families_keep_their_states_and_pages(family):
+def test_other_families_keep_their_states_and_pages(family, always_shared):
     """Recurrent states, windows, latents and chunks follow their beams: the same search with one whole pass per beam."""
     from dispec_b200 import SeqEntry
     util = importlib.import_module(f"{family}_util")
@@ -115,7 +122,7 @@ def test_other_families_keep_their_states_and_pages(family):
         check(engine, logits_of, prompts, 3, 9, 1.0, None, 2e-3)
 
 
-def test_bfloat16_scores_are_the_models_own():
+def test_bfloat16_scores_are_the_models_own(always_shared):
     with tempfile.TemporaryDirectory() as td:
         config, weights = ru.make_model_folder(td, "c", dtype="bfloat16")
         engine = engine_for(td, "bfloat16", ru.TINY["c"]["page_size"], 4)
@@ -128,6 +135,29 @@ def test_bfloat16_scores_are_the_models_own():
                 # logits are off by up to 5e-2 in bfloat16, as the tests of steps have it; a mean of twelve log-probabilities, each
                 # off by twice as much
                 assert abs(log_probability(logits_of, prompt, h.tokens) / 12 - h.score) <= 0.1
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_shared_pages_are_read_once_a_prompt(dtype, monkeypatch):
+    """The attention of shared pages is called in every layer of every step whose beams share enough."""
+    from dispec_b200 import ops
+    from dispec_b200.engine import runner
+    calls = []
+    real = ops.shared_prefix_attention
+    monkeypatch.setattr(ops, "shared_prefix_attention", lambda *a, **kw: calls.append(a[6].tolist()) or real(*a, **kw))
+    with tempfile.TemporaryDirectory() as td:
+        config, _ = ru.make_model_folder(td, "a", dtype=dtype)
+        engine = engine_for(td, dtype, 16, 4)
+        prompts = [ru.random_ids(100, config["vocab_size"], 1), ru.random_ids(40, config["vocab_size"], 2)]
+        engine.generate(prompts, 5)
+        assert not calls  # (not worth it)
+        monkeypatch.setattr(runner, "SHARED_BYTES", {torch.bfloat16: 1, torch.float32: 1})
+        engine.generate(prompts, 5)
+        layers = config["num_hidden_layers"]
+        assert len(calls) == 4 * layers and all(c == [96, 32] for c in calls)
+        calls.clear()
+        engine.generate([ru.random_ids(7, config["vocab_size"], 1)], 5)  # no page is full
+        assert not calls
 
 
 def test_more_prompts_than_fit_at_once_and_again():
