@@ -1,7 +1,7 @@
 // Attention of rows over the paged cache on the fifth-generation tensor cores, bfloat16 in, 32-bit softmax and accumulation.  What
 // the rows are, how the work is cut and what a row sees is said by a type `Work` (TreeWork in tree_schedule.cuh: nodes of drafted
-// trees; SharedWork in shared_schedule.cuh: sequences with a shared beginning).  Compiled once per head size
-// (-DDSP_HEAD_DIM=64 or 128) and Work.
+// trees).  Compiled once per head size (-DDSP_HEAD_DIM=64 or 128).  The tile's layout and the treatment of its values are
+// shared_attn_many.cuh's as well (SharedWork in shared_schedule.cuh).
 //
 // One CTA an SM walks its run of units: for each item's share, 128 query rows of one key/value head and key tiles of 64.
 // S = Q K^T and O += P V are tcgen05.mma with S, O and the A operands Q and P in tensor memory; keys and values arrive by
@@ -508,15 +508,13 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
     const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - M);
     const float w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - M);
     const float denom = ml0.y * w0 + ml1.y * w1;
-    const float inv = slot >= 0 || Work::ROW_PARTS ? 1.f : denom == 0.f ? 0.f : 1.f / denom;
+    const float inv = slot >= 0 ? 1.f : denom == 0.f ? 0.f : 1.f / denom;
     const float f0 = w0 * inv, f1 = w1 * inv;
     if (quarter * 32 < nrows) {
       Rows4 rows;
-      if (slot < 0) rows = rows_of(t, Work::ROW_PARTS ? (size_t)sh.KVH * G * D : (size_t)p.a.out_stride);
+      if (slot < 0) rows = rows_of(t, (size_t)p.a.out_stride);
       bf16* out = (bf16*)p.a.out + (lane & 3) * 8;
       float* part = p.a.scratch.part_o + ((size_t)slot * BM + r4) * D + (lane & 3) * 4;
-      float* of_rows = nullptr;
-      if constexpr (Work::ROW_PARTS) of_rows = p.a.scratch.rows_o + (size_t)t.part * sh.rows * sh.KVH * G * D + (lane & 3) * 4;
 #pragma unroll 1
       for (int c0 = g * (D / 2); c0 < (g + 1) * (D / 2); c0 += 32) {
         uint32_t ov[32], ow[32];
@@ -532,7 +530,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
 #pragma unroll
           for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * f0);
         }
-        if (slot >= 0 || Work::ROW_PARTS) {
+        if (slot >= 0) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint4 x[4];
@@ -541,13 +539,8 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
               x[c] = make_uint4(ov[16 * h + 4 * c], ov[16 * h + 4 * c + 1], ov[16 * h + 4 * c + 2], ov[16 * h + 4 * c + 3]);
             transpose4(x);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (Work::ROW_PARTS && slot < 0) {
-                if (k < rows.n) *reinterpret_cast<uint4*>(of_rows + rows.at[k] + c0 + 16 * h) = x[k];
-              } else if (r4 + k < nrows) {
-                *reinterpret_cast<uint4*>(part + k * D + c0 + 16 * h) = x[k];
-              }
-            }
+            for (int k = 0; k < 4; ++k)
+              if (r4 + k < nrows) *reinterpret_cast<uint4*>(part + k * D + c0 + 16 * h) = x[k];
           }
         } else {
           uint4 x[4];
@@ -566,13 +559,6 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
         __syncwarp();
       }
       if (g == 0 && slot >= 0 && row_ok) reinterpret_cast<float2*>(p.a.scratch.part_ml)[(size_t)slot * BM + r] = make_float2(M, denom);
-      if constexpr (Work::ROW_PARTS) {
-        if (g == 0 && slot < 0 && row_ok) {
-          const int node = (row0 + r) / G, head = row0 + r - node * G;
-          const size_t at = ((size_t)t.part * sh.rows + t.first + node) * sh.KVH * G + t.head * G + head;
-          reinterpret_cast<float2*>(p.a.scratch.rows_ml)[at] = make_float2(M, denom);
-        }
-      }
     }
     tc_fence_before();
     __syncwarp();
@@ -680,7 +666,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
       const bool row_ok = r < nrows;
       const bool warp_ok = quarter * 32 < nrows;  // a warp without rows only keeps the barriers going
       const int node = row_ok ? t.first + (row0 + r) / G : t.first;
-      const auto row = Work::keep_row(p.a, t, node);
+      const auto row = Work::row(p.a, t, node);
       m_run = -INFINITY;
       l_run = 0.f;
       bool ok = true;
@@ -691,7 +677,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
         // what the row sees of a tile that not every row sees whole, while its scores are being formed
         const bool some = Work::any_hidden(sh, t, row, key0);
         unsigned long long seen = ~0ull;
-        if (some && warp_ok) seen = row_ok ? Work::seen_keys(p.a, t, Work::row_of(p.a, t, row), key0) : 0ull;
+        if (some && warp_ok) seen = row_ok ? Work::seen_keys(p.a, t, row, key0) : 0ull;
         // the tile's scores; and the group's previous O[g] += P V has to be complete before O[g] is rescaled and P[g] rewritten (no
         // arrival for a tile comes before every warp's for the one before has been counted)
         if (!__all_sync(0xffffffffu, j == 0 ? mbar_wait(&s_full[g], count & 1)
@@ -784,7 +770,7 @@ rows_attn_tcgen05_kernel(const __grid_constant__ Params<Work> p, const __grid_co
         if (__all_sync(0xffffffffu, mbar_wait(&o_done[g], (count - 1) & 1))) {
           if (odd_share[g] == share && warp_ok) {  // (every warp of the group has arrived for that product)
             tc_fence_after();
-            add_odd_values(p, t, g, 2, Work::row_of(p.a, t, row), row_ok, o_addr);
+            add_odd_values(p, t, g, 2, row, row_ok, o_addr);
             __syncwarp();
             ask_queries(next, brings && next.seq >= 0, x);  // (asked for again: they need not live through the call)
           }

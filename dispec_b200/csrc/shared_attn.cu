@@ -237,6 +237,7 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   if (tensor_cores) {
     typedef int (*Kernel)(const DspSharedAttention*, cudaStream_t);
     int rc = 0;
+    a.beside = use_many;
     if (use_many) {
       DspSharedAttention x = a;
       x.sh = many.sh;
@@ -253,7 +254,8 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   }
   // threads that share a row and head: one for eight of the parts that a shared part's item may have, by the CTAs that there are for
   // each and by its key tiles
-  const long quads = D / 4, row_heads = R * columns / D, parts = min(ctas / min(groups * KVH, ctas), (long)a.sh.most_ctx / KEYS_PER_TILE);
+  const long quads = D / 4, row_heads = R * columns / D, of_part = use_many ? many.ctas : ctas,
+             parts = min(of_part / min(groups * KVH, of_part), (long)a.sh.most_ctx / KEYS_PER_TILE);
   int share = 1;
   while (quads * share * 2 <= COMBINE_THREADS && share * 16 <= parts) share *= 2;
   const long of_block = COMBINE_THREADS / (quads * share);

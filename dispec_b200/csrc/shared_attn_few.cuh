@@ -308,7 +308,9 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
     for (int k = 0; k < 8; ++k) mbar_init(&known[k], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_wait();
+  // Behind the kernel for many rows, which was behind its own wait when this one began, nothing that is read here is still being written,
+  // and the results lie apart: the wait is for the end (the merge waits for this kernel alone).
+  if (!p.a.beside) pdl_wait();
   shared::make_plan(sh, *reinterpret_cast<shared::Groups*>(ring), run, blockIdx.x, gridDim.x);
   fence_async_smem();  // (the ring's memory was written by threads, and TMA writes it next)
   __syncthreads();
@@ -394,6 +396,7 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
       mbar_arrive(&known[share & 7]);
     }
     pdl_launch_dependents();
+    if (p.a.beside) pdl_wait();
     if (!ok) {
       if (lane == 0) atomicOr(p.a.err, DSP_ERR_WAIT_LIMIT);
       // let copies that are still on their way land before the shared memory goes away

@@ -85,6 +85,7 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
+  pdl_launch_dependents();  // (the other kernel's CTAs begin where these end, and do not wait for them)
   shared::make_plan(sh, plan.groups, plan.run, blockIdx.x, gridDim.x);  // (meets)
   tc_fence_before();
   __syncthreads();
@@ -173,7 +174,6 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
       shares[share % KNOWN].seq = -1;
       mbar_arrive(&known[share % KNOWN]);
     }
-    pdl_launch_dependents();
   } else if (warp <= 2) {
     // ---- products of row tile g
     const int g = warp - 1;

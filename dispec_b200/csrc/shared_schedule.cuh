@@ -9,7 +9,7 @@
 // runs, one per CTA, wherever that falls, so that few long beginnings load every SM as well as many short sequences, and nothing
 // about lengths is needed on the host.
 //
-// Two kernels may share the work: beginnings with more than `many` rows a head go to one whose tiles have 128 rows, the rest to
+// Two kernels may share the work: beginnings with more than `many` rows a head go to one whose tiles have 256 rows, the rest to
 // one with smaller tiles.  Where all beginnings of the first have R row tiles, teams of R CTAs walk the same keys with one row
 // tile each, which then come from memory once and from the L2 for the others.
 //
@@ -386,6 +386,7 @@ struct DspSharedAttention {
   long q_stride, out_stride;
   int pt_stride, table_width, D, page_size, num_pages, ctas;
   float scale;
+  int beside;  // the kernel for few rows is launched behind the one for many
   int* err;
 };
 
@@ -415,10 +416,6 @@ struct SharedWork {
     const int length = a.sh.length(node);
     return {max(t.from, a.sh.window > 0 ? length - a.sh.window : 0), min(t.end, length)};
   }
-  // what a softmax thread keeps of its row through a share: few tiles are not seen whole, and its length is read again for them
-  static __device__ __forceinline__ int keep_row(const Args&, const Share&, int node) { return node; }
-  static __device__ __forceinline__ Row row_of(const Args& a, const Share& t, int node) { return row(a, t, node); }
-  static __device__ __forceinline__ bool any_hidden(const Shape& sh, const Share& t, int, int key0) { return !whole(sh, t, key0); }
   static __device__ __forceinline__ unsigned long long seen_keys(const Args&, const Share&, const Row& row, int key0) {
     const int lo = max(row.lo - key0, 0), n = min(row.hi - key0, KEYS_PER_TILE) - lo;  // bits lo .. lo + n - 1
     return n <= 0 ? 0ull : n >= 64 ? ~0ull : ((1ull << n) - 1ull) << lo;

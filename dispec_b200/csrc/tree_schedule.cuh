@@ -320,9 +320,6 @@ struct TreeWork {
     return key0 <= t.ctx - KEYS_PER_TILE && (sh.window <= 0 || key0 > t.ctx + t.n - 1 - sh.window);
   }
   static __device__ __forceinline__ Row row(const Args& a, const Share&, int node) { return {node, a.sh.window > 0 ? a.depth[node] : 0}; }
-  // what a softmax thread keeps of its row through a share: all of it
-  static __device__ __forceinline__ Row keep_row(const Args& a, const Share& t, int node) { return row(a, t, node); }
-  static __device__ __forceinline__ Row row_of(const Args&, const Share&, const Row& row) { return row; }
   // by a whole warp: a row of it may not see every key of the tile
   static __device__ __forceinline__ bool any_hidden(const Shape& sh, const Share& t, const Row& row, int key0) {
     return key0 > t.ctx - KEYS_PER_TILE || (sh.window > 0 && __any_sync(0xffffffffu, key0 < t.ctx + row.depth - sh.window + 1));
