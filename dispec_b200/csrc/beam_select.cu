@@ -359,6 +359,7 @@ beam_groups_kernel(const Args a) {
   __shared__ int found, opened;
   __shared__ Candidate best_of_warp[WARPS], taken;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, group = blockIdx.x;
+  if (a.rows == 0) pdl_wait();  // (else the kernel in front was behind its own wait when this one began)
   const int first = a.group_start[group], end = a.group_start[group + 1];
   int* parent = a.parent + (size_t)group * n;
   int* token = a.token + (size_t)group * n;
@@ -576,7 +577,7 @@ extern "C" int dsp_beam_select(const DspTensor* t, cudaStream_t stream) {
   const int sms = dsp_num_sms();
   const long pieces = (V + PIECE - 1) / PIECE, most_ctas = (sms > 0 ? sms : 1) * PIECES_CTAS;
   const long run = max((R * pieces + most_ctas - 1) / most_ctas, 1L), ctas = (R * pieces + run - 1) / run;
-  SELECT_REQUIRE(R * pieces <= 0x7fffffff, "%ld rows of %ld logits are too many for one call", R, V);
+  SELECT_REQUIRE(R * pieces <= 1 << 30, "%ld rows of %ld logits are too many for one call", R, V);
   Args a = {};
   const long need = layout(a, (float*)scratch.data, R, pieces, ctas, n);
   SELECT_REQUIRE(scratch.contiguous && scratch.device == logits.device && scratch.dims == 1 && scratch.dtype == DSP_T_F32 &&

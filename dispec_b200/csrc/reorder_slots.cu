@@ -133,7 +133,7 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
   REORDER_REQUIRE(tensor_is(src, DSP_T_I32, src.device, 1, n) && tensor_is(dst, DSP_T_I32, src.device, 1, n),
                   "src and dst must be contiguous int32 of one length on one device");
   Args a = {};
-  uintptr_t bits = 0;
+  uintptr_t bits = 0, ends[MAX_POOLS];
   const DspTensor& first = t[2];
   for (long p = 0; p < pools; ++p) {
     const DspTensor& x = t[2 + p];
@@ -147,8 +147,10 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
     a.pools[p].slots = (int)x.size[1];
     REORDER_REQUIRE(x.size[1] <= 0x7fffffff, "pool %ld has too many slots", p);
     bits |= (uintptr_t)x.data | (uintptr_t)a.pools[p].row_bytes;
+    const uintptr_t at = (uintptr_t)x.data;
+    ends[p] = at + (uintptr_t)(x.size[0] * x.size[1] * a.pools[p].row_bytes);
     for (long o = 0; o < p; ++o)
-      REORDER_REQUIRE(a.pools[o].data != a.pools[p].data || a.pools[p].row_bytes == 0, "pools %ld and %ld are the same memory", o, p);
+      REORDER_REQUIRE(at >= ends[o] || ends[p] <= (uintptr_t)a.pools[o].data, "pools %ld and %ld have parts of the same memory", o, p);
   }
   if (n == 0) return 0;
   // the widest pieces that all rows consist of; as much of an entry in a block as it can hold

@@ -7,7 +7,7 @@
 // A sum over keys may be taken in parts: with m the largest score of a part, l = sum exp(s_j - m) and a = sum exp(s_j - m) v_j, parts
 // join as  M = max m,  o = sum a exp(m - M) / sum l exp(m - M).  So the shared keys are read once for all sequences of a group,
 // whose rows fill the tiles of a matrix product, and each sequence's own keys once for its G rows.  A row that sees nothing gives 0.
-// The work is cut as shared_schedule.cuh says; the kernels: shared_attn_few.cuh, rows_attn_tcgen05.cuh where many rows share keys,
+// The work is cut as shared_schedule.cuh says; the kernels: shared_attn_few.cuh, shared_attn_many.cuh where many rows share keys,
 // rows_attn.cuh in 32-bit arithmetic.
 #include "merge_parts.cuh"
 #include "rows_attn.cuh"
@@ -23,10 +23,11 @@ constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
 // where 16 take 1.3).  (256 sequences behind shared parts of 2,050, 28 heads of 128 on 4: 105.7, 103.7, 100.4 and 100.8 us with 0 to 3 for
 // the kernel for few rows; 8 groups of 5 behind 4,101: 39.7, 33.9, 31.1, 32.0.  In 32 bits a key tile takes 8 us, and nothing is
 // small beside it: 2 groups of 5 behind 701, 12 heads on 2: 21.6, 25.2, 32.2.)
-// A kernel more is some 17 us more: one group of 224 rows a head of 128, 4 heads, shared parts of 4,000, 8,000 and 32,000 tokens: 48, 50
-// and 70 us with both kernels, 38, 51 and 119 with the one for few alone; of 112 rows 8,000 and 32,000: 46 and 63, 43 and 80; of
-// 320 rows, 8 heads, 4,000, 8,000 and 32,768: 74, 78 and 121, 64, 84 and 213.
-constexpr long MANY_UNITS = 16;
+// A kernel more is some 7 us more, which so many of its tiles an SM repay.  One group of 16 and 64 sequences of 28 heads on 4, and of
+// 40 of 64 on 8, heads of 128, with both kernels and with the one for few alone: shared parts of 4,000 tokens (3.4, 11.9 and 17.0 tiles
+// an SM) 25.2, 39.7 and 43.0 us and 21.3, 39.2 and 48.6; of 8,000 26.2, 43.6 and 50.6 and 28.1, 65.1 and 72.1; of 32,000 39.3, 69.8
+// and 94.2 and 55.2, 160.5 and 211.9.  8 groups of 16 with 28 heads: 1,000 tokens (6.1) 37.3 and 35.2, 2,000 (12.1) 39.1 and 43.5.
+constexpr long MANY_UNITS = 12;
 constexpr int EXTRA_FEW = 2, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
 
 // Joins a row's partial results: `quads` neighbouring threads have four columns each of a row and head, and where rows are few, so many
@@ -166,8 +167,8 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
                  "ctx_len [%ld], group_start [%ld] and prefix_len [%ld] must be contiguous int32 on the device of q", R, groups + 1, groups);
   SHARED_REQUIRE(is_page_table(table, q.device, R), "page_table must be int32 [%ld, pages], neighbouring pages side by side", R);
   SHARED_REQUIRE(out.dtype == q.dtype && out.device == q.device && out.dims == 2 && out.size[0] == R && out.size[1] == columns &&
-                     (R == 0 || out.stride[1] == 1 || columns == 1),
-                 "out must be like the queries [%ld, %ld] with neighbouring columns", R, columns);
+                     (R == 0 || out.stride[1] == 1 || columns == 1) && (R <= 1 || out.stride[0] >= columns),
+                 "out must be like the queries [%ld, %ld] with neighbouring columns, no two rows in one place", R, columns);
   SHARED_REQUIRE(R <= 0x7fffffff && pages <= 0x7fffffff && page >= 1 && page <= 0x7fffffff && o->sms >= 1 && table.stride[0] <= 0x7fffffff,
                  "sizes out of range");
   if (R == 0 || groups == 0) return 0;

@@ -61,8 +61,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     what = "shared_prefix_attention"
     if not q.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")
-    if q.dim() != 2 or k_pool.dim() != 4:
-        _refuse(what, "q [R, H * D] and two pools [pages, heads, page_size, D] expected")
+    if q.dim() != 2 or k_pool.dim() != 4 or page_table.dim() != 2:
+        _refuse(what, "q [R, H * D], two pools [pages, heads, page_size, D] and a page_table [R, pages of a sequence] expected")
     if out is None:
         out = q.new_empty(q.shape)
     dev = q.get_device()
@@ -76,7 +76,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     tile, ctas = (64, 2 * sms) if tensor_cores else (32, sms * (1 if dim > 128 else 2))
     items = (rows * share // tile + groups + 1 + rows * -(-share // tile)) * kv_heads + 1
     rest = ctas * tile * (dim + 2) + items
-    many = tensor_cores and rows * share > 64 * groups  # (it may be)
+    # (the rule by which the kernel for many rows is taken as well: csrc/shared_attn.cu)
+    many = tensor_cores and rows * share > 64 * groups and (
+        -(-rows * share // 64) * kv_heads * (page_table.shape[1] * page // 64 + 1) > 12 * sms)
     if many:
         rest += sms * 256 * (dim + 2) + (rows * share // 256 + groups + 1) * kv_heads + 1
     scratch = prefix_len.new_empty(2 * (rows * kv_heads * share * (dim + 2) + rest))
@@ -127,7 +129,8 @@ def reorder_slots(pools: list, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Slots of caches or states follow a choice, in place: ``pool[:, dst[i]] = pool[:, src[i]]`` for all i and every pool, as
     though all were read before any is written (a slot may be read by several and written by another).
 
-    ``pools``: up to 64 contiguous tensors [layers, slots, ...] of three to five dimensions with the same number of slots;
+    ``pools``: up to 64 contiguous tensors [layers, slots, ...] of three to five dimensions, float32, bfloat16, int32 or int64,
+    with the same number of slots and no memory in common;
     ``src``, ``dst`` int32 [n], n up to 8,192, ``dst`` ascending: what does not ascend, or names a slot that is not there, is
     left from there on and recorded as a device error."""
     what = "reorder_slots"

@@ -51,6 +51,9 @@ def test_attention_types_sizes_and_options_are_refused():
     assert "int32" in attention(prefix=described(I64, (1,)))
     assert "page_table" in attention(table=(2, 8)) and "page_table" in attention(table=(3, 8, 1))
     assert "like the queries" in attention(out=described(BF16, (3, 32)))
+    assert "two rows in one place" in attention(out=described(F32, (3, 32), (0, 1), contiguous=0))
+    assert "two rows in one place" in attention(out=described(F32, (3, 32), (16, 1), contiguous=0))
+    assert "scratch" in attention(q=described(F32, (3, 32), (0, 1), contiguous=0))
     assert "16 bytes" in attention(q=described(F32, (3, 32), data=(1 << 20) + 4))
     assert "16 bytes" in attention(q=described(F32, (3, 32), (33, 1), contiguous=0))
 
@@ -101,5 +104,9 @@ def test_reorder_refusals():
     assert "three to five" in reorder([described(BF16, (2, 8))]) and "three to five" in reorder([described(-1, (2, 8, 4))])
     assert "three to five" in reorder([described(BF16, (2, 8, 4), (64, 8, 2))]) and "three to five" in reorder([described(BF16, (2, 8, 4), device=1)])
     assert "slots" in reorder([good, described(BF16, (2, 9, 4, 16), data=1 << 22)])
+    behind = described(BF16, (2, 8, 4, 16), data=(1 << 20) + 2 * 8 * 4 * 16 * 2)
+    inside = described(BF16, (2, 8, 4, 16), data=(1 << 20) + 8 * 4 * 16 * 2)
+    assert "current device" in reorder([good, behind]) and "current device" in reorder([behind, good])
+    assert "same memory" in reorder([good, inside]) and "same memory" in reorder([inside, behind])
     assert "one length" in reorder([good], src=described(I32, (3,))) and "one length" in reorder([good], dst=described(I64, (2,)))
     assert "8192" in reorder([good], n=8193)

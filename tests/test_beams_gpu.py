@@ -22,6 +22,53 @@ def i32(v):
 
 
 # ------------------------------------------------------------------------------------- attention
+def long_pages(table):
+    """Places for so many tokens more that the kernel for many rows a key is taken where there are such."""
+    return torch.nn.functional.pad(table, (0, 1600), value=-1)
+
+
+@pytest.mark.parametrize("groups", [[(300, [301 + j % 5 for j in range(70)])], [(130, [131] * 40), (700, [701] * 40), (64, [90] * 40)],
+                                    [(900, [905] * 60), (200, [201, 210]), (70, [80] * 33), (5, [300])],
+                                    [(90, [100] * 17 + [0, 40] * 9)] * 2, [(1, [2] * 70)], [(5000, [5001] * 33)], [(63, [64] * 64)],
+                                    [(64, [63] * 65), (0, [5] * 65), (129, [0] * 65)]])
+@pytest.mark.parametrize("dim,window,page_size,scatter", [(128, 0, 16, True), (64, 0, 16, True), (128, 60, 16, True), (64, 130, 16, False),
+                                                          (128, 0, 8, True), (128, 0, 64, False), (64, 90, 32, True)])
+def test_attention_kernel_for_many_rows(groups, dim, window, page_size, scatter):
+    case = SharedCase(groups, 8, 2, dim, BF16, window=window, page_size=page_size, scatter=scatter)
+    case.table = long_pages(case.table)
+    case.check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(7, 1), (16, 1), (28, 4), (64, 8), (65, 1), (3, 3)])
+def test_attention_head_layouts_of_many_rows(heads, kv_heads):
+    case = SharedCase([(200, [203] * 90), (500, [501, 560] * 50)], heads, kv_heads, 128, BF16)
+    case.table = long_pages(case.table)
+    case.check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_hidden_keys_of_many_rows_may_be_anything(bad, window, dim):
+    """What a row does not see does not reach it; a value that is not finite reaches the rows that see it."""
+    case = SharedCase([(230, [231, 300, 200, 105] * 20)], 8, 2, dim, BF16, window=window)
+    case.table = long_pages(case.table)
+    want, bound = case.plain()
+    hidden = 202  # behind the last key of half of the sequences, in the part that the others see
+    page, o = int(case.table[0, hidden // 16]), hidden % 16
+    sees = torch.tensor([any(j == hidden for _, j in case.keys(0, r)) for r in range(80)])
+    assert sees.any() and not sees.all()
+    case.v[page, :, o] = bad
+    got = case.run().double().cpu()
+    assert ((got - want).abs() <= bound)[~sees].all() and not torch.isfinite(got[sees]).any()
+    case.k[page, :, o] = bad
+    got = case.run().double().cpu()
+    assert ((got - want).abs() <= bound)[~sees].all()
+    no_device_error()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("groups", [[(0, [1])], [(1, [1, 1])], [(0, [0, 1, 0])], [(64, [65, 64, 70])], [(63, [64, 65]), (65, [66, 130, 65])],
                                     [(100, [101]), (100, [101, 140])], [(40, [30, 50, 0, 40])], [(100, [0, 0]), (7, [9, 8])],
@@ -211,6 +258,68 @@ def test_attention_lengths_beyond_the_pages_are_cut():
     assert ops.device_error() == 1  # (the table is three places wider than the pages that are there: their keys are hidden)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("bad", [-2, -2 ** 31, 2 ** 31 - 1])
+def test_attention_pages_of_any_number_are_reported(dtype, bad):
+    """In the shared part of many rows, in that of few, and in a sequence's own: the other rows keep their results."""
+    from dispec_b200 import ops
+    case = SharedCase([(700, [720] * 70), (90, [100, 101]), (0, [40])], 8, 2, 128, dtype)
+    case.table = long_pages(case.table)
+    want = case.run()
+    for row, page, spoilt in ((0, 3, range(70)), (70, 2, (70, 71)), (72, 1, (72,)), (71, 6, (71,))):
+        table = case.table.clone()
+        case.table[row, page] = bad
+        got = case.run()
+        case.table = table
+        rest = [r for r in range(73) if r not in spoilt]
+        assert ops.device_error() == 1 and torch.isfinite(got).all() and torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("groups,heads,kv_heads,dim", [([(16000, [16010, 16001])], 2, 1, 128), ([(11, [12, 9000, 14, 11])], 4, 1, 64),
+                                                       ([(9000, [9001])], 1, 1, 32), ([(7000, [7040] * 70)], 2, 1, 64)])
+def test_attention_items_of_many_parts(dtype, groups, heads, kv_heads, dim):
+    """A row's partial results come from many CTAs, and several threads join them."""
+    SharedCase(groups, heads, kv_heads, dim, dtype).check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_calls_behind_and_beside_one_another(dtype):
+    """Calls of few and of many rows in turn, without a pause, in a graph, and on two streams at once."""
+    from dispec_b200 import ops
+    cases = [SharedCase([(900, [905 + j % 7 for j in range(70)])], 8, 2, 128, dtype, seed=1), SharedCase([(300, [310, 305])], 8, 2, 128, dtype, seed=2),
+             SharedCase([(640, [700] * 40), (900, [901] * 30)], 8, 2, 128, dtype, seed=3)]
+    calls = []
+    for case in cases:
+        q, k, v, table, lens, starts, prefix = case.tensors()
+        table = long_pages(table)
+        calls.append(lambda t=(q, k, v, table, lens, starts, prefix), c=case: ops.shared_prefix_attention(*t, scale=c.scale))
+    want = []
+    for call in calls:
+        want.append(call())
+        torch.cuda.synchronize()
+    turns = [0, 1, 2, 1, 0, 2] * 3
+    got = [calls[i]() for i in turns]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for n, i in enumerate(turns):
+        with torch.cuda.stream(sides[n % 2]):
+            got.append(calls[i]())
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            got += [calls[i]() for i in turns]
+    for _ in range(2):
+        for graph, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for x, i in zip(got, turns * 4))
+    no_device_error()
+
+
 def test_attention_refusals():
     from dispec_b200 import ops
     from dispec_b200.ops import KernelError
@@ -365,6 +474,19 @@ def test_select_same_bits_again_in_a_graph_and_on_another_stream():
     again = call()
     torch.cuda.synchronize()
     assert torch.equal(again.token, third.token) and not torch.equal(again.token, first.token)
+
+
+def test_select_without_rows_follows_what_comes_before_it():
+    """The groups are read when the kernels in front have written them."""
+    from dispec_b200 import ops
+    logits, scores = random_choice(64, 40001, seed=8)
+    logits, scores = logits.to(DEV), scores.to(DEV)
+    starts = i32([0, 32, 64])
+    for _ in range(20):
+        first = ops.beam_select(logits, scores, starts, count=8)
+        none = ops.beam_select(logits[:0], scores[:0], first.parent[0, :3] * 0, count=8)
+        assert (none.parent == -1).all() and (none.token == -1).all() and (none.score == -math.inf).all()
+    no_device_error()
 
 
 @pytest.mark.parametrize("starts", [[0, 3, 2, 4], [-1, 2, 3, 4], [0, 2, 3, 9]])
