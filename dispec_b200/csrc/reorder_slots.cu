@@ -2,8 +2,11 @@
 //     pool[:, dst[i]] = pool[:, src[i]]   for all i, as though all were read before any is written.
 //
 // Bytes of different columns have nothing to do with each other.  So a block takes some columns of one layer of one pool for
-// ALL i: it holds them in registers, eight pieces a thread, meets, and writes them.  A slot may be read by several and
+// ALL i: it holds them in shared memory or in registers, meets, and writes them.  A slot may be read by several and
 // written by another in one call, in place and without a copy of anything, and no block waits for another.
+//
+// Memory bounds it: 906 MB in rows of 32 KB (48 layers of keys and values, read and written) take 161 us, 151 MB in rows of 512 KB
+// (12 layers of states) 25.6: 5.6 and 5.9 TB/s.
 //
 // dst ascends, so that no slot is written twice; what does not ascend, or names a slot that is not there, is left from there on
 // and recorded.
@@ -48,7 +51,8 @@ __device__ __forceinline__ int sound_entries(const Args& a, const Pool& pool, in
 }
 
 // Rows of whole 16-byte pieces and up to BULK_ENTRIES entries: the columns of an entry are one bulk copy into shared memory and one
-// back.
+// back (of 96 bytes at least).  The same copies through registers, eight pieces a thread, take 203 and 32.7 us where these take 161 and
+// 25.6; more entries, and rows of other sizes, go that way.
 constexpr int BULK_THREADS = 128, BULK_ENTRIES = 512, BULK_BYTES = 48 * 1024;
 __global__ void __launch_bounds__(BULK_THREADS)
 reorder_bulk_kernel(const __grid_constant__ Args a) {

@@ -7,10 +7,17 @@
 // where pages follow one another), and while one is between two shares the other one reads.  A warp requests, four work:
 // of 16, 32 or 64 rows (MT = 1, 2, 4 row tiles of 16) warp w has row tile w % MT and 16 MT of a tile's keys, with a running
 // maximum, sum and accumulator of its own, so that no warp waits for another inside a share; at its end the 4 / MT warps
-// of a row tile join theirs.  The products are mma.sync m16n8k16: 64 rows and keys take 1,024 cycles of an SM's tensor pipe
-// where their tile takes 1,400 from memory, and sixteen rows would leave seven eighths of a tcgen05 tile of 128 empty, which
-// puts its rows through tensor memory and the whole block through a barrier for every share (5.6 us a share of one tile; 128
-// sequences of 1,000 tokens ...).
+// of a row tile join theirs.  The products are mma.sync m16n8k16 (8 cycles each): 64 rows and keys take 1,024 cycles of an SM's
+// tensor pipe where their tile takes 1,400 from memory, and sixteen rows would leave seven eighths of a tcgen05 tile of 128 empty,
+// which puts its rows through tensor memory and the whole block through a barrier for every share.
+//
+// What bounds it: with sixteen rows the way from memory once it is full (148 sequences of 1,000 tokens, 28 heads of 128 on 4: 303 MB
+// in 58 us behind 6 us in which the runs are found, 5.2 TB/s; 1,150 cycles a tile and CTA are work), with 33 to 64 rows its own
+// instructions (3,100 cycles a tile and CTA for 35, 3,750 for 64: products 1,024, reads of keys and values by every row tile 1,024,
+// the softmax between them): 8 groups of 5 behind 4,101 tokens, 28 heads on 4: 30.9 us, 70 MB.  In calls this short the beginnings
+// count: 3.7 us until the runs are found, 3.5 until the first tile is there, 3 for the first steps' instructions.
+// Tried and not kept: all 64 keys of a tile in one step (the same 3,750 cycles, and spills), fragments loaded a step ahead of
+// their products (3,900).
 #pragma once
 #include "shared_schedule.cuh"
 #include "rows_attn_tcgen05.cuh"
@@ -417,6 +424,7 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
     const bool ended = !ok || t.seq < 0;
     const int row0 = t.row_tile << FEW_SHIFT, nrows = min(FEW_ROWS, t.n * G - row0), head = t.head;
     const int MT = nrows <= 16 ? 1 : nrows <= 32 ? 2 : 4;
+    const bool has_rows = (warp & (MT - 1)) * 16 < nrows;  // (of a warp with a fourth row tile, of 48 rows, none)
     const int part = warp / MT, at_row = (warp & (MT - 1)) * 16 + gid;  // of the tile's rows: this one and the eighth behind it
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -450,7 +458,7 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
         const Tile tl = {k_s, v_s, key0, bad, ragged};
         if (MT == 1)
           few_step<1>(tl, t, part, page_shift, scale, q, lo, hi, o, m, l);
-        else
+        else if (has_rows)
 #pragma unroll 1
           for (int block = part * MT; block < (part + 1) * MT; block += 2)
             few_step<2>(tl, t, block, page_shift, scale, q, lo, hi, o, m, l);
