@@ -203,6 +203,7 @@ def build_all(head_dims=(16, 32, 64, 128)) -> list[str]:
         if d in (64, 128):
             libs.append(prefill_attention_library(d))
             libs.append(tree_attention_library(d))
+        if d in (32, 64, 128):
             libs.append(shared_attention_library(d))
     libs += [mixer_library(name) for name in MIXER_LIBRARIES]
     # the attention with widths of their own for keys and values is compiled per pair of widths

@@ -27,20 +27,11 @@
 // some; that was not tried).
 #pragma once
 #include "packed2.cuh"
-#include "tcgen05_common.cuh"
-
-#ifndef DSP_HEAD_DIM
-#error "compile with -DDSP_HEAD_DIM=<head size>"
-#endif
-#define DSP_CAT2(a, b) a##b
-#define DSP_CAT(a, b) DSP_CAT2(a, b)
+#include "paged_tile.cuh"
 
 namespace {
-using namespace tc;
-
-constexpr int D = DSP_HEAD_DIM;
 static_assert(D == 64 || D == 128, "this kernel is built for head sizes 64 and 128");
-constexpr int BM = 1 << ROW_SHIFT_TENSOR_CORES, BN = KEYS_PER_TILE, THREADS = 384;
+constexpr int BM = 1 << ROW_SHIFT_TENSOR_CORES, THREADS = 384;
 // Key tiles of a share go to two issuing warps in turn, and each waits for its own tiles only.  With an even ring the tiles of a
 // share in one slot all belong to one of them; with an odd one a warp that is ahead (its tile landed, an older one of the
 // other's has not) could take the slot's last phase but one for the phase it waits for.  From share to share a slot may change
@@ -52,12 +43,6 @@ constexpr int SHARES = 4;      // the shares remembered: the next two, the prese
 constexpr int BAD_SLOTS = 16;  // a tile's unreadable pages are remembered until its softmax has begun
 static_assert(BAD_SLOTS >= K_STAGES + 4, "a slot is rewritten K_STAGES + 4 tiles later at the earliest");
 constexpr int PV_WARP = 10, S1_WARP = 11;
-constexpr int KD = D / 64;
-// A tile in shared memory lies as the pages are brought (tcgen05_common.cuh): [group of 8 keys][slice of 64 columns][8 rows of 128
-// bytes], a page's rows in one TMA request.
-constexpr int SLICE = KEY_SLICE;
-constexpr int GROUP = KD * SLICE;
-constexpr int KV_BYTES = BN / 8 * GROUP;
 constexpr int SMEM_BYTES = (K_STAGES + V_STAGES) * KV_BYTES + 1024;
 // tensor memory, 32-bit columns
 constexpr int S_COLS = BN;
@@ -72,13 +57,7 @@ static_assert(Q_COL + D / 2 <= TMEM_COLS, "tensor memory layout");
 // 8 trees of 16 the same with both.  The larger call decides.  The result's error is the same to four digits (2.305e-3 of its size
 // against 64 bits, 2.342e-3 behind 32,768).  Heads of 64, with half of the products to a weight: no difference, none.
 constexpr int EX2_FMA = D == 128 ? 2 : 0;
-constexpr float RESCALE_STEP = 8.f;  // the running maximum follows the true one in steps of 2^8
 
-// Two bfloat16 values: one that is not finite; the same with 0 in its place.
-__device__ __forceinline__ bool has_odd(uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
-__device__ __forceinline__ uint32_t without_odd(uint32_t x) {
-  return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
-}
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");

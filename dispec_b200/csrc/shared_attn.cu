@@ -143,7 +143,7 @@ struct DspSharedOptions {  // as ops/beams.py packs them
   double scale;
 };
 
-// Addresses of the tensor-core kernels' entry points for this head size, or 0: `few`, `many`.
+// Addresses of the tensor-core kernels' entry points for this head size, or 0: `few`, `many` (heads of 32 have none).
 // tensors: q, key pool, value pool, page table, ctx_len, group_start, prefix_len, out, scratch.
 extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* o, cudaStream_t stream) {
   const DspTensor &q = t[0], &k = t[1], &v = t[2], &table = t[3], &ctx = t[4], &start = t[5], &prefix = t[6], &out = t[7], &scratch = t[8];
@@ -176,7 +176,7 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   const long piece = q.dtype == DSP_T_F32 ? 4 : 8;  // elements of 16 bytes
   SHARED_REQUIRE(bits % 16 == 0 && (R == 1 || (q.stride[0] % piece == 0 && out.stride[0] % piece == 0)), "rows must begin on 16 bytes");
   // the tensor-core kernels are built for these page sizes; everything else takes the 32-bit kernel
-  const bool tensor_cores = o->few != 0 && o->many != 0 && q.dtype == DSP_T_BF16 && (D == 64 || D == 128) &&
+  const bool tensor_cores = o->few != 0 && q.dtype == DSP_T_BF16 && (D == 32 || D == 64 || D == 128) &&
                             (page == 8 || page == 16 || page == 32 || page == 64) && pages > 0;
   const long ctas = o->sms * (tensor_cores ? FEW_CTAS : D > 128 ? 1 : 2);  // (by shared memory two CTAs an SM)
   DspSharedAttention a = {};
@@ -195,7 +195,7 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   // Where groups have more rows a head on average than a tile of the kernel for few, and their shared parts may be so long (as long
   // as their pages) that each SM has MANY_UNITS of its tiles or more, the shared parts of those that do are the other kernel's.
   const long units = (R * a.sh.G + FEW_ROWS_OF_A_TILE - 1) / FEW_ROWS_OF_A_TILE * KVH * (table.size[1] * page / KEYS_PER_TILE + 1);
-  const bool use_many = tensor_cores && R * a.sh.G > groups * FEW_ROWS_OF_A_TILE && units > MANY_UNITS * o->sms;
+  const bool use_many = tensor_cores && o->many != 0 && R * a.sh.G > groups * FEW_ROWS_OF_A_TILE && units > MANY_UNITS * o->sms;
   a.sh.many = use_many ? FEW_ROWS_OF_A_TILE : 0x7fffffff;
   // places are counted in 32 bits, a tile of keys beyond the last among them
   a.sh.most_ctx = (int)min(table.size[1] * page, 1L << 30);

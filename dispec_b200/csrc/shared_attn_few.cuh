@@ -1,6 +1,6 @@
 // Attention of sequences with a shared beginning where few rows meet a key: each sequence's own keys (G rows), and shared
 // beginnings of few sequences.  bfloat16 in, 32-bit softmax and accumulation (the formula: shared_attn.cu; how the work is cut:
-// shared_schedule.cuh).  Compiled once per head size (-DDSP_HEAD_DIM=64 or 128).
+// shared_schedule.cuh).  Compiled once per head size (-DDSP_HEAD_DIM=32, 64 or 128).
 //
 // Such a share is its keys' way from memory: 512 bytes a key and head of 128, for up to 64 rows.  So two CTAs an SM keep a ring
 // of key tiles on its way that runs on from share to share (tiles of 64 keys, requested by TMA page by page, or in one request
@@ -16,11 +16,14 @@
 // instructions (3,100 cycles a tile and CTA for 35, 3,750 for 64: products 1,024, reads of keys and values by every row tile 1,024,
 // the softmax between them): 8 groups of 5 behind 4,101 tokens, 28 heads on 4: 30.9 us, 70 MB.  In calls this short the beginnings
 // count: 3.7 us until the runs are found, 3.5 until the first tile is there, 3 for the first steps' instructions.
+// Heads of 32, 28 on 4: those 8 groups 25.4 us (103 in 32-bit arithmetic), 148 sequences of 1,000 tokens 35.2 (185); they have no kernel for
+// many rows: 64 sequences of 40 heads on 8 behind 32,768 tokens 118 us (849).
 // Tried and not kept: all 64 keys of a tile in one step (the same 3,750 cycles, and spills), fragments loaded a step ahead of
-// their products (3,900).
+// their products (3,900), 200 registers a thread (three warps of an SM's quarter have 16,384 together: one CTA an SM, 43.6 us).
 #pragma once
 #include "shared_schedule.cuh"
-#include "rows_attn_tcgen05.cuh"
+#include "packed2.cuh"
+#include "paged_tile.cuh"
 
 namespace {
 constexpr int FEW_SHIFT = ROW_SHIFT_FEW, FEW_ROWS = 1 << FEW_SHIFT, FEW_WARPS = 4, FEW_THREADS = 32 * (FEW_WARPS + 1);
@@ -92,21 +95,22 @@ __device__ __forceinline__ void few_step(const Tile& tl, const shared::Share& t,
   {
     // (two chains of products for each eight keys where there is one block only)
     float odd[NB == 1 ? 2 : 1][4] = {};
+    constexpr int EACH = 4 / NB < D / 16 ? 4 / NB : D / 16;  // steps of 16 columns that are loaded together
 #pragma unroll
-    for (int k0 = 0; k0 < D / 16; k0 += 4 / NB) {
-      uint32_t b[NB][4 / NB][4];
+    for (int k0 = 0; k0 < D / 16; k0 += EACH) {
+      uint32_t b[NB][EACH][4];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         const int row = c0 + n * 16 + (m8 >> 1) * 8 + l8;
-        const uint32_t base = tl.k_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
+        const uint32_t base = tl.k_s + row_at(row);
 #pragma unroll
-        for (int k = 0; k < 4 / NB; ++k) {
+        for (int k = 0; k < EACH; ++k) {
           const int chunk = (k0 + k) * 2 + (m8 & 1);
-          ldmatrix4(b[n][k], base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+          ldmatrix4(b[n][k], base + piece_at(chunk, l8));
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4 / NB; ++k)
+      for (int k = 0; k < EACH; ++k)
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           mma16(NB == 1 && (k & 1) ? odd[0] : sc[2 * n], q[k0 + k], b[n][k][0], b[n][k][1]);
@@ -173,13 +177,13 @@ __device__ __forceinline__ void few_step(const Tile& tl, const shared::Share& t,
 #pragma unroll
   for (int c = 0; c < NB; ++c) {
     const int row = c0 + c * 16 + (m8 & 1) * 8 + l8;
-    const uint32_t base = tl.v_s + (uint32_t)(row >> 3) * GROUP + (uint32_t)(row & 7) * 128u;
+    const uint32_t base = tl.v_s + row_at(row);
     if (!tl.ragged) {
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
         const int chunk = n * 2 + (m8 >> 1);
         uint32_t b[4];
-        ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+        ldmatrix4_trans(b, base + piece_at(chunk, l8));
         mma16(o[2 * n], pk[c], b[0], b[1]);
         mma16(o[2 * n + 1], pk[c], b[2], b[3]);
       }
@@ -189,7 +193,7 @@ __device__ __forceinline__ void few_step(const Tile& tl, const shared::Share& t,
       for (int n = 0; n < D / 16; ++n) {
         const int chunk = n * 2 + (m8 >> 1);
         uint32_t b[4];
-        ldmatrix4_trans(b, base + (uint32_t)(chunk >> 3) * SLICE + (uint32_t)(((chunk & 7) ^ l8) << 4));
+        ldmatrix4_trans(b, base + piece_at(chunk, l8));
 #pragma unroll
         for (int j = 0; j < 4; ++j) b[j] &= j & 1 ? mask1 : mask0;
         if (mixed) {
@@ -210,13 +214,13 @@ __device__ __forceinline__ void few_step(const Tile& tl, const shared::Share& t,
       if (!((alive >> c) & 1u)) continue;
       const int key = key0 + c0 + c, at = c0 + c;
       const bool sees0 = key >= lo[0] && key < hi[0], sees1 = key >= lo[1] && key < hi[1];
-      const uint32_t line = tl.v_s + (uint32_t)(at >> 3) * GROUP + (uint32_t)(at & 7) * 128u + (uint32_t)tq * 4u;
+      const uint32_t line = tl.v_s + row_at(at) + (uint32_t)tq * 4u;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
         uint32_t x;
         asm volatile("ld.shared.u32 %0, [%1];"
                      : "=r"(x)
-                     : "r"(line + (uint32_t)(n >> 3) * SLICE + (uint32_t)(((n & 7) ^ (at & 7)) << 4))
+                     : "r"(line + piece_at(n, at & 7))
                      : "memory");
         const float x0 = __uint_as_float(x << 16), x1 = __uint_as_float(x & 0xffff0000u);
         if (!isfinite(x0)) {
@@ -424,8 +428,8 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
     const bool ended = !ok || t.seq < 0;
     const int row0 = t.row_tile << FEW_SHIFT, nrows = min(FEW_ROWS, t.n * G - row0), head = t.head;
     const int MT = nrows <= 16 ? 1 : nrows <= 32 ? 2 : 4;
-    const bool has_rows = (warp & (MT - 1)) * 16 < nrows;  // (of a warp with a fourth row tile, of 48 rows, none)
-    const int part = warp / MT, at_row = (warp & (MT - 1)) * 16 + gid;  // of the tile's rows: this one and the eighth behind it
+    const int first_block = warp / MT * MT, end_block = (warp & (MT - 1)) * 16 < nrows ? first_block + MT : 0;  // (of a row tile without rows: none)
+    const int at_row = (warp & (MT - 1)) * 16 + gid;  // of the tile's rows: this one and the eighth behind it
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -457,10 +461,10 @@ shared_attn_few_kernel(const __grid_constant__ FewParams p, const __grid_constan
         const bool ragged = bad != 0u || !SharedWork::whole(sh, t, key0);
         const Tile tl = {k_s, v_s, key0, bad, ragged};
         if (MT == 1)
-          few_step<1>(tl, t, part, page_shift, scale, q, lo, hi, o, m, l);
-        else if (has_rows)
+          few_step<1>(tl, t, first_block, page_shift, scale, q, lo, hi, o, m, l);
+        else
 #pragma unroll 1
-          for (int block = part * MT; block < (part + 1) * MT; block += 2)
+          for (int block = first_block; block < end_block; block += 2)
             few_step<2>(tl, t, block, page_shift, scale, q, lo, hi, o, m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);

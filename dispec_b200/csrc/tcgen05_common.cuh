@@ -380,13 +380,14 @@ constexpr int KEY_SLICE = 8 * 128;
 // `pages_per_box` neighbouring pages.
 inline bool make_map_pages(CUtensorMap* map, const void* base, long num_pages, int heads, int page_size, int D, int pages_per_box) {
   EncodeTiled fn = encode_fn();
-  if (fn == nullptr || D % 64 != 0 || num_pages < pages_per_box) return false;
-  cuuint64_t dims[5] = {64u, 8u, (cuuint64_t)D / 64, (cuuint64_t)heads * (page_size / 8), (cuuint64_t)num_pages};
-  cuuint64_t strides[4] = {(cuuint64_t)D * 2, 128u, (cuuint64_t)8 * D * 2, (cuuint64_t)heads * page_size * D * 2};
-  cuuint32_t box[5] = {64u, 8u, (cuuint32_t)D / 64, (cuuint32_t)(page_size / 8), (cuuint32_t)pages_per_box};
+  const cuuint32_t columns = D == 32 ? 32u : 64u;  // of a slice: heads of 32 have one of half the width
+  if (fn == nullptr || D % columns != 0 || num_pages < pages_per_box) return false;
+  cuuint64_t dims[5] = {columns, 8u, (cuuint64_t)D / columns, (cuuint64_t)heads * (page_size / 8), (cuuint64_t)num_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)D * 2, columns * 2u, (cuuint64_t)8 * D * 2, (cuuint64_t)heads * page_size * D * 2};
+  cuuint32_t box[5] = {columns, 8u, (cuuint32_t)D / columns, (cuuint32_t)(page_size / 8), (cuuint32_t)pages_per_box};
   cuuint32_t elem[5] = {1, 1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, D == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // `group`: of the pool's head's first group of 8 keys in its page

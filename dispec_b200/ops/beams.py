@@ -36,7 +36,9 @@ def _tensor_core_call(dim: int) -> tuple:
     calls = _tensor_core_calls.get(dim)
     if calls is None:
         lib = L.shared_attention_library(dim)
-        calls = tuple(L.address_of(lib, f"dsp_shared_attention_{rows}_d{dim}") for rows in ("few", "many"))
+        # (heads of 32 have no kernel for many rows)
+        calls = tuple(L.address_of(lib, f"dsp_shared_attention_{rows}_d{dim}") if rows == "few" or dim >= 64 else 0
+                      for rows in ("few", "many"))
         _tensor_core_calls[dim] = calls
     return calls
 
@@ -69,7 +71,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     (rows, columns), (_, kv_heads, page, dim) = q.shape, k_pool.shape
     sms = tuning._sm_count.get(dev) or tuning.sm_count(dev)
     # the tensor-core kernels are built for these head sizes and pages
-    tensor_cores = q.dtype is torch.bfloat16 and dim in (64, 128) and page in (8, 16, 32, 64)
+    tensor_cores = q.dtype is torch.bfloat16 and dim in (32, 64, 128) and page in (8, 16, 32, 64)
     # scratch of this call alone (calls on several streams do not meet in it): two partial results for each row, and for each
     # kernel two of a tile of rows for each CTA and what the merge has to know of every item (csrc/shared_schedule.cuh)
     share, groups = columns // max(1, kv_heads * dim), prefix_len.numel()
@@ -77,7 +79,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     items = (rows * share // tile + groups + 1 + rows * -(-share // tile)) * kv_heads + 1
     rest = ctas * tile * (dim + 2) + items
     # (the rule by which the kernel for many rows is taken as well: csrc/shared_attn.cu)
-    many = tensor_cores and rows * share > 64 * groups and (
+    many = tensor_cores and dim >= 64 and rows * share > 64 * groups and (
         -(-rows * share // 64) * kv_heads * (page_table.shape[1] * page // 64 + 1) > 12 * sms)
     if many:
         rest += sms * 256 * (dim + 2) + (rows * share // 256 + groups + 1) * kv_heads + 1

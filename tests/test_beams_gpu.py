@@ -48,6 +48,33 @@ def test_attention_head_layouts_of_many_rows(heads, kv_heads):
     no_device_error()
 
 
+@pytest.mark.parametrize("groups", [[(0, [1])], [(0, [0, 1, 0])], [(64, [65, 64, 70])], [(63, [64, 65]), (65, [66, 130, 65])],
+                                    [(100, [101]), (100, [101, 140])], [(40, [30, 50, 0, 40])], [(700, [701] * 40)], [(3, [5, 4])] * 90])
+@pytest.mark.parametrize("heads,kv_heads,window,page_size,scatter", [(12, 2, 0, 16, True), (3, 1, 0, 8, True), (28, 4, 60, 32, True),
+                                                                     (8, 8, 0, 64, False), (33, 1, 7, 16, False), (40, 8, 130, 8, False)])
+def test_attention_heads_of_32(groups, heads, kv_heads, window, page_size, scatter):
+    SharedCase(groups, heads, kv_heads, 32, BF16, window=window, page_size=page_size, scatter=scatter).check()
+    no_device_error()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dim", [32, 64])
+def test_attention_hidden_keys_of_few_rows_may_be_anything(bad, dim):
+    """What a row does not see does not reach it; a value that is not finite reaches the rows that see it."""
+    case = SharedCase([(130, [131, 200, 100, 135]), (20, [40, 21])], 8, 2, dim, BF16)
+    want, bound = case.plain()
+    hidden = 105  # behind the third sequence's last key, in the part that the others see
+    page, o = int(case.table[0, hidden // 16]), hidden % 16
+    sees = torch.tensor([any(j == hidden for _, j in case.keys(0, r)) for r in range(4)] + [False] * 2)
+    case.v[page, :, o] = bad
+    got = case.run().double().cpu()
+    assert ((got - want).abs() <= bound)[~sees].all() and not torch.isfinite(got[sees]).any()
+    case.k[page, :, o] = bad
+    got = case.run().double().cpu()
+    assert ((got - want).abs() <= bound)[~sees].all()
+    no_device_error()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("window", [0, 90])
 @pytest.mark.parametrize("dim", [64, 128])
