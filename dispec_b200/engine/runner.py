@@ -215,14 +215,24 @@ class ModelRunner:
     @torch.inference_mode()
     def fork(self, pairs: list) -> None:
         """For each (request, new one): the new one goes on from where the request is, with pages in common and a copy of the
-        page that both will write to and of the states."""
+        page that both will write to and of the states.  Where one cannot, none is there."""
         pages = [[] for _ in self.cache.groups]
-        slots = []
+        slots, there, origin = [], [], {}
         for req_id, new_id in pairs:
-            slot, copies = self.cache.fork(req_id, new_id)
-            slots.append((slot, self.cache.state_slot(req_id)))
+            try:
+                slot, copies = self.cache.fork(req_id, new_id)
+            except Exception:
+                for r in there:
+                    self.release(r)
+                raise
+            there.append(new_id)
+            # (what is itself new here is copied from where it comes from: all is read before anything is written)
+            old = self.cache.state_slot(req_id)
+            origin[slot] = origin.get(old, old)
+            slots.append((slot, origin[slot]))
             for g, page, copy in copies:
-                pages[g].append((copy, page))
+                origin[g, copy] = origin.get((g, page), page)
+                pages[g].append((copy, origin[g, copy]))
         for named, moves in zip(self.storage.pools, pages):
             self._copy_slots(list(named.values()), moves)
         self._copy_slots([b.view(1, b.shape[0], -1) for b in self.states.buffers], slots)
@@ -233,8 +243,10 @@ class ModelRunner:
             return
         moves = sorted(moves)
         numbers = torch.tensor([d for d, _ in moves] + [s for _, s in moves], dtype=torch.int32).to(self.device)
+        dst, src = numbers[:len(moves)], numbers[len(moves):]
         for i in range(0, len(pools), 64):
-            ops.reorder_slots(pools[i:i + 64], numbers[len(moves):], numbers[:len(moves)])
+            for k in range(0, len(moves), 8192):  # (copies are new: none of them is read)
+                ops.reorder_slots(pools[i:i + 64], src[k:k + 8192], dst[k:k + 8192])
 
     # -------------------------------------------------------- captured all-decode steps
     def _context_class(self, entries: list) -> int:

@@ -195,6 +195,24 @@ def test_a_pool_too_small_raises_and_leaves_nothing_behind():
         assert len(engine.generate([[1, 2, 3]], 4)[0]) == 1
 
 
+def test_forks_of_which_one_cannot_be_take_nothing():
+    from dispec_b200 import SeqEntry
+    with tempfile.TemporaryDirectory() as td:
+        ru.make_model_folder(td, "a", dtype="float32")
+        run = engine_for(td, "float32", 16, 2).runner
+        run.admit("x")
+        run.step([SeqEntry("x", list(range(40)), 0, [])])
+        for pairs, error in (([("x", "y"), ("x", "y")], ValueError), ([("x", "y"), ("z", "w")], KeyError)):
+            with pytest.raises(error):
+                run.fork(pairs)
+            run.cache.check()
+            assert run.cache.live_requests() == ["x"]
+        run.fork([("x", "y"), ("y", "z")])
+        run.cache.check()
+        logits, _ = run.beam_step([[SeqEntry(r, [7], 40) for r in "xyz"]], [[0]])
+        assert torch.equal(logits[0], logits[1]) and torch.equal(logits[0], logits[2])
+
+
 def test_refusals():
     from dispec_b200 import SeqEntry
     with tempfile.TemporaryDirectory() as td:

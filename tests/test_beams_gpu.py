@@ -347,6 +347,27 @@ def test_attention_calls_behind_and_beside_one_another(dtype):
     no_device_error()
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (BF16, 32), (F32, 128)])
+@pytest.mark.parametrize("groups,long", [([(100, [131, 101, 140]), (0, [90])], False), ([(300, [311] * 70)], True)])
+def test_attention_pools_beyond_32_bits(dtype, dim, groups, long):
+    """More than 2^31 numbers in a pool, and the pages that are read are its last ones."""
+    case = SharedCase(groups, 8, 2, dim, dtype)
+    if long:
+        case.table = long_pages(case.table)
+    q, k, v, table, lens, starts, prefix = case.tensors()
+    first = (2 ** 31 + 2 ** 24) // k[0].numel() - k.shape[0]
+    pools = []
+    for pool in (k, v):
+        big = torch.empty((first + k.shape[0], *k.shape[1:]), dtype=dtype, device=DEV)
+        big[first:] = pool
+        pools.append(big)
+    from dispec_b200 import ops
+    got = ops.shared_prefix_attention(q, *pools, torch.where(table < 0, table, table + first), lens, starts, prefix, scale=case.scale)
+    want, bound = case.plain()
+    assert ((got.double().cpu() - want).abs() <= bound).all()
+    no_device_error()
+
+
 def test_attention_refusals():
     from dispec_b200 import ops
     from dispec_b200.ops import KernelError
@@ -529,6 +550,22 @@ def test_select_groups_outside_the_rows_are_reported(starts):
             assert ((got.parent[g] >= a) & (got.parent[g] < b)).all()
 
 
+def test_select_logits_beyond_32_bits():
+    rows, vocab = 15000, 152064
+    from dispec_b200 import ops
+    logits = torch.empty((rows, vocab), dtype=BF16, device=DEV).normal_(std=2.5)
+    scores = -torch.rand(rows, device=DEV)
+    got = ops.beam_select(logits, scores, torch.arange(0, rows + 1, 5, dtype=torch.int32, device=DEV), count=10)
+    for g in (0, 1500, 2999):
+        of = slice(5 * g, 5 * g + 5)
+        alone = ops.beam_select(logits[of].clone(), scores[of].clone(), i32([0, 5]), count=10)
+        assert torch.equal(got.token[g], alone.token[0]) and torch.equal(got.parent[g], alone.parent[0] + 5 * g) and torch.equal(got.score[g], alone.score[0])
+    of = slice(rows - 5, rows)
+    parent, token, best = plain_select(logits[of].cpu(), scores[of].cpu(), [0, 5], 10)
+    assert (got.score[-1].cpu().double() - best[0]).abs().max() <= select_tolerance(vocab, 30.0)
+    no_device_error()
+
+
 def test_select_refusals():
     from dispec_b200 import ops
     from dispec_b200.ops import KernelError
@@ -610,6 +647,19 @@ def test_reorder_slots_that_do_not_ascend_or_are_not_there_are_reported(src, dst
     want[:, dst[:kept]] = p[:, src[:kept]]
     ops.reorder_slots([p], i32(src), i32(dst))
     assert ops.device_error() == 16 and torch.equal(p, want)
+
+
+@pytest.mark.parametrize("shape", [(40, 2 ** 16), (40, 2 ** 16 - 2)])
+def test_reorder_pools_beyond_32_bits(shape):
+    """More than 2^32 bytes in front of the slots, in both ways of copying."""
+    p = torch.zeros((2, 900, *shape), dtype=BF16, device=DEV)
+    p[:, 890:] = torch.randn((2, 10, *shape), device=DEV).to(BF16)
+    want = p[:, 890:].clone()
+    want[:, [0, 3, 9]] = want[:, [9, 0, 5]]
+    from dispec_b200 import ops
+    ops.reorder_slots([p], i32([899, 890, 895]), i32([890, 893, 899]))
+    assert torch.equal(p[:, 890:], want) and not p[:, :890].any()
+    no_device_error()
 
 
 def test_reorder_refusals():
