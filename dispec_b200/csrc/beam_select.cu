@@ -14,7 +14,9 @@
 // not depend on how rows are dealt out.
 // What does not exceed the n-th best so far is left alone; what does is put aside, and now and then the list is put in order anew by
 // counting.  Of a part's first piece a lower bound of the n-th best, which few others reach, costs no search: of each of the 8 warps
-// the ceil(n / 8)-th largest of its lanes' maxima, of these the smallest: at least n logits are as large.  Where too many reach it
+// the ceil(n / 8)-th largest of its lanes' maxima, of these the smallest: at least n logits are as large.  (Of a row of 1,093 bfloat16
+// logits, which five warps have among them, so do four of these; with all eight, three of them empty, nothing was bounded: 96 rows 15
+// us for 307.)  Where too many reach it
 // (many equal logits), the piece's exact bound is bisected.  A block a group then merges the sums of its rows' parts and picks n
 // of their lists.
 //
@@ -28,7 +30,7 @@
 
 namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 32, PIECE = THREADS * EACH;
-constexpr int MAX_COUNT = 8 * 32;  // each warp vouches for an eighth of the wanted
+constexpr int MAX_COUNT = 8 * 32;  // each warp vouches for an eighth of the wanted, and has so many lanes
 constexpr int CAP = 1024;          // candidates of a group that are put in order by counting
 constexpr int ASIDE = 32;          // logits that are put aside before a part's list is put in order (which costs as many steps as it has entries)
 constexpr int LIST_CAP = 2 * MAX_COUNT + 2 * ASIDE;
@@ -111,7 +113,8 @@ __device__ __forceinline__ int block_sum(int mine, int* of_warp) {
 }
 
 // Where more logits of a piece reach a bound than can be put in order: the n-th largest by bisection, and where its equals are more
-// than wanted, the last column taken.  By the whole block; the n go to list[aside] and on.
+// than wanted, the last column taken.  By the whole block; the n go to list[aside] and on.  (Some 280 us a piece: rows of equal logits, and
+// counts from 190 on, which the lanes' maxima bound too loosely for the list.)
 template <int WIDE>
 __device__ __noinline__ void exact_bound(const float* x, uint32_t limit, int n, int first, unsigned long long* list,
                                          int aside, int* found, int* of_warp) {
@@ -256,8 +259,10 @@ beam_pieces_kernel(const Args a) {
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) a.stats[(size_t)p * WARPS + warp] = make_float2(top, sum);
     if (fresh) {
-      const uint32_t kth = warp_kth(ordered(mine), (n + WARPS - 1) / WARPS - 1);
-      if (lane == 0) bounds[warp] = kth;
+      // (each warp whose lanes all have logits vouches for an equal part of the wanted; where there are too few of them, none does)
+      const int whole = max(1, min(WARPS, there / (32 * WIDE))), each = whole == WARPS ? (n + WARPS - 1) / WARPS : (n + whole - 1) / whole;
+      const uint32_t kth = each <= 32 ? warp_kth(ordered(mine), each - 1) : NOTHING;
+      if (lane == 0) bounds[warp] = warp < whole ? kth : 0xffffffffu;
       for (int i = tid; i < n; i += THREADS) list[i] = 0;
       if (tid == 0) found = n;
       aside = n;

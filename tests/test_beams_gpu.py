@@ -433,6 +433,14 @@ def test_select_vocabularies(dtype, vocab, count):
     check_choice(logits, scores, [0, 4, 4, 5, 9], count)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [3, 31, 127, 128, 129, 255, 256, 257, 511, 640, 1023, 1024, 1093, 1792, 2047, 2049, 8192 + 130])
+@pytest.mark.parametrize("count", [1, 11, 33, 64, 200])
+def test_select_rows_that_few_warps_have(dtype, vocab, count):
+    logits, scores = random_choice(9, vocab, seed=vocab + count, dtype=dtype)
+    check_choice(logits, scores, [0, 3, 4, 9], count)
+
+
 @pytest.mark.parametrize("starts", [[0, 300], list(range(301)), [0, 1, 1, 150, 300], [5, 40]])
 def test_select_groups(starts):
     logits, scores = random_choice(300, 5000, seed=1)
