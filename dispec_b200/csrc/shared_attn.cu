@@ -200,7 +200,7 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   // places are counted in 32 bits, a tile of keys beyond the last among them
   a.sh.most_ctx = (int)min(table.size[1] * page, 1L << 30);
   // Units are counted in 32 bits: those of all items, each over as many tokens as a sequence's pages hold.
-  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (2 * (a.sh.most_ctx / KEYS_PER_TILE + 1) + EXTRA_MANY),
+  SHARED_REQUIRE(R * a.sh.G <= 0x7fffffff && a.sh.items() <= 0x7fffffff / (2 * (a.sh.most_ctx / KEYS_PER_TILE + 1 + EXTRA_MANY)),
                  "%ld rows of %ld heads over pages for %d tokens a sequence are too many for one call", R, columns / D, a.sh.most_ctx);
   DspSharedAttention many = a;
   many.sh.is_many = 1;

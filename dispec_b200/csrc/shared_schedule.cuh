@@ -4,10 +4,10 @@
 // P_g = prefix_len[g] tokens are the same for all of them and are read through the pages of its first sequence.  A segment is
 // either such a beginning with the rows of all the group's sequences, or one sequence's keys behind it with its own G rows (a
 // group of one has no shared part: all its keys are one segment).  An item is one tile of query rows of one key/value head of
-// one segment; it walks the key tiles of 64 that any of its rows sees, and is counted as so many units, twice as many where a tile
-// has more than `heavy` rows, and `extra` more, which stand for its beginning and end.  All units, in the order (shared parts, sequences; row tile, head, key tile), are cut into equal
-// runs, one per CTA, wherever that falls, so that few long beginnings load every SM as well as many short sequences, and nothing
-// about lengths is needed on the host.
+// one segment; it walks the key tiles of 64 that any of its rows sees, and is counted as so many units and `extra` more, which stand for
+// its beginning and end, all twice where a tile has more than `heavy` rows.  All units, in the order (shared parts, sequences; row tile,
+// head, key tile), are cut into equal runs, one per CTA, wherever that falls, so that few long beginnings load every SM as well as many
+// short sequences, and nothing about lengths is needed on the host.
 //
 // Two kernels may share the work: beginnings with more than `many` rows a head go to one whose tiles have 256 rows, the rest to
 // one with smaller tiles.  Where all beginnings of the first have R row tiles, teams of R CTAs walk the same keys with one row
@@ -128,7 +128,7 @@ __device__ __forceinline__ Segment segment(const Shape& sh, const Groups& groups
 // Units of a segment, or with teams of one of its row tiles (which all weigh the same then).
 __device__ __forceinline__ int units_of(const Shape& sh, const Segment& x, bool teams) {
   if (x.key_tiles <= 0) return 0;
-  return sh.KVH * ((teams ? 0 : (x.row_tiles - 1) * (x.key_tiles * x.weight + sh.extra)) + x.key_tiles * (teams ? 1 : x.last_weight) + sh.extra);
+  return sh.KVH * (x.key_tiles + sh.extra) * (teams ? 1 : (x.row_tiles - 1) * x.weight + x.last_weight);
 }
 
 // Where a CTA's run begins.
@@ -283,11 +283,11 @@ struct Walk {
     if (teams > 1) {
       at.row_tile = cta % teams;
     } else {
-      const int whole = sh.KVH * (key_tiles * weights[0] + sh.extra);
+      const int whole = sh.KVH * (key_tiles + sh.extra) * weights[0];
       at.row_tile = min((u - item_start) / whole, row_tiles - 1);
       item_start += at.row_tile * whole;
     }
-    const int cost = key_tiles * weight() + sh.extra;
+    const int cost = (key_tiles + sh.extra) * weight();
     at.head = (u - item_start) / cost;
     item_start += at.head * cost;
     return share(sh) || next(sh);
@@ -333,7 +333,7 @@ struct Walk {
   // the run's part of the present item; false: it has no key tile
   __device__ __forceinline__ bool share(const Shape& sh) {
     // (so many key tiles lie in front of a unit of the item)
-    const int w = weight(), first_tile = item_start + sh.extra, item_end = first_tile + key_tiles * w, stop = min(end, item_end);
+    const int w = weight(), first_tile = item_start + sh.extra * w, item_end = first_tile + key_tiles * w, stop = min(end, item_end);
     const int before = max(u - first_tile, 0) >> (w - 1), upto = max(stop - first_tile, 0) >> (w - 1);
     begins = before == 0;
     at.kt_begin = lo_tile + before;
@@ -346,7 +346,7 @@ struct Walk {
     Note x = {-1, {cta, 1, (short)teams}};
     if (begins) {
       x.item = sh.item(at.part, at.group, at.first, at.row_tile, at.head);
-      x.record.parts = (short)((item_start + sh.extra + key_tiles * weight() - 1) / chunk - cta / teams + 1);
+      x.record.parts = (short)((item_start + (sh.extra + key_tiles) * weight() - 1) / chunk - cta / teams + 1);
     }
     return x;
   }
