@@ -53,23 +53,20 @@ constexpr uint32_t NOTHING = 0x007fffffu;  // ordered(-inf)
 constexpr unsigned long long NOTHING64 = 0x000fffffffffffffull;
 
 // The k-th largest (from 0) of the lanes' numbers: they are sorted across the warp.
-template <typename K>
-__device__ __forceinline__ K warp_kth(K x, int k) {
+__device__ __forceinline__ uint32_t warp_kth(uint32_t x, int k) {
   const int lane = threadIdx.x & 31;
-  if constexpr (sizeof(K) == 4) {
-    if (k < 4) {  // one after the other is quicker
-      for (int i = 0; i < k; ++i) {
-        const uint32_t those = __ballot_sync(0xffffffffu, x == __reduce_max_sync(0xffffffffu, x));
-        if (lane == __ffs(those) - 1) x = 0;
-      }
-      return __reduce_max_sync(0xffffffffu, x);
+  if (k < 4) {  // one after the other is quicker
+    for (int i = 0; i < k; ++i) {
+      const uint32_t those = __ballot_sync(0xffffffffu, x == __reduce_max_sync(0xffffffffu, x));
+      if (lane == __ffs(those) - 1) x = 0;
     }
+    return __reduce_max_sync(0xffffffffu, x);
   }
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int step = size >> 1; step > 0; step >>= 1) {
-      const K y = __shfl_xor_sync(0xffffffffu, x, step);
+      const uint32_t y = __shfl_xor_sync(0xffffffffu, x, step);
       const bool larger = ((lane & step) == 0) == ((lane & size) == 0);  // this lane keeps the larger one
       x = (x > y) == larger ? x : y;
     }

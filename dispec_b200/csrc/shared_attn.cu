@@ -19,16 +19,17 @@ using namespace shared;
 
 constexpr int FEW_CTAS = 2;                                 // an SM (shared_attn_few.cuh)
 constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
-// What an item's beginning and end cost, in key tiles; rows of a tile that takes twice as long (64 rows 2.5 us a key tile and CTA
-// where 16 take 1.3).  (256 sequences behind shared parts of 2,050, 28 heads of 128 on 4: 105.7, 103.7, 100.4 and 100.8 us with 0 to 3 for
-// the kernel for few rows; 8 groups of 5 behind 4,101: 39.7, 33.9, 31.1, 32.0.  In 32 bits a key tile takes 8 us, and nothing is
-// small beside it: 2 groups of 5 behind 701, 12 heads on 2: 21.6, 25.2, 32.2.)
+// What an item's beginning and end cost, in key tiles; rows of a tile of which all takes twice as long (64 rows 2 us a key tile and CTA
+// where 16 take 0.6).  8 groups of 5 behind 4,101 tokens with 130 of their own, 28 heads of 128 on 4, and 7 groups of 50 behind 56 with
+// 97, 16 on 4, with 0 to 5: 48.5, 42.6, 39.3, 35.8, 37.0, 36.4 us and 72.6, 61.0, 54.9, 50.6, 50.4, 49.3; with 3, and twice from above 16
+// rows, 32, and never: 35.5, 35.8, 38.8 and 50.5, 50.6, 70.5.  (In 32 bits a key tile takes 8 us, and nothing is small beside it: 2 groups
+// of 5 behind 701, 12 heads on 2, with 0 to 2: 21.6, 25.2, 32.2.)
 // A kernel more is some 7 us more, which so many of its tiles an SM repay.  One group of 16 and 64 sequences of 28 heads on 4, and of
 // 40 of 64 on 8, heads of 128, with both kernels and with the one for few alone: shared parts of 4,000 tokens (3.4, 11.9 and 17.0 tiles
 // an SM) 25.2, 39.7 and 43.0 us and 21.3, 39.2 and 48.6; of 8,000 26.2, 43.6 and 50.6 and 28.1, 65.1 and 72.1; of 32,000 39.3, 69.8
 // and 94.2 and 55.2, 160.5 and 211.9.  8 groups of 16 with 28 heads: 1,000 tokens (6.1) 37.3 and 35.2, 2,000 (12.1) 39.1 and 43.5.
 constexpr long MANY_UNITS = 12;
-constexpr int EXTRA_FEW = 2, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
+constexpr int EXTRA_FEW = 3, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
 
 // Joins a row's partial results: `quads` neighbouring threads have four columns each of a row and head, and where rows are few, so many
 // threads more (`share`) divide the partial results of a row among them, up to one for each CTA (8 rows behind 16,384 tokens, 12 heads
