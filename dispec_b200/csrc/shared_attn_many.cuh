@@ -58,7 +58,7 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
   // whose buffer the softmax of tile n has left.
   __shared__ uint32_t bad_pages[16];
   static_assert(MANY_STAGES / 2 + 2 < 16, "tiles that may be looked at");
-  __shared__ int odd_share;      // the last share in which numbers were taken out of the values
+  __shared__ int odd_share[KNOWN];  // share k in k % KNOWN: numbers were taken out of its values (one group may be a share ahead)
   __shared__ uint32_t tmem_slot;
   __shared__ shared::Plan plan;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -86,7 +86,7 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
       mbar_init(&left[k], 10);  // the warps of the products and the softmax warps
       mbar_init(&cleaned[k], 4);
     }
-    odd_share = -1;
+    for (int k = 0; k < KNOWN; ++k) odd_share[k] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
@@ -387,7 +387,7 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
           const int sv = (2 * tile + 1) % MANY_STAGES;
           ok = __all_sync(0xffffffffu, mbar_wait(&full[sv], (2 * tile / MANY_STAGES) & 1));
           if (!ok) break;
-          if (clean_values<SharedWork>(p, t, smem_u32(ring + sv * KV_BYTES), t.kt_begin + j, bad, r)) odd_share = share;
+          if (clean_values<SharedWork>(p, t, smem_u32(ring + sv * KV_BYTES), t.kt_begin + j, bad, r)) odd_share[share % KNOWN] = share;
           __syncwarp();
           if (lane == 0) mbar_arrive(&cleaned[tile & 7]);
         }
@@ -418,7 +418,7 @@ shared_attn_many_kernel(const __grid_constant__ Params<SharedWork> p, const __gr
       }
       if (!ok) break;
       tc_fence_after();
-      if (odd_share == share && warp_ok) {
+      if (odd_share[share % KNOWN] == share && warp_ok) {
         add_odd_values<SharedWork>(p, t, 0, 1, SharedWork::row(p.a, t, node), row_ok, o_addr);
         __syncwarp();
       }

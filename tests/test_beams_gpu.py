@@ -347,6 +347,22 @@ def test_attention_calls_behind_and_beside_one_another(dtype):
     no_device_error()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_values_that_are_not_finite_in_many_shares_a_cta(dim):
+    """Shares of few key tiles follow one another in a CTA, each with such a value that some of its rows see."""
+    case = SharedCase([(100 + 64 * (g % 3), [101 + 64 * (g % 3), 300, 90, 95] * 20) for g in range(24)], 8, 2, dim, BF16)
+    case.table = long_pages(case.table)
+    want, bound = case.plain()
+    for g in range(24):
+        page = int(case.table[case.starts[g], 95 // 16])
+        case.v[page, :, 95 % 16] = float("inf")
+    sees = torch.tensor([n > 95 for n in case.lens])
+    for _ in range(3):
+        got = case.run().double().cpu()
+        assert ((got - want).abs() <= bound)[~sees].all() and not torch.isfinite(got[sees]).any()
+    no_device_error()
+
+
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (BF16, 32), (F32, 128)])
 @pytest.mark.parametrize("groups,long", [([(100, [131, 101, 140]), (0, [90])], False), ([(300, [311] * 70)], True)])
 def test_attention_pools_beyond_32_bits(dtype, dim, groups, long):
