@@ -28,10 +28,10 @@ GRAPH_CONTEXT_CLASSES = (2048, 8192, 32768, 131072, 524288)
 
 # Bytes of keys and values that reading shared pages once has to save in a layer.  The attention of shared pages is three launches
 # where that of single tokens is one: some 10 us, in which 100 MB come from the L2 and the memory.  A layer of a step, heads of 128,
-# shared and each its own: 8 beams behind 4,096 tokens, 28 heads on 4 (59 MB) 42 and 37 us, 4 behind 16,384 (101 MB) 46 and 50, 8 behind
-# 16,384 (235 MB) 53 and 73, 32 behind 16,384 (1 GB) 76 and 191; 8 behind 16,384, 12 heads on 2 (117 MB) 41 and 40.  In 32 bits the
+# shared and each its own: 8 beams behind 4,096 tokens, 28 heads on 4 (59 MB) 41 and 37 us, 4 behind 16,384 (101 MB) 45 and 50, 8 behind
+# 16,384 (235 MB) 54 and 75, 32 behind 16,384 (1 GB) 75 and 188; 8 behind 16,384, 12 heads on 2 (117 MB) 39 and 41.  In 32 bits the
 # attention of single tokens is bound by its arithmetic, and the products of shared pages are of tiles of rows: 2 beams behind
-# 64 tokens, 12 heads on 2 (0.1 MB) 60 and 57 us, behind 256 (0.5 MB) 61 and 70, behind 16,384 86 and 1,260.
+# 64 tokens, 12 heads on 2 (0.1 MB) 61 and 58 us, behind 256 (0.5 MB) 62 and 71, behind 16,384 87 and 1,264.
 SHARED_BYTES = {torch.bfloat16: 100_000_000, torch.float32: 500_000}
 MAX_SHARED_GROUPS = 1024  # of a call (ops/beams.py)
 
