@@ -5,8 +5,8 @@
 // ALL i: it holds them in shared memory or in registers, meets, and writes them.  A slot may be read by several and
 // written by another in one call, in place and without a copy of anything, and no block waits for another.
 //
-// Memory bounds it: 906 MB in rows of 32 KB (48 layers of keys and values, read and written) take 161 us, 151 MB in rows of 512 KB
-// (12 layers of states) 25.6: 5.6 and 5.9 TB/s.
+// Memory bounds it: 906 MB in rows of 32 KB (48 layers of keys and values, read and written) take 136 us, 151 MB in rows of 512 KB
+// (12 layers of states) 23.6: 6.6 and 6.4 TB/s.
 //
 // dst ascends, so that no slot is written twice; what does not ascend, or names a slot that is not there, is left from there on
 // and recorded.
@@ -51,9 +51,10 @@ __device__ __forceinline__ int sound_entries(const Args& a, const Pool& pool, in
 }
 
 // Rows of whole 16-byte pieces and up to BULK_ENTRIES entries: the columns of an entry are one bulk copy into shared memory and one
-// back (of 96 bytes at least).  The same copies through registers, eight pieces a thread, take 203 and 32.7 us where these take 161 and
-// 25.6; more entries, and rows of other sizes, go that way.
-constexpr int BULK_THREADS = 128, BULK_ENTRIES = 512, BULK_BYTES = 48 * 1024;
+// back, of whole lines of 128 bytes where six blocks an SM hold them, else of 96 bytes at least.  The two calls above: 136 and 23.6 us; with
+// 48 KB a block and copies of 336 and 4,096 bytes 160 and 24.9; lines, and room for 48 KB all the same (four blocks an SM) 165; lines with
+// 74 KB 140 and 25.3.  Through registers, eight pieces a thread, 203 and 32.7; more entries, and rows of other sizes, go that way.
+constexpr int BULK_THREADS = 128, BULK_ENTRIES = 512, BULK_BYTES = 48 * 1024, LINE_BYTES = 37 * 1024;
 __global__ void __launch_bounds__(BULK_THREADS)
 reorder_bulk_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(128) unsigned char stage[];
@@ -163,7 +164,7 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
   const int threads = n <= 512 ? 256 : 1024;  // (rows of 64 bytes at least up to 2,048 entries)
   REORDER_REQUIRE(n <= (long)threads * EACH, "%ld slots to be copied, at most %d", n, 1024 * EACH);
   while ((n << (a.chunk_shift + 1)) <= (long)threads * EACH) ++a.chunk_shift;
-  const long chunk_bytes = bulk ? BULK_BYTES / n / 16 * 16 : piece << a.chunk_shift;
+  const long chunk_bytes = bulk ? (n * 128 <= LINE_BYTES ? LINE_BYTES / n / 128 * 128 : BULK_BYTES / n / 16 * 16) : piece << a.chunk_shift;
   a.chunk_bytes = (int)chunk_bytes;
   long blocks = 0;
   for (long p = 0; p < pools; ++p) {
@@ -193,7 +194,7 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
       DSP_CUDA(cudaFuncSetAttribute(reorder_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BULK_BYTES));
       if (device >= 0) allowed[device] = true;
     }
-    const int rc = go(reorder_bulk_kernel, BULK_THREADS, BULK_BYTES);
+    const int rc = go(reorder_bulk_kernel, BULK_THREADS, (size_t)(n * chunk_bytes));
     if (rc != 0) return rc;
   } else {
     const int rc = threads == 256 ? (piece == 16 ? go(reorder_kernel<uint4, 256>, 256, 0) : piece == 4 ? go(reorder_kernel<uint32_t, 256>, 256, 0)

@@ -639,6 +639,15 @@ def test_reorder_all_slots_at_once(n):
         reorder([pool(2, n, 3, 40), pool(1, n, 8, dtype=F32)], order, src)
 
 
+@pytest.mark.parametrize("n", [11, 12, 144, 147, 148, 149, 295, 296, 297, 384])
+def test_reorder_whole_lines_and_parts_of_them(n):
+    """Entries whose columns are copied by lines of 128 bytes and by less, with rows that are no multiple of either."""
+    for shape in ((8, 208), (5, 8), (2, 16, 128)):
+        src = torch.randperm(n + 5, generator=torch.Generator().manual_seed(n))[:n].tolist()
+        reorder([pool(2, n + 5, *shape, dtype=BF16)], src, list(range(5, n + 5)))
+        no_device_error()
+
+
 def test_reorder_many_pools_of_different_rows():
     pools = [pool(1 + s % 3, 9, 1 + s % 5, 8 * (1 + s % 7), dtype=(BF16, F32)[s % 2], seed=s) for s in range(64)]
     reorder(pools, [8, 0, 3, 3], [0, 1, 2, 8])
