@@ -41,7 +41,7 @@ template <typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS, 3)
 shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch scratch, const SharedScratch scratch_many,
                       T* __restrict__ out, long out_stride, int D, int ctas, int ctas_many, int share) {
-  __shared__ int start[MAX_GROUPS + 1];
+  __shared__ Starts starts;
   __shared__ float4 sums[COMBINE_THREADS];
   __shared__ float2 mls[COMBINE_THREADS];
   const int H = sh.KVH * sh.G, quads = D / 4, per_row = quads * share, tid = threadIdx.x;
@@ -50,15 +50,14 @@ shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch s
   const int mine = in_row / quads, d = (in_row - mine * quads) * 4;  // which of the row's parts; its columns
   const int row = in_block < of_block ? (int)min(row_head / H, (long)sh.rows) : sh.rows, h = (int)(row_head % H);
   const int head = h / sh.G, of_head = h - head * sh.G;
-  for (int k = tid; k <= sh.groups; k += COMBINE_THREADS) start[k] = sh.group_start[k];
   const int length = row < sh.rows ? sh.length(row) : 0;  // (asked for with the groups)
-  __syncthreads();
-  const int g = row < sh.rows ? group_of(start, sh.groups, sh.rows, row) : -1;
+  starts.bring(sh);
+  const int g = row < sh.rows ? group_of(starts, sh.groups, row) : -1;
   bool many = false, sees[2] = {false, false};  // the shared part was the other kernel's
   int of_tile[2] = {0, 0};
   long item[2] = {0, 0};
   if (g >= 0) {
-    const int first = start[g], n = start[g + 1] - first;
+    const int first = starts.start[g], n = starts.start[g + 1] - first;
     const int prefix = n > 1 ? min(max(0, sh.prefix_len[g]), sh.most_ctx) : 0, lo = sh.window > 0 ? max(0, length - sh.window) : 0;
     many = (long)n * sh.G > sh.many;
     // an item of which the row sees a key is there, and has a record

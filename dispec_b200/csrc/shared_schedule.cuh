@@ -16,6 +16,10 @@
 // Every item leaves a partial result (32-bit sums that are not divided yet, running maximum, sum of weights): in the place of its
 // rows, `rows_o`, where one CTA had all of it, else one in each CTA's scratch slots (2 c + 1 for the item that begins in CTA c,
 // 2 c for the one that began before).  A record of each item says which; shared_combine_kernel merges a row's two items.
+//
+// Which groups there are is settled before anything is counted: one that is not inside the rows, or does not begin behind those before
+// it, is left out, so that the groups that are there ascend and a row is in one of them at most.  All that counts units, walks them or
+// merges goes by that (a row that lay in two groups for one of them made runs longer than what there was to walk).
 #pragma once
 #include "rows_schedule.cuh"
 
@@ -48,8 +52,45 @@ struct Shape {
   __device__ __forceinline__ int length(int row) const { return min(max(0, ctx_len[row]), most_ctx); }
 };
 
-// The group of a row, -1: in none.
-__device__ __forceinline__ int group_of(const int* start, int groups, int rows, int row) {
+// Where groups begin, in shared memory.
+struct Starts {
+  int start[MAX_GROUPS + 1];
+  uint32_t out[MAX_GROUPS / 32];  // bit g % 32 of word g / 32: group g is left out
+
+  // By the whole block, which meets: brings them.  Returns whether some are left out; then the others' places stay as they are, and
+  // what is left out fills the gaps between them.
+  __device__ __forceinline__ bool bring(const Shape& sh) {
+    const int tid = threadIdx.x;
+    bool bad = false;
+    for (int g = tid; g < sh.groups; g += blockDim.x) {
+      const int first = sh.group_start[g], end = sh.group_start[g + 1];
+      start[g] = first;
+      if (g + 1 == sh.groups) start[g + 1] = end;
+      bad |= first < 0 || end < first || end > sh.rows;
+    }
+    if (tid < MAX_GROUPS / 32) out[tid] = 0;
+    if (!__syncthreads_or(bad)) return false;
+    if (tid == 0) {
+      int at = 0, end = start[0];  // of the last group that is there; in the list as it came
+      for (int g = 0; g < sh.groups; ++g) {
+        const int first = end;
+        end = start[g + 1];
+        const bool there = first >= at && end >= first && end <= sh.rows;
+        start[g] = there ? first : at;
+        if (there)
+          at = end;
+        else
+          out[g >> 5] |= 1u << (g & 31);
+      }
+      start[sh.groups] = at;
+    }
+    __syncthreads();
+    return true;
+  }
+  __device__ __forceinline__ bool left_out(int g) const { return (out[g >> 5] >> (g & 31)) & 1u; }
+};
+// The group of a row, -1: in none.  The starts ascend.
+__device__ __forceinline__ int group_of(const int* start, int groups, int row) {
   int lo = 0, hi = groups;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -58,12 +99,17 @@ __device__ __forceinline__ int group_of(const int* start, int groups, int rows, 
     else
       hi = mid;
   }
-  return start[lo] <= row && row < start[lo + 1] && start[lo] >= 0 && start[lo + 1] <= rows ? lo : -1;
+  return start[lo] <= row && row < start[lo + 1] ? lo : -1;
+}
+__device__ __forceinline__ int group_of(const Starts& s, int groups, int row) {
+  const int g = group_of(s.start, groups, row);
+  return g >= 0 && !s.left_out(g) ? g : -1;
 }
 
 // What a CTA has to know of the groups while it finds its run.
 struct Groups {
-  int start[MAX_GROUPS + 1], prefix[MAX_GROUPS], shortest[MAX_GROUPS], longest[MAX_GROUPS];
+  Starts starts;
+  int prefix[MAX_GROUPS], shortest[MAX_GROUPS], longest[MAX_GROUPS];
   int of_warp[32], most_tiles[32], least_tiles[32];
 };
 struct Segment {
@@ -78,13 +124,13 @@ __device__ __forceinline__ void set_weights(const Shape& sh, Segment& x) {
   x.weight = sh.rows_per_tile() > sh.heavy ? 2 : 1;
   x.last_weight = x.n * sh.G - ((x.row_tiles - 1) << sh.row_shift) > sh.heavy ? 2 : 1;
 }
-// The shared part of group g, whose sequences have between `shortest` and `longest` tokens.
+// The shared part of group g (`first` -1: it is left out), whose sequences have between `shortest` and `longest` tokens.
 __device__ __forceinline__ Segment shared_part(const Shape& sh, int g, int first, int end, int prefix, int shortest, int longest) {
   Segment x = {};
   x.group = g;
   x.first = first;
   x.n = end - first;
-  if (first < 0 || end > sh.rows || x.n < 2 || ((long)x.n * sh.G > sh.many) != (sh.is_many != 0)) return x;
+  if (first < 0 || x.n < 2 || ((long)x.n * sh.G > sh.many) != (sh.is_many != 0)) return x;
   x.end = min(prefix, longest);
   x.all_end = min(prefix, shortest);
   if (sh.window > 0) {
@@ -115,15 +161,15 @@ __device__ __forceinline__ Segment own_part(const Shape& sh, int row, int g, int
   set_weights(sh, x);
   return x;
 }
-// `near`: a group that the row may be in, looked at first.
+// `near`: a group that is there and that the row may be in, looked at first.
 __device__ __forceinline__ Segment segment(const Shape& sh, const Groups& groups, int s, int near = -1) {
   const int row = s - sh.groups;
+  const int* start = groups.starts.start;
   if (row < 0)
-    return shared_part(sh, s, groups.start[s], groups.start[s + 1], groups.prefix[s], groups.shortest[s], groups.longest[s]);
-  if (near < 0 || row < groups.start[near] || row >= groups.start[near + 1] || groups.start[near + 1] > sh.rows)
-    near = group_of(groups.start, sh.groups, sh.rows, row);
+    return shared_part(sh, s, groups.starts.left_out(s) ? -1 : start[s], start[s + 1], groups.prefix[s], groups.shortest[s], groups.longest[s]);
+  if (near < 0 || row < start[near] || row >= start[near + 1]) near = group_of(groups.starts, sh.groups, row);
   const int at = max(near, 0);
-  return own_part(sh, row, near, groups.start[at], groups.start[at + 1], groups.prefix[at]);
+  return own_part(sh, row, near, start[at], start[at + 1], groups.prefix[at]);
 }
 // Units of a segment, or with teams of one of its row tiles (which all weigh the same then).
 __device__ __forceinline__ int units_of(const Shape& sh, const Segment& x, bool teams) {
@@ -137,6 +183,9 @@ struct Run {
   int total, chunk;            // all units (of one row tile, with teams); units of a run
   int teams;                   // CTAs that walk the same keys
   int segment, segment_start;  // of the CTA's first unit (-1: there is none)
+  int segments;
+  bool some_out;               // groups are left out, these:
+  uint32_t out[MAX_GROUPS / 32];
   Segment ahead[AHEAD];
 };
 struct Plan {
@@ -148,19 +197,19 @@ struct Plan {
 __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& run, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int own_length = tid < sh.rows ? sh.length(tid) : 0;  // (asked for with the groups)
-  for (int g = tid; g <= sh.groups; g += threads) {
-    groups.start[g] = sh.group_start[g];
-    if (g == sh.groups) break;
+  for (int g = tid; g < sh.groups; g += threads) {
     groups.prefix[g] = min(max(0, sh.prefix_len[g]), sh.most_ctx);
     groups.shortest[g] = 0x7fffffff;
     groups.longest[g] = 0;
   }
   if (tid == 0) run.segment = -1;
-  __syncthreads();
-  for (int g = tid; g < sh.groups; g += threads)
-    if (groups.start[g] < 0 || groups.start[g + 1] < groups.start[g] || groups.start[g + 1] > sh.rows) atomicOr(sh.err, DSP_ERR_BAD_GROUP);
+  const bool some_out = groups.starts.bring(sh);
+  if (some_out) {
+    if (tid == 0) atomicOr(sh.err, DSP_ERR_BAD_GROUP);
+    if (tid < MAX_GROUPS / 32) run.out[tid] = groups.starts.out[tid];
+  }
   for (int row = tid; row < sh.rows; row += threads) {
-    const int length = row == tid ? own_length : sh.length(row), g = group_of(groups.start, sh.groups, sh.rows, row);
+    const int length = row == tid ? own_length : sh.length(row), g = group_of(groups.starts, sh.groups, row);
     if (g < 0) continue;
     atomicMin(&groups.shortest[g], length);
     atomicMax(&groups.longest[g], length);
@@ -225,6 +274,8 @@ __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& 
     run.total = total;
     run.chunk = chunk;
     run.teams = team_size;
+    run.segments = segments;
+    run.some_out = some_out;
   }
   __syncthreads();
   if (run.segment >= 0) {
@@ -300,9 +351,11 @@ struct Walk {
     if (segment_at - run_->segment < AHEAD) {
       x = run_->ahead[segment_at - run_->segment];
     } else if (row < 0) {
-      const int g = segment_at, first = sh.group_start[g], last = sh.group_start[g + 1];
+      const int g = segment_at;
+      const bool out = run_->some_out && ((run_->out[g >> 5] >> (g & 31)) & 1u);
+      const int first = out ? -1 : sh.group_start[g], last = sh.group_start[g + 1];
       int shortest = 0x7fffffff, longest = 0;
-      if (first >= 0 && last <= sh.rows)
+      if (!out)
         for (int r = first + (int)(threadIdx.x & 31); r < last; r += 32) {
           const int length = sh.length(r);
           shortest = min(shortest, length);
@@ -311,7 +364,15 @@ struct Walk {
       x = shared_part(sh, g, first, last, min(max(0, sh.prefix_len[g]), sh.most_ctx), __reduce_min_sync(0xffffffffu, shortest),
                       __reduce_max_sync(0xffffffffu, longest));
     } else {
-      const int g = group_of(sh.group_start, sh.groups, sh.rows, row), at = max(g, 0);
+      int g = -1;
+      if (!run_->some_out) {
+        g = group_of(sh.group_start, sh.groups, row);
+      } else {  // (the list does not ascend)
+        for (int k = threadIdx.x & 31; k < sh.groups; k += 32)
+          if (!((run_->out[k >> 5] >> (k & 31)) & 1u) && sh.group_start[k] <= row && row < sh.group_start[k + 1]) g = k;
+        g = __reduce_max_sync(0xffffffffu, g);
+      }
+      const int at = max(g, 0);
       x = own_part(sh, row, g, sh.group_start[at], sh.group_start[at + 1], min(max(0, sh.prefix_len[at]), sh.most_ctx));
     }
     at.seq = at.first = x.first;
@@ -358,8 +419,9 @@ struct Walk {
         at.head = 0;
         if (teams > 1 || ++at.row_tile == row_tiles) {
           if (teams == 1) at.row_tile = 0;
-          do ++segment_at;
-          while (!enter(sh));  // (there is such a segment: units are left)
+          do {
+            if (++segment_at >= run_->segments) return false;  // (units are left, so there is such a segment)
+          } while (!enter(sh));
         }
       }
     } while (!share(sh));

@@ -58,8 +58,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q . k_j),   max(0, n - window) <= j < n  (window 0: all j < n)
 
     zero where there is none.  Pages that no row of the group sees may be gone from the tables.  32-bit sums and softmax; the
-    result [R, H * D] is rounded once.  Rows of no group are left as they are; a group whose sequences are not all among the R
-    is recorded as a device error and left out.  At most 1,024 groups.  Nothing is read back."""
+    result [R, H * D] is rounded once.  Rows of no group are left as they are; a group whose sequences are not all among the R,
+    or that does not begin behind the groups before it, is recorded as a device error and left out.  At most 1,024 groups.  Nothing is read back."""
     what = "shared_prefix_attention"
     if not q.is_cuda:
         _refuse(what, "CUDA tensors only (there is no CPU path)")

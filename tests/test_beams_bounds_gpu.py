@@ -1,0 +1,59 @@
+"""Operators on beams whose device lists overlap or point outside the arrays: recorded, left out, and everything else as it was."""
+import pytest
+import torch
+
+from beams_util import SharedCase
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+DEV = "cuda:0"
+LAST = 2 ** 31 - 1
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# dtype, head size, places for so many tokens that the kernel for many rows a key is taken
+KERNELS = [(BF16, 128, False), (BF16, 64, True), (BF16, 32, False), (F32, 64, False)]
+
+
+@pytest.mark.parametrize("dtype,dim,long", KERNELS)
+@pytest.mark.parametrize("groups,starts,prefix", [
+    # behind the group that there is, one that has two of its rows, and an empty one
+    ([(90, [130 + j % 70 for j in range(301)])], [0, 301, 299, 301, 301], [90, 0, 4000, 0]),
+    ([(400, [405 + j % 9 for j in range(90)])], [0, 90, 20, 90, 50, 90], [400, 0, 64, 0, 64]),
+    # groups that end beyond the rows or begin in front of them, between others that are there
+    ([(70, [90] * 40), (130, [140, 131])], [0, 40, LAST, 40, 42], [70, 9, 9, 130]),
+    ([(70, [90] * 40), (130, [140, 131])], [0, 40, -LAST - 1, 40, 42], [70, 9, 9, 130]),
+    ([(70, [90] * 5), (0, [60]), (130, [140, 131])], [-3, LAST, 0, 5, 6, 8, 7, 6, 8, 9], [9, 9, 70, 0, 130, 7, 7, 8, 9])])
+def test_attention_groups_that_overlap_are_left_out(dtype, dim, long, groups, starts, prefix):
+    from dispec_b200 import ops
+    case = SharedCase(groups, 8, 2, dim, dtype)
+    if long:
+        case.table = torch.nn.functional.pad(case.table, (0, 1600), value=-1)
+    want, bound = case.plain()
+    q, k, v, table, lens, _, _ = case.tensors()
+    out = torch.full((q.shape[0], q.shape[1]), 7.0, dtype=dtype, device=DEV)
+    for _ in range(3):
+        ops.shared_prefix_attention(q, k, v, table, lens, i32(starts), i32(prefix), scale=case.scale, out=out)
+        got = out.double().cpu()
+        assert ops.device_error() == 16 and ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,dim,long", KERNELS)
+def test_attention_rows_between_groups_that_are_there_stay(dtype, dim, long):
+    """Every other group is out; its rows are in none."""
+    from dispec_b200 import ops
+    lengths = [100 + 7 * r % 60 for r in range(60)]
+    case = SharedCase([(0, [n]) for n in lengths], 8, 2, dim, dtype)
+    if long:
+        case.table = torch.nn.functional.pad(case.table, (0, 1600), value=-1)
+    want, bound = case.plain()
+    q, k, v, table, lens, _, _ = case.tensors()
+    starts = [x for r in range(0, 60, 3) for x in (r, r + 1, LAST)] + [60]  # rows 0, 3, 6, ...
+    out = torch.full((60, q.shape[1]), 7.0, dtype=dtype, device=DEV)
+    ops.shared_prefix_attention(q, k, v, table, lens, i32(starts), i32([50] * 60), scale=case.scale, out=out)
+    got = out.double().cpu()
+    there = torch.arange(60) % 3 == 0
+    assert ops.device_error() == 16 and ((got - want).abs() <= bound)[there].all() and (got[~there] == 7).all()
