@@ -60,6 +60,10 @@ typedef __nv_bfloat16 bf16;
 // before that (fetching weights, computing addresses) overlaps the tail of its predecessor.
 // pdl_launch_dependents() lets the next kernel's launch begin.  Without the launch attribute
 // both calls do nothing.
+//
+// One kernel reads more than weights in front of its wait: the attention of single tokens (attn_mma.cu) reads page tables,
+// lengths and stored keys and values, which no kernel of its step writes.  So a kernel that moves what is stored never calls
+// pdl_launch_dependents(), not even behind its wait: the kernel after it then begins when it is complete.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

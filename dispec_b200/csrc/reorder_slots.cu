@@ -8,6 +8,9 @@
 // Memory bounds it: 906 MB in rows of 32 KB (48 layers of keys and values, read and written) take 136 us, 151 MB in rows of 512 KB
 // (12 layers of states) 23.6: 6.6 and 6.4 TB/s.
 //
+// The next kernel does not begin before the last block has left: what is written here are stored keys and values too, which the
+// attention of single tokens reads in front of its wait.
+//
 // dst ascends, so that no slot is written twice; what does not ascend, or names a slot that is not there, is left from there on
 // and recorded.
 #include "tcgen05_common.cuh"
@@ -70,7 +73,6 @@ reorder_bulk_kernel(const __grid_constant__ Args a) {
     tc::mbar_init(&landed, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_launch_dependents();
   pdl_wait();
   const int count = sound_entries(a, pool, &bad);
   if (count == 0) return;
@@ -103,7 +105,6 @@ reorder_kernel(const __grid_constant__ Args a) {
   const int tid = threadIdx.x;
   const Pool& pool = pool_of(a);
   const int block = blockIdx.x - pool.first_block, layer = block / pool.chunks, chunk = block - layer * pool.chunks;
-  pdl_launch_dependents();
   pdl_wait();
   const int count = sound_entries(a, pool, &bad);
   const long in_row = pool.row_bytes / (long)sizeof(Piece);
