@@ -37,8 +37,7 @@ __global__ void __launch_bounds__(THREADS)
 tree_keep_kernel(const __grid_constant__ Args a) {
   __shared__ int from_page[THREADS], from_at[THREADS], to_page[THREADS], to_at[THREADS];  // of a node; from_page -1: it stays
   __shared__ int stop;  // first node that does not come after the one in front of it
-  pdl_wait();
-  pdl_launch_dependents();
+  pdl_wait();  // (the next kernel may read what is moved here in front of its own wait, and begins when this one is complete)
   const int s = blockIdx.y, tid = threadIdx.x;
   int block = blockIdx.x, which = 0;
   while (block >= a.pool[which].blocks) block -= a.pool[which++].blocks;

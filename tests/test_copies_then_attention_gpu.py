@@ -70,3 +70,27 @@ def test_attention_behind_reordered_pages(seqs, tokens, layers):
     dst, src = i32(range(n)), [i32(range(n, 2 * n)), i32(range(2 * n, 3 * n))]
     many_times(lambda c: ops.reorder_slots([k, v], src[c], dst), lambda: step.attend(k[-1], v[-1]), 2)
     ops.raise_on_device_error("test")
+
+
+@pytest.mark.parametrize("seqs,tokens,layers", [(2, 200, 12), (16, 1000, 6)])
+def test_attention_behind_an_accepted_branch(seqs, tokens, layers):
+    """The branch's keys and values lie, once moved, in front of the newest token, in pages that the attention asks for early."""
+    from dispec_b200 import ops
+    nodes = 96  # behind them lie the newest token and as many nodes again
+    pages = -(-(tokens + 2 * nodes) // PAGE)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    k, v = (torch.randn(layers, seqs * pages, KVH, PAGE, DIM, generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    table = torch.randperm(seqs * pages, generator=torch.Generator().manual_seed(5)).to(torch.int32).view(seqs, pages).to(DEV)
+    step = Step([tokens + nodes // 2] * seqs, table)
+    stored, count = i32([tokens] * seqs), i32([nodes // 2] * seqs)
+    # node j's branch: every second node from j on, so that each call moves other numbers to the same places
+    paths = [i32([[c + 2 * j for j in range(nodes // 2)]] * seqs).contiguous() for c in (0, 1)]
+    first = [x.clone() for x in (k, v)]
+
+    def move(c):
+        k.copy_(first[0])
+        v.copy_(first[1])
+        ops.keep_path([k, v], table, stored, paths[c], count)
+
+    many_times(move, lambda: step.attend(k[-1], v[-1]), 2)
+    ops.raise_on_device_error("test")
