@@ -51,7 +51,7 @@ shared_combine_kernel(const Shape sh, const Shape sh_many, const SharedScratch s
   const int row = in_block < of_block ? (int)min(row_head / H, (long)sh.rows) : sh.rows, h = (int)(row_head % H);
   const int head = h / sh.G, of_head = h - head * sh.G;
   const int length = row < sh.rows ? sh.length(row) : 0;  // (asked for with the groups)
-  starts.bring(sh);
+  starts.bring(sh, Starts::ask(sh));
   const int g = row < sh.rows ? group_of(starts, sh.groups, row) : -1;
   bool many = false, sees[2] = {false, false};  // the shared part was the other kernel's
   int of_tile[2] = {0, 0};

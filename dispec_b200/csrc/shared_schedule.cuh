@@ -57,13 +57,20 @@ struct Starts {
   int start[MAX_GROUPS + 1];
   uint32_t out[MAX_GROUPS / 32];  // bit g % 32 of word g / 32: group g is left out
 
-  // By the whole block, which meets: brings them.  Returns whether some are left out; then the others' places stay as they are, and
-  // what is left out fills the gaps between them.
-  __device__ __forceinline__ bool bring(const Shape& sh) {
+  struct Own {  // begin and end of the group with the thread's number
+    int first, end;
+  };
+  static __device__ __forceinline__ Own ask(const Shape& sh) {
+    const int tid = threadIdx.x;
+    return tid < sh.groups ? Own{sh.group_start[tid], sh.group_start[tid + 1]} : Own{0, 0};
+  }
+  // By the whole block, which meets: brings them (`own`: asked for before, with what else is wanted, so that the answers come together).
+  // Returns whether some are left out; then the others' places stay as they are, and what is left out fills the gaps between them.
+  __device__ __forceinline__ bool bring(const Shape& sh, const Own& own) {
     const int tid = threadIdx.x;
     bool bad = false;
     for (int g = tid; g < sh.groups; g += blockDim.x) {
-      const int first = sh.group_start[g], end = sh.group_start[g + 1];
+      const int first = g == tid ? own.first : sh.group_start[g], end = g == tid ? own.end : sh.group_start[g + 1];
       start[g] = first;
       if (g + 1 == sh.groups) start[g + 1] = end;
       bad |= first < 0 || end < first || end > sh.rows;
@@ -197,13 +204,15 @@ struct Plan {
 __device__ __forceinline__ void make_plan(const Shape& sh, Groups& groups, Run& run, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int own_length = tid < sh.rows ? sh.length(tid) : 0;  // (asked for with the groups)
+  const int own_prefix = tid < sh.groups ? sh.prefix_len[tid] : 0;
+  const Starts::Own own_group = Starts::ask(sh);
   for (int g = tid; g < sh.groups; g += threads) {
-    groups.prefix[g] = min(max(0, sh.prefix_len[g]), sh.most_ctx);
+    groups.prefix[g] = min(max(0, g == tid ? own_prefix : sh.prefix_len[g]), sh.most_ctx);
     groups.shortest[g] = 0x7fffffff;
     groups.longest[g] = 0;
   }
   if (tid == 0) run.segment = -1;
-  const bool some_out = groups.starts.bring(sh);
+  const bool some_out = groups.starts.bring(sh, own_group);
   if (some_out) {
     if (tid == 0) atomicOr(sh.err, DSP_ERR_BAD_GROUP);
     if (tid < MAX_GROUPS / 32) run.out[tid] = groups.starts.out[tid];
