@@ -10,6 +10,8 @@ dispec/engine/model_runner.py:188-231) with the bookkeeping its callers do by ha
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from dispec_b200 import ops
@@ -32,7 +34,10 @@ GRAPH_CONTEXT_CLASSES = (2048, 8192, 32768, 131072, 524288)
 # 16,384 (235 MB) 54 and 75, 32 behind 16,384 (1 GB) 75 and 188; 8 behind 16,384, 12 heads on 2 (117 MB) 39 and 41.  In 32 bits the
 # attention of single tokens is bound by its arithmetic, and the products of shared pages are of tiles of rows: 2 beams behind
 # 64 tokens, 12 heads on 2 (0.1 MB) 61 and 58 us, behind 256 (0.5 MB) 62 and 71, behind 16,384 87 and 1,264.
-SHARED_BYTES = {torch.bfloat16: 100_000_000, torch.float32: 500_000}
+# Where single tokens have a tensor-core kernel and shared pages the 32-bit one (bfloat16 heads other than 32, 64 and 128, pages of other
+# than 8 to 64 tokens), never: a layer of a step, 28 heads of 96 on 4, 8 groups of 5 behind 4,101 tokens 440 and 294 us, 64 beams behind
+# 32,768 1,931 and 1,225.  (What is not listed counts as the model's type.)
+SHARED_BYTES = {torch.bfloat16: 100_000_000, torch.float32: 500_000, "32 bits for tensor cores": math.inf}
 MAX_SHARED_GROUPS = 1024  # of a call (ops/beams.py)
 
 
@@ -69,6 +74,12 @@ class ModelRunner:
         self._group_windows = [g.window for g in groups]
         self._group_pages = list(counts)
         self._graphs: dict = {}
+        # per cache group: how its mixers read pages that sequences share
+        self._shared_by: list = [set() for _ in groups]
+        for call, label in zip(model.schedule, model.call_cache):
+            by = model.layers[call.layer].mixer.takes_shared(page_size, self.dtype)
+            if label is not None and by is not None:
+                self._shared_by[model.placement[label].group].add(by)
 
     # ---------------------------------------------------------------- request lifecycle
     def admit(self, req_id, prompt_len: int = 0, max_total_len: int = 0, max_chunk: int = 1) -> None:
@@ -201,7 +212,8 @@ class ModelRunner:
                 prefixes.append(known[c] * self.page_size if len(of) > 1 else 0)
                 of_window = prefixes[-1] if spec.window <= 0 else max(0, min(prefixes[-1], prefixes[-1] + spec.window - of[0].start - 1))
                 saved += (len(of) - 1) * of_window * sum(t.num_heads * t.width for t in spec.tensors) * self.dtype.itemsize
-            worth.append(n <= MAX_SHARED_GROUPS and saved >= SHARED_BYTES[self.dtype])
+            least = max((SHARED_BYTES.get(by, SHARED_BYTES[self.dtype]) for by in self._shared_by[c]), default=math.inf)
+            worth.append(n <= MAX_SHARED_GROUPS and saved >= least)
         numbers = torch.tensor(starts + prefixes, dtype=torch.int32).to(self.device)
         if any(worth):
             ctx.shared = SharedStep(numbers[:n + 1], [numbers[n + 1 + c * n:n + 1 + (c + 1) * n] if w else None for c, w in enumerate(worth)])

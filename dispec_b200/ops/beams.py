@@ -16,6 +16,19 @@ _ATTENTION = struct.Struct("4qd")
 _PIECE = 8192  # logits of a piece of a row (csrc/beam_select.cu)
 
 
+# The tensor-core kernels are built for these head sizes and pages, and bfloat16; everything else takes the 32-bit kernel.
+TENSOR_CORE_DIMS, TENSOR_CORE_PAGES = (32, 64, 128), (8, 16, 32, 64)
+
+
+def on_tensor_cores(dim: int, page_size: int, dtype: torch.dtype) -> bool:
+    return dtype is torch.bfloat16 and dim in TENSOR_CORE_DIMS and page_size in TENSOR_CORE_PAGES
+
+
+def takes_heads(dim: int) -> bool:
+    """Heads of which there is a kernel at all."""
+    return dim % 8 == 0 and 8 <= dim <= 256
+
+
 def _refuse(what: str, message: str):
     raise L.KernelError(f"{what}: {message}")
 
@@ -70,8 +83,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     dev = q.get_device()
     (rows, columns), (_, kv_heads, page, dim) = q.shape, k_pool.shape
     sms = tuning._sm_count.get(dev) or tuning.sm_count(dev)
-    # the tensor-core kernels are built for these head sizes and pages
-    tensor_cores = q.dtype is torch.bfloat16 and dim in (32, 64, 128) and page in (8, 16, 32, 64)
+    tensor_cores = on_tensor_cores(dim, page, q.dtype)
     # scratch of this call alone (calls on several streams do not meet in it): two partial results for each row, and for each
     # kernel two of a tile of rows for each CTA and what the merge has to know of every item (csrc/shared_schedule.cuh)
     share, groups = columns // max(1, kv_heads * dim), prefix_len.numel()

@@ -19,6 +19,7 @@ import torch
 
 from dispec_b200 import ops
 from dispec_b200.ops import attention as attn_ops
+from dispec_b200.ops import beams
 from dispec_b200.ops import norm32 as norm32_ops
 from dispec_b200.ops import short_conv as conv_ops
 from dispec_b200.cache.manager import CacheTensor
@@ -120,7 +121,15 @@ class GQAAttention(Mixer):
                                  scale, fused_rope=fused)
         return ops.linear(out, self.w_o, self.b_o, residual=residual, out=residual, then_norm=then_norm)
 
-    takes_trees = takes_shared = True
+    takes_trees = True
+
+    def takes_shared(self, page_size, dtype):
+        if not beams.takes_heads(self.head_dim):
+            return None
+        # the arithmetic of the kernel that single tokens have otherwise, where the one for shared pages has no less
+        if not attn_ops.tensor_core_supported(self.head_dim, self.num_heads // self.num_kv_heads, dtype):
+            return torch.float32
+        return torch.bfloat16 if beams.on_tensor_cores(self.head_dim, page_size, dtype) else "32 bits for tensor cores"
 
     def _shared(self, ctx, qkv, cache, inv_freq, rotary_dim, scale):
         """A step of beams: single tokens, whose sequences share pages group by group."""

@@ -105,8 +105,11 @@ class Part:
     graph_safe = True
     # True for a mixer whose forward takes a step of drafted trees (``ctx.tree``, see engine/batch.py)
     takes_trees = False
-    # True for a mixer that reads pages which sequences share once for all of them (``ctx.shared``); others read them for each
-    takes_shared = False
+
+    def takes_shared(self, page_size: int, dtype: torch.dtype):
+        """How a mixer reads pages that sequences share once for all of them (``ctx.shared``), as a key of SHARED_BYTES
+        (engine/runner.py), which says when that is worth it; None: it reads them for each."""
+        return None
 
     def tensor_specs(self) -> dict[str, TensorSpec]:
         return {}

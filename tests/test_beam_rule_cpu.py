@@ -1,0 +1,45 @@
+"""Which mixers read pages that sequences share once for all of them, and by kernels of which arithmetic."""
+import importlib
+import math
+
+import pytest
+import torch
+
+import replay_util as ru
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def mixers(config):
+    from dispec_b200 import build_model, load_model_config
+    model = build_model(load_model_config(config))
+    return [model.layers[call.layer].mixer for call in model.schedule]
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,page,dtype,by", [
+    (128, 28, 4, 16, BF16, BF16), (64, 16, 4, 8, BF16, BF16), (32, 3, 1, 64, BF16, BF16), (32, 3, 1, 64, F32, F32), (128, 12, 2, 16, F32, F32),
+    # single tokens have a tensor-core kernel there, shared pages have none
+    (96, 28, 4, 16, BF16, "32 bits for tensor cores"), (16, 4, 2, 16, BF16, "32 bits for tensor cores"), (256, 8, 2, 16, BF16, "32 bits for tensor cores"),
+    (128, 28, 4, 4, BF16, "32 bits for tensor cores"), (64, 16, 4, 128, BF16, "32 bits for tensor cores"), (64, 16, 4, 24, BF16, "32 bits for tensor cores"),
+    # neither has one
+    (24, 8, 2, 16, BF16, F32), (8, 4, 2, 16, BF16, F32), (64, 130, 2, 16, BF16, F32), (96, 28, 4, 16, F32, F32),
+    # no kernel takes these heads
+    (20, 4, 2, 16, F32, None), (20, 4, 2, 16, BF16, None), (12, 4, 2, 8, F32, None), (264, 4, 2, 16, F32, None)])
+def test_heads_of_every_kind(dim, heads, kv_heads, page, dtype, by):
+    for mixer in mixers(dict(ru.CONFIG_A, head_dim=dim, num_attention_heads=heads, num_key_value_heads=kv_heads)):
+        assert mixer.takes_shared(page, dtype) == by
+
+
+def test_there_is_a_threshold_for_each():
+    from dispec_b200.engine.runner import SHARED_BYTES
+    assert SHARED_BYTES[BF16] > 0 and SHARED_BYTES[F32] > 0 and SHARED_BYTES["32 bits for tensor cores"] == math.inf
+
+
+@pytest.mark.parametrize("family", ["puludra", "murutar", "desalix", "milivik", "bepepel", "pikalorn"])
+def test_other_mixers_read_them_for_each(family):
+    from dispec_b200.parts.attention import GQAAttention
+    util = importlib.import_module(f"{family}_util")
+    for name in sorted(util.CONFIGS):
+        for mixer in mixers(util.CONFIGS[name]["config"]):
+            if type(mixer) is not GQAAttention:
+                assert mixer.takes_shared(16, BF16) is None and mixer.takes_shared(16, F32) is None
