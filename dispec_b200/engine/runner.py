@@ -20,6 +20,7 @@ from dispec_b200.cache.storage import CacheStorage, StateStorage
 from dispec_b200.engine.batch import (HostStaging, SeqEntry, SharedStep, StepPlanLayout, TreeEntry, build_context,
                                       build_tree_context)
 from dispec_b200.ops import library as _library
+from dispec_b200.ops.beams import ON_FMA_UNITS
 from dispec_b200.models.model import DecoderModel
 
 # Context lengths for which a captured decode step is laid out (the last class is the engine's
@@ -28,16 +29,46 @@ from dispec_b200.models.model import DecoderModel
 GRAPH_CONTEXT_CLASSES = (2048, 8192, 32768, 131072, 524288)
 
 
-# Bytes of keys and values that reading shared pages once has to save in a layer.  The attention of shared pages is three launches
-# where that of single tokens is one: some 10 us, in which 100 MB come from the L2 and the memory.  A layer of a step, heads of 128,
-# shared and each its own: 8 beams behind 4,096 tokens, 28 heads on 4 (59 MB) 41 and 37 us, 4 behind 16,384 (101 MB) 45 and 50, 8 behind
-# 16,384 (235 MB) 54 and 75, 32 behind 16,384 (1 GB) 75 and 188; 8 behind 16,384, 12 heads on 2 (117 MB) 39 and 41.  In 32 bits the
-# attention of single tokens is bound by its arithmetic, and the products of shared pages are of tiles of rows: 2 beams behind
-# 64 tokens, 12 heads on 2 (0.1 MB) 61 and 58 us, behind 256 (0.5 MB) 62 and 71, behind 16,384 87 and 1,264.
+# Bytes of keys and values that reading shared pages once has to save in a layer: the attention of shared pages is three launches and
+# one of the rotation where that of single tokens is one.  A layer of a step as the engine runs it, eagerly and read back (models of 8 to
+# 14 layers, layer by layer both), shared and each its own, us: 28 heads of 128 on 4, 4 beams behind 16,384 tokens (101 MB) 160 and
+# 160, 8 behind 16,384 (235 MB) 174 and 184, 32 behind 16,384 (1 GB) 272 and 380, 32 groups of 4 behind 500 (98 MB) 259 and 243, 8 of 5
+# behind 4,101 (268 MB) 220 and 254; 12 on 2, 8 groups of 5 (134 MB) 169 and 159; 40 on 8, 8 behind 4,096 (117 MB) 175 and 170, 4
+# behind 16,384 (201 MB) 187 and 192; 28 heads of 32 on 4, 32 behind 16,384 (260 MB) 196 and 237.  In 32 bits the attention of single
+# tokens is bound by its arithmetic, and the products of shared pages are of tiles of rows: 12 on 2, 2 beams behind 64 tokens (0.1 MB) 154
+# and 155, behind 256 (0.5 MB) 155 and 167, 8 behind 4,096 173 and 457.
 # Where single tokens have a tensor-core kernel and shared pages the 32-bit one (bfloat16 heads other than 32, 64 and 128, pages of other
-# than 8 to 64 tokens), never: a layer of a step, 28 heads of 96 on 4, 8 groups of 5 behind 4,101 tokens 440 and 294 us, 64 beams behind
-# 32,768 1,931 and 1,225.  (What is not listed counts as the model's type.)
-SHARED_BYTES = {torch.bfloat16: 100_000_000, torch.float32: 500_000, "32 bits for tensor cores": math.inf}
+# than 8 to 64 tokens), a tile of 32 rows takes as long with five of them.  28 heads of 96 on 4 never gain, 64 beams behind 32,768
+# tokens 1,931 and 1,225; one or two heads a key head do from 16 rows on: 8 of 96 on 8, 8 groups of 5 behind 4,101 (403 MB) 430 and 305, 8
+# beams behind 32,768 (705 MB) 362 and 297, 16 behind 16,384 (755 MB) 279 and 305, 32 (1.6 GB) 375 and 540; 16 of 80 on 8, 32 behind 4,096
+# (325 MB) 228 and 210, 16 behind 16,384 (629 MB) 275 and 294; 8 of 16 on 4, 64 behind 32,768 (528 MB) 899 and 1,115; 16 of 128 on 8, pages
+# of 128 tokens, 32 behind 4,096 (520 MB) 203 and 189.  Narrower heads take longer a byte, here and below.
+# (What is not listed counts as the model's type.)
+SHARED_BYTES = {torch.bfloat16: 150_000_000, torch.float32: 500_000, ON_FMA_UNITS: 600_000_000}
+FILLED_ROWS = 16
+# A step that reads shared pages once runs layer by layer, which takes the host 105 us a layer; others of a dense decoder run behind one
+# call (ops/dense_chain.py), and take as long as the device does.  So such a step has to read so many times SHARED_BYTES a layer, or the
+# device waits for the host: weights, and keys and values by what a byte of them takes (1.4 times a weight's with heads of 128).  Behind one call and shared: 12 heads of 128 on 2, 8 beams behind 16,384 tokens (0.28 GB so counted) 98
+# and 152, 32 behind 16,384 (0.85 GB) 214 and 206; 16 of 64 on 4, 8 behind 16,384 (0.30 GB) 99 and 153, 16 groups of 8 behind 4,101 (1.1 GB)
+# 291 and 252; 28 on 4, 8 behind 16,384 (0.84 GB) 190 and 174.
+CHAIN_SHARED_BYTES, KEY_BYTE = 4, 1.4
+
+
+def _time_of_a_byte(dim: int) -> float:
+    """Of keys and values, beside heads of 128: a fit to the figures above."""
+    return math.sqrt(128 / dim)
+
+
+def _least_saved(by: tuple, dtype: torch.dtype, dim: int, sequences: float) -> float:
+    """Bytes that reading shared pages once has to save, for a mixer that does so "by" (``Part.takes_shared``) and so many sequences a
+    group."""
+    kernel, heads = by
+    least = SHARED_BYTES.get(kernel, SHARED_BYTES[dtype])
+    if kernel != ON_FMA_UNITS:
+        return least
+    return least / _time_of_a_byte(dim) * (FILLED_ROWS / min(FILLED_ROWS, heads * sequences)) ** 4
+
+
 MAX_SHARED_GROUPS = 1024  # of a call (ops/beams.py)
 
 
@@ -201,19 +232,27 @@ class ModelRunner:
             self.cache.extend(e.req_id, e.start + 1)
         ctx, _ = build_context([SeqEntry(e.req_id, e.tokens, e.start, [0]) for e in entries], self.cache, self.storage, self.states,
                                self.staging, self.dtype, self.device, self.model.attention_tile_tokens, self.vocab_size)
-        n, starts, prefixes, worth = len(groups), [0], [], []
+        n, starts, prefixes, worth, reads = len(groups), [0], [], [], []
         for of in groups:
             starts.append(starts[-1] + len(of))
         for c, spec in enumerate(self.cache.groups):
-            saved = 0  # bytes that need not be read in a layer
+            saved = seen = 0  # tokens that need not be read, and that are seen
             for of, known in zip(groups, shared):
                 if len(of) > 1:
                     known[c] = self.cache.shared_pages([e.req_id for e in of], c, known[c])
                 prefixes.append(known[c] * self.page_size if len(of) > 1 else 0)
                 of_window = prefixes[-1] if spec.window <= 0 else max(0, min(prefixes[-1], prefixes[-1] + spec.window - of[0].start - 1))
-                saved += (len(of) - 1) * of_window * sum(t.num_heads * t.width for t in spec.tensors) * self.dtype.itemsize
-            least = max((SHARED_BYTES.get(by, SHARED_BYTES[self.dtype]) for by in self._shared_by[c]), default=math.inf)
-            worth.append(n <= MAX_SHARED_GROUPS and saved >= least)
+                saved += (len(of) - 1) * of_window
+                seen += sum(e.start + 1 if spec.window <= 0 else min(e.start + 1, spec.window) for e in of)
+            token = sum(t.num_heads * t.width for t in spec.tensors) * self.dtype.itemsize
+            dim = max(t.width for t in spec.tensors)
+            reads.append(spec.num_slots * seen * token * _time_of_a_byte(dim))
+            least = max((_least_saved(by, self.dtype, dim, len(entries) / n) for by in self._shared_by[c]), default=math.inf)
+            worth.append(n <= MAX_SHARED_GROUPS and saved * token >= least)
+        if self.model.dense_chain:
+            a_layer = self._layer_bytes() + KEY_BYTE * sum(reads) / sum(spec.num_slots for spec in self.cache.groups)
+            if a_layer < CHAIN_SHARED_BYTES * SHARED_BYTES[self.dtype]:
+                worth = [False] * len(worth)
         numbers = torch.tensor(starts + prefixes, dtype=torch.int32).to(self.device)
         if any(worth):
             ctx.shared = SharedStep(numbers[:n + 1], [numbers[n + 1 + c * n:n + 1 + (c + 1) * n] if w else None for c, w in enumerate(worth)])
@@ -223,6 +262,12 @@ class ModelRunner:
             self._poison(self.cache.commit(e.req_id, e.start + 1))
         self.num_steps += 1
         return logits, numbers[:n + 1]
+
+    def _layer_bytes(self) -> int:
+        """Weights of a layer of a dense decoder."""
+        block = self.model.layers[self.model.schedule[0].layer]
+        return sum(w.numel() * w.element_size() for w in (block.mixer.w_qkv, block.mixer.w_o, block.feed_forward.w_gate_up,
+                                                          block.feed_forward.w_down))
 
     @torch.inference_mode()
     def fork(self, pairs: list) -> None:

@@ -18,6 +18,7 @@ _PIECE = 8192  # logits of a piece of a row (csrc/beam_select.cu)
 
 # The tensor-core kernels are built for these head sizes and pages, and bfloat16; everything else takes the 32-bit kernel.
 TENSOR_CORE_DIMS, TENSOR_CORE_PAGES = (32, 64, 128), (8, 16, 32, 64)
+ON_FMA_UNITS = "32 bits for tensor cores"  # that kernel, where single tokens have one on the tensor cores
 
 
 def on_tensor_cores(dim: int, page_size: int, dtype: torch.dtype) -> bool:

@@ -124,12 +124,15 @@ class GQAAttention(Mixer):
     takes_trees = True
 
     def takes_shared(self, page_size, dtype):
+        group = self.num_heads // self.num_kv_heads
         if not beams.takes_heads(self.head_dim):
             return None
         # the arithmetic of the kernel that single tokens have otherwise, where the one for shared pages has no less
-        if not attn_ops.tensor_core_supported(self.head_dim, self.num_heads // self.num_kv_heads, dtype):
-            return torch.float32
-        return torch.bfloat16 if beams.on_tensor_cores(self.head_dim, page_size, dtype) else "32 bits for tensor cores"
+        if not attn_ops.tensor_core_supported(self.head_dim, group, dtype):
+            return torch.float32, group
+        if beams.on_tensor_cores(self.head_dim, page_size, dtype):
+            return torch.bfloat16, group
+        return (beams.ON_FMA_UNITS, group) if group <= 2 else None
 
     def _shared(self, ctx, qkv, cache, inv_freq, rotary_dim, scale):
         """A step of beams: single tokens, whose sequences share pages group by group."""

@@ -107,8 +107,8 @@ class Part:
     takes_trees = False
 
     def takes_shared(self, page_size: int, dtype: torch.dtype):
-        """How a mixer reads pages that sequences share once for all of them (``ctx.shared``), as a key of SHARED_BYTES
-        (engine/runner.py), which says when that is worth it; None: it reads them for each."""
+        """How a mixer reads pages that sequences share once for all of them (``ctx.shared``): a key of SHARED_BYTES (engine/runner.py),
+        which says when that is worth it, and query heads a key head; None: it reads them for each."""
         return None
 
     def tensor_specs(self) -> dict[str, TensorSpec]:
