@@ -289,6 +289,10 @@ beam_pieces_kernel(const Args a) {
     }
     if (__syncthreads_or(!ok)) {  // a copy did not arrive: the block leaves together
       if (tid == 0) atomicOr(a.err, DSP_ERR_WAIT_LIMIT);
+      // the parts that are left have no entries (the groups' kernel goes by what stands there)
+      const int last_row = (end - 1) / a.pieces;
+      for (int r = row + tid; r <= last_row; r += THREADS) a.parts[blockIdx.x + r] = (uint32_t)r << 16;
+      if (tid == 0 && end % a.pieces == 0) a.parts[blockIdx.x + last_row + 1] = (uint32_t)last_row << 16;
       // let copies that are still on their way land before the shared memory goes away
 #pragma unroll 1
       for (int i = 0; i < 2000; ++i) __nanosleep(100);

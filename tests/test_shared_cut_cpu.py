@@ -1,96 +1,12 @@
 """How the attention of sequences with a shared beginning is cut, run on the host: csrc/shared_schedule.cuh compiled by the C++ compiler,
 a block's threads as coroutines that meet where its threads do.  Every key tile that a row of a group sees is walked once, no other
 is, and every walk ends."""
-import os
 import random
-import shutil
 import subprocess
 
 import pytest
 
-ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-CSRC = os.path.join(ROOT, "dispec_b200", "csrc")
-
-# What common.cuh gives the schedule, for threads that run in turn.
-COMMON = r"""
-#pragma once
-#include <stdint.h>
-#include <stdio.h>
-#include <stdlib.h>
-#include <ucontext.h>
-#include <algorithm>
-#include <functional>
-#include <vector>
-using std::max;
-using std::min;
-#define __device__
-#define __host__
-#define __forceinline__ inline
-#define __noinline__
-struct float2 { float x, y; };
-struct Dim { int x; };
-enum { DSP_ERR_BAD_GROUP = 16 };
-inline Dim threadIdx, blockDim;
-
-// A block of coroutines.  A thread that meets others gives way until all of them have come.
-struct Block {
-  struct Thread { ucontext_t at; std::vector<char> stack; bool done; };
-  struct Meeting { int expected = 0, come = 0; long turn = 0; int any = 0, result = 0; int values[1024]; int out[1024]; };
-  std::vector<Thread> threads;
-  std::vector<Meeting> warps;
-  Meeting all;
-  ucontext_t home;
-  int now = 0;
-  std::function<void()> work;
-  static Block*& current() { static Block* b; return b; }
-  static void enter() { Block* b = current(); b->work(); b->threads[b->now].done = true; }
-  void run(int n, std::function<void()> f) {
-    work = f, current() = this, blockDim.x = n;
-    threads.resize(n), warps.resize((n + 31) / 32);
-    all.expected = n, all.come = 0;
-    for (auto& w : warps) w.expected = 32, w.come = 0;
-    for (auto& t : threads) {
-      t.stack.resize(1 << 16), t.done = false;
-      getcontext(&t.at);
-      t.at.uc_stack.ss_sp = t.stack.data(), t.at.uc_stack.ss_size = t.stack.size(), t.at.uc_link = &home;
-      makecontext(&t.at, enter, 0);
-    }
-    for (long idle = 0; idle < 1000000; ++idle) {
-      bool left = false;
-      for (now = 0; now < n; ++now)
-        if (!threads[now].done) left = true, threadIdx.x = now, swapcontext(&home, &threads[now].at);
-      if (!left) return;
-    }
-    fprintf(stderr, "threads wait for one another\n"), exit(3);
-  }
-  void meet(Meeting& m, int place, int value) {
-    const long turn = m.turn;
-    m.values[place] = value;
-    if (++m.come == m.expected) {
-      std::copy(m.values, m.values + m.expected, m.out);
-      m.come = 0, ++m.turn;
-      return;
-    }
-    while (m.turn == turn) swapcontext(&threads[now].at, &home);
-  }
-};
-inline int* meet_all(int value = 0) { Block* b = Block::current(); b->meet(b->all, threadIdx.x, value); return b->all.out; }
-inline int* meet_warp(int value) {
-  Block* b = Block::current();
-  Block::Meeting& w = b->warps[threadIdx.x / 32];
-  b->meet(w, threadIdx.x % 32, value);
-  return w.out;
-}
-inline void __syncthreads() { meet_all(); }
-inline int __syncthreads_or(int x) { const int* v = meet_all(x != 0); int any = 0; for (int i = 0; i < blockDim.x; ++i) any |= v[i]; meet_all(); return any; }
-inline int __reduce_max_sync(unsigned, int x) { const int* v = meet_warp(x); const int r = *std::max_element(v, v + 32); meet_warp(0); return r; }
-inline int __reduce_min_sync(unsigned, int x) { const int* v = meet_warp(x); const int r = *std::min_element(v, v + 32); meet_warp(0); return r; }
-inline int __shfl_xor_sync(unsigned, int x, int o) { const int r = meet_warp(x)[(threadIdx.x % 32) ^ o]; meet_warp(0); return r; }
-inline int __shfl_up_sync(unsigned, int x, int o) { const int l = threadIdx.x % 32, r = meet_warp(x)[l < o ? l : l - o]; meet_warp(0); return r; }
-inline void atomicOr(int* p, int x) { *p |= x; }
-inline void atomicMin(int* p, int x) { *p = min(*p, x); }
-inline void atomicMax(int* p, int x) { *p = max(*p, x); }
-"""
+import host_block
 
 # Reads a call, walks every CTA's run, and writes the shares.
 PROGRAM = r"""
@@ -136,20 +52,13 @@ int main() {
 
 @pytest.fixture(scope="module")
 def walk(tmp_path_factory):
-    cxx = os.environ.get("CXX") or shutil.which("g++")
-    if not cxx:
-        pytest.skip("no C++ compiler")
-    at = tmp_path_factory.mktemp("cut")
-    for name in ("shared_schedule.cuh", "rows_schedule.cuh"):
-        shutil.copy(os.path.join(CSRC, name), at)
-    (at / "common.cuh").write_text(COMMON)
-    (at / "walk.cpp").write_text("#include <string.h>\n" + PROGRAM)
-    subprocess.run([cxx, "-std=c++20", "-O2", "-w", "-I", str(at), str(at / "walk.cpp"), "-o", str(at / "walk")], check=True)
+    names = ("shared_schedule.cuh", "rows_schedule.cuh")
+    program = host_block.compiled(tmp_path_factory.mktemp("cut"), {name: host_block.source(name) for name in names}, PROGRAM)
 
     def of(starts, prefix, ctx, kv_heads=2, group=4, window=0, most_ctx=1 << 20, row_shift=6, extra=3, heavy=32, many=1 << 20, is_many=False,
            ctas=24, threads=160):
         numbers = [len(prefix), len(ctx), kv_heads, group, window, most_ctx, row_shift, extra, heavy, -many if is_many else many, ctas, threads]
-        done = subprocess.run([str(at / "walk")], input=" ".join(map(str, numbers + starts + prefix + ctx)), capture_output=True, text=True, timeout=120)
+        done = subprocess.run([program], input=" ".join(map(str, numbers + starts + prefix + ctx)), capture_output=True, text=True, timeout=120)
         assert done.returncode == 0, (done.returncode, done.stderr)
         *lines, last = done.stdout.splitlines()
         shares = [tuple(map(int, line.split())) for line in lines]
