@@ -158,8 +158,8 @@ extern "C" int dsp_shared_attention(const DspTensor* t, const DspSharedOptions* 
   SHARED_REQUIRE(R == 0 || q.stride[1] == 1 || columns == 1, "the columns of q must be neighbours");
   SHARED_REQUIRE(D % 8 == 0 && D >= 8 && D <= 256 && KVH > 0 && columns > 0 && columns % D == 0 && columns / D % KVH == 0,
                  "%ld query columns on %ld heads of %ld (a multiple of 8 up to 256)", columns, KVH, D);
-  SHARED_REQUIRE(o->scale > 0. && o->scale <= 3e38 && o->window >= 0 && o->window <= 0x7fffffff,
-                 "scale %g must be positive, window %ld not negative", o->scale, o->window);
+  SHARED_REQUIRE(is_scale(o->scale) && o->window >= 0 && o->window <= 0x7fffffff,
+                 "scale %g must be positive and finite in 32 bits, window %ld not negative", o->scale, o->window);
   SHARED_REQUIRE(prefix.dims == 1 && prefix.size[0] <= MAX_GROUPS, "prefix_len must be one-dimensional, of at most %d groups", MAX_GROUPS);
   const long groups = prefix.size[0];
   SHARED_REQUIRE(tensor_is(ctx, DSP_T_I32, q.device, 1, R) && tensor_is(start, DSP_T_I32, q.device, 1, groups + 1) &&

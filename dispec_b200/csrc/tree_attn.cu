@@ -100,8 +100,8 @@ extern "C" int dsp_tree_attention(const DspTensor* t, const DspTreeOptions* o, c
   const long S = ctx.size[0], words = visible.dims == 2 ? visible.size[1] : 0;
   DSP_REQUIRE(tensor_is(visible, DSP_T_I64, q.device, 2, T, words) && words >= 1 && 64 * words >= o->max_nodes,
               "tree_attention: visible must be contiguous int64 [%ld, words] with a bit for each of %ld nodes", T, o->max_nodes);
-  DSP_REQUIRE(o->scale > 0. && o->window >= 0 && o->window <= 0x7fffffff && o->max_nodes >= 1,
-              "tree_attention: scale %g must be positive, window %ld not negative, max_nodes %ld at least 1", o->scale, o->window,
+  DSP_REQUIRE(is_scale(o->scale) && o->window >= 0 && o->window <= 0x7fffffff && o->max_nodes >= 1,
+              "tree_attention: scale %g must be positive and finite in 32 bits, window %ld not negative, max_nodes %ld at least 1", o->scale, o->window,
               o->max_nodes);
   DSP_REQUIRE(tensor_is(ctx, DSP_T_I32, q.device, 1, S) && tensor_is(start, DSP_T_I32, q.device, 1, S + 1),
               "tree_attention: ctx_len [%ld] and node_start [%ld] must be contiguous int32 on the device of q", S, S + 1);

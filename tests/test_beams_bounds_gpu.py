@@ -57,3 +57,15 @@ def test_attention_rows_between_groups_that_are_there_stay(dtype, dim, long):
     got = out.double().cpu()
     there = torch.arange(60) % 3 == 0
     assert ops.device_error() == 16 and ((got - want).abs() <= bound)[there].all() and (got[~there] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,dim,long", KERNELS)
+@pytest.mark.parametrize("scale", [1e-44, 1e-38])
+def test_attention_of_the_smallest_scales(dtype, dim, long, scale):
+    """All weights are one, and hidden keys have none."""
+    from dispec_b200 import ops
+    case = SharedCase([(100, [130, 101, 90] * 30), (9, [20])], 8, 2, dim, dtype, scale=scale)
+    if long:
+        case.table = torch.nn.functional.pad(case.table, (0, 1600), value=-1)
+    case.check()
+    ops.raise_on_device_error("test")
