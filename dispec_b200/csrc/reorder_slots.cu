@@ -178,6 +178,11 @@ extern "C" int dsp_reorder_slots(const DspTensor* t, long pools, cudaStream_t st
   }
   if (blocks == 0) return 0;
   REORDER_REQUIRE(current_device() == src.device, "the tensors are on device %d, the current device is %d", src.device, current_device());
+  // (blocks read the lists while others write)
+  for (const DspTensor* list : {&src, &dst})
+    for (long p = 0; p < pools; ++p)
+      REORDER_REQUIRE((uintptr_t)list->data >= ends[p] || (uintptr_t)list->data + 4 * (uintptr_t)n <= (uintptr_t)a.pools[p].data,
+                      "src or dst lies in pool %ld", p);
   a.src = (const int*)src.data;
   a.dst = (const int*)dst.data;
   a.count = (int)n;

@@ -145,7 +145,7 @@ def reorder_slots(pools: list, src: torch.Tensor, dst: torch.Tensor) -> None:
     though all were read before any is written (a slot may be read by several and written by another).
 
     ``pools``: up to 64 contiguous tensors [layers, slots, ...] of three to five dimensions, float32, bfloat16, int32 or int64,
-    with the same number of slots and no memory in common;
+    with the same number of slots and no memory in common, with each other or with ``src`` and ``dst``;
     ``src``, ``dst`` int32 [n], n up to 8,192, ``dst`` ascending: what does not ascend, or names a slot that is not there, is
     left from there on and recorded as a device error."""
     what = "reorder_slots"

@@ -69,3 +69,22 @@ def test_attention_of_the_smallest_scales(dtype, dim, long, scale):
         case.table = torch.nn.functional.pad(case.table, (0, 1600), value=-1)
     case.check()
     ops.raise_on_device_error("test")
+
+
+def test_reorder_lists_in_a_pool_are_refused():
+    """Blocks would read them while others write there."""
+    from dispec_b200 import ops
+    from dispec_b200.ops import KernelError
+    pool = torch.arange(2 * 8 * 16, dtype=torch.int32, device=DEV).view(2, 8, 16) % 8
+    before = pool.clone()
+    inside, apart = pool.view(-1)[4:6], i32([1, 2])
+    for src, dst in ((inside, apart), (apart, inside), (pool.view(-1)[-2:], apart), (apart, pool.view(-1)[:2])):
+        with pytest.raises(KernelError, match="pool 1"):
+            ops.reorder_slots([torch.zeros(1, 8, 4, dtype=torch.int32, device=DEV), pool], src, dst)
+    assert torch.equal(pool, before)
+    both = i32([0, 1] + list(range(100, 164)) + [2, 5])  # beside a pool is not in it
+    want = both[2:66].view(2, 8, 4).clone()
+    want[:, [2, 5]] = want[:, [0, 1]]
+    ops.reorder_slots([both[2:66].view(2, 8, 4)], both[:2], both[66:])
+    assert torch.equal(both[2:66].view(2, 8, 4), want)
+    assert ops.device_error() == 0
