@@ -100,6 +100,10 @@ class BeamSearchEngine:
             raise ValueError(f"length_penalty={length_penalty}")
         if max_new_tokens <= 0:
             return [[] for _ in prompts]
+        try:
+            max_new_tokens ** abs(length_penalty)
+        except OverflowError:
+            raise ValueError(f"length_penalty={length_penalty}: {max_new_tokens} tokens to this power cannot be counted") from None
         at_once = self.max_num_seqs // self.beam_width
         out = []
         for i in range(0, len(prompts), at_once):
