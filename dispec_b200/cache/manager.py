@@ -271,6 +271,10 @@ class CacheManager:
         """How many first pages all these requests share (``known``: so many do, as the caller knows)."""
         tables = [self._requests[r].tables[group] for r in req_ids]
         n = min(len(t) for t in tables)
+        # a longer request may since have given back pages that a shorter one still reads: those are not shared any more
+        first_live = [self._requests[r].first_live[group] for r in req_ids]
+        if min(first_live) != max(first_live):
+            known = min(known, min(first_live))
         while known < n and all(t[known] == tables[0][known] for t in tables):
             known += 1
         return min(known, n)

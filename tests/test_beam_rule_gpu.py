@@ -136,3 +136,32 @@ def test_sixteen_rows_of_heads_without_a_kernel_on_tensor_cores(monkeypatch):
     few = beams_behind(run, 96, 11, "few")
     assert shared_calls(run, monkeypatch, [names[:11]], 16385) == 0  # 503 MB
     assert shared_calls(run, monkeypatch, [[n] for n in few], 96) == 0
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_sequences_of_different_lengths_behind_a_window(first, monkeypatch):
+    """The longer one has given back pages that the shorter one reads, and that were known to be shared."""
+    from dispec_b200 import SeqEntry, ops
+    from dispec_b200.engine import runner
+    monkeypatch.setattr(runner, "SHARED_BYTES", {F32: 1})
+    run = runner_of("float32", head_dim=32, use_sliding_window=True, sliding_window=40, max_window_layers=1,
+                    layer_types=["full_attention", "sliding_attention"])
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    for pools in run.storage.pools:
+        for pool in pools.values():
+            pool.normal_(generator=gen)
+    names = beams_behind(run, 64, 2)
+    known = [[0, 0]]
+    run.beam_step([[SeqEntry(n, [5], 64) for n in names]], known)
+    assert known == [[4, 4]]
+    at = [130, 70]  # the window begins at 91 and 31
+    for n, length in zip(names, at):
+        run.cache.extend(n, length)
+        run.cache.commit(n, length)
+    others = [(n, "other") for n in names]
+    run.fork(list(zip(names, others)))
+    entries = lambda of: [SeqEntry(of[i], [7 + i], at[i]) for i in (first, 1 - first)]
+    got = run.beam_step([entries(names)], known)[0]
+    monkeypatch.setattr(runner, "SHARED_BYTES", {F32: math.inf})
+    want = run.beam_step([entries(others)], [[0, 0]])[0]
+    assert ops.device_error() == 0 and (got - want).abs().max() <= 1e-4 * max(1.0, float(want.abs().max()))
