@@ -10,6 +10,7 @@ dispec/engine/model_runner.py:188-231) with the bookkeeping its callers do by ha
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -105,12 +106,6 @@ class ModelRunner:
         self._group_windows = [g.window for g in groups]
         self._group_pages = list(counts)
         self._graphs: dict = {}
-        # per cache group: how its mixers read pages that sequences share
-        self._shared_by: list = [set() for _ in groups]
-        for call, label in zip(model.schedule, model.call_cache):
-            by = model.layers[call.layer].mixer.takes_shared(page_size, self.dtype)
-            if label is not None and by is not None:
-                self._shared_by[model.placement[label].group].add(by)
 
     # ---------------------------------------------------------------- request lifecycle
     def admit(self, req_id, prompt_len: int = 0, max_total_len: int = 0, max_chunk: int = 1) -> None:
@@ -262,6 +257,17 @@ class ModelRunner:
             self._poison(self.cache.commit(e.req_id, e.start + 1))
         self.num_steps += 1
         return logits, numbers[:n + 1]
+
+    @functools.cached_property
+    def _shared_by(self) -> list:
+        """Per cache group: how its mixers read pages that sequences share."""
+        of = [set() for _ in self.cache.groups]
+        for call, label in zip(self.model.schedule, self.model.call_cache):
+            if label is not None:
+                by = self.model.layers[call.layer].mixer.takes_shared(self.page_size, self.dtype)
+                if by is not None:
+                    of[self.model.placement[label].group].add(by)
+        return of
 
     def _layer_bytes(self) -> int:
         """Weights of a layer of a dense decoder."""
