@@ -56,7 +56,8 @@ __device__ __forceinline__ int sound_entries(const Args& a, const Pool& pool, in
 // Rows of whole 16-byte pieces and up to BULK_ENTRIES entries: the columns of an entry are one bulk copy into shared memory and one
 // back, of whole lines of 128 bytes where six blocks an SM hold them, else of 96 bytes at least.  The two calls above: 136 and 23.6 us; with
 // 48 KB a block and copies of 336 and 4,096 bytes 160 and 24.9; lines, and room for 48 KB all the same (four blocks an SM) 165; lines with
-// 74 KB 140 and 25.3.  Through registers, eight pieces a thread, 203 and 32.7; more entries, and rows of other sizes, go that way.
+// 74 KB 140 and 25.3.  Through registers, eight pieces a thread, 203 and 32.7; more entries, and rows of other sizes, go that way
+// (rows of 32 KB in 24 layers, behind a flushed L2: 512 entries 3.4 TB/s, 513 3.0; rows of 32,776 bytes 2.1).
 constexpr int BULK_THREADS = 128, BULK_ENTRIES = 512, BULK_BYTES = 48 * 1024, LINE_BYTES = 37 * 1024;
 __global__ void __launch_bounds__(BULK_THREADS)
 reorder_bulk_kernel(const __grid_constant__ Args a) {

@@ -8,7 +8,8 @@
 // join as  M = max m,  o = sum a exp(m - M) / sum l exp(m - M).  So the shared keys are read once for all sequences of a group,
 // whose rows fill the tiles of a matrix product, and each sequence's own keys once for its G rows.  A row that sees nothing gives 0.
 // The work is cut as shared_schedule.cuh says; the kernels: shared_attn_few.cuh, shared_attn_many.cuh where many rows share keys,
-// rows_attn.cuh in 32-bit arithmetic.
+// rows_attn.cuh in 32-bit arithmetic, which bfloat16 heads without a tensor-core kernel take too (8 groups of 5 behind 4,096 tokens
+// with 130 of their own, 28 heads on 4: of 96 222 us, of 128 on the tensor cores 43, each call behind a flushed L2).
 #include "merge_parts.cuh"
 #include "rows_attn.cuh"
 #include "shared_schedule.cuh"
@@ -28,6 +29,9 @@ constexpr long FEW_ROWS_OF_A_TILE = 1 << ROW_SHIFT_FEW;
 // 40 of 64 on 8, heads of 128, with both kernels and with the one for few alone: shared parts of 4,000 tokens (3.4, 11.9 and 17.0 tiles
 // an SM) 25.2, 39.7 and 43.0 us and 21.3, 39.2 and 48.6; of 8,000 26.2, 43.6 and 50.6 and 28.1, 65.1 and 72.1; of 32,000 39.3, 69.8
 // and 94.2 and 55.2, 160.5 and 211.9.  8 groups of 16 with 28 heads: 1,000 tokens (6.1) 37.3 and 35.2, 2,000 (12.1) 39.1 and 43.5.
+// Groups and lengths are the device's, so the rule goes by rows a group on average and by the pages that a sequence may have: one
+// group of many rows among many of one goes to the kernel for few, in tiles of 64 that each read the shared keys, and short
+// beginnings in wide page tables pay for the kernel more.
 constexpr long MANY_UNITS = 12;
 constexpr int EXTRA_FEW = 3, HEAVY_FEW = 32, EXTRA_32BIT = 0, EXTRA_MANY = 5;
 

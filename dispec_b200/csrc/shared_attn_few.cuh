@@ -14,7 +14,7 @@
 // What bounds it: with sixteen rows the way from memory once it is full (148 sequences of 1,000 tokens, 28 heads of 128 on 4: 303 MB
 // in 58 us behind 6 us in which the runs are found, 5.2 TB/s; 1,150 cycles a tile and CTA are work), with 33 to 64 rows its own
 // instructions (3,100 cycles a tile and CTA for 35, 3,750 for 64: products 1,024, reads of keys and values by every row tile 1,024,
-// the softmax between them): 8 groups of 5 behind 4,101 tokens, 28 heads on 4: 30.4 us, 60 MB.  In calls this short the beginnings
+// the softmax between them): 8 groups of 5 behind 4,101 tokens, 28 heads on 4: 29.7 us, 60 MB.  In calls this short the beginnings
 // count: 3.7 us until the runs are found, 3.5 until the first tile is there, 3 for the first steps' instructions.
 // Heads of 32, 28 on 4: those 8 groups 25.4 us (103 in 32-bit arithmetic), 148 sequences of 1,000 tokens 35.2 (185); they have no kernel for
 // many rows: 64 sequences of 40 heads on 8 behind 32,768 tokens 118 us (849).

@@ -11,7 +11,8 @@
 //
 // Two kernels may share the work: beginnings with more than `many` rows a head go to one whose tiles have 256 rows, the rest to
 // one with smaller tiles.  Where all beginnings of the first have R row tiles, teams of R CTAs walk the same keys with one row
-// tile each, which then come from memory once and from the L2 for the others.
+// tile each, which then come from memory once and from the L2 for the others.  CTAs beyond the last whole team have nothing to do
+// (75 row tiles, some 2,400 sequences of 8 rows a head, leave 73 of 148 idle), and a last row tile of few rows has as many as a full one.
 //
 // Every item leaves a partial result (32-bit sums that are not divided yet, running maximum, sum of weights): in the place of its
 // rows, `rows_o`, where one CTA had all of it, else one in each CTA's scratch slots (2 c + 1 for the item that begins in CTA c,
