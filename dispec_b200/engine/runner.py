@@ -263,10 +263,10 @@ class ModelRunner:
         """Per cache group: how its mixers read pages that sequences share."""
         of = [set() for _ in self.cache.groups]
         for call, label in zip(self.model.schedule, self.model.call_cache):
-            if label is not None:
-                by = self.model.layers[call.layer].mixer.takes_shared(self.page_size, self.dtype)
-                if by is not None:
-                    of[self.model.placement[label].group].add(by)
+            takes = getattr(self.model.layers[call.layer].mixer, "takes_shared", None)  # (a mixer need not know of it)
+            by = takes(self.page_size, self.dtype) if takes is not None and label is not None else None
+            if by is not None:
+                of[self.model.placement[label].group].add(by)
         return of
 
     def _layer_bytes(self) -> int:

@@ -50,3 +50,15 @@ def test_other_mixers_read_them_for_each(family):
         for mixer in mixers(util.CONFIGS[name]["config"]):
             if type(mixer) is not GQAAttention:
                 assert mixer.takes_shared(16, BF16) is None and mixer.takes_shared(16, F32) is None
+
+
+def test_mixers_that_know_nothing_of_it_and_ones_without_a_cache():
+    from types import SimpleNamespace as N
+    from dispec_b200.engine.runner import ModelRunner
+    takes, states = N(takes_shared=lambda page, dtype: (dtype, page)), N(takes_shared=lambda page, dtype: 1 / 0)
+    layers = [N(mixer=m) for m in (takes, N(), states, takes)]
+    run = object.__new__(ModelRunner)
+    run.cache, run.page_size, run.dtype = N(groups=[0, 1, 2]), 16, BF16
+    run.model = N(schedule=[N(layer=i) for i in (0, 1, 2, 3)], layers=layers, call_cache=[0, 1, None, 2],
+                  placement={0: N(group=0), 1: N(group=1), 2: N(group=0)})
+    assert run._shared_by == [{(BF16, 16)}, set(), set()]
