@@ -88,3 +88,36 @@ def test_reorder_lists_in_a_pool_are_refused():
     ops.reorder_slots([both[2:66].view(2, 8, 4)], both[:2], both[66:])
     assert torch.equal(both[2:66].view(2, 8, 4), want)
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("masked", [-1e9, torch.finfo(torch.bfloat16).min])
+@pytest.mark.parametrize("kept,count", [(3, 8), (20, 8), (20, 40), (9000, 256)])
+def test_select_rows_masked_by_a_finite_number(dtype, masked, kept, count):
+    """Most of a piece is equal, and it may take masked tokens to fill the choice: the lowest ones."""
+    from beams_util import plain_select, select_tolerance
+    from dispec_b200 import ops
+    gen = torch.Generator().manual_seed(kept)
+    logits = torch.full((6, 30000), masked)
+    for row in logits:
+        row[torch.randperm(30000, generator=gen)[:kept]] = 2.5 * torch.randn(kept, generator=gen)
+    logits, scores = logits.to(dtype), -10 * torch.rand(6, generator=gen)
+    starts = [0, 4, 6]
+    got = ops.beam_select(logits.to(DEV), scores.to(DEV), i32(starts), count=count)
+    parent, token, key = plain_select(logits.float(), scores, starts, count)
+    assert ops.device_error() == 0 and (got.parent >= 0).all()
+    # scores are rounded to 32 bits, and those of masked tokens are as large as the mask
+    tolerance = select_tolerance(30000, 30.0) + key.abs() * 2.0 ** -23
+    assert ((got.score.cpu().double() - key).abs() <= tolerance).all()
+    sure = torch.ones_like(key, dtype=torch.bool)  # where the next in line is not as good
+    sure[:, 1:] &= (key[:, :-1] - key[:, 1:]) > 2 * tolerance[:, 1:]
+    sure[:, :-1] &= (key[:, :-1] - key[:, 1:]) > 2 * tolerance[:, :-1]
+    sure[:, -1] = False
+    assert torch.equal(got.parent.cpu()[sure].long(), parent[sure]) and torch.equal(got.token.cpu()[sure].long(), token[sure])
+    # of one row's masked tokens, which are all equal, the lowest are taken, in order
+    for g in range(2):
+        p, t = got.parent[g].cpu(), got.token[g].cpu()
+        for r in set(p.tolist()):
+            mine = t[(p == r) & (logits[p.long(), t.long()] == logits.min())]
+            lowest = (logits[r] == logits.min()).nonzero()[:len(mine), 0]
+            assert torch.equal(mine.long(), lowest)
